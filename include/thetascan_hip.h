@@ -53,8 +53,10 @@ extern "C" {
  *     ts_rotary_tables, ts_causal_attention_fwd, ts_scale_add_norm_fwd and
  *     ts_contract_sums; bf16 scans take up to 384 keys and 512 values; the 64
  *     rows of a token group of a GN stream have to lie within 4 GiB (a row
- *     stride of 32 Mi elements and more was taken before). */
-#define TS_ABI_VERSION 18
+ *     stride of 32 Mi elements and more was taken before).
+ * 19: ts_delta_fwd / ts_delta_bwd / ts_delta_step (with their workspace sizes)
+ *     and ts_policy_loss_fwd / ts_policy_loss_bwd; nothing earlier changed. */
+#define TS_ABI_VERSION 19
 
 enum ts_status {
   TS_OK = 0,
@@ -1245,6 +1247,56 @@ typedef struct ts_memory_grads {
 int ts_memory_bwd(const ts_memory_desc* desc, const ts_memory_io* io, const ts_memory_grads* grads,
                   const void* saved, size_t saved_bytes, void* scratch, size_t scratch_bytes,
                   hipStream_t stream);
+
+/* ------------------------------------------------ gated delta rule */
+
+/* Per batch and value head, from the state S [dk,dv] (fp32):
+ *   S <- a_t S;  u = b_t (v_t - S^T k_t);  S <- S + k_t u^T;  out_t = S^T q_t
+ * with a_t = exp(decay_t) (decay <= 0).  q, k [B,Hk,T,dk] (value head h reads
+ * head h / (H / Hkeys)), v, out [B,H,T,dv]; dk <= 128, dv <= 512. */
+typedef struct ts_delta_desc {
+  int32_t B, Hk, H, T, dk, dv; /* dk and dv multiples of 16 bytes              */
+  int32_t dtype;               /* of q, k, v, out and their gradients          */
+  int32_t beta_dtype;          /* ts_dtype of beta and of its gradient         */
+  int32_t decay_dtype;
+  int32_t keep;                /* the workspace is kept for ts_delta_bwd       */
+} ts_delta_desc;
+
+typedef struct ts_delta_io {
+  ts_strided q, k, v;     /* rows 16-byte aligned                                */
+  ts_strided beta, decay; /* [B,H,T], any strides; decay NULL: none; strides
+                             (0, s, 0): one retention a head                     */
+  ts_strided out;
+  const int64_t* lengths; /* [B] or NULL: tokens of each sequence.  Tokens behind
+                             it are not read, give zeros, and leave the state   */
+  const float* state;     /* [B,H,dk,dv] contiguous, or NULL (zero)             */
+  float* state_out;       /* the state after the last token, or NULL            */
+} ts_delta_io;
+
+int ts_delta_workspace_bytes(const ts_delta_desc* desc, size_t* bytes);
+
+/* The chunked form over T tokens.  workspace: 16-byte aligned; where desc.keep,
+ * it is ts_delta_bwd's `saved`. */
+int ts_delta_fwd(const ts_delta_desc* desc, const ts_delta_io* io, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream);
+
+/* The recurrent form for few tokens, one read and one write of the state
+ * (16-byte aligned; state_out may be state).  No workspace. */
+int ts_delta_step(const ts_delta_desc* desc, const ts_delta_io* io, hipStream_t stream);
+
+typedef struct ts_delta_grads {
+  ts_strided dout;         /* [B,H,T,dv], rows 16-byte aligned                   */
+  ts_strided dq, dk, dv;   /* out, of the inputs' shapes and dtype               */
+  void* dbeta;             /* out [B,H,T] contiguous, beta's dtype               */
+  void* ddecay;            /* out [B,H,T] contiguous, decay's dtype, or NULL     */
+  void* ddecay_head;       /* out [H] for one retention a head, or NULL          */
+  const float* dstate_out; /* gradient of state_out, or NULL (zero)              */
+  float* dstate;           /* out, gradient of state, or NULL                    */
+} ts_delta_grads;
+
+int ts_delta_bwd_workspace_bytes(const ts_delta_desc* desc, size_t* bytes);
+int ts_delta_bwd(const ts_delta_desc* desc, const ts_delta_io* io, const ts_delta_grads* grads, const void* saved,
+                 size_t saved_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -3,6 +3,7 @@ hand-written gfx950 ``hip`` scan backend underneath."""
 from .api import ThetaScan
 from .state import ThetaScanState
 from .decode import DecodeGraph
+from ._core.ops.delta import gated_delta_rule
 from .config import (
     Backend,
     BankMode,
@@ -36,5 +37,5 @@ __all__ = [
     "DecodeGraph", "KernelBSplineScaleMode", "KernelConfig", "KernelFeatureMap", "KernelReLU2ThresholdMode",
     "KernelReadNormalization", "KernelSharpnessMode", "KernelSparsity", "KernelValueRepresentation",
     "RegularizationConfig", "RoPEConfig", "RoPEMode", "RoPEPlacement", "RuntimeConfig", "TemporalConfig",
-    "TemporalMode", "ThetaScan", "ThetaScanConfig", "ThetaScanState",
+    "TemporalMode", "ThetaScan", "ThetaScanConfig", "ThetaScanState", "gated_delta_rule",
 ]

@@ -1,0 +1,303 @@
+"""The gated delta rule: a causal memory that writes what it does not yet know.
+
+:func:`gated_delta_rule` is the error-correcting counterpart of the additive
+scans (:func:`.scan_hip.linattn`), with the same streams and retentions.  From
+the fp32 state ``S`` [dk, dv] of a value head, token after token::
+
+    S <- a_t S                        # the retention, a = exp(log a)
+    u  = beta_t (v_t - S^T k_t)       # what the memory misses, times the write strength
+    S <- S + k_t u^T
+    out_t = S^T q_t
+
+Whole sequences run in chunks of 64 tokens on MFMA (ts_delta_fwd, with
+ts_delta_bwd for the gradients); a few tokens against a carried state, without
+gradients, run token by token in one pass over the state (ts_delta_step).  Both
+are the same function of their inputs.
+
+bf16 inputs: products take bf16 operands and fp32 sums; everything that feeds the
+state in the forward (the state itself, what is written, the chunk's inverse)
+enters as a bf16 pair hi + lo, so the returned state is exact to about 1e-5; the
+outputs and the gradients carry bf16's rounding.  fp32 inputs compute in fp32.
+A non-finite value in a token that counts spreads over its chunk of 64 tokens
+and everything after it.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from ... import _lib
+from .dispatch import HipOp
+from .scan_hip import _kernel_view, _vec
+
+MAX_KEYS, MAX_VALUES = 128, 512
+# tokens that the recurrent form takes (without gradients)
+STEP_TOKENS = 8
+
+
+def _on(device: torch.device):
+    """The device a launch needs as the current one (a no-op where it is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _width(dtype: torch.dtype, n: int) -> int:
+    vec = _vec(dtype)
+    return -(-n // vec) * vec
+
+
+def _gate(t: torch.Tensor | None, heads: bool = False) -> _lib.Strided:
+    if t is None:
+        return _lib.Strided(None, 0, 0, 0)
+    if heads:
+        return _lib.Strided(t.data_ptr(), 0, t.stride(0), 0)
+    return _lib.Strided(t.data_ptr(), *t.stride())
+
+
+def _desc(q, k, v, beta, decay, keep: bool) -> _lib.DeltaDesc:
+    B, Hk, T, dk = q.shape
+    return _lib.DeltaDesc(B, Hk, v.shape[1], T, _width(q.dtype, dk), _width(q.dtype, v.shape[-1]),
+                          _lib.dtype_code(q.dtype), _lib.dtype_code(beta.dtype),
+                          _lib.TS_F32 if decay is None else _lib.dtype_code(decay.dtype), int(keep))
+
+
+def _padded_state(state: torch.Tensor | None, dk: int, dv: int) -> torch.Tensor | None:
+    if state is None:
+        return None
+    if state.shape[-2:] == (dk, dv) and state.is_contiguous() and state.data_ptr() % 16 == 0:
+        return state
+    out = state.new_zeros(*state.shape[:2], dk, dv)
+    out[..., :state.shape[-2], :state.shape[-1]] = state
+    return out
+
+
+def _rows_like(x: torch.Tensor, dtype: torch.dtype, width: int) -> torch.Tensor:
+    """[B,H,T,width] in x's own order: token-major memory for a projection's heads."""
+    B, H, T, _ = x.shape
+    if H > 1 and T > 1 and x.stride(1) < x.stride(2):
+        return x.new_empty(B, T, H, width, dtype=dtype).transpose(1, 2)
+    return x.new_empty(B, H, T, width, dtype=dtype)
+
+
+def _io(q, k, v, beta, decay, lengths, out, state, state_out) -> _lib.DeltaIO:
+    return _lib.DeltaIO(_lib.strided(q), _lib.strided(k), _lib.strided(v), _gate(beta),
+                        _gate(decay, decay is not None and decay.ndim == 1), _lib.strided(out), _lib.ptr(lengths),
+                        _lib.ptr(state), _lib.ptr(state_out))
+
+
+def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, step: bool, state_out=None):
+    """``(out, state or None, workspace or None)`` at the padded widths' slices."""
+    lib = _lib.load()
+    desc = _desc(q, k, v, beta, decay, keep)
+    B, H, T, dv = v.shape
+    dk, dkp, dvp = q.shape[-1], desc.dk, desc.dv
+    q, k, v4 = (_kernel_view(x) for x in (q, k, v))
+    out = _rows_like(v, q.dtype, dvp)
+    given = _padded_state(state, dkp, dvp)
+    final = None
+    if want_state:
+        if state_out is not None and (dkp, dvp) == (dk, dv) and state_out.data_ptr() % 16 == 0:
+            final = state_out
+        else:
+            final = torch.empty(B, H, dkp, dvp, dtype=torch.float32, device=q.device)
+    io = _io(q, k, v4, beta, decay, lengths, out, given, final)
+    work = None
+    with _on(q.device):
+        stream = _lib.stream_handle(q.device)
+        if step:
+            with _lib.timed("ts_delta_step", lambda: _lib.nbytes(q, k, v4, out, given, final)):
+                status = lib.ts_delta_step(ctypes.byref(desc), ctypes.byref(io), stream)
+            _lib.check(status, "ts_delta_step")
+        else:
+            work = torch.empty(_workspace_bytes(desc), dtype=torch.uint8, device=q.device)
+            with _lib.timed("ts_delta_fwd", lambda: _lib.nbytes(q, k, v4, beta, decay, out, given, final)):
+                status = lib.ts_delta_fwd(ctypes.byref(desc), ctypes.byref(io), work.data_ptr(), work.numel(), stream)
+            _lib.check(status, "ts_delta_fwd")
+    if final is not None and final is not state_out:
+        final = final[..., :dk, :dv]
+        if (dkp, dvp) != (dk, dv):
+            final = final.contiguous()
+        if state_out is not None:
+            final = state_out.copy_(final)
+    return out[..., :dv], final, work
+
+
+def _workspace_bytes(desc: _lib.DeltaDesc) -> int:
+    n = ctypes.c_size_t()
+    _lib.check(_lib.load().ts_delta_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), "ts_delta_workspace_bytes")
+    return n.value
+
+
+def _forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor | None,
+             state: torch.Tensor | None, lengths: torch.Tensor | None, want_state: bool, keep: bool,
+             step: bool) -> list[torch.Tensor]:
+    out, final, work = _launch(q, k, v, beta, decay, state, lengths, want_state, keep, step)
+    none = q.new_empty(0, dtype=torch.float32)
+    return [out, none if final is None else final, work if keep else q.new_empty(0, dtype=torch.uint8)]
+
+
+def _forward_fake(q, k, v, beta, decay, state, lengths, want_state, keep, step):
+    B, H, _, dv = v.shape
+    out = _rows_like(v, q.dtype, _width(q.dtype, dv))[..., :dv]
+    nbytes = _workspace_bytes(_desc(q, k, v, beta, decay, True)) if keep else 0
+    return [out, q.new_empty((B, H, q.shape[-1], dv) if want_state else (0,), dtype=torch.float32),
+            q.new_empty(nbytes, dtype=torch.uint8)]
+
+
+def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor,
+                   v: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor | None, state: torch.Tensor | None,
+                   lengths: torch.Tensor | None, saved: torch.Tensor, need_state: bool) -> list[torch.Tensor]:
+    lib = _lib.load()
+    desc = _desc(q, k, v, beta, decay, True)
+    B, H, T, dv = v.shape
+    Hk, dk, dkp, dvp = q.shape[1], q.shape[-1], desc.dk, desc.dv
+    q4, k4, v4 = (_kernel_view(x) for x in (q, k, v))
+    if dout is None:
+        dout = torch.zeros(B, H, T, dvp, dtype=q.dtype, device=q.device)
+    do4 = _kernel_view(dout.to(q.dtype))
+    given = None if dfinal is None else _padded_state(dfinal.to(torch.float32), dkp, dvp)
+    dq, dk_, dv_ = _rows_like(q, q.dtype, dkp), _rows_like(k, q.dtype, dkp), _rows_like(v, q.dtype, dvp)
+    dbeta = torch.empty(B, H, T, dtype=beta.dtype, device=q.device)
+    per_head = decay is not None and decay.ndim == 1
+    ddecay = None
+    if decay is not None:
+        ddecay = torch.empty((H,) if per_head else (B, H, T), dtype=decay.dtype, device=q.device)
+    dstate = torch.empty(B, H, dkp, dvp, dtype=torch.float32, device=q.device) if need_state else None
+    # (the forward's output and states play no part here: out takes dout's rows)
+    io = _io(q4, k4, v4, beta, decay, lengths, do4, None, None)
+    grads = _lib.DeltaGrads(_lib.strided(do4), _lib.strided(dq), _lib.strided(dk_), _lib.strided(dv_), dbeta.data_ptr(),
+                            None if per_head else _lib.ptr(ddecay), _lib.ptr(ddecay) if per_head else None,
+                            _lib.ptr(given), _lib.ptr(dstate))
+    n = ctypes.c_size_t()
+    _lib.check(lib.ts_delta_bwd_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), "ts_delta_bwd_workspace_bytes")
+    work = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+    with _on(q.device), _lib.timed("ts_delta_bwd", lambda: _lib.nbytes(q4, k4, v4, do4, dq, dk_, dv_, dbeta, ddecay)):
+        status = lib.ts_delta_bwd(ctypes.byref(desc), ctypes.byref(io), ctypes.byref(grads), saved.data_ptr(),
+                                  saved.numel(), work.data_ptr(), work.numel(), _lib.stream_handle(q.device))
+    _lib.check(status, "ts_delta_bwd")
+    none = q.new_empty(0)
+    return [dq[..., :dk], dk_[..., :dk], dv_[..., :dv], dbeta, none if ddecay is None else ddecay,
+            none if dstate is None else dstate[..., :dk, :dv]]
+
+
+def _backward_fake(dout, dfinal, q, k, v, beta, decay, state, lengths, saved, need_state):
+    def rows(x):
+        return _rows_like(x, q.dtype, _width(q.dtype, x.shape[-1]))[..., :x.shape[-1]]
+
+    none = q.new_empty(0)
+    B, H, _, dv = v.shape
+    return [rows(q), rows(k), rows(v), beta.new_empty(beta.shape), none if decay is None else decay.new_empty(decay.shape),
+            q.new_empty(B, H, q.shape[-1], dv, dtype=torch.float32) if need_state else none]
+
+
+def _setup(ctx, inputs, output):
+    q, k, v, beta, decay, state, lengths, want_state, keep, step = inputs
+    ctx.need_state = state is not None and state.requires_grad
+    ctx.want_state = want_state
+    ctx.need_decay = decay is not None and decay.requires_grad
+    ctx.save_for_backward(q, k, v, beta, decay, state, lengths, output[2])
+
+
+def _backward(ctx, grads, bwd):
+    q, k, v, beta, decay, state, lengths, saved = ctx.saved_tensors
+    dout, dfinal = grads[0], grads[1] if ctx.want_state else None
+    if dout is None and dfinal is None:
+        return (None,) * 10
+    dq, dk, dv, dbeta, ddecay, dstate = bwd(dout, dfinal, q, k, v, beta, decay, state, lengths, saved, ctx.need_state)
+    return (dq, dk, dv, dbeta, ddecay if ctx.need_decay else None, dstate if ctx.need_state else None, None, None, None,
+            None)
+
+
+_delta_op = HipOp("gated_delta", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,
+                  backward_fake=_backward_fake, setup=_setup, backward=_backward)
+
+
+def _token_gate(t: torch.Tensor, name: str, B: int, H: int, T: int) -> torch.Tensor:
+    if t.ndim == 4 and t.shape[-1] == 1:
+        t = t.squeeze(-1)
+    if tuple(t.shape) != (B, H, T):
+        raise ValueError(f"gated_delta_rule: {name} must be [B,H,T] or [B,H,T,1] = {(B, H, T)}, got {tuple(t.shape)}")
+    return t
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor,
+                     retention: torch.Tensor | None = None, *, state: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, return_state: bool = False,
+                     state_out: torch.Tensor | None = None):
+    """Outputs [B,H,T,dv] of the gated delta rule (module docstring), and with
+    ``return_state`` the fp32 state [B,H,dk,dv] after the last token.
+
+    ``q``, ``k`` [B,Hk,T,dk] and ``v`` [B,H,T,dv] (bf16 or fp32, any strides; H a
+    multiple of Hk: value head h reads the keys and queries of head h // (H / Hk));
+    ``beta`` [B,H,T] or [B,H,T,1] the write strengths; ``retention`` the log
+    retentions (at most zero, -inf a reset): None, one per value head [H], or one
+    per token [B,H,T] or [B,H,T,1].  Keys are taken as given: the memory is stable
+    where ``beta_t |k_t|^2`` is at most 2.  dk is at most 128, dv at most 512.
+
+    ``state`` continues from the fp32 state of an earlier call (None: zero).
+    ``lengths`` [B] (integers, on the GPU, clamped to [0, T]) makes a padded batch:
+    tokens at or past a sequence's length are not read, give zeros and gradients of
+    zero, and leave its state as it was.  ``state_out`` (without gradients only) is
+    the contiguous fp32 tensor to write the new state into; it may be ``state``.
+
+    Differentiable in q, k, v, beta, the retention and the state.
+    """
+    tensors = (q, k, v, beta)
+    for name, x in zip(("q", "k", "v"), tensors):
+        if x.ndim != 4:
+            raise ValueError(f"gated_delta_rule: {name} must be [B,H,T,D], got {tuple(x.shape)}")
+    B, Hk, T, dk = q.shape
+    H, dv = v.shape[1], v.shape[3]
+    if tuple(k.shape) != (B, Hk, T, dk) or v.shape[0] != B or v.shape[2] != T:
+        raise ValueError(f"gated_delta_rule: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if B < 1 or Hk < 1 or dk < 1 or dv < 1 or H < 1 or H % Hk:
+        raise ValueError(f"gated_delta_rule: {H} value heads over {Hk} key heads, {B} sequences, widths {dk} and {dv}")
+    if dk > MAX_KEYS or dv > MAX_VALUES:
+        raise NotImplementedError(f"gated_delta_rule: at most {MAX_KEYS} keys and {MAX_VALUES} values, got {dk} and {dv}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"gated_delta_rule: q, k and v of one dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
+    beta = _token_gate(beta, "beta", B, H, T)
+    if retention is not None and retention.ndim == 1:
+        if retention.numel() != H:
+            raise ValueError(f"gated_delta_rule: a static retention has one entry per value head ({H}), "
+                             f"got {retention.numel()}")
+    elif retention is not None:
+        if retention.ndim == 4 and retention.shape[-1] != 1:
+            raise NotImplementedError("gated_delta_rule: one retention per token and head (no per-channel decay)")
+        retention = _token_gate(retention, "retention", B, H, T)
+    for x in (q, beta) if retention is None else (q, beta, retention):
+        _lib.dtype_code(x.dtype)
+    for name, s in (("state", state), ("state_out", state_out)):
+        if s is not None and (tuple(s.shape) != (B, H, dk, dv) or s.dtype != torch.float32):
+            raise ValueError(f"gated_delta_rule: {name} must be fp32 {(B, H, dk, dv)}, got {s.dtype} {tuple(s.shape)}")
+    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"gated_delta_rule: lengths must be integers [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
+    everything = [x for x in (*tensors, retention, state, lengths, state_out) if x is not None]
+    if not all(x.is_cuda for x in everything):
+        raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")
+    if any(x.device != q.device for x in everything):
+        raise ValueError("gated_delta_rule: tensors on several devices")
+    if lengths is not None:
+        lengths = lengths.to(torch.int64).contiguous()
+    record = torch.is_grad_enabled() and any(x.requires_grad for x in everything)
+    if state_out is not None:
+        if record or state_out.requires_grad:
+            raise ValueError("gated_delta_rule: state_out takes no part in gradients: call it without them")
+        if not state_out.is_contiguous():
+            raise ValueError("gated_delta_rule: state_out must be contiguous")
+    if T == 0:
+        final = torch.zeros(B, H, dk, dv, dtype=torch.float32, device=q.device) if state is None else state.clone()
+        if state_out is not None:
+            final = state_out.copy_(final)
+        out = v.new_empty(B, H, 0, dv)
+        return (out, final) if return_state else out
+    step = not record and T <= STEP_TOKENS
+    if state_out is not None:
+        with torch.no_grad():
+            out, final, _ = _launch(q, k, v, beta, retention, state, lengths, True, False, step, state_out)
+        return (out, final) if return_state else out
+    out, final, _ = _delta_op(q, k, v, beta, retention, state, lengths, bool(return_state), record, step)
+    return (out, final) if return_state else out

@@ -545,7 +545,22 @@ class RetentionIO(ctypes.Structure):
 FEAT_RELU2 = 0
 FEAT_SOFTMAX = 1
 
-ABI_VERSION = 18  # the include/thetascan_hip.h these bindings are written for
+class DeltaDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "Hk", "H", "T", "dk", "dv", "dtype", "beta_dtype", "decay_dtype",
+                                              "keep")]
+
+
+class DeltaIO(ctypes.Structure):
+    _fields_ = [(n, Strided) for n in ("q", "k", "v", "beta", "decay", "out")] + [
+        (n, ctypes.c_void_p) for n in ("lengths", "state", "state_out")]
+
+
+class DeltaGrads(ctypes.Structure):
+    _fields_ = [(n, Strided) for n in ("dout", "dq", "dk", "dv")] + [
+        (n, ctypes.c_void_p) for n in ("dbeta", "ddecay", "ddecay_head", "dstate_out", "dstate")]
+
+
+ABI_VERSION = 19  # the include/thetascan_hip.h these bindings are written for
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -696,6 +711,12 @@ def load() -> ctypes.CDLL:
         lib.ts_stack_heads.argtypes = [P(StackDesc), P(Strided), ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_rotary_tables.argtypes = [ctypes.c_void_p] + [ctypes.c_int32] * 3 + [ctypes.c_void_p] * 3
         lib.ts_causal_attention_fwd.argtypes = [P(AttentionDesc), Strided, Strided, Strided, Strided, ctypes.c_void_p]
+        lib.ts_delta_workspace_bytes.argtypes = [P(DeltaDesc), P(ctypes.c_size_t)]
+        lib.ts_delta_fwd.argtypes = [P(DeltaDesc), P(DeltaIO), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.ts_delta_step.argtypes = [P(DeltaDesc), P(DeltaIO), ctypes.c_void_p]
+        lib.ts_delta_bwd_workspace_bytes.argtypes = [P(DeltaDesc), P(ctypes.c_size_t)]
+        lib.ts_delta_bwd.argtypes = [P(DeltaDesc), P(DeltaIO), P(DeltaGrads), ctypes.c_void_p, ctypes.c_size_t,
+                                     ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.ts_scale_add_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 6
         lib.ts_scale_add_norm_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 4 + [ctypes.c_float] + [
             ctypes.c_void_p] * 4

@@ -1,0 +1,181 @@
+// Shared parts of the gated delta rule's kernels (gfx950): chunk layout of the
+// workspace and operand helpers.
+//
+// Mathematics (per batch and value head, state S [dk, dv] fp32):
+//   S_t = a_t S_{t-1} + k_t u_t^T,  u_t = b_t (v_t - a_t S_{t-1}^T k_t),  o_t = S_t^T q_t
+// For a chunk of 64 tokens with entering state S0 and G_t = sum_{s<=t} log a_s in it:
+//   L_ti = b_t e^{G_t - G_i} k_t.k_i  (i < t),   Ti = (I + L)^-1
+//   P_ti = e^{G_t - G_i} q_t.k_i      (i <= t)
+//   U = Ti b (V - e^G K S0),   O = e^G Q S0 + P U,   S' = e^{G_63} S0 + K^T (e^{G_63 - G} U)
+// Every exponent is a difference of sums over a range of tokens: at most zero
+// for retentions, and formed in fp64, so a reset (log a = -inf, taken as -1000)
+// costs its neighbours no digits.
+//
+// A token at or past its sequence's length reads as q = k = v = 0, b = 0,
+// log a = 0: it writes nothing, and its row and column of Ti are the identity's.
+#pragma once
+
+#include "ts_common.h"
+#include "ts_tokens.h"
+
+namespace ts {
+
+constexpr int kChunk = 64;
+constexpr double kLog2e = 1.4426950408889634074;
+
+// A lower triangular 64 x 64 matrix as MFMA operands: row block r (16 rows)
+// and contraction step s (32 columns), the six that hold the triangle.  Lane
+// (l16, g) owns row 16r + l16 and columns 32s + 16(j >> 2) + 4g + (j & 3), the
+// order in which accumulators of 16-row blocks 2s, 2s+1 hold their rows.
+constexpr int kTri = 6;
+__device__ __forceinline__ constexpr int tri(int r, int s) { return r < 2 ? r : (r == 2 ? 2 + s : 4 + s); }
+
+// Elements of one fragment set in the workspace.
+constexpr int kTriElems = kTri * 64 * 8;
+
+// The inverse and P are kept as bf16 pairs hi + lo (fp32: once): where keys are
+// alike, sums over the chunk cancel, and what one rounding leaves does not.
+template <typename E> struct TriSets { static constexpr int N = 1; };
+template <> struct TriSets<bf16> { static constexpr int N = 2; };
+
+// Per chunk, in bytes: the inverse, P, and e^G, e^{G_63 - G}, b (fp32 x 64 each).
+constexpr size_t kVecBytes = 3 * kChunk * sizeof(float);
+template <typename E> __host__ __device__ constexpr size_t prep_bytes() {
+  return (size_t)2 * TriSets<E>::N * kTriElems * sizeof(E) + kVecBytes;
+}
+
+struct DeltaP {
+  int B, Hk, H, rep, T, dk, dv, nc;  // nc: chunks of T
+  int dvp;                           // dv rounded up to 16
+  int beta_bf16, decay_bf16;
+  ts_strided q, k, v, beta, decay, out;
+  const int64_t* lengths;  // [B] or null
+  const float* state;      // [B,H,dk,dv] or null (zero)
+  float* state_out;        // or null
+  char* prep;              // [B*H*nc] of prep_bytes
+  void* u;                 // kept: [B*H*nc][dvp][64]
+  void* s0;                // kept: [B*H*nc][dvp][DK]
+  // backward
+  ts_strided dout, dq, dkey, dval;
+  void* dbeta;   // [B,H,T] of beta's dtype
+  void* ddecay;  // [B,H,T], decay's dtype (or fp32), or null
+  int ddecay_bf16, grad_f32;  // grad_f32: dq and dkey are fp32 (value heads that share keys)
+  const float* dstate_out;  // gradient of the final state or null
+  float* dstate;            // gradient of the entering state or null
+  void* dr;                 // [B*H*nc][dvp][64]
+  void* ds;                 // [B*H*nc][dvp][DK]
+};
+
+__device__ __forceinline__ int delta_len(const DeltaP& p, int b) {
+  if (!p.lengths) return p.T;
+  const int64_t n = p.lengths[b];
+  return n < 0 ? 0 : (n > p.T ? p.T : (int)n);
+}
+__device__ __forceinline__ float gate_at(const ts_strided& s, int bf, int64_t i) {
+  return bf ? tof(((const bf16*)s.ptr)[i]) : ((const float*)s.ptr)[i];
+}
+
+template <typename E>
+__device__ __forceinline__ typename Frag<E>::f8 zero8() {
+  typename Frag<E>::f8 z;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = (E)0.0f;
+  return z;
+}
+__device__ __forceinline__ floatx4 zero4() { return floatx4{0.f, 0.f, 0.f, 0.f}; }
+
+// Accumulators of two 16-row blocks as an operand, in one rounding (hi) and
+// what that leaves (lo): hi + lo holds 16 bits and more.  fp32 keeps everything
+// in hi.
+template <typename E> struct Split;
+template <> struct Split<bf16> {
+  bf16x8 hi, lo;
+  __device__ __forceinline__ Split(floatx4 a, floatx4 b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = (bf16)a[i];
+      hi[4 + i] = (bf16)b[i];
+      lo[i] = (bf16)(a[i] - (float)hi[i]);
+      lo[4 + i] = (bf16)(b[i] - (float)hi[4 + i]);
+    }
+  }
+};
+template <> struct Split<float> {
+  floatx8 hi;
+  __device__ __forceinline__ Split(floatx4 a, floatx4 b) { hi = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+};
+// c + x (y.hi + y.lo) and c + (y.hi + y.lo) x
+__device__ __forceinline__ floatx4 mma_split(bf16x8 x, const Split<bf16>& y, floatx4 c) {
+  return mma32(x, y.hi, mma32(x, y.lo, c));
+}
+__device__ __forceinline__ floatx4 mma_split(floatx8 x, const Split<float>& y, floatx4 c) { return mma32(x, y.hi, c); }
+__device__ __forceinline__ floatx4 mma_split(const Split<bf16>& y, bf16x8 x, floatx4 c) {
+  return mma32(y.hi, x, mma32(y.lo, x, c));
+}
+__device__ __forceinline__ floatx4 mma_split(const Split<float>& y, floatx8 x, floatx4 c) { return mma32(y.hi, x, c); }
+
+// Eight columns of an LDS row in accumulator order (32s + 4g.., 32s + 16 + 4g..).
+template <typename E>
+__device__ __forceinline__ typename Frag<E>::f8 row_perm(const E* row, int s, int g) {
+  return LdsIO<E>::cat(LdsIO<E>::ld4(row + 32 * s + 4 * g), LdsIO<E>::ld4(row + 32 * s + 16 + 4 * g));
+}
+
+// Operand of the transposed triangle from its LDS copy: row 16r + l16 of Tr^T,
+// contraction step s (rows of Tr in accumulator order).
+template <typename E> struct TriT;
+template <> struct TriT<bf16> {
+  typedef short shortx4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+  static __device__ __forceinline__ bf16x8 get(const bf16* t, int r, int s, int lane) {
+    const int g = lane >> 4, j = lane & 15;
+    const int at = (j & 3) * 128 + (4 * g + (j >> 2)) * 8 + (r & 1) * 4;
+    shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(t + tri(2 * s + 1, r >> 1) * 512 + at));
+    shortx4 lo = {0, 0, 0, 0};
+    // (row block 2s of step s is past the triangle for the odd block beside it)
+    if (2 * s >= r) lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(t + tri(2 * s, r >> 1) * 512 + at));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+template <> struct TriT<float> {
+  static __device__ __forceinline__ floatx8 get(const float* t, int r, int s, int lane) {
+    const int g = lane >> 4, l16 = lane & 15;
+    floatx8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int rb = 2 * s + (e >> 2);  // row block of Tr
+      const int at = (l16 >> 2) * 128 + (4 * g + (e & 3)) * 8 + (r & 1) * 4 + (l16 & 3);
+      v[e] = rb >= r ? t[tri(rb, r >> 1) * 512 + at] : 0.f;
+    }
+    return v;
+  }
+};
+
+// A [64 x W] token tile on its way from global memory to LDS rows of pitch W +
+// pad: vector idx = tid + i * threads.  Rows at or past `len` and columns at or
+// past `width` (a multiple of a vector) are zero.
+template <typename E, int W, int THREADS>
+struct ChunkTile {
+  static constexpr int VEC = 16 / (int)sizeof(E);
+  static constexpr int PER = W / VEC;
+  static constexpr int SLOTS = kChunk * PER / THREADS;
+  uint4 r[SLOTS];
+  __device__ __forceinline__ void fetch(const E* base, int64_t st, int t0, int len, int width, int tid) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int idx = tid + i * THREADS, row = idx / PER, c = (idx % PER) * VEC;
+      r[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (t0 + row < len && c < width) r[i] = *(const uint4*)(base + (int64_t)(t0 + row) * st + c);
+    }
+  }
+  __device__ __forceinline__ void store(E* dst, int pitch, int tid) const {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int idx = tid + i * THREADS;
+      *(uint4*)(dst + (idx / PER) * pitch + (idx % PER) * VEC) = r[i];
+    }
+  }
+};
+
+int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const char* what);
+
+}  // namespace ts

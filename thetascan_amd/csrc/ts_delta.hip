@@ -1,0 +1,500 @@
+// Gated delta rule over whole sequences, forward (gfx950); the mathematics is in
+// ts_delta.h.
+//
+// delta_prepare: one wave a chunk, nothing shared between chunks.  K K^T and
+// Q K^T on MFMA straight from global rows, the decay between every pair, and the
+// inverse of the unit lower triangular I + L: the four 16 x 16 diagonal blocks by
+// substitution (a lane per row), the six below them by fp32 MFMA,
+// Ti_ij = -Ti_ii sum_k L_ik Ti_kj.
+//
+// delta_forward: the chain over the chunks.  A column of the state needs no
+// other column, so a wave owns 16 value columns of one head for the whole
+// sequence, its state in accumulators, and an accumulator is the next product's
+// operand without leaving the registers (rows of the accumulator are the
+// contraction).  Every operand that is not an input is a bf16 pair hi + lo: the
+// state is the long sum here and keeps about 1e-5 over any length, and an output
+// is rounded once.
+
+#include "ts_delta.h"
+
+#include <string.h>
+
+namespace ts {
+
+template <typename E>
+__device__ __forceinline__ typename Frag<E>::f8 global8(const E* row, int c, int width, bool on) {
+  constexpr int VEC = 16 / (int)sizeof(E);
+  uint4 raw[8 / VEC];
+#pragma unroll
+  for (int i = 0; i < 8 / VEC; ++i) {
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (on && c + i * VEC < width) raw[i] = *(const uint4*)(row + c + i * VEC);
+  }
+  return __builtin_bit_cast(typename Frag<E>::f8, raw);
+}
+
+constexpr int kDiagPitch = 20;
+
+// One fragment of a triangular matrix into its sets, and one read back.
+__device__ __forceinline__ void put_tri(bf16* m, int r, int s, int lane, const Split<bf16>& f) {
+  bf16* at = m + (tri(r, s) * 64 + lane) * 8;
+  *(bf16x8*)at = f.hi;
+  *(bf16x8*)(at + kTriElems) = f.lo;
+}
+__device__ __forceinline__ void put_tri(float* m, int r, int s, int lane, const Split<float>& f) {
+  *(floatx8*)(m + (tri(r, s) * 64 + lane) * 8) = f.hi;
+}
+// c + m x of a pair each: what the two remainders make together (2^-16) is left out.
+__device__ __forceinline__ floatx4 mma_tri(const bf16* m, int r, int s, int lane, const Split<bf16>& x, floatx4 c) {
+  const bf16* at = m + (tri(r, s) * 64 + lane) * 8;
+  const bf16x8 hi = *(const bf16x8*)at, lo = *(const bf16x8*)(at + kTriElems);
+  return mma32(hi, x.hi, mma32(hi, x.lo, mma32(lo, x.hi, c)));
+}
+__device__ __forceinline__ floatx4 mma_tri(const float* m, int r, int s, int lane, const Split<float>& x, floatx4 c) {
+  return mma32(*(const floatx8*)(m + (tri(r, s) * 64 + lane) * 8), x.hi, c);
+}
+// The same with the sides exchanged (the transposed result).
+__device__ __forceinline__ floatx4 mma_tri_t(const bf16* m, int r, int s, int lane, const Split<bf16>& x, floatx4 c) {
+  const bf16* at = m + (tri(r, s) * 64 + lane) * 8;
+  const bf16x8 hi = *(const bf16x8*)at, lo = *(const bf16x8*)(at + kTriElems);
+  return mma32(x.hi, hi, mma32(x.lo, hi, mma32(x.hi, lo, c)));
+}
+__device__ __forceinline__ floatx4 mma_tri_t(const float* m, int r, int s, int lane, const Split<float>& x, floatx4 c) {
+  return mma32(x.hi, *(const floatx8*)(m + (tri(r, s) * 64 + lane) * 8), c);
+}
+
+template <typename E, int DK>
+__global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
+  typedef LdsIO<E> IO;
+  __shared__ __align__(16) double gs[4][kChunk];
+  __shared__ __align__(16) float diag[4][4 * 16 * kDiagPitch];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+  const int64_t n = (int64_t)blockIdx.x * 4 + wv;
+  if (n >= (int64_t)p.B * p.H * p.nc) return;
+  const int c = (int)(n % p.nc), bh = (int)(n / p.nc), b = bh / p.H, h = bh % p.H;
+  const int t0 = c * kChunk, len = delta_len(p, b);
+  if (t0 >= len) return;
+  double* G = gs[wv];
+  float* dg = diag[wv];
+
+  // log decays, their running sum, and the vectors the chain reads
+  const bool seen = t0 + lane < len;
+  double sum = 0.0;
+  float beta = 0.f;
+  if (seen) {
+    beta = gate_at(p.beta, p.beta_bf16, b * p.beta.sb + h * p.beta.sh + (int64_t)(t0 + lane) * p.beta.st);
+    if (p.decay.ptr) {
+      const float la =
+          gate_at(p.decay, p.decay_bf16, b * p.decay.sb + h * p.decay.sh + (int64_t)(t0 + lane) * p.decay.st);
+      sum = la < -1000.f ? -1000.0 : (double)la;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double below = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += below;
+  }
+  G[lane] = sum;
+  char* prep = p.prep + n * (int64_t)prep_bytes<E>();
+  E* tri_t = (E*)prep;
+  E* tri_p = tri_t + TriSets<E>::N * kTriElems;
+  float* vec = (float*)(tri_p + TriSets<E>::N * kTriElems);
+  vec[lane] = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
+  vec[kChunk + lane] = __builtin_amdgcn_exp2f((float)((__shfl(sum, 63, 64) - sum) * kLog2e));
+  vec[2 * kChunk + lane] = beta;
+  wave_lds_sync();
+
+  // K K^T and Q K^T, the lower blocks: column t = l16 of block rt, rows i = 4g.. of block ri
+  const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
+  const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
+  floatx4 kk[10], qk[10];
+#pragma unroll
+  for (int i = 0; i < 10; ++i) kk[i] = qk[i] = zero4();
+#pragma unroll
+  for (int s = 0; s < DK / 32; ++s) {
+    typename Frag<E>::f8 kf[4], qf[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = t0 + 16 * r + l16;
+      kf[r] = global8<E>(kb + (int64_t)t * p.k.st, 32 * s + 8 * g, p.dk, t < len);
+      qf[r] = global8<E>(qb + (int64_t)t * p.q.st, 32 * s + 8 * g, p.dk, t < len);
+    }
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+      for (int ri = 0; ri <= rt; ++ri) {
+        const int at = rt * (rt + 1) / 2 + ri;
+        kk[at] = mma32(kf[ri], kf[rt], kk[at]);
+        qk[at] = mma32(kf[ri], qf[rt], qk[at]);
+      }
+  }
+  // times the decay between the pair, masked: P, and L in kk
+  const floatx4 z4 = zero4();
+#pragma unroll
+  for (int rt = 0; rt < 4; ++rt) {
+    const double gt = G[16 * rt + l16];
+    const float bt = __shfl(beta, 16 * rt + l16, 64);
+#pragma unroll
+    for (int ri = 0; ri <= rt; ++ri) {
+      const int at = rt * (rt + 1) / 2 + ri;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 16 * ri + 4 * g + j, t = 16 * rt + l16;
+        const float d = __builtin_amdgcn_exp2f((float)((gt - G[i]) * kLog2e));
+        qk[at][j] = i <= t ? qk[at][j] * d : 0.f;
+        kk[at][j] = i < t ? kk[at][j] * d * bt : 0.f;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s <= rt / 2; ++s) {
+      const int at = rt * (rt + 1) / 2 + 2 * s;
+      put_tri(tri_p, rt, s, lane, Split<E>(qk[at], 2 * s + 1 <= rt ? qk[2 * s + 1 <= rt ? at + 1 : at] : z4));
+    }
+  }
+  // diagonal blocks: block g, row l16 of it per lane.  L_gg^T in LDS, [column][row]
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dg[(16 * r + 4 * g + j) * kDiagPitch + l16] = kk[r * (r + 1) / 2 + r][j];
+  wave_lds_sync();
+  float x[16];
+#pragma unroll
+  for (int col = 15; col >= 0; --col) {
+    float lrow[16];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const floatx4 w = *(const floatx4*)(dg + (16 * g + col) * kDiagPitch + 4 * v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) lrow[4 * v + j] = w[j];
+    }
+    float acc = col == l16 ? 1.f : 0.f;
+#pragma unroll
+    for (int s = 15; s > col; --s) acc = fmaf(-x[s], lrow[s], acc);
+    x[col] = acc;
+  }
+  wave_lds_sync();
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+    *(floatx4*)(dg + (16 * g + l16) * kDiagPitch + 4 * v) = floatx4{x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]};
+  wave_lds_sync();
+  // ac[..]: rows in registers (the next contraction), tr[..]: columns in
+  // registers (lane l16 a row), the form of the stored operands
+  floatx4 ac[6], tr[10];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) tr[r * (r + 1) / 2 + r] = *(const floatx4*)(dg + (16 * r + l16) * kDiagPitch + 4 * g);
+#pragma unroll
+  for (int r = 0; r < 3; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ac[r * (r + 1) / 2 + r][j] = dg[(16 * r + 4 * g + j) * kDiagPitch + l16];
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+#pragma unroll
+    for (int j = i - 1; j >= 0; --j) {
+      floatx4 y = z4;
+#pragma unroll
+      for (int k = j; k < i; ++k) y = mma16(kk[i * (i + 1) / 2 + k], ac[k * (k + 1) / 2 + j], y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = -y[e];
+      const floatx4 ti = tr[i * (i + 1) / 2 + i];
+      tr[i * (i + 1) / 2 + j] = mma16(y, ti, z4);
+      if (i < 3) ac[i * (i + 1) / 2 + j] = mma16(ti, y, z4);
+    }
+#pragma unroll
+  for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+    for (int s = 0; s <= rt / 2; ++s) {
+      const int at = rt * (rt + 1) / 2 + 2 * s;
+      put_tri(tri_t, rt, s, lane, Split<E>(tr[at], 2 * s + 1 <= rt ? tr[2 * s + 1 <= rt ? at + 1 : at] : z4));
+    }
+}
+
+template <typename E, int DK, int NW>
+struct ForwardLds {
+  static constexpr int PITCH = DK + 16 / (int)sizeof(E);
+  E k[2][kChunk * PITCH];
+  E q[2][kChunk * PITCH];
+};
+
+template <typename E, int DK, int NW, bool KEEP>
+__global__ __launch_bounds__(64 * NW) void delta_forward_kernel(DeltaP p) {
+  typedef LdsIO<E> IO;
+  typedef ForwardLds<E, DK, NW> Lds;
+  constexpr int PITCH = Lds::PITCH, KB = DK / 16, KS = DK / 32;
+  extern __shared__ __align__(16) char smem[];
+  Lds& lds = *(Lds*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
+  const int col0 = ((int)blockIdx.y * NW + w) * 16, col = col0 + l16;
+  const bool mine = col0 < p.dvp, on = col < p.dv;  // (a wave past the columns only helps staging)
+  const int len = delta_len(p, b), chunks = (len + kChunk - 1) / kChunk;
+  const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
+  const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
+  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh + col;
+  E* ob = (E*)p.out.ptr + b * p.out.sb + h * p.out.sh + col0 + 4 * g;
+  const bool out_on = col0 + 4 * g < p.dv;
+
+  floatx4 S[KB];
+#pragma unroll
+  for (int d = 0; d < KB; ++d) {
+    S[d] = zero4();
+    if (p.state && on) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * d + 4 * g + i;
+        if (row < p.dk) S[d][i] = p.state[((int64_t)bh * p.dk + row) * p.dv + col];
+      }
+    }
+  }
+  ChunkTile<E, DK, 64 * NW> kt, qt;
+  E vr[16];
+  auto fetch = [&](int c) {
+    const int t0 = c * kChunk;
+    kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
+    qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 16 * r + 4 * g + i;
+        vr[4 * r + i] = (E)0.0f;
+        if (on && t < len) vr[4 * r + i] = vb[(int64_t)t * p.v.st];
+      }
+  };
+  if (chunks) fetch(0);
+  for (int c = 0; c < chunks; ++c) {
+    const int buf = c & 1, t0 = c * kChunk;
+    kt.store(lds.k[buf], PITCH, tid);
+    qt.store(lds.q[buf], PITCH, tid);
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = tof(vr[i]);
+    if (c + 1 < chunks) fetch(c + 1);
+    // this chunk is staged; the other buffer was last read before this barrier
+    __syncthreads();
+    if (!mine) continue;
+    const E* ks = lds.k[buf];
+    const E* qs = lds.q[buf];
+    const int64_t n = (int64_t)bh * p.nc + c;
+    const char* prep = p.prep + n * (int64_t)prep_bytes<E>();
+    const E* tri_t = (const E*)prep;
+    const E* tri_p = tri_t + TriSets<E>::N * kTriElems;
+    const float* vec = (const float*)(tri_p + TriSets<E>::N * kTriElems);
+
+    if constexpr (KEEP) {
+      E* s0 = (E*)p.s0 + (n * p.dvp + col) * DK + 4 * g;
+#pragma unroll
+      for (int d = 0; d < KB; ++d) IO::st4(s0 + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
+    }
+    // R = b (V - e^G K S0)
+    floatx4 R[4];
+    {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) R[r] = zero4();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const Split<E> sf(S[2 * s], S[2 * s + 1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) R[r] = mma_split(row_perm<E>(ks + (16 * r + l16) * PITCH, s, g), sf, R[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const floatx4 eg = *(const floatx4*)(vec + 16 * r + 4 * g);
+      const floatx4 be = *(const floatx4*)(vec + 2 * kChunk + 16 * r + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) R[r][i] = be[i] * fmaf(-eg[i], R[r][i], v[4 * r + i]);
+    }
+    // U = Ti R
+    floatx4 U[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) U[r] = zero4();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Split<E> rf(R[2 * s], R[2 * s + 1]);
+#pragma unroll
+      for (int r = 2 * s; r < 4; ++r) U[r] = mma_tri(tri_t, r, s, lane, rf, U[r]);
+    }
+    if constexpr (KEEP) {
+      E* u = (E*)p.u + (n * p.dvp + col) * kChunk + 4 * g;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) IO::st4(u + 16 * r, U[r][0], U[r][1], U[r][2], U[r][3]);
+    }
+    // O^T = S0^T Q^T e^G + U^T P^T: lane l16 a token, four columns
+    {
+      floatx4 O[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) O[r] = zero4();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const Split<E> sf(S[2 * s], S[2 * s + 1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) O[r] = mma_split(sf, row_perm<E>(qs + (16 * r + l16) * PITCH, s, g), O[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float eg = vec[16 * r + l16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[r][i] *= eg;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const Split<E> uf(U[2 * s], U[2 * s + 1]);
+#pragma unroll
+        for (int r = 2 * s; r < 4; ++r) O[r] = mma_tri_t(tri_p, r, s, lane, uf, O[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = t0 + 16 * r + l16;
+        const bool in = t < len;
+        if (t < p.T && out_on)
+          IO::st4(ob + (int64_t)t * p.out.st, in ? O[r][0] : 0.f, in ? O[r][1] : 0.f, in ? O[r][2] : 0.f,
+                  in ? O[r][3] : 0.f);
+      }
+    }
+    // S = e^{G_63} S0 + K^T (e^{G_63 - G} U)
+    const float whole = vec[kChunk - 1];
+#pragma unroll
+    for (int d = 0; d < KB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[d][i] *= whole;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const floatx4 tail = *(const floatx4*)(vec + kChunk + 16 * r + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) U[r][i] *= tail[i];
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Split<E> uf(U[2 * s], U[2 * s + 1]);
+#pragma unroll
+      for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(ks, PITCH, 16 * d, s, lane), uf, S[d]);
+    }
+  }
+  if (!mine) return;
+  // tokens behind the length, chunk by chunk (those of its own chunk are written above)
+  for (int t = chunks * kChunk + l16; t < p.T; t += 16)
+    if (out_on) IO::st4(ob + (int64_t)t * p.out.st, 0.f, 0.f, 0.f, 0.f);
+  if (p.state_out && on) {
+#pragma unroll
+    for (int d = 0; d < KB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * d + 4 * g + i;
+        if (row < p.dk) p.state_out[((int64_t)bh * p.dk + row) * p.dv + col] = S[d][i];
+      }
+  }
+}
+
+int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const char* what) {
+  if (!d || d->B < 1 || d->Hk < 1 || d->H < 1 || d->H % d->Hk || d->T < 0 || d->dk < 1 || d->dv < 1)
+    return fail(TS_ERR_VALUE, "%s: bad shape", what);
+  if (d->dtype != TS_BF16 && d->dtype != TS_F32) return fail(TS_ERR_NOT_IMPLEMENTED, "%s: bf16 or fp32 only", what);
+  const int vec = d->dtype == TS_BF16 ? 8 : 4;
+  if (d->dk > 128 || d->dv > 512)
+    return fail(TS_ERR_NOT_IMPLEMENTED, "%s: at most 128 keys and 512 values, got %d and %d", what, d->dk, d->dv);
+  if (d->dk % vec || d->dv % vec) return fail(TS_ERR_VALUE, "%s: widths must be multiples of 16 bytes", what);
+  if ((int64_t)d->B * d->H > 0x7fffffff || d->T > 0x7fffffff - 64)
+    return fail(TS_ERR_NOT_IMPLEMENTED, "%s: too many heads or tokens", what);
+  if (!p) return TS_OK;
+  memset(p, 0, sizeof(*p));
+  p->B = d->B; p->Hk = d->Hk; p->H = d->H; p->rep = d->H / d->Hk; p->T = d->T; p->dk = d->dk; p->dv = d->dv;
+  p->nc = (d->T + kChunk - 1) / kChunk;
+  p->dvp = (d->dv + 15) / 16 * 16;
+  p->beta_bf16 = d->beta_dtype == TS_BF16;
+  p->decay_bf16 = d->decay_dtype == TS_BF16;
+  if (!io) return TS_OK;
+  auto rows = [&](const ts_strided& s) {
+    return s.ptr && ((uintptr_t)s.ptr & 15u) == 0 && s.sb % vec == 0 && s.sh % vec == 0 && s.st % vec == 0;
+  };
+  if (!rows(io->q) || !rows(io->k) || !rows(io->v) || !rows(io->out))
+    return fail(TS_ERR_VALUE, "%s: q, k, v and out need 16-byte aligned rows", what);
+  if (!io->beta.ptr) return fail(TS_ERR_VALUE, "%s: missing beta", what);
+  p->q = io->q; p->k = io->k; p->v = io->v; p->out = io->out; p->beta = io->beta; p->decay = io->decay;
+  p->lengths = io->lengths; p->state = io->state; p->state_out = io->state_out;
+  return TS_OK;
+}
+
+}  // namespace ts
+
+namespace {
+
+using ts::DeltaP;
+using ts::fail;
+
+int padded_keys(int dk) { return dk <= 64 ? 64 : 128; }
+
+struct Sizes {
+  size_t prep, u, s0;  // bytes of each part; u and s0 only where kept
+};
+Sizes sizes(const ts_delta_desc* d) {
+  const size_t es = d->dtype == TS_BF16 ? 2 : 4;
+  const size_t n = (size_t)d->B * d->H * ((d->T + 63) / 64), dvp = (d->dv + 15) / 16 * 16;
+  Sizes s;
+  s.prep = n * (d->dtype == TS_BF16 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>());
+  s.u = n * dvp * 64 * es;
+  s.s0 = n * dvp * padded_keys(d->dk) * es;
+  return s;
+}
+
+template <typename E, int DK, int NW>
+int launch_forward(const DeltaP& p, hipStream_t stream) {
+  const dim3 grid((unsigned)(p.B * p.H), (unsigned)((p.dvp / 16 + NW - 1) / NW)), block(64 * NW);
+  const int lds = (int)sizeof(ts::ForwardLds<E, DK, NW>);
+  const void* fn = p.u ? (const void*)ts::delta_forward_kernel<E, DK, NW, true>
+                       : (const void*)ts::delta_forward_kernel<E, DK, NW, false>;
+  if (ts::ensure_lds_limit(fn, lds) != hipSuccess) return fail(TS_ERR_RUNTIME, "delta: LDS of %d bytes", lds);
+  if (p.u)
+    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, NW, true>), grid, block, lds, stream, p);
+  else
+    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, NW, false>), grid, block, lds, stream, p);
+  return TS_OK;
+}
+
+template <typename E, int DK>
+int forward(const DeltaP& p, hipStream_t stream) {
+  const int64_t n = (int64_t)p.B * p.H * p.nc;
+  hipLaunchKernelGGL((ts::delta_prepare_kernel<E, DK>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, p);
+  return launch_forward<E, DK, 1>(p, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ts_delta_workspace_bytes(const ts_delta_desc* d, size_t* bytes) {
+  const int rc = ts::delta_check(d, nullptr, nullptr, "delta");
+  if (rc) return rc;
+  const Sizes s = sizes(d);
+  if (bytes) *bytes = s.prep + (d->keep ? s.u + s.s0 : 0);
+  return TS_OK;
+}
+
+int ts_delta_fwd(const ts_delta_desc* d, const ts_delta_io* io, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream) {
+  DeltaP p;
+  if (!io) return fail(TS_ERR_VALUE, "delta: missing tensors");
+  const int rc = ts::delta_check(d, io, &p, "delta");
+  if (rc) return rc;
+  if (d->T == 0) return TS_OK;
+  const Sizes s = sizes(d);
+  if (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < s.prep + (d->keep ? s.u + s.s0 : 0))
+    return fail(TS_ERR_VALUE, "delta: the workspace is missing, misaligned or too small");
+  if (((int64_t)p.B * p.H * p.nc + 3) / 4 > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta: grid too large");
+  p.prep = (char*)workspace;
+  if (d->keep) {
+    p.u = p.prep + s.prep;
+    p.s0 = p.prep + s.prep + s.u;
+  }
+  const bool narrow = d->dk <= 64;
+  int rc2;
+  if (d->dtype == TS_BF16)
+    rc2 = narrow ? forward<ts::bf16, 64>(p, stream) : forward<ts::bf16, 128>(p, stream);
+  else
+    rc2 = narrow ? forward<float, 64>(p, stream) : forward<float, 128>(p, stream);
+  if (rc2) return rc2;
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(TS_ERR_RUNTIME, "delta: launch failed: %s", hipGetErrorString(e));
+  return TS_OK;
+}
+
+}  // extern "C"

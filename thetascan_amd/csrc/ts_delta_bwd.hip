@@ -1,0 +1,655 @@
+// Gated delta rule, backward (gfx950); notation of ts_delta.h, X' the gradient
+// of X, dS the gradient of the state behind a chunk.
+//
+//   dU = P^T dO + e^{G_63 - G} K dS,   dR = Ti^T dU,   dV = b dR
+//   dS0 = e^{G_63} dS + Q^T (e^G dO) - K^T (b e^G dR)
+//   A = e^{G_t - G_i} (dO U^T)_ti (i <= t),   M = -b e^{G_t - G_i} (dR U^T)_ti (i < t)
+//   dQ = A K + e^G dO S0^T
+//   dK = A^T Q + (M + M^T) K + e^{G_63 - G} U dS^T - b e^G dR S0^T
+//   db_t = dR_t.U_t / b_t,   or dR_t.(v_t - e^{G_t} S0^T k_t - sum_i e^{G_t - G_i} k_t.k_i U_i) where b_t = 0
+//   dG_t = sum_i X_ti - sum_i X_it + e^{G_t} q_t.(S0 dO_t) - b e^{G_t} k_t.(S0 dR_t) - f_t,
+//     X = A (Q K^T) + M (K K^T) elementwise,  f_t = e^{G_63 - G_t} k_t.(dS U_t)
+//   dG_63 += sum_t f_t + e^{G_63} <S0, dS>;   dlog a_t = sum_{s >= t} dG_s
+//
+// delta_chain walks the chunks backwards, a wave per 16 value columns as in the
+// forward; it leaves dR and dS per chunk and writes dV.  delta_grads takes the
+// chunks on their own: one workgroup each, a wave per 16 tokens.
+
+#include "ts_delta.h"
+
+#include <string.h>
+
+namespace ts {
+
+template <typename E, int DK>
+struct ChainLds {
+  static constexpr int PITCH = DK + 16 / (int)sizeof(E);
+  E k[kChunk * PITCH];
+  E q[kChunk * PITCH];
+  E t[kTriElems];
+  E p[kTriElems];
+};
+
+template <typename E, int DK, int NW>
+__global__ __launch_bounds__(64 * NW) void delta_chain_kernel(DeltaP p) {
+  typedef LdsIO<E> IO;
+  typedef typename Frag<E>::f8 f8;
+  typedef ChainLds<E, DK> Lds;
+  constexpr int PITCH = Lds::PITCH, KB = DK / 16, KS = DK / 32, THREADS = 64 * NW;
+  constexpr int TRI_VECS = kTriElems * (int)sizeof(E) / 16, TRI_SLOTS = (TRI_VECS + THREADS - 1) / THREADS;
+  extern __shared__ __align__(16) char smem[];
+  Lds& lds = *(Lds*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
+  const int col0 = ((int)blockIdx.y * NW + w) * 16, col = col0 + l16;
+  const bool mine = col0 < p.dvp, on = col < p.dv;
+  const int len = delta_len(p, b), chunks = (len + kChunk - 1) / kChunk;
+  const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
+  const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
+  const E* db = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh + col;
+  E* vb = (E*)p.dval.ptr + b * p.dval.sb + h * p.dval.sh + col;
+
+  floatx4 S[KB];  // dS
+#pragma unroll
+  for (int d = 0; d < KB; ++d) {
+    S[d] = zero4();
+    if (p.dstate_out && on) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * d + 4 * g + i;
+        if (row < p.dk) S[d][i] = p.dstate_out[((int64_t)bh * p.dk + row) * p.dv + col];
+      }
+    }
+  }
+  ChunkTile<E, DK, THREADS> kt, qt;
+  uint4 tt[TRI_SLOTS], tp[TRI_SLOTS];
+  E dr[16];  // this wave's columns of dO, rows in accumulator order
+  auto prep_of = [&](int c) { return (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>()); };
+  auto fetch = [&](int c) {
+    const int t0 = c * kChunk;
+    kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
+    qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
+    const uint4* mt = (const uint4*)prep_of(c);
+    const uint4* mp = (const uint4*)(prep_of(c) + TriSets<E>::N * kTriElems);
+#pragma unroll
+    for (int i = 0; i < TRI_SLOTS; ++i) {
+      const int idx = min(tid + i * THREADS, TRI_VECS - 1);
+      tt[i] = mt[idx];
+      tp[i] = mp[idx];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 16 * r + 4 * g + i;
+        dr[4 * r + i] = (E)0.0f;
+        if (on && t < len) dr[4 * r + i] = db[(int64_t)t * p.dout.st];
+      }
+  };
+  if (chunks) fetch(chunks - 1);
+  for (int c = chunks - 1; c >= 0; --c) {
+    const int t0 = c * kChunk;
+    const int64_t n = (int64_t)bh * p.nc + c;
+    const float* vec = (const float*)(prep_of(c) + 2 * TriSets<E>::N * kTriElems);
+    // the last chunk's operands have been read
+    __syncthreads();
+    kt.store(lds.k, PITCH, tid);
+    qt.store(lds.q, PITCH, tid);
+#pragma unroll
+    for (int i = 0; i < TRI_SLOTS; ++i) {
+      const int idx = tid + i * THREADS;
+      if (idx < TRI_VECS) {
+        ((uint4*)lds.t)[idx] = tt[i];
+        ((uint4*)lds.p)[idx] = tp[i];
+      }
+    }
+    f8 of[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) of[s][j] = dr[8 * s + j];
+    if (c) fetch(c - 1);
+    __syncthreads();
+    if (!mine) continue;
+
+    E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 4 * g;
+#pragma unroll
+    for (int d = 0; d < KB; ++d) IO::st4(ds + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
+    // dU = P^T dO + e^{G_63 - G} K dS
+    floatx4 X[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) X[r] = zero4();
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const Split<E> sf(S[2 * s], S[2 * s + 1]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) X[r] = mma_split(row_perm<E>(lds.k + (16 * r + l16) * PITCH, s, g), sf, X[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const floatx4 tail = *(const floatx4*)(vec + kChunk + 16 * r + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) X[r][i] *= tail[i];
+#pragma unroll
+      for (int s = r / 2; s < 2; ++s) X[r] = mma32(TriT<E>::get(lds.p, r, s, lane), of[s], X[r]);
+    }
+    // dR = Ti^T dU
+    floatx4 R[4];
+    {
+      const Split<E> u0(X[0], X[1]), u1(X[2], X[3]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        R[r] = mma_split(TriT<E>::get(lds.t, r, 1, lane), u1, zero4());
+        if (r < 2) R[r] = mma_split(TriT<E>::get(lds.t, r, 0, lane), u0, R[r]);
+      }
+    }
+    E* dro = (E*)p.dr + (n * p.dvp + col) * kChunk + 4 * g;
+    const float whole = vec[kChunk - 1];
+    float od[16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      IO::st4(dro + 16 * r, R[r][0], R[r][1], R[r][2], R[r][3]);
+      const floatx4 eg = *(const floatx4*)(vec + 16 * r + 4 * g);
+      const floatx4 be = *(const floatx4*)(vec + 2 * kChunk + 16 * r + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 16 * r + 4 * g + i;
+        const float dv = be[i] * R[r][i];
+        if (t < p.T && on) vb[(int64_t)t * p.dval.st] = cvt<E>(t < len ? dv : 0.f);
+        R[r][i] = -eg[i] * dv;
+        od[4 * r + i] = eg[i] * tof(of[r / 2][4 * (r & 1) + i]);
+      }
+    }
+    // dS0
+#pragma unroll
+    for (int d = 0; d < KB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[d][i] *= whole;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Split<E> rf(R[2 * s], R[2 * s + 1]);
+      const Split<E> qf(floatx4{od[8 * s], od[8 * s + 1], od[8 * s + 2], od[8 * s + 3]},
+                        floatx4{od[8 * s + 4], od[8 * s + 5], od[8 * s + 6], od[8 * s + 7]});
+#pragma unroll
+      for (int d = 0; d < KB; ++d) {
+        S[d] = mma_split(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, S[d]);
+        S[d] = mma_split(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
+      }
+    }
+  }
+  if (!mine) return;
+  if (on)
+    for (int t = chunks * kChunk + g; t < p.T; t += 4) vb[(int64_t)t * p.dval.st] = (E)0.0f;
+  if (p.dstate && on) {
+#pragma unroll
+    for (int d = 0; d < KB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * d + 4 * g + i;
+        if (row < p.dk) p.dstate[((int64_t)bh * p.dk + row) * p.dv + col] = S[d][i];
+      }
+  }
+}
+
+// Value columns of a pass of delta_grads.
+template <typename E> constexpr int kGradCols = sizeof(E) == 2 ? 64 : 32;
+
+template <typename E, int DK>
+struct GradsLds {
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VB = kGradCols<E>, VP = VB + PAD, TP = kChunk + PAD;
+  struct Pass {
+    E dout[kChunk * VP], u[VB * TP], dr[VB * TP], s0[VB * PITCH], ds[VB * PITCH];
+  };
+  struct Pairs {
+    E a[kChunk * TP], m[kChunk * TP];
+  };
+  E k[kChunk * PITCH], q[kChunk * PITCH];
+  union {
+    Pass pass;
+    Pairs pairs;
+  };
+  double G[kChunk];
+  float cols[4][kChunk], base[kChunk], f[kChunk], red[4];
+};
+
+// [rows x W] contiguous rows -> LDS; rows at or past `rows` are zero.
+template <typename E, int ROWS, int W>
+__device__ __forceinline__ void stage_rows(const E* src, int rows, E* dst, int pitch, int tid) {
+  constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC;
+#pragma unroll
+  for (int i = 0; i < ROWS * PER / 256; ++i) {
+    const int idx = tid + i * 256, row = idx / PER, c = (idx % PER) * VEC;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) v = *(const uint4*)(src + row * W + c);
+    *(uint4*)(dst + row * pitch + c) = v;
+  }
+}
+
+template <typename E, int DK>
+__global__ __launch_bounds__(256) void delta_grads_kernel(DeltaP p) {
+  typedef LdsIO<E> IO;
+  typedef TokFrag<E> TF;
+  typedef typename Frag<E>::f8 f8;
+  typedef GradsLds<E, DK> Lds;
+  constexpr int PITCH = Lds::PITCH, VB = Lds::VB, VP = Lds::VP, TP = Lds::TP, KB = DK / 16, KS = DK / 32;
+  extern __shared__ __align__(16) char smem[];
+  Lds& lds = *(Lds*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t n = blockIdx.x;
+  const int c = (int)(n % p.nc), bh = (int)(n / p.nc), b = bh / p.H, h = bh % p.H;
+  const int t0 = c * kChunk, len = delta_len(p, b);
+  const int64_t gate0 = (int64_t)bh * p.T + t0;
+  const int t = 16 * w + l16;  // this lane's token of the chunk
+  auto put_gate = [&](void* dst, int bf, int64_t i, float v) {
+    if (bf)
+      ((bf16*)dst)[i] = (bf16)v;
+    else
+      ((float*)dst)[i] = v;
+  };
+  // gradient rows of a token: columns 16d + 4g ..
+  auto put_row = [&](const ts_strided& s, int d, const floatx4& v) {
+    if (t0 + t >= p.T || 16 * d + 4 * g >= p.dk) return;
+    const int64_t at = b * s.sb + h * s.sh + (int64_t)(t0 + t) * s.st + 16 * d + 4 * g;
+    if (p.grad_f32)
+      *(floatx4*)((float*)s.ptr + at) = v;
+    else
+      IO::st4((E*)s.ptr + at, v[0], v[1], v[2], v[3]);
+  };
+  if (t0 >= len) {  // a chunk behind the sequence
+#pragma unroll
+    for (int d = 0; d < KB; ++d) {
+      put_row(p.dq, d, zero4());
+      put_row(p.dkey, d, zero4());
+    }
+    if (tid < kChunk && t0 + tid < p.T) {
+      put_gate(p.dbeta, p.beta_bf16, gate0 + tid, 0.f);
+      if (p.ddecay) put_gate(p.ddecay, p.ddecay_bf16, gate0 + tid, 0.f);
+    }
+    return;
+  }
+  const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
+  const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
+  {
+    ChunkTile<E, DK, 256> kt, qt;
+    kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
+    qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
+    kt.store(lds.k, PITCH, tid);
+    qt.store(lds.q, PITCH, tid);
+  }
+  const float* vec =
+      (const float*)((const E*)(p.prep + n * (int64_t)prep_bytes<E>()) + 2 * TriSets<E>::N * kTriElems);
+  const float eg = vec[t], tail = vec[kChunk + t], be = vec[2 * kChunk + t], whole = vec[kChunk - 1];
+  if (w == 0) {
+    double sum = 0.0;
+    if (p.decay.ptr && t0 + lane < len) {
+      const float la =
+          gate_at(p.decay, p.decay_bf16, b * p.decay.sb + h * p.decay.sh + (int64_t)(t0 + lane) * p.decay.st);
+      sum = la < -1000.f ? -1000.0 : (double)la;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double below = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += below;
+    }
+    lds.G[lane] = sum;
+  }
+  // where a token's b is zero, db takes its values' rows too
+  const bool zero_b = t0 + t < len && fabsf(be) < 1e-30f;
+  const bool any_zero = __any(zero_b);
+
+  floatx4 dp[4], ru[4], z[KB], y[KB], fu[KB], rv = zero4();
+#pragma unroll
+  for (int r = 0; r < 4; ++r) dp[r] = ru[r] = zero4();
+#pragma unroll
+  for (int d = 0; d < KB; ++d) z[d] = y[d] = fu[d] = zero4();
+  float inner = 0.f;  // this thread's part of <S0, dS>
+  const E* ob = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh;
+  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh;
+  for (int v0 = 0; v0 < p.dvp; v0 += VB) {
+    __syncthreads();
+    {
+      ChunkTile<E, VB, 256> ot;
+      ot.fetch(ob + v0, p.dout.st, t0, len, p.dv - v0, tid);
+      ot.store(lds.pass.dout, VP, tid);
+    }
+    const int rows = p.dvp - v0;
+    stage_rows<E, VB, kChunk>((const E*)p.u + (n * p.dvp + v0) * kChunk, rows, lds.pass.u, TP, tid);
+    stage_rows<E, VB, kChunk>((const E*)p.dr + (n * p.dvp + v0) * kChunk, rows, lds.pass.dr, TP, tid);
+    stage_rows<E, VB, DK>((const E*)p.s0 + (n * p.dvp + v0) * DK, rows, lds.pass.s0, PITCH, tid);
+    stage_rows<E, VB, DK>((const E*)p.ds + (n * p.dvp + v0) * DK, rows, lds.pass.ds, PITCH, tid);
+    __syncthreads();
+    for (int i = tid; i < VB * DK / 4; i += 256) {
+      const int row = i / (DK / 4), cc = (i % (DK / 4)) * 4;
+      float a[4], bb[4];
+      ld4f<E>(lds.pass.s0 + row * PITCH + cc, a);
+      ld4f<E>(lds.pass.ds + row * PITCH + cc, bb);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) inner = fmaf(a[e], bb[e], inner);
+    }
+#pragma unroll
+    for (int s = 0; s < VB / 32; ++s) {
+      const f8 of = row_perm<E>(lds.pass.dout + t * VP, s, g);
+      const f8 rf = TF::get(lds.pass.dr, TP, 16 * w, s, lane), uw = TF::get(lds.pass.u, TP, 16 * w, s, lane);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r <= w) {
+          const f8 uf = TF::get(lds.pass.u, TP, 16 * r, s, lane);
+          dp[r] = mma32(uf, of, dp[r]);
+          ru[r] = mma32(uf, rf, ru[r]);
+        }
+#pragma unroll
+      for (int d = 0; d < KB; ++d) {
+        const f8 sf = TF::get(lds.pass.s0, PITCH, 16 * d, s, lane);
+        z[d] = mma32(sf, of, z[d]);
+        y[d] = mma32(sf, rf, y[d]);
+        fu[d] = mma32(TF::get(lds.pass.ds, PITCH, 16 * d, s, lane), uw, fu[d]);
+      }
+      if (any_zero) {
+        E v8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int cc = v0 + 32 * s + 16 * (j >> 2) + 4 * g + (j & 3);
+          v8[j] = (E)0.0f;
+          if (cc < p.dv && t0 + t < len) v8[j] = vb[(int64_t)(t0 + t) * p.v.st + cc];
+        }
+        f8 vf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vf[j] = v8[j];
+        rv = mma32(vf, rf, rv);
+      }
+    }
+  }
+  // pairs (i, t): rows i = 16r + 4g + j, column t
+  const double gt = lds.G[t];
+  float rows_x = 0.f, rows_n = 0.f;
+  float cx[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) cx[i] = 0.f;
+  float diag = 0.f, diag_v = 0.f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r <= w) {
+      floatx4 kk = zero4(), qk = zero4();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const f8 ki = IO::ld8(lds.k + (16 * r + l16) * PITCH + 32 * s + 8 * g);
+        kk = mma32(ki, IO::ld8(lds.k + t * PITCH + 32 * s + 8 * g), kk);
+        qk = mma32(ki, IO::ld8(lds.q + t * PITCH + 32 * s + 8 * g), qk);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 16 * r + 4 * g + j;
+        const float d = __builtin_amdgcn_exp2f((float)((gt - lds.G[i]) * kLog2e));
+        if (i == t) {
+          diag = ru[r][j];
+          diag_v = rv[j];
+        }
+        const float a = i <= t ? dp[r][j] * d : 0.f, m = i < t ? ru[r][j] * d : 0.f;
+        const float xa = a * qk[j], xn = m * kk[j];
+        rows_x += xa;
+        rows_n += xn;
+        cx[4 * r + j] = fmaf(-be, xn, xa);
+        dp[r][j] = a;
+        ru[r][j] = -be * m;
+      }
+    } else {
+      dp[r] = ru[r] = zero4();
+    }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) cx[i] += __shfl_xor(cx[i], o, 64);
+    if (l16 == 0) lds.cols[w][16 * (i >> 2) + 4 * g + (i & 3)] = cx[i];
+  }
+  __syncthreads();  // the last pass has been read: the pair matrices take its place
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    IO::st4(lds.pairs.a + t * TP + 16 * r + 4 * g, dp[r][0], dp[r][1], dp[r][2], dp[r][3]);
+    IO::st4(lds.pairs.m + t * TP + 16 * r + 4 * g, ru[r][0], ru[r][1], ru[r][2], ru[r][3]);
+  }
+  // state terms of the gates, and of the rows
+  float zq = 0.f, yk = 0.f, fk = 0.f;
+#pragma unroll
+  for (int d = 0; d < KB; ++d) {
+    float qv[4], kv[4];
+    ld4f<E>(lds.q + t * PITCH + 16 * d + 4 * g, qv);
+    ld4f<E>(lds.k + t * PITCH + 16 * d + 4 * g, kv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      zq = fmaf(z[d][i], qv[i], zq);
+      yk = fmaf(y[d][i], kv[i], yk);
+      fk = fmaf(fu[d][i], kv[i], fk);
+      z[d][i] *= eg;
+      fu[d][i] = fmaf(tail, fu[d][i], -be * eg * y[d][i]);
+    }
+  }
+  zq = sum_g(zq) * eg;
+  yk = sum_g(yk) * eg;
+  fk = sum_g(fk) * tail;
+  rows_x = sum_g(rows_x);
+  rows_n = sum_g(rows_n);
+  if (g == 0) {
+    lds.base[t] = rows_x - be * rows_n + zq - be * yk - fk;
+    lds.f[t] = fk;
+  }
+  if (g == (l16 >> 2) && t0 + t < p.T) {  // the lane that holds (t, t)
+    const float v = t0 + t >= len ? 0.f : zero_b ? diag_v - yk - rows_n : diag / be;
+    put_gate(p.dbeta, p.beta_bf16, gate0 + t, v);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) inner += __shfl_xor(inner, o, 64);
+  if (lane == 0) lds.red[w] = inner;
+  __syncthreads();
+  // dQ^T = K^T A^T + .., dK^T = Q^T A + K^T (M + M^T)^T + ..
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const f8 af = IO::from_acc(dp[2 * s], dp[2 * s + 1]), mf = IO::from_acc(ru[2 * s], ru[2 * s + 1]);
+    const f8 at = TF::get(lds.pairs.a, TP, 16 * w, s, lane), mt = TF::get(lds.pairs.m, TP, 16 * w, s, lane);
+#pragma unroll
+    for (int d = 0; d < KB; ++d) {
+      const f8 kf = TF::get(lds.k, PITCH, 16 * d, s, lane);
+      if (2 * s <= w) {
+        z[d] = mma32(kf, af, z[d]);
+        fu[d] = mma32(kf, mf, fu[d]);
+      }
+      if (2 * s + 1 >= w) {
+        fu[d] = mma32(kf, mt, fu[d]);
+        fu[d] = mma32(TF::get(lds.q, PITCH, 16 * d, s, lane), at, fu[d]);
+      }
+    }
+  }
+  const bool in = t0 + t < len;
+#pragma unroll
+  for (int d = 0; d < KB; ++d) {
+    put_row(p.dq, d, in ? z[d] : zero4());
+    put_row(p.dkey, d, in ? fu[d] : zero4());
+  }
+  if (w == 0 && p.ddecay) {
+    double dg = (double)lds.base[lane];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) dg -= (double)lds.cols[r][lane];
+    double total = (double)lds.f[lane];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
+    total += (double)whole * ((double)lds.red[0] + lds.red[1] + lds.red[2] + lds.red[3]);
+    if (lane == 63) dg += total;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double above = __shfl_down(dg, o, 64);
+      if (lane + o < 64) dg += above;
+    }
+    if (t0 + lane < p.T) put_gate(p.ddecay, p.ddecay_bf16, gate0 + lane, t0 + lane < len ? (float)dg : 0.f);
+  }
+}
+
+// Rows of `rep` value heads added up, in head order: x [B,H,T,W] fp32
+// contiguous -> out [B,H/rep,T,W].
+template <typename E>
+__global__ __launch_bounds__(256) void delta_group_sum_kernel(const float* x, ts_strided out, int Hk, int rep, int T,
+                                                              int W, int64_t total) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int cols = W / 4, c = (int)(i % cols) * 4;
+    const int64_t row = i / cols;
+    const int t = (int)(row % T);
+    const int64_t bk = row / T;
+    const int b = (int)(bk / Hk), hk = (int)(bk % Hk);
+    floatx4 sum = zero4();
+    for (int r = 0; r < rep; ++r) {
+      const floatx4 v = *(const floatx4*)(x + ((bk * rep + r) * T + t) * W + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += v[e];
+    }
+    LdsIO<E>::st4((E*)out.ptr + b * out.sb + hk * out.sh + (int64_t)t * out.st + c, sum[0], sum[1], sum[2], sum[3]);
+  }
+}
+
+// out[h] = sum over batch and time of x [B,H,T] (a static retention's gradient).
+template <typename O>
+__global__ __launch_bounds__(256) void delta_head_sum_kernel(const float* x, O* out, int B, int H, int T) {
+  __shared__ double part[256];
+  const int h = blockIdx.x, tid = threadIdx.x;
+  double sum = 0.0;
+  for (int b = 0; b < B; ++b) {
+    const float* row = x + ((int64_t)b * H + h) * T;
+    for (int t = tid; t < T; t += 256) sum += (double)row[t];
+  }
+  part[tid] = sum;
+  __syncthreads();
+  for (int o = 128; o >= 1; o >>= 1) {
+    if (tid < o) part[tid] += part[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) out[h] = (O)(float)part[0];
+}
+
+}  // namespace ts
+
+namespace {
+
+using ts::DeltaP;
+using ts::fail;
+
+template <typename E, int DK>
+int backward(const DeltaP& p, hipStream_t stream) {
+  const int chain = (int)sizeof(ts::ChainLds<E, DK>), grads = (int)sizeof(ts::GradsLds<E, DK>);
+  if (ts::ensure_lds_limit((const void*)ts::delta_chain_kernel<E, DK, 1>, chain) != hipSuccess ||
+      ts::ensure_lds_limit((const void*)ts::delta_grads_kernel<E, DK>, grads) != hipSuccess)
+    return fail(TS_ERR_RUNTIME, "delta bwd: LDS of %d bytes", grads);
+  hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK, 1>), dim3((unsigned)(p.B * p.H), (unsigned)(p.dvp / 16)), dim3(64),
+                     chain, stream, p);
+  hipLaunchKernelGGL((ts::delta_grads_kernel<E, DK>), dim3((unsigned)((int64_t)p.B * p.H * p.nc)), dim3(256), grads,
+                     stream, p);
+  return TS_OK;
+}
+
+// One axis: which heads share keys, and their fp32 rows' sums.
+template <typename E>
+void group_sum(const DeltaP& p, const float* x, const ts_strided& out, hipStream_t stream) {
+  const int64_t total = (int64_t)p.B * p.Hk * p.T * (p.dk / 4), blocks = (total + 255) / 256;
+  hipLaunchKernelGGL((ts::delta_group_sum_kernel<E>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0,
+                     stream, x, out, p.Hk, p.rep, p.T, p.dk, total);
+}
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+
+extern "C" {
+
+int ts_delta_bwd_workspace_bytes(const ts_delta_desc* d, size_t* bytes) {
+  const int rc = ts::delta_check(d, nullptr, nullptr, "delta bwd");
+  if (rc) return rc;
+  const size_t es = d->dtype == TS_BF16 ? 2 : 4;
+  const size_t n = (size_t)d->B * d->H * ((d->T + 63) / 64), dvp = (d->dv + 15) / 16 * 16;
+  size_t total = n * dvp * (64 + (d->dk <= 64 ? 64 : 128)) * es;
+  if (d->H != d->Hk) total += align16(2 * (size_t)d->B * d->H * d->T * d->dk * sizeof(float));
+  if (bytes) *bytes = total + align16((size_t)d->B * d->H * d->T * sizeof(float));
+  return TS_OK;
+}
+
+int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_grads* gr, const void* saved,
+                 size_t saved_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  DeltaP p;
+  if (!io || !gr) return fail(TS_ERR_VALUE, "delta bwd: missing tensors");
+  int rc = ts::delta_check(d, io, &p, "delta bwd");
+  if (rc) return rc;
+  if (d->T == 0) return TS_OK;
+  size_t need = 0, kept = 0;
+  rc = ts_delta_bwd_workspace_bytes(d, &need);
+  if (rc) return rc;
+  ts_delta_desc whole = *d;
+  whole.keep = 1;
+  rc = ts_delta_workspace_bytes(&whole, &kept);
+  if (rc) return rc;
+  if (!saved || ((uintptr_t)saved & 15u) || saved_bytes < kept || !workspace || ((uintptr_t)workspace & 15u) ||
+      workspace_bytes < need)
+    return fail(TS_ERR_VALUE, "delta bwd: the saved buffer or the workspace is missing, misaligned or too small");
+  const int vec = d->dtype == TS_BF16 ? 8 : 4;
+  auto rows = [&](const ts_strided& s, int v) {
+    return s.ptr && ((uintptr_t)s.ptr & 15u) == 0 && s.sb % v == 0 && s.sh % v == 0 && s.st % v == 0;
+  };
+  if (!rows(gr->dout, vec) || !rows(gr->dq, 4) || !rows(gr->dk, 4) || !gr->dv.ptr || !gr->dbeta)
+    return fail(TS_ERR_VALUE, "delta bwd: missing gradients, or rows that are not aligned");
+  const int64_t chunks = (int64_t)p.B * p.H * p.nc;
+  if (chunks > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta bwd: grid too large");
+  const size_t es = d->dtype == TS_BF16 ? 2 : 4, dkp = d->dk <= 64 ? 64 : 128;
+  const size_t u = (size_t)chunks * p.dvp * 64 * es, s0 = (size_t)chunks * p.dvp * dkp * es;
+  p.prep = (char*)saved;
+  p.u = (char*)saved + (kept - u - s0);
+  p.s0 = (char*)saved + (kept - s0);
+  char* ws = (char*)workspace;
+  p.dr = ws;
+  p.ds = ws + u;
+  ws += u + s0;
+  p.dout = gr->dout; p.dval = gr->dv; p.dq = gr->dq; p.dkey = gr->dk;
+  p.dbeta = gr->dbeta; p.ddecay = gr->ddecay; p.ddecay_bf16 = p.decay_bf16;
+  p.dstate_out = gr->dstate_out; p.dstate = gr->dstate;
+  float *gq = nullptr, *gk = nullptr;
+  if (p.rep > 1) {
+    // per value head in fp32, added up over the heads of a key afterwards
+    const int64_t n = (int64_t)p.B * p.H * p.T * p.dk;
+    gq = (float*)ws;
+    gk = gq + n;
+    ws += align16(2 * (size_t)n * sizeof(float));
+    const ts_strided f = {gq, (int64_t)p.H * p.T * p.dk, (int64_t)p.T * p.dk, p.dk};
+    p.dq = f;
+    p.dkey = f;
+    p.dkey.ptr = gk;
+    p.grad_f32 = 1;
+  } else {
+    p.grad_f32 = d->dtype == TS_F32;
+  }
+  if (gr->ddecay_head) {  // one retention a head: its tokens' gradients, then their sum
+    p.ddecay = ws;
+    p.ddecay_bf16 = 0;
+  }
+  const bool narrow = d->dk <= 64;
+  if (d->dtype == TS_BF16)
+    rc = narrow ? backward<ts::bf16, 64>(p, stream) : backward<ts::bf16, 128>(p, stream);
+  else
+    rc = narrow ? backward<float, 64>(p, stream) : backward<float, 128>(p, stream);
+  if (rc) return rc;
+  if (p.rep > 1) {
+    if (d->dtype == TS_BF16) {
+      group_sum<ts::bf16>(p, gq, gr->dq, stream);
+      group_sum<ts::bf16>(p, gk, gr->dk, stream);
+    } else {
+      group_sum<float>(p, gq, gr->dq, stream);
+      group_sum<float>(p, gk, gr->dk, stream);
+    }
+  }
+  if (gr->ddecay_head) {
+    if (d->decay_dtype == TS_BF16)
+      hipLaunchKernelGGL((ts::delta_head_sum_kernel<ts::bf16>), dim3(p.H), dim3(256), 0, stream, (const float*)p.ddecay,
+                         (ts::bf16*)gr->ddecay_head, p.B, p.H, p.T);
+    else
+      hipLaunchKernelGGL((ts::delta_head_sum_kernel<float>), dim3(p.H), dim3(256), 0, stream, (const float*)p.ddecay,
+                         (float*)gr->ddecay_head, p.B, p.H, p.T);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(TS_ERR_RUNTIME, "delta bwd: launch failed: %s", hipGetErrorString(e));
+  return TS_OK;
+}
+
+}  // extern "C"
