@@ -55,7 +55,8 @@ extern "C" {
  *     rows of a token group of a GN stream have to lie within 4 GiB (a row
  *     stride of 32 Mi elements and more was taken before).
  * 19: ts_delta_fwd / ts_delta_bwd / ts_delta_step (with their workspace sizes)
- *     and ts_policy_loss_fwd / ts_policy_loss_bwd; nothing earlier changed. */
+ *     and ts_policy_loss_fwd / ts_policy_loss_bwd /
+ *     ts_policy_loss_parts; nothing earlier changed. */
 #define TS_ABI_VERSION 19
 
 enum ts_status {
@@ -1297,6 +1298,42 @@ typedef struct ts_delta_grads {
 int ts_delta_bwd_workspace_bytes(const ts_delta_desc* desc, size_t* bytes);
 int ts_delta_bwd(const ts_delta_desc* desc, const ts_delta_io* io, const ts_delta_grads* grads, const void* saved,
                  size_t saved_bytes, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------ clipped policy loss */
+
+/* Rows of logits z (element stride `stride`) with y = cap tanh(z / cap) (cap 0:
+ * y = z), lp = log softmax(y)[token], r = exp(lp - old):
+ *   loss = sum_n w [ -min(r A, clip(r, 1 - low, 1 + high) A)
+ *                    + kl (exp(ref - lp) - (ref - lp) - 1) ]
+ * A row of weight zero is not read.  A token outside [0, V) makes its row NaN. */
+typedef struct ts_policy_desc {
+  int64_t rows, stride;
+  int32_t V, dtype;
+  float cap;
+  int32_t reserved;
+  double kl, low, high;
+} ts_policy_desc;
+
+typedef struct ts_policy_io {
+  const void* logits;
+  const int64_t* tokens;                /* [rows] */
+  const float *old_log_probs;           /* [rows] (loss only)                    */
+  const float *ref_log_probs;           /* [rows] or NULL: no KL term            */
+  const float *advantages;              /* [rows] (loss only)                    */
+  const float *weights;                 /* [rows] or NULL: 1 / rows each         */
+  float *log_probs;                     /* out [rows], zero where not read       */
+  float *coef, *lse;                    /* out [rows] and [2, rows], kept for the
+                                           backward                              */
+  double *parts;                        /* scratch, ts_policy_loss_parts of them */
+  float *loss;                          /* out [1], or NULL: log_probs only      */
+} ts_policy_io;
+
+int ts_policy_loss_parts(const ts_policy_desc* desc, int64_t* parts);
+int ts_policy_loss_fwd(const ts_policy_desc* desc, const ts_policy_io* io, hipStream_t stream);
+/* dlogits [rows, V] contiguous from the forward's coef and lse and the loss's
+ * gradient dloss (fp32, on the device). */
+int ts_policy_loss_bwd(const ts_policy_desc* desc, const ts_policy_io* io, const float* dloss, void* dlogits,
+                       hipStream_t stream);
 
 #ifdef __cplusplus
 }

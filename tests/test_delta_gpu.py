@@ -361,11 +361,12 @@ def test_other_stream_and_empty_sequence(cuda):
     assert out.shape == (1, 2, 0, 64) and torch.equal(S, s["state"]) and S is not s["state"]
 
 
-def test_compiled_call_is_the_eager_one(cuda):
+@pytest.mark.parametrize("decay", ["token", "head", None])
+def test_compiled_call_is_the_eager_one(cuda, decay):
     import thetascan_amd as ts
 
-    s = on_gpu(inputs(1, 2, 2, 80, 64, 64, BF, seed=14), cuda, True)
-    args = [s[n] for n in ("q", "k", "v", "beta", "decay")]
+    s = on_gpu(inputs(1, 2, 2, 80, 64, 64, BF, seed=14, decay=decay), cuda, True)
+    args = [s[n] for n in ("q", "k", "v", "beta", "decay") if s[n] is not None]
 
     def f(*a):
         return ts.gated_delta_rule(*a) * 2.0

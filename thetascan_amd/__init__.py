@@ -4,6 +4,7 @@ from .api import ThetaScan
 from .state import ThetaScanState
 from .decode import DecodeGraph
 from ._core.ops.delta import gated_delta_rule
+from ._core.ops.policy import policy_loss, token_log_probs
 from .config import (
     Backend,
     BankMode,
@@ -37,5 +38,6 @@ __all__ = [
     "DecodeGraph", "KernelBSplineScaleMode", "KernelConfig", "KernelFeatureMap", "KernelReLU2ThresholdMode",
     "KernelReadNormalization", "KernelSharpnessMode", "KernelSparsity", "KernelValueRepresentation",
     "RegularizationConfig", "RoPEConfig", "RoPEMode", "RoPEPlacement", "RuntimeConfig", "TemporalConfig",
-    "TemporalMode", "ThetaScan", "ThetaScanConfig", "ThetaScanState", "gated_delta_rule",
+    "TemporalMode", "ThetaScan", "ThetaScanConfig", "ThetaScanState", "gated_delta_rule", "policy_loss",
+    "token_log_probs",
 ]

@@ -27,7 +27,7 @@ SOURCES = ("ts_scan.hip", "ts_scan_wide.hip", "ts_scan_views.hip", "ts_features.
            "ts_contract.hip", "ts_readout.hip", "ts_anchor.hip", "ts_kmap.hip", "ts_gnact.hip", "ts_absmass.hip",
            "ts_rownorm.hip", "ts_rowglue.hip", "ts_bankread.hip",
            "ts_views_bwd.hip", "ts_step.hip", "ts_attention.hip",
-           "ts_delta.hip", "ts_delta_bwd.hip", "ts_delta_step.hip")
+           "ts_delta.hip", "ts_delta_bwd.hip", "ts_delta_step.hip", "ts_policy.hip")
 
 HIPCC_FLAGS = (
     f"--offload-arch={ARCH}",

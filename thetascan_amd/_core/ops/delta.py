@@ -178,19 +178,18 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
         status = lib.ts_delta_bwd(ctypes.byref(desc), ctypes.byref(io), ctypes.byref(grads), saved.data_ptr(),
                                   saved.numel(), work.data_ptr(), work.numel(), _lib.stream_handle(q.device))
     _lib.check(status, "ts_delta_bwd")
-    none = q.new_empty(0)
-    return [dq[..., :dk], dk_[..., :dk], dv_[..., :dv], dbeta, none if ddecay is None else ddecay,
-            none if dstate is None else dstate[..., :dk, :dv]]
+    return [dq[..., :dk], dk_[..., :dk], dv_[..., :dv], dbeta, q.new_empty(0) if ddecay is None else ddecay,
+            q.new_empty(0) if dstate is None else dstate[..., :dk, :dv]]
 
 
 def _backward_fake(dout, dfinal, q, k, v, beta, decay, state, lengths, saved, need_state):
     def rows(x):
         return _rows_like(x, q.dtype, _width(q.dtype, x.shape[-1]))[..., :x.shape[-1]]
 
-    none = q.new_empty(0)
     B, H, _, dv = v.shape
-    return [rows(q), rows(k), rows(v), beta.new_empty(beta.shape), none if decay is None else decay.new_empty(decay.shape),
-            q.new_empty(B, H, q.shape[-1], dv, dtype=torch.float32) if need_state else none]
+    return [rows(q), rows(k), rows(v), beta.new_empty(beta.shape),
+            q.new_empty(0) if decay is None else decay.new_empty(decay.shape),
+            q.new_empty((B, H, q.shape[-1], dv) if need_state else (0,), dtype=torch.float32)]
 
 
 def _setup(ctx, inputs, output):

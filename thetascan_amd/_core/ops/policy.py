@@ -1,0 +1,169 @@
+"""The clipped policy loss with a KL term, on (soft-capped) logits.
+
+What follows rollouts where the soft-capped cross entropy
+(:func:`.rowglue.softcap_cross_entropy`) follows plain text: per row n of the
+logits, with ``y = cap tanh(z / cap)`` (or z), ``lp = log softmax(y)[token]`` and
+``r = exp(lp - old)``::
+
+    loss = sum_n w_n [ -min(r A, clip(r, 1 - low, 1 + high) A)
+                       + kl (exp(ref - lp) - (ref - lp) - 1) ]
+
+One pass over the logits a direction (ts_policy_loss_fwd, ts_policy_loss_bwd):
+neither the capped logits nor the probabilities are stored.  A row of weight zero
+(a prompt's, a padding's) is not read.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ... import _lib
+from .delta import _on
+from .dispatch import HipOp
+
+
+def _desc(z: torch.Tensor, cap: float, kl: float = 0.0, low: float = 0.0, high: float = 0.0) -> _lib.PolicyDesc:
+    return _lib.PolicyDesc(z.shape[0], z.stride(0) if z.shape[0] > 1 else z.shape[1], z.shape[1],
+                           _lib.dtype_code(z.dtype), cap, 0, kl, low, high)
+
+
+def _rows(z: torch.Tensor) -> torch.Tensor:
+    """Logits [rows, V] with contiguous rows (any distance apart)."""
+    return z if z.stride(1) == 1 or z.shape[1] == 1 else z.contiguous()
+
+
+def _forward(z: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, adv: torch.Tensor, ref: torch.Tensor | None,
+             weights: torch.Tensor | None, low: float, high: float, kl: float, cap: float) -> list[torch.Tensor]:
+    lib = _lib.load()
+    z = _rows(z)
+    rows = z.shape[0]
+    desc = _desc(z, cap, kl, low, high)
+    n = ctypes.c_int64()
+    _lib.check(lib.ts_policy_loss_parts(ctypes.byref(desc), ctypes.byref(n)), "ts_policy_loss_parts")
+    loss = torch.empty((), dtype=torch.float32, device=z.device)
+    lp = torch.empty(rows, dtype=torch.float32, device=z.device)
+    coef = torch.empty_like(lp)
+    lse = torch.empty(2, rows, dtype=torch.float32, device=z.device)
+    parts = torch.empty(max(n.value, 1), dtype=torch.float64, device=z.device)
+    io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), old.data_ptr(), _lib.ptr(ref), adv.data_ptr(),
+                       _lib.ptr(weights), lp.data_ptr(), coef.data_ptr(), lse.data_ptr(), parts.data_ptr(),
+                       loss.data_ptr())
+    with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tokens, old, adv, ref, weights, lp)):
+        status = lib.ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
+    _lib.check(status, "ts_policy_loss_fwd")
+    return [loss, lp, coef, lse]
+
+
+def _forward_fake(z, tokens, old, adv, ref, weights, low, high, kl, cap):
+    row = z.new_empty(z.shape[0], dtype=torch.float32)
+    return [z.new_empty((), dtype=torch.float32), row, torch.empty_like(row), row.new_empty(2, z.shape[0])]
+
+
+def _backward_impl(g: torch.Tensor, z: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | None,
+                   coef: torch.Tensor, lse: torch.Tensor, cap: float) -> torch.Tensor:
+    lib = _lib.load()
+    z = _rows(z)
+    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    g32 = g.detach().to(torch.float32).reshape(1).contiguous()
+    io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), None, None, None, _lib.ptr(weights), None, coef.data_ptr(),
+                       lse.data_ptr(), None, None)
+    desc = _desc(z, cap)
+    with _on(z.device), _lib.timed("ts_policy_loss_bwd", lambda: _lib.nbytes(z, tokens, dz)):
+        status = lib.ts_policy_loss_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(),
+                                        _lib.stream_handle(z.device))
+    _lib.check(status, "ts_policy_loss_bwd")
+    return dz
+
+
+def _backward_fake(g, z, tokens, weights, coef, lse, cap):
+    return z.new_empty(z.shape)
+
+
+def _setup(ctx, inputs, output):
+    z, tokens, weights, ctx.cap = inputs[0], inputs[1], inputs[5], inputs[9]
+    ctx.save_for_backward(z, tokens, weights, output[2], output[3])
+
+
+def _backward(ctx, grads, bwd):
+    if grads[0] is None:
+        return (None,) * 10
+    z, tokens, weights, coef, lse = ctx.saved_tensors
+    return (bwd(grads[0], z, tokens, weights, coef, lse, ctx.cap), *(None,) * 9)
+
+
+_policy_op = HipOp("policy_loss", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,
+                   backward_fake=_backward_fake, setup=_setup, backward=_backward)
+
+
+def _flat(what: str, logits: torch.Tensor, tokens: torch.Tensor, softcap: float | None,
+          rows: dict) -> tuple[torch.Tensor, torch.Tensor, float, dict]:
+    """The logits as [rows, V], the tokens and per-row tensors (fp32) as [rows]."""
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits must be [..., V], got {tuple(logits.shape)}")
+    shape = logits.shape[:-1]
+    if tokens.shape != shape or tokens.dtype != torch.int64:
+        raise ValueError(f"{what}: tokens must be int64 {tuple(shape)}, got {tokens.dtype} {tuple(tokens.shape)}")
+    for name, x in rows.items():
+        if x is not None and (x.shape != shape or not (x.is_floating_point() or name == "weights")):
+            raise ValueError(f"{what}: {name} must be floating-point {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
+    cap = 0.0 if softcap is None else float(softcap)
+    if softcap is not None and not 0.0 < cap < float("inf"):
+        raise ValueError(f"{what}: softcap must be positive (None: no cap), got {softcap}")
+    _lib.dtype_code(logits.dtype)
+    given = [logits, tokens, *(x for x in rows.values() if x is not None)]
+    if not all(x.is_cuda for x in given):
+        raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")
+    if any(x.device != logits.device for x in given):
+        raise ValueError(f"{what}: tensors on several devices")
+    flat = {name: None if x is None else x.detach().to(torch.float32).reshape(-1).contiguous()
+            for name, x in rows.items()}
+    return logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1).contiguous(), cap, flat
+
+
+def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor, *,
+                ref_log_probs: torch.Tensor | None = None, weights: torch.Tensor | None = None,
+                clip: float | tuple[float, float] = 0.2, kl: float = 0.0,
+                softcap: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(loss, log_probs)``: the clipped policy loss (module docstring; a
+    scalar, differentiable in the logits) and the tokens' present
+    log-probabilities (fp32, without a gradient).
+
+    ``logits`` [..., V] in bf16 or fp32, ``tokens`` int64 [...] (one outside [0, V)
+    makes the loss NaN), ``old_log_probs`` and ``advantages`` [...], as
+    ``ref_log_probs``, which the KL term needs (``kl`` > 0).  ``clip`` is the
+    distance of the clipping borders from 1, below and above.  ``weights`` [...]
+    multiplies each row's loss (default: the mean over all rows); a row of weight
+    zero may hold anything in any input, and gives a log-probability of zero and a
+    gradient of zero.  ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.
+    """
+    low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
+    low, high, kl = float(low), float(high), float(kl)
+    if not (0.0 <= low <= 1.0 and 0.0 <= high < float("inf")):
+        raise ValueError(f"policy_loss: clip must lie in [0, 1] below and be at least 0 above, got {clip}")
+    if not 0.0 <= kl < float("inf"):
+        raise ValueError(f"policy_loss: kl must be at least 0, got {kl}")
+    if kl and ref_log_probs is None:
+        raise ValueError("policy_loss: the KL term needs ref_log_probs")
+    z, tok, cap, r = _flat("policy_loss", logits, tokens, softcap,
+                           {"old_log_probs": old_log_probs, "advantages": advantages,
+                            "ref_log_probs": ref_log_probs if kl else None, "weights": weights})
+    loss, lp, _, _ = _policy_op(z, tok, r["old_log_probs"], r["advantages"], r["ref_log_probs"], r["weights"], low, high,
+                                kl, cap)
+    return loss, lp.detach().view(tokens.shape)
+
+
+@torch.no_grad()
+def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, softcap: float | None = None) -> torch.Tensor:
+    """The tokens' log-probabilities [...] (fp32, without a gradient) under the
+    (soft-capped) logits [..., V]: what :func:`policy_loss` takes as
+    ``old_log_probs`` and ``ref_log_probs``, in the same arithmetic."""
+    z, tok, cap, _ = _flat("token_log_probs", logits.detach(), tokens, softcap, {})
+    z = _rows(z)
+    lp = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
+    io = _lib.PolicyIO(z.data_ptr(), tok.data_ptr(), None, None, None, None, lp.data_ptr(), None, None, None, None)
+    desc = _desc(z, cap)
+    with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tok, lp)):
+        status = _lib.load().ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
+    _lib.check(status, "ts_policy_loss_fwd")
+    return lp.view(tokens.shape)

@@ -560,6 +560,17 @@ class DeltaGrads(ctypes.Structure):
         (n, ctypes.c_void_p) for n in ("dbeta", "ddecay", "ddecay_head", "dstate_out", "dstate")]
 
 
+class PolicyDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("stride", ctypes.c_int64), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("cap", ctypes.c_float), ("reserved", ctypes.c_int32), ("kl", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double)]
+
+
+class PolicyIO(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "tokens", "old_log_probs", "ref_log_probs", "advantages",
+                                               "weights", "log_probs", "coef", "lse", "parts", "loss")]
+
+
 ABI_VERSION = 19  # the include/thetascan_hip.h these bindings are written for
 
 _lock = threading.Lock()
@@ -717,6 +728,9 @@ def load() -> ctypes.CDLL:
         lib.ts_delta_bwd_workspace_bytes.argtypes = [P(DeltaDesc), P(ctypes.c_size_t)]
         lib.ts_delta_bwd.argtypes = [P(DeltaDesc), P(DeltaIO), P(DeltaGrads), ctypes.c_void_p, ctypes.c_size_t,
                                      ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.ts_policy_loss_parts.argtypes = [P(PolicyDesc), P(ctypes.c_int64)]
+        lib.ts_policy_loss_fwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p]
+        lib.ts_policy_loss_bwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_scale_add_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 6
         lib.ts_scale_add_norm_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 4 + [ctypes.c_float] + [
             ctypes.c_void_p] * 4

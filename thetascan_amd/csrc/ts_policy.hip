@@ -1,0 +1,391 @@
+// Clipped policy loss with a KL term on (soft-capped) logits, forward and
+// backward (gfx950).
+//
+//   y = cap tanh(z / cap) (or z);  lp = y_tok - log sum_v e^{y_v};  r = e^{lp - old}
+//   loss = sum_n w_n [ -min(r A, clip(r, 1 - low, 1 + high) A) + kl (e^{ref - lp} - (ref - lp) - 1) ]
+//   dloss/dlp = w [ -r A where not clipped + kl (1 - e^{ref - lp}) ]
+//   dz_v = dloss/dlp (1[v = tok] - e^{y_v - lse}) (1 - (y_v / cap)^2)
+//
+// Bound by the logits' bytes: a row is read once a direction, by one wave (or by
+// a workgroup where it is long), with a running maximum and sum.  The sums of
+// exponentials are fp32; a row's own terms are formed in fp64, for several rows
+// at once (a lane each, after the rows of its wave), and the rows are added in
+// fp64 in a fixed order: normalized advantages all but cancel in the sum.  A row
+// of weight zero is not read; its log-probability is given as zero, its gradient
+// too.
+
+#include "ts_common.h"
+#include "ts_tokens.h"
+
+#include <string.h>
+
+namespace ts {
+
+constexpr float kLog2eF = 1.44269504088896340736f;
+constexpr double kLn2 = 0.69314718055994530942;
+struct PolicyP {
+  int64_t rows, stride;
+  int V;
+  float cap;
+  double kl, low, high;
+  const void* z;
+  const int64_t* tokens;
+  const float *old, *ref, *adv, *w;
+  float *lp, *coef;
+  float* lse;  // [2][rows]: the maximum, and log2 of the sum of e^{x - maximum}
+  double* part;
+  const float* g;
+  void* dz;
+};
+
+// A logit as the softmax takes it, x, and e^x relative to a maximum.  Without a
+// cap x is the logit itself (the lowest finite one too, whose multiple by log2 e
+// is none); with a cap, x = log2 e cap tanh(z / cap) = log2 e (cap - 2 cap r) with
+// r = 1 / (1 + e^{2 z / cap}).
+template <bool CAP>
+struct Logit {
+  float in, mul, add;
+  __device__ __forceinline__ explicit Logit(float cap)
+      : in(CAP ? 2.f * kLog2eF / cap : 0.f), mul(-2.f * cap * kLog2eF), add(cap * kLog2eF) {}
+  __device__ __forceinline__ float sig(float z) const { return rcp(1.f + __builtin_amdgcn_exp2f(z * in)); }
+  __device__ __forceinline__ float operator()(float z) const { return CAP ? fmaf(sig(z), mul, add) : z; }
+};
+template <bool CAP>
+__device__ __forceinline__ float ex(float d) {
+  return __builtin_amdgcn_exp2f(CAP ? d : d * kLog2eF);
+}
+constexpr float kLowest = -3.402823466e38f;
+
+// The parts of a row: `head` elements before its first 16-byte boundary, then
+// `vecs` vectors, then a tail.
+template <typename E>
+struct RowSpan {
+  int head, vecs;
+  __device__ __forceinline__ RowSpan(const E* row, int V) {
+    constexpr int N = Vec16<E>::N;
+    head = min(V, (int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(E)));
+    vecs = (V - head) / N;
+  }
+};
+
+// WPR waves a row, R rows one after the other whose terms are formed together.
+template <typename E, bool CAP, int WPR, int R>
+__global__ __launch_bounds__(WPR <= 4 ? 256 : 64 * WPR) void policy_fwd_kernel(PolicyP p) {
+  constexpr int N = Vec16<E>::N, THREADS = WPR <= 4 ? 256 : 64 * WPR, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
+  constexpr int U = 4;
+  __shared__ float sm[WPR == 1 ? 1 : THREADS / 64], ss[WPR == 1 ? 1 : THREADS / 64];
+  __shared__ double sums[THREADS / 64];
+  const int tid = threadIdx.x, lane = tid & 63, gi = tid / LANES, li = tid % LANES;
+  const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + gi) * R;
+  const Logit<CAP> f(p.cap);
+  float mine_m = 0.f, mine_s = 1.f;  // of the row this lane finishes
+  for (int k = 0; k < R; ++k) {
+    const int64_t n = row0 + k;
+    // (uniform over the row's threads; with several waves a row over the workgroup)
+    if (n >= p.rows) break;
+    if (p.w && p.w[n] == 0.f) continue;
+    const E* row = (const E*)p.z + n * p.stride;
+    const RowSpan<E> span(row, p.V);
+    const Vec16<E>* vec = (const Vec16<E>*)(row + span.head);
+    float m = kLowest, s = 0.f;
+    auto one = [&](float x) {
+      const float top = fmaxf(m, x);
+      s = fmaf(s, ex<CAP>(m - top), ex<CAP>(x - top));
+      m = top;
+    };
+    for (int i = li; i < span.vecs; i += LANES * U) {
+      Vec16<E> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * LANES < span.vecs) v[u].raw = vec[i + u * LANES].raw;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * LANES < span.vecs) {
+          float x[N], top = m;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            x[j] = f(tof(v[u].e[j]));
+            top = fmaxf(top, x[j]);
+          }
+          s *= ex<CAP>(m - top);
+#pragma unroll
+          for (int j = 0; j < N; ++j) s += ex<CAP>(x[j] - top);
+          m = top;
+        }
+    }
+    if (li < span.head) one(f(tof(row[li])));
+    for (int i = span.head + span.vecs * N + li; i < p.V; i += LANES) one(f(tof(row[i])));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2);
+      s = s * ex<CAP>(m - top) + s2 * ex<CAP>(m2 - top);
+      m = top;
+    }
+    if constexpr (WPR > 1) {
+      const int w0 = gi * WPR;
+      if (lane == 0) {
+        sm[tid >> 6] = m;
+        ss[tid >> 6] = s;
+      }
+      __syncthreads();
+      m = kLowest;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) m = fmaxf(m, sm[w0 + w]);
+      s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) s = fmaf(ss[w0 + w], ex<CAP>(sm[w0 + w] - m), s);
+      __syncthreads();
+    }
+    if (li == k) {
+      mine_m = m;
+      mine_s = s;
+    }
+  }
+  // the rows' own terms, a lane each
+  double term = 0.0;
+  const int64_t n = row0 + li;
+  if (li < R && n < p.rows) {
+    const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
+    float coef = 0.f, logs = 0.f, lpf = 0.f;
+    if (w != 0.f) {
+      const double l2 = log2((double)mine_s), top = CAP ? (double)mine_m * kLn2 : (double)mine_m;
+      const int64_t tok = p.tokens[n];
+      double y = (double)NAN;  // a token that is none of the row's
+      if (tok >= 0 && tok < p.V) {
+        y = (double)tof(((const E*)p.z)[n * p.stride + tok]);
+        if (CAP) y = (double)p.cap * tanh(y / (double)p.cap);
+      }
+      const double lp = (y - top) - l2 * kLn2;
+      logs = (float)l2;
+      lpf = (float)lp;
+      if (p.adv) {
+        const double A = (double)p.adv[n], r = exp(lp - (double)p.old[n]);
+        const double edge = A > 0.0 ? 1.0 + p.high : 1.0 - p.low;
+        const bool flat = (A > 0.0 && r > edge) || (A < 0.0 && r < edge);
+        term = -(flat ? edge : r) * A;
+        double slope = flat ? 0.0 : -r * A;
+        if (p.ref) {
+          const double d = (double)p.ref[n] - lp, e = expm1(d);
+          term += p.kl * (e - d);
+          slope -= p.kl * e;
+        }
+        term *= (double)w;
+        coef = (float)(slope * (double)w);
+      }
+    }
+    p.lp[n] = lpf;
+    if (p.coef) {
+      p.coef[n] = coef;
+      p.lse[n] = mine_m;
+      p.lse[p.rows + n] = logs;
+    }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int o = R / 2; o >= 1; o >>= 1) term += __shfl_xor(term, o, 64);
+  if (lane == 0) sums[tid >> 6] = term;
+  __syncthreads();
+  if (tid == 0) {
+    double total = 0.0;
+    for (int i = 0; i < GROUPS; ++i) total += sums[i * WPR];
+    p.part[blockIdx.x] = total;
+  }
+}
+
+__global__ __launch_bounds__(256) void policy_sum_kernel(const double* part, int64_t n, float* loss) {
+  __shared__ double s[256];
+  const int tid = threadIdx.x;
+  double sum = 0.0;
+  for (int64_t i = tid; i < n; i += 256) sum += part[i];
+  s[tid] = sum;
+  __syncthreads();
+  for (int o = 128; o >= 1; o >>= 1) {
+    if (tid < o) s[tid] += s[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) loss[0] = (float)s[0];
+}
+
+template <typename E, bool CAP, int WPR>
+__global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
+  constexpr int N = Vec16<E>::N, LANES = 64 * WPR, GROUPS = 256 / LANES, U = 4;
+  const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
+  const int64_t n = (int64_t)blockIdx.x * GROUPS + gi;
+  if (n >= p.rows) return;
+  const float c = p.coef[n] * p.g[0], top = p.lse[n], logs = p.lse[p.rows + n];
+  const int64_t tok = p.tokens[n];
+  const bool read = !p.w || p.w[n] != 0.f;
+  const Logit<CAP> f(p.cap);
+  const E* row = (const E*)p.z + n * p.stride;
+  E* out = (E*)p.dz + n * (int64_t)p.V;
+  auto grad = [&](float z, int v) {
+    float x = z, slope = 1.f;
+    if (CAP) {
+      const float r = f.sig(z);
+      x = fmaf(r, f.mul, f.add);
+      slope = 4.f * r * (1.f - r);
+    }
+    const float prob = __builtin_amdgcn_exp2f(CAP ? (x - top) - logs : fmaf(x - top, kLog2eF, -logs));
+    return c * ((v == tok ? 1.f : 0.f) - prob) * slope;
+  };
+  // the output's vectors; where the logits' do not start with them, they are read element by element
+  const RowSpan<E> span(out, p.V);
+  const bool together = (((uintptr_t)(row + span.head)) & 15) == 0;
+  for (int i = li + (int)blockIdx.y * LANES * U; i < span.vecs; i += (int)gridDim.y * LANES * U) {
+    Vec16<E> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].raw = make_uint4(0u, 0u, 0u, 0u);
+      const int at = i + u * LANES;
+      if (at < span.vecs && read) {
+        if (together)
+          v[u].raw = ((const Vec16<E>*)(row + span.head))[at].raw;
+        else
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[u].e[j] = row[span.head + at * N + j];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = i + u * LANES;
+      if (at < span.vecs) {
+        Vec16<E> o;
+        o.raw = make_uint4(0u, 0u, 0u, 0u);
+        if (read)
+#pragma unroll
+          for (int j = 0; j < N; ++j) o.e[j] = cvt<E>(grad(tof(v[u].e[j]), span.head + at * N + j));
+        ((Vec16<E>*)(out + span.head))[at].raw = o.raw;
+      }
+    }
+  }
+  if (blockIdx.y) return;
+  if (li < span.head) out[li] = read ? cvt<E>(grad(tof(row[li]), li)) : (E)0.0f;
+  for (int i = span.head + span.vecs * N + li; i < p.V; i += LANES)
+    out[i] = read ? cvt<E>(grad(tof(row[i]), i)) : (E)0.0f;
+}
+
+}  // namespace ts
+
+namespace {
+
+using ts::fail;
+using ts::PolicyP;
+
+// Rows of up to 2048 logits take a wave each (no barrier); longer ones a
+// workgroup of four, or of sixteen waves where the rows alone leave most of the
+// CUs without one.
+int waves_of(const PolicyP& p) { return p.V <= 2048 ? 1 : (p.rows < 256 && p.V > 8192 ? 16 : 4); }
+
+// A row's fp64 terms cost a wave about as much as 1500 of its logits: where there
+// are rows enough to keep every CU busy all the same, eight rows share one pass.
+bool shares_terms(const PolicyP& p) { return p.rows * waves_of(p) >= 8 * 8192; }
+
+int64_t forward_blocks(const PolicyP& p) {
+  const int64_t per = (waves_of(p) == 1 ? 4 : 1) * (shares_terms(p) ? 8 : 1);
+  return (p.rows + per - 1) / per;
+}
+
+template <typename E, bool CAP, int WPR>
+void forward(const PolicyP& p, hipStream_t stream) {
+  const dim3 grid((unsigned)forward_blocks(p)), block(WPR <= 4 ? 256 : 64 * WPR);
+  if (shares_terms(p))
+    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, WPR, 8>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, WPR, 1>), grid, block, 0, stream, p);
+}
+template <typename E, bool CAP>
+void forward(const PolicyP& p, hipStream_t stream) {
+  switch (waves_of(p)) {
+    case 1: return forward<E, CAP, 1>(p, stream);
+    case 4: return forward<E, CAP, 4>(p, stream);
+    default: return forward<E, CAP, 16>(p, stream);
+  }
+}
+template <typename E, bool CAP>
+void backward(const PolicyP& p, hipStream_t stream) {
+  // a row's vectors split over workgroups where the rows are few
+  const int64_t rows = p.V <= 2048 ? (p.rows + 3) / 4 : p.rows;
+  int parts = 1;
+  if (p.V > 2048)
+    while (rows * parts < 1024 && parts * 8192 < p.V) parts *= 2;
+  const dim3 grid((unsigned)rows, (unsigned)parts);
+  if (p.V <= 2048)
+    hipLaunchKernelGGL((ts::policy_bwd_kernel<E, CAP, 1>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((ts::policy_bwd_kernel<E, CAP, 4>), grid, dim3(256), 0, stream, p);
+}
+
+int setup(const ts_policy_desc* d, const void* z, const int64_t* tokens, PolicyP* p) {
+  if (!d || d->rows < 0 || d->V < 1 || d->stride < 0 || !(d->cap >= 0.f) || !(d->low >= 0.0 && d->low <= 1.0) ||
+      !(d->high >= 0.0) || !(d->kl >= 0.0))
+    return fail(TS_ERR_VALUE, "policy_loss: bad shape, cap, clip range or KL coefficient");
+  if (d->dtype != TS_BF16 && d->dtype != TS_F32) return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: bf16 or fp32 only");
+  if (d->rows > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: too many rows");
+  if (d->rows && (!z || !tokens || ((uintptr_t)z & (d->dtype == TS_BF16 ? 1u : 3u))))
+    return fail(TS_ERR_VALUE, "policy_loss: missing or misaligned logits or tokens");
+  memset(p, 0, sizeof(*p));
+  p->rows = d->rows; p->V = d->V; p->stride = d->stride; p->cap = d->cap;
+  p->kl = d->kl; p->low = d->low; p->high = d->high;
+  p->z = z; p->tokens = tokens;
+  return TS_OK;
+}
+
+int finish(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(TS_ERR_RUNTIME, "%s: launch failed: %s", what, hipGetErrorString(e));
+  return TS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ts_policy_loss_parts(const ts_policy_desc* d, int64_t* parts) {
+  PolicyP p;
+  const int rc = setup(d, (const void*)16, (const int64_t*)16, &p);
+  if (rc) return rc;
+  if (parts) *parts = forward_blocks(p);
+  return TS_OK;
+}
+
+int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStream_t stream) {
+  PolicyP p;
+  if (!io) return fail(TS_ERR_VALUE, "policy_loss: missing tensors");
+  const int rc = setup(d, io->logits, io->tokens, &p);
+  if (rc) return rc;
+  if (d->rows && !io->log_probs) return fail(TS_ERR_VALUE, "policy_loss: no place for the log-probabilities");
+  if (io->loss && (!io->parts || (d->rows && (!io->old_log_probs || !io->advantages || !io->coef || !io->lse))))
+    return fail(TS_ERR_VALUE, "policy_loss: missing tensors");
+  p.old = io->old_log_probs; p.ref = io->ref_log_probs; p.adv = io->loss ? io->advantages : nullptr; p.w = io->weights;
+  p.lp = io->log_probs; p.coef = io->loss ? io->coef : nullptr; p.lse = io->lse;
+  p.part = io->loss ? io->parts : nullptr;
+  if (d->rows) {
+    if (d->dtype == TS_BF16)
+      p.cap > 0.f ? forward<ts::bf16, true>(p, stream) : forward<ts::bf16, false>(p, stream);
+    else
+      p.cap > 0.f ? forward<float, true>(p, stream) : forward<float, false>(p, stream);
+  }
+  if (io->loss)
+    hipLaunchKernelGGL(ts::policy_sum_kernel, dim3(1), dim3(256), 0, stream, (const double*)io->parts,
+                       d->rows ? forward_blocks(p) : 0, io->loss);
+  return finish("policy_loss");
+}
+
+int ts_policy_loss_bwd(const ts_policy_desc* d, const ts_policy_io* io, const float* dloss, void* dlogits,
+                       hipStream_t stream) {
+  PolicyP p;
+  if (!io) return fail(TS_ERR_VALUE, "policy_loss bwd: missing tensors");
+  const int rc = setup(d, io->logits, io->tokens, &p);
+  if (rc) return rc;
+  if (d->rows == 0) return TS_OK;
+  if (!io->coef || !io->lse || !dloss || !dlogits || ((uintptr_t)dlogits & (d->dtype == TS_BF16 ? 1u : 3u)))
+    return fail(TS_ERR_VALUE, "policy_loss bwd: missing or misaligned tensors");
+  p.w = io->weights; p.coef = io->coef; p.lse = io->lse; p.g = dloss; p.dz = dlogits;
+  if (d->dtype == TS_BF16)
+    p.cap > 0.f ? backward<ts::bf16, true>(p, stream) : backward<ts::bf16, false>(p, stream);
+  else
+    p.cap > 0.f ? backward<float, true>(p, stream) : backward<float, false>(p, stream);
+  return finish("policy_loss bwd");
+}
+
+}  // extern "C"
