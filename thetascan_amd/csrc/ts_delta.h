@@ -176,6 +176,42 @@ struct ChunkTile {
   }
 };
 
+// A chunk's record of delta_prepare, copied as it stands.
+template <typename E, int THREADS, size_t BYTES>
+struct Linear {
+  static constexpr int VECS = (int)(BYTES / 16), SLOTS = (VECS + THREADS - 1) / THREADS;
+  floatx4 r[SLOTS];
+  __device__ __forceinline__ void fetch(const void* src, int tid) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) r[i] = ((const floatx4*)src)[min(tid + i * THREADS, VECS - 1)];
+  }
+  __device__ __forceinline__ void store(void* dst, int tid) const {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+      if (tid + i * THREADS < VECS) ((floatx4*)dst)[tid + i * THREADS] = r[i];
+  }
+};
+
+// Four consecutive rows of column c0 + l16 of an LDS tile, from row r0 + 4g.
+template <typename E>
+__device__ __forceinline__ floatx4 col4(const E* rows, int pitch, int r0, int c0, int lane);
+template <>
+__device__ __forceinline__ floatx4 col4<bf16>(const bf16* rows, int pitch, int r0, int c0, int lane) {
+  typedef short shortx4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+  const int g = lane >> 4, j = lane & 15;
+  const bf16* a = rows + (r0 + 4 * g + (j >> 2)) * pitch + c0 + 4 * (j & 3);
+  const bf16x4 v = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)a));
+  return floatx4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+template <>
+__device__ __forceinline__ floatx4 col4<float>(const float* rows, int pitch, int r0, int c0, int lane) {
+  const float* a = rows + (r0 + 4 * (lane >> 4)) * pitch + c0 + (lane & 15);
+  return floatx4{a[0], a[pitch], a[2 * pitch], a[3 * pitch]};
+}
+
+constexpr int kLdsBytes = 160 * 1024;
+
 int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const char* what);
 
 }  // namespace ts

@@ -208,28 +208,31 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
     }
 }
 
-template <typename E, int DK, int NW>
-struct ForwardLds {
-  static constexpr int PITCH = DK + 16 / (int)sizeof(E);
-  E k[2][kChunk * PITCH];
-  E q[2][kChunk * PITCH];
+// What the waves of a workgroup read of one chunk.
+template <typename E, int DK>
+struct ForwardChunk {
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD;
+  E k[kChunk * PITCH], q[kChunk * PITCH], v[kChunk * VP];
+  __align__(16) char prep[prep_bytes<E>()];
 };
+template <typename E, int DK>
+constexpr int kForwardBufs = 2 * sizeof(ForwardChunk<E, DK>) <= kLdsBytes ? 2 : 1;
 
-template <typename E, int DK, int NW, bool KEEP>
-__global__ __launch_bounds__(64 * NW) void delta_forward_kernel(DeltaP p) {
+template <typename E, int DK, bool KEEP>
+__global__ __launch_bounds__(256) void delta_forward_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
-  typedef ForwardLds<E, DK, NW> Lds;
-  constexpr int PITCH = Lds::PITCH, KB = DK / 16, KS = DK / 32;
+  typedef ForwardChunk<E, DK> Chunk;
+  constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32, BUFS = kForwardBufs<E, DK>;
   extern __shared__ __align__(16) char smem[];
-  Lds& lds = *(Lds*)smem;
+  Chunk* lds = (Chunk*)smem;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-  const int col0 = ((int)blockIdx.y * NW + w) * 16, col = col0 + l16;
+  const int base = (int)blockIdx.y * 64, col0 = base + w * 16, col = col0 + l16;
   const bool mine = col0 < p.dvp, on = col < p.dv;  // (a wave past the columns only helps staging)
   const int len = delta_len(p, b), chunks = (len + kChunk - 1) / kChunk;
   const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
-  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh + col;
+  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh + base;
   E* ob = (E*)p.out.ptr + b * p.out.sb + h * p.out.sh + col0 + 4 * g;
   const bool out_on = col0 + 4 * g < p.dv;
 
@@ -245,38 +248,32 @@ __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(DeltaP p) {
       }
     }
   }
-  ChunkTile<E, DK, 64 * NW> kt, qt;
-  E vr[16];
+  ChunkTile<E, DK, 256> kt, qt;
+  ChunkTile<E, 64, 256> vt;
+  Linear<E, 256, prep_bytes<E>()> pt;
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
     kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
     qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t0 + 16 * r + 4 * g + i;
-        vr[4 * r + i] = (E)0.0f;
-        if (on && t < len) vr[4 * r + i] = vb[(int64_t)t * p.v.st];
-      }
+    vt.fetch(vb, p.v.st, t0, len, p.dv - base, tid);
+    pt.fetch(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>(), tid);
   };
   if (chunks) fetch(0);
   for (int c = 0; c < chunks; ++c) {
-    const int buf = c & 1, t0 = c * kChunk;
-    kt.store(lds.k[buf], PITCH, tid);
-    qt.store(lds.q[buf], PITCH, tid);
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = tof(vr[i]);
+    const int t0 = c * kChunk;
+    Chunk& ch = lds[BUFS == 2 ? c & 1 : 0];
+    if (BUFS == 1) __syncthreads();  // the last chunk has been read
+    kt.store(ch.k, PITCH, tid);
+    qt.store(ch.q, PITCH, tid);
+    vt.store(ch.v, VP, tid);
+    pt.store(ch.prep, tid);
     if (c + 1 < chunks) fetch(c + 1);
     // this chunk is staged; the other buffer was last read before this barrier
     __syncthreads();
     if (!mine) continue;
-    const E* ks = lds.k[buf];
-    const E* qs = lds.q[buf];
+    const E *ks = ch.k, *qs = ch.q;
     const int64_t n = (int64_t)bh * p.nc + c;
-    const char* prep = p.prep + n * (int64_t)prep_bytes<E>();
-    const E* tri_t = (const E*)prep;
+    const E* tri_t = (const E*)ch.prep;
     const E* tri_p = tri_t + TriSets<E>::N * kTriElems;
     const float* vec = (const float*)(tri_p + TriSets<E>::N * kTriElems);
 
@@ -301,8 +298,9 @@ __global__ __launch_bounds__(64 * NW) void delta_forward_kernel(DeltaP p) {
     for (int r = 0; r < 4; ++r) {
       const floatx4 eg = *(const floatx4*)(vec + 16 * r + 4 * g);
       const floatx4 be = *(const floatx4*)(vec + 2 * kChunk + 16 * r + 4 * g);
+      const floatx4 v = col4<E>(ch.v, VP, 16 * r, 16 * w, lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) R[r][i] = be[i] * fmaf(-eg[i], R[r][i], v[4 * r + i]);
+      for (int i = 0; i < 4; ++i) R[r][i] = be[i] * fmaf(-eg[i], R[r][i], v[i]);
     }
     // U = Ti R
     floatx4 U[4];
@@ -436,25 +434,20 @@ Sizes sizes(const ts_delta_desc* d) {
   return s;
 }
 
-template <typename E, int DK, int NW>
-int launch_forward(const DeltaP& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.B * p.H), (unsigned)((p.dvp / 16 + NW - 1) / NW)), block(64 * NW);
-  const int lds = (int)sizeof(ts::ForwardLds<E, DK, NW>);
-  const void* fn = p.u ? (const void*)ts::delta_forward_kernel<E, DK, NW, true>
-                       : (const void*)ts::delta_forward_kernel<E, DK, NW, false>;
-  if (ts::ensure_lds_limit(fn, lds) != hipSuccess) return fail(TS_ERR_RUNTIME, "delta: LDS of %d bytes", lds);
-  if (p.u)
-    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, NW, true>), grid, block, lds, stream, p);
-  else
-    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, NW, false>), grid, block, lds, stream, p);
-  return TS_OK;
-}
-
 template <typename E, int DK>
 int forward(const DeltaP& p, hipStream_t stream) {
   const int64_t n = (int64_t)p.B * p.H * p.nc;
+  const int lds = (int)sizeof(ts::ForwardChunk<E, DK>) * ts::kForwardBufs<E, DK>;
+  const void* fn = p.u ? (const void*)ts::delta_forward_kernel<E, DK, true>
+                       : (const void*)ts::delta_forward_kernel<E, DK, false>;
+  if (ts::ensure_lds_limit(fn, lds) != hipSuccess) return fail(TS_ERR_RUNTIME, "delta: LDS of %d bytes", lds);
   hipLaunchKernelGGL((ts::delta_prepare_kernel<E, DK>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, p);
-  return launch_forward<E, DK, 1>(p, stream);
+  const dim3 grid((unsigned)(p.B * p.H), (unsigned)((p.dvp + 63) / 64));
+  if (p.u)
+    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, true>), grid, dim3(256), lds, stream, p);
+  else
+    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, false>), grid, dim3(256), lds, stream, p);
+  return TS_OK;
 }
 
 }  // namespace

@@ -21,32 +21,33 @@
 
 namespace ts {
 
+// What the waves of a workgroup read of one chunk: the triangles in one rounding.
 template <typename E, int DK>
-struct ChainLds {
-  static constexpr int PITCH = DK + 16 / (int)sizeof(E);
-  E k[kChunk * PITCH];
-  E q[kChunk * PITCH];
-  E t[kTriElems];
-  E p[kTriElems];
+struct ChainChunk {
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD;
+  E k[kChunk * PITCH], q[kChunk * PITCH], o[kChunk * VP];
+  E t[kTriElems], p[kTriElems];
+  float vec[3 * kChunk];
 };
+template <typename E, int DK>
+constexpr int kChainBufs = 2 * sizeof(ChainChunk<E, DK>) <= kLdsBytes ? 2 : 1;
 
-template <typename E, int DK, int NW>
-__global__ __launch_bounds__(64 * NW) void delta_chain_kernel(DeltaP p) {
+template <typename E, int DK>
+__global__ __launch_bounds__(256) void delta_chain_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef typename Frag<E>::f8 f8;
-  typedef ChainLds<E, DK> Lds;
-  constexpr int PITCH = Lds::PITCH, KB = DK / 16, KS = DK / 32, THREADS = 64 * NW;
-  constexpr int TRI_VECS = kTriElems * (int)sizeof(E) / 16, TRI_SLOTS = (TRI_VECS + THREADS - 1) / THREADS;
+  typedef ChainChunk<E, DK> Chunk;
+  constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32, BUFS = kChainBufs<E, DK>;
   extern __shared__ __align__(16) char smem[];
-  Lds& lds = *(Lds*)smem;
+  Chunk* bufs = (Chunk*)smem;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-  const int col0 = ((int)blockIdx.y * NW + w) * 16, col = col0 + l16;
+  const int base = (int)blockIdx.y * 64, col0 = base + w * 16, col = col0 + l16;
   const bool mine = col0 < p.dvp, on = col < p.dv;
   const int len = delta_len(p, b), chunks = (len + kChunk - 1) / kChunk;
   const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
-  const E* db = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh + col;
+  const E* db = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh + base;
   E* vb = (E*)p.dval.ptr + b * p.dval.sb + h * p.dval.sh + col;
 
   floatx4 S[KB];  // dS
@@ -61,56 +62,40 @@ __global__ __launch_bounds__(64 * NW) void delta_chain_kernel(DeltaP p) {
       }
     }
   }
-  ChunkTile<E, DK, THREADS> kt, qt;
-  uint4 tt[TRI_SLOTS], tp[TRI_SLOTS];
-  E dr[16];  // this wave's columns of dO, rows in accumulator order
-  auto prep_of = [&](int c) { return (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>()); };
+  ChunkTile<E, DK, 256> kt, qt;
+  ChunkTile<E, 64, 256> ot;
+  Linear<E, 256, kTriElems * sizeof(E)> tt, tp;
+  float vv = 0.f;
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
     kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
     qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
-    const uint4* mt = (const uint4*)prep_of(c);
-    const uint4* mp = (const uint4*)(prep_of(c) + TriSets<E>::N * kTriElems);
-#pragma unroll
-    for (int i = 0; i < TRI_SLOTS; ++i) {
-      const int idx = min(tid + i * THREADS, TRI_VECS - 1);
-      tt[i] = mt[idx];
-      tp[i] = mp[idx];
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t0 + 16 * r + 4 * g + i;
-        dr[4 * r + i] = (E)0.0f;
-        if (on && t < len) dr[4 * r + i] = db[(int64_t)t * p.dout.st];
-      }
+    ot.fetch(db, p.dout.st, t0, len, p.dv - base, tid);
+    const E* prep = (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>());
+    tt.fetch(prep, tid);
+    tp.fetch(prep + TriSets<E>::N * kTriElems, tid);
+    vv = ((const float*)(prep + 2 * TriSets<E>::N * kTriElems))[min(tid, 3 * kChunk - 1)];
   };
   if (chunks) fetch(chunks - 1);
   for (int c = chunks - 1; c >= 0; --c) {
     const int t0 = c * kChunk;
     const int64_t n = (int64_t)bh * p.nc + c;
-    const float* vec = (const float*)(prep_of(c) + 2 * TriSets<E>::N * kTriElems);
-    // the last chunk's operands have been read
-    __syncthreads();
+    Chunk& lds = bufs[BUFS == 2 ? c & 1 : 0];
+    if (BUFS == 1) __syncthreads();  // the last chunk has been read
     kt.store(lds.k, PITCH, tid);
     qt.store(lds.q, PITCH, tid);
-#pragma unroll
-    for (int i = 0; i < TRI_SLOTS; ++i) {
-      const int idx = tid + i * THREADS;
-      if (idx < TRI_VECS) {
-        ((uint4*)lds.t)[idx] = tt[i];
-        ((uint4*)lds.p)[idx] = tp[i];
-      }
-    }
-    f8 of[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) of[s][j] = dr[8 * s + j];
+    ot.store(lds.o, VP, tid);
+    tt.store(lds.t, tid);
+    tp.store(lds.p, tid);
+    if (tid < 3 * kChunk) lds.vec[tid] = vv;
     if (c) fetch(c - 1);
+    // this chunk is staged; the other buffer was last read before this barrier
     __syncthreads();
     if (!mine) continue;
+    const float* vec = lds.vec;
+    f8 of[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) of[s] = TokFrag<E>::get(lds.o, VP, 16 * w, s, lane);
 
     E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 4 * g;
 #pragma unroll
@@ -532,12 +517,13 @@ using ts::fail;
 
 template <typename E, int DK>
 int backward(const DeltaP& p, hipStream_t stream) {
-  const int chain = (int)sizeof(ts::ChainLds<E, DK>), grads = (int)sizeof(ts::GradsLds<E, DK>);
-  if (ts::ensure_lds_limit((const void*)ts::delta_chain_kernel<E, DK, 1>, chain) != hipSuccess ||
+  const int chain = (int)sizeof(ts::ChainChunk<E, DK>) * ts::kChainBufs<E, DK>;
+  const int grads = (int)sizeof(ts::GradsLds<E, DK>);
+  if (ts::ensure_lds_limit((const void*)ts::delta_chain_kernel<E, DK>, chain) != hipSuccess ||
       ts::ensure_lds_limit((const void*)ts::delta_grads_kernel<E, DK>, grads) != hipSuccess)
     return fail(TS_ERR_RUNTIME, "delta bwd: LDS of %d bytes", grads);
-  hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK, 1>), dim3((unsigned)(p.B * p.H), (unsigned)(p.dvp / 16)), dim3(64),
-                     chain, stream, p);
+  hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK>), dim3((unsigned)(p.B * p.H), (unsigned)((p.dvp + 63) / 64)),
+                     dim3(256), chain, stream, p);
   hipLaunchKernelGGL((ts::delta_grads_kernel<E, DK>), dim3((unsigned)((int64_t)p.B * p.H * p.nc)), dim3(256), grads,
                      stream, p);
   return TS_OK;
