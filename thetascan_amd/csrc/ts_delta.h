@@ -38,8 +38,10 @@ constexpr int kTriElems = kTri * 64 * 8;
 template <typename E> struct TriSets { static constexpr int N = 1; };
 template <> struct TriSets<bf16> { static constexpr int N = 2; };
 
-// Per chunk, in bytes: the inverse, P, and e^G, e^{G_63 - G}, b (fp32 x 64 each).
-constexpr size_t kVecBytes = 3 * kChunk * sizeof(float);
+// Per chunk, in bytes: the inverse, P, and e^G, e^{G_63 - G}, b (fp32 x 64 each,
+// zero past the length) and e^{G_63}.
+constexpr int kVec = 3 * kChunk + 4;
+constexpr size_t kVecBytes = kVec * sizeof(float);
 template <typename E> __host__ __device__ constexpr size_t prep_bytes() {
   return (size_t)2 * TriSets<E>::N * kTriElems * sizeof(E) + kVecBytes;
 }
@@ -84,6 +86,12 @@ __device__ __forceinline__ typename Frag<E>::f8 zero8() {
 }
 __device__ __forceinline__ floatx4 zero4() { return floatx4{0.f, 0.f, 0.f, 0.f}; }
 
+__device__ __forceinline__ unsigned pack2(float x, float y) {
+  typedef float floatx2 __attribute__((ext_vector_type(2)));
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2{x, y}), bf16x2));
+}
+
 // Accumulators of two 16-row blocks as an operand, in one rounding (hi) and
 // what that leaves (lo): hi + lo holds 16 bits and more.  fp32 keeps everything
 // in hi.
@@ -91,13 +99,18 @@ template <typename E> struct Split;
 template <> struct Split<bf16> {
   bf16x8 hi, lo;
   __device__ __forceinline__ Split(floatx4 a, floatx4 b) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      hi[i] = (bf16)a[i];
-      hi[4 + i] = (bf16)b[i];
-      lo[i] = (bf16)(a[i] - (float)hi[i]);
-      lo[4 + i] = (bf16)(b[i] - (float)hi[4 + i]);
-    }
+    uint4 h, l;
+    two(a[0], a[1], h.x, l.x);
+    two(a[2], a[3], h.y, l.y);
+    two(b[0], b[1], h.z, l.z);
+    two(b[2], b[3], h.w, l.w);
+    hi = __builtin_bit_cast(bf16x8, h);
+    lo = __builtin_bit_cast(bf16x8, l);
+  }
+  // (two elements to a conversion: one at a time takes a conversion each and their packing)
+  static __device__ __forceinline__ void two(float x, float y, unsigned& h, unsigned& l) {
+    h = pack2(x, y);
+    l = pack2(x - __uint_as_float(h << 16), y - __uint_as_float(h & 0xffff0000u));
   }
 };
 template <> struct Split<float> {
@@ -150,36 +163,63 @@ template <> struct TriT<float> {
   }
 };
 
-// A [64 x W] token tile on its way from global memory to LDS rows of pitch W +
-// pad: vector idx = tid + i * threads.  Rows at or past `len` and columns at or
-// past `width` (a multiple of a vector) are zero.
+// A [64 x W] token tile on its way from global memory to LDS rows: vector idx =
+// tid + i * THREADS.  Columns at or past `width` (a multiple of a vector) are
+// zero.  Loads have no branches, so that the wait for them is counted: rows at or
+// past `len` read the last row instead, and what is made of them meets zeros (b,
+// e^G and e^{G_63 - G}, and the rows of the triangles, of tokens past the length).
 template <typename E, int W, int THREADS>
 struct ChunkTile {
   static constexpr int VEC = 16 / (int)sizeof(E);
   static constexpr int PER = W / VEC;
   static constexpr int SLOTS = kChunk * PER / THREADS;
   uint4 r[SLOTS];
-  __device__ __forceinline__ void fetch(const E* base, int64_t st, int t0, int len, int width, int tid) {
+  unsigned off[SLOTS];  // bytes from the chunk's first row (the host checks that they fit)
+  unsigned col[SLOTS];  // those of its column
+  unsigned row_bytes;
+  bool narrow;
+  __device__ __forceinline__ void init(int64_t st, int width, int tid) {
+    row_bytes = (unsigned)(st * (int)sizeof(E));
+    narrow = width < W;
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
-      const int idx = tid + i * THREADS, row = idx / PER, c = (idx % PER) * VEC;
-      r[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (t0 + row < len && c < width) r[i] = *(const uint4*)(base + (int64_t)(t0 + row) * st + c);
+      const int idx = tid + i * THREADS, c = (idx % PER) * VEC;
+      col[i] = c < width ? c * (unsigned)sizeof(E) : 0u;
+      off[i] = (unsigned)(idx / PER) * row_bytes + col[i];
     }
   }
-  __device__ __forceinline__ void store(E* dst, int pitch, int tid) const {
+  __device__ __forceinline__ void fetch(const E* base, int64_t st, int t0, int len) {
+    const char* first = (const char*)(base + (int64_t)t0 * st);
+    const unsigned last = (unsigned)(min(len - t0, kChunk) - 1) * row_bytes;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) r[i] = *(const uint4*)(first + min(off[i], last + col[i]));
+  }
+  __device__ __forceinline__ void store(E* dst, int pitch, int width, int tid) {
+    if (narrow) {  // uniform
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i)
+        if (((tid + i * THREADS) % PER) * VEC >= width) r[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
       const int idx = tid + i * THREADS;
       *(uint4*)(dst + (idx / PER) * pitch + (idx % PER) * VEC) = r[i];
     }
   }
+  // Rows at or past the length zeroed (a kernel that takes its tile on its own).
+  __device__ __forceinline__ void clear(int t0, int len, int tid) {
+    if (t0 + kChunk <= len) return;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i)
+      if (t0 + (tid + i * THREADS) / PER >= len) r[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
 };
 
-// A chunk's record of delta_prepare, copied as it stands.
+// A chunk's record of delta_prepare, copied as it stands (to whole slots).
 template <typename E, int THREADS, size_t BYTES>
 struct Linear {
   static constexpr int VECS = (int)(BYTES / 16), SLOTS = (VECS + THREADS - 1) / THREADS;
+  static constexpr size_t LDS = (size_t)SLOTS * THREADS * 16;
   floatx4 r[SLOTS];
   __device__ __forceinline__ void fetch(const void* src, int tid) {
 #pragma unroll
@@ -187,10 +227,12 @@ struct Linear {
   }
   __device__ __forceinline__ void store(void* dst, int tid) const {
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i)
-      if (tid + i * THREADS < VECS) ((floatx4*)dst)[tid + i * THREADS] = r[i];
+    for (int i = 0; i < SLOTS; ++i) ((floatx4*)dst)[tid + i * THREADS] = r[i];
   }
 };
+
+// Every load so far has landed (counted from here, a loop's waits are for its own).
+__device__ __forceinline__ void loads_landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // Four consecutive rows of column c0 + l16 of an LDS tile, from row r0 + 4g.
 template <typename E>

@@ -99,9 +99,13 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
   E* tri_t = (E*)prep;
   E* tri_p = tri_t + TriSets<E>::N * kTriElems;
   float* vec = (float*)(tri_p + TriSets<E>::N * kTriElems);
-  vec[lane] = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
-  vec[kChunk + lane] = __builtin_amdgcn_exp2f((float)((__shfl(sum, 63, 64) - sum) * kLog2e));
+  const double last = __shfl(sum, 63, 64);
+  const float eg = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
+  const float tail = __builtin_amdgcn_exp2f((float)((last - sum) * kLog2e));
+  vec[lane] = seen ? eg : 0.f;
+  vec[kChunk + lane] = seen ? tail : 0.f;
   vec[2 * kChunk + lane] = beta;
+  if (lane == 63) vec[3 * kChunk] = eg;
   wave_lds_sync();
 
   // K K^T and Q K^T, the lower blocks: column t = l16 of block rt, rows i = 4g.. of block ri
@@ -213,13 +217,13 @@ template <typename E, int DK>
 struct ForwardChunk {
   static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD;
   E k[kChunk * PITCH], q[kChunk * PITCH], v[kChunk * VP];
-  __align__(16) char prep[prep_bytes<E>()];
+  __align__(16) char prep[Linear<E, 256, prep_bytes<E>()>::LDS];
 };
 template <typename E, int DK>
 constexpr int kForwardBufs = 2 * sizeof(ForwardChunk<E, DK>) <= kLdsBytes ? 2 : 1;
 
 template <typename E, int DK, bool KEEP>
-__global__ __launch_bounds__(256) void delta_forward_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef ForwardChunk<E, DK> Chunk;
   constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32, BUFS = kForwardBufs<E, DK>;
@@ -250,24 +254,28 @@ __global__ __launch_bounds__(256) void delta_forward_kernel(DeltaP p) {
   }
   ChunkTile<E, DK, 256> kt, qt;
   ChunkTile<E, 64, 256> vt;
+  kt.init(p.k.st, p.dk, tid);
+  qt.init(p.q.st, p.dk, tid);
+  vt.init(p.v.st, p.dv - base, tid);
   Linear<E, 256, prep_bytes<E>()> pt;
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
-    kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
-    qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
-    vt.fetch(vb, p.v.st, t0, len, p.dv - base, tid);
+    kt.fetch(kb, p.k.st, t0, len);
+    qt.fetch(qb, p.q.st, t0, len);
+    vt.fetch(vb, p.v.st, t0, len);
     pt.fetch(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>(), tid);
   };
   if (chunks) fetch(0);
+  loads_landed();
   for (int c = 0; c < chunks; ++c) {
     const int t0 = c * kChunk;
     Chunk& ch = lds[BUFS == 2 ? c & 1 : 0];
     if (BUFS == 1) __syncthreads();  // the last chunk has been read
-    kt.store(ch.k, PITCH, tid);
-    qt.store(ch.q, PITCH, tid);
-    vt.store(ch.v, VP, tid);
+    kt.store(ch.k, PITCH, p.dk, tid);
+    qt.store(ch.q, PITCH, p.dk, tid);
+    vt.store(ch.v, VP, p.dv - base, tid);
     pt.store(ch.prep, tid);
-    if (c + 1 < chunks) fetch(c + 1);
+    fetch(min(c + 1, chunks - 1));
     // this chunk is staged; the other buffer was last read before this barrier
     __syncthreads();
     if (!mine) continue;
@@ -350,7 +358,7 @@ __global__ __launch_bounds__(256) void delta_forward_kernel(DeltaP p) {
       }
     }
     // S = e^{G_63} S0 + K^T (e^{G_63 - G} U)
-    const float whole = vec[kChunk - 1];
+    const float whole = vec[3 * kChunk];
 #pragma unroll
     for (int d = 0; d < KB; ++d)
 #pragma unroll
@@ -407,6 +415,10 @@ int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const 
   if (!rows(io->q) || !rows(io->k) || !rows(io->v) || !rows(io->out))
     return fail(TS_ERR_VALUE, "%s: q, k, v and out need 16-byte aligned rows", what);
   if (!io->beta.ptr) return fail(TS_ERR_VALUE, "%s: missing beta", what);
+  // (a chunk's rows are addressed in 32 bits from its first)
+  const int64_t reach = ((int64_t)1 << 31) / (ts::kChunk * (16 / vec));
+  for (int64_t st : {io->q.st, io->k.st, io->v.st})
+    if (st < 0 || st >= reach) return fail(TS_ERR_NOT_IMPLEMENTED, "%s: 64 rows must lie within 2 GiB", what);
   p->q = io->q; p->k = io->k; p->v = io->v; p->out = io->out; p->beta = io->beta; p->decay = io->decay;
   p->lengths = io->lengths; p->state = io->state; p->state_out = io->state_out;
   return TS_OK;

@@ -26,14 +26,15 @@ template <typename E, int DK>
 struct ChainChunk {
   static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD;
   E k[kChunk * PITCH], q[kChunk * PITCH], o[kChunk * VP];
-  E t[kTriElems], p[kTriElems];
-  float vec[3 * kChunk];
+  __align__(16) char t[Linear<E, 256, kTriElems * sizeof(E)>::LDS];
+  __align__(16) char p[Linear<E, 256, kTriElems * sizeof(E)>::LDS];
+  float vec[256];
 };
 template <typename E, int DK>
 constexpr int kChainBufs = 2 * sizeof(ChainChunk<E, DK>) <= kLdsBytes ? 2 : 1;
 
 template <typename E, int DK>
-__global__ __launch_bounds__(256) void delta_chain_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef typename Frag<E>::f8 f8;
   typedef ChainChunk<E, DK> Chunk;
@@ -64,31 +65,35 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaP p) {
   }
   ChunkTile<E, DK, 256> kt, qt;
   ChunkTile<E, 64, 256> ot;
+  kt.init(p.k.st, p.dk, tid);
+  qt.init(p.q.st, p.dk, tid);
+  ot.init(p.dout.st, p.dv - base, tid);
   Linear<E, 256, kTriElems * sizeof(E)> tt, tp;
   float vv = 0.f;
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
-    kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
-    qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
-    ot.fetch(db, p.dout.st, t0, len, p.dv - base, tid);
+    kt.fetch(kb, p.k.st, t0, len);
+    qt.fetch(qb, p.q.st, t0, len);
+    ot.fetch(db, p.dout.st, t0, len);
     const E* prep = (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>());
     tt.fetch(prep, tid);
     tp.fetch(prep + TriSets<E>::N * kTriElems, tid);
-    vv = ((const float*)(prep + 2 * TriSets<E>::N * kTriElems))[min(tid, 3 * kChunk - 1)];
+    vv = ((const float*)(prep + 2 * TriSets<E>::N * kTriElems))[min(tid, kVec - 1)];
   };
   if (chunks) fetch(chunks - 1);
+  loads_landed();
   for (int c = chunks - 1; c >= 0; --c) {
     const int t0 = c * kChunk;
     const int64_t n = (int64_t)bh * p.nc + c;
     Chunk& lds = bufs[BUFS == 2 ? c & 1 : 0];
     if (BUFS == 1) __syncthreads();  // the last chunk has been read
-    kt.store(lds.k, PITCH, tid);
-    qt.store(lds.q, PITCH, tid);
-    ot.store(lds.o, VP, tid);
+    kt.store(lds.k, PITCH, p.dk, tid);
+    qt.store(lds.q, PITCH, p.dk, tid);
+    ot.store(lds.o, VP, p.dv - base, tid);
     tt.store(lds.t, tid);
     tp.store(lds.p, tid);
-    if (tid < 3 * kChunk) lds.vec[tid] = vv;
-    if (c) fetch(c - 1);
+    lds.vec[tid] = vv;
+    fetch(max(c - 1, 0));
     // this chunk is staged; the other buffer was last read before this barrier
     __syncthreads();
     if (!mine) continue;
@@ -116,7 +121,7 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaP p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) X[r][i] *= tail[i];
 #pragma unroll
-      for (int s = r / 2; s < 2; ++s) X[r] = mma32(TriT<E>::get(lds.p, r, s, lane), of[s], X[r]);
+      for (int s = r / 2; s < 2; ++s) X[r] = mma32(TriT<E>::get((const E*)lds.p, r, s, lane), of[s], X[r]);
     }
     // dR = Ti^T dU
     floatx4 R[4];
@@ -124,12 +129,12 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaP p) {
       const Split<E> u0(X[0], X[1]), u1(X[2], X[3]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        R[r] = mma_split(TriT<E>::get(lds.t, r, 1, lane), u1, zero4());
-        if (r < 2) R[r] = mma_split(TriT<E>::get(lds.t, r, 0, lane), u0, R[r]);
+        R[r] = mma_split(TriT<E>::get((const E*)lds.t, r, 1, lane), u1, zero4());
+        if (r < 2) R[r] = mma_split(TriT<E>::get((const E*)lds.t, r, 0, lane), u0, R[r]);
       }
     }
     E* dro = (E*)p.dr + (n * p.dvp + col) * kChunk + 4 * g;
-    const float whole = vec[kChunk - 1];
+    const float whole = vec[3 * kChunk];
     float od[16];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -257,14 +262,18 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaP p) {
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
   {
     ChunkTile<E, DK, 256> kt, qt;
-    kt.fetch(kb, p.k.st, t0, len, p.dk, tid);
-    qt.fetch(qb, p.q.st, t0, len, p.dk, tid);
-    kt.store(lds.k, PITCH, tid);
-    qt.store(lds.q, PITCH, tid);
+    kt.init(p.k.st, p.dk, tid);
+    qt.init(p.q.st, p.dk, tid);
+    kt.fetch(kb, p.k.st, t0, len);
+    qt.fetch(qb, p.q.st, t0, len);
+    kt.clear(t0, len, tid);
+    qt.clear(t0, len, tid);
+    kt.store(lds.k, PITCH, p.dk, tid);
+    qt.store(lds.q, PITCH, p.dk, tid);
   }
   const float* vec =
       (const float*)((const E*)(p.prep + n * (int64_t)prep_bytes<E>()) + 2 * TriSets<E>::N * kTriElems);
-  const float eg = vec[t], tail = vec[kChunk + t], be = vec[2 * kChunk + t], whole = vec[kChunk - 1];
+  const float eg = vec[t], tail = vec[kChunk + t], be = vec[2 * kChunk + t], whole = vec[3 * kChunk];
   if (w == 0) {
     double sum = 0.0;
     if (p.decay.ptr && t0 + lane < len) {
@@ -295,8 +304,10 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaP p) {
     __syncthreads();
     {
       ChunkTile<E, VB, 256> ot;
-      ot.fetch(ob + v0, p.dout.st, t0, len, p.dv - v0, tid);
-      ot.store(lds.pass.dout, VP, tid);
+      ot.init(p.dout.st, p.dv - v0, tid);
+      ot.fetch(ob + v0, p.dout.st, t0, len);
+      ot.clear(t0, len, tid);
+      ot.store(lds.pass.dout, VP, p.dv - v0, tid);
     }
     const int rows = p.dvp - v0;
     stage_rows<E, VB, kChunk>((const E*)p.u + (n * p.dvp + v0) * kChunk, rows, lds.pass.u, TP, tid);
@@ -577,6 +588,8 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
   };
   if (!rows(gr->dout, vec) || !rows(gr->dq, 4) || !rows(gr->dk, 4) || !gr->dv.ptr || !gr->dbeta)
     return fail(TS_ERR_VALUE, "delta bwd: missing gradients, or rows that are not aligned");
+  if (gr->dout.st < 0 || gr->dout.st >= ((int64_t)1 << 31) / (64 * (16 / vec)))
+    return fail(TS_ERR_NOT_IMPLEMENTED, "delta bwd: 64 rows must lie within 2 GiB");
   const int64_t chunks = (int64_t)p.B * p.H * p.nc;
   if (chunks > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta bwd: grid too large");
   const size_t es = d->dtype == TS_BF16 ? 2 : 4, dkp = d->dk <= 64 ? 64 : 128;
