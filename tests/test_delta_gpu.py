@@ -377,3 +377,29 @@ def test_compiled_call_is_the_eager_one(cuda, decay):
     for a, b in zip(torch.autograd.grad(out, args, torch.ones_like(out)),
                     torch.autograd.grad(got, args, torch.ones_like(got))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,dk,dv,ragged", [(1024, 64, 64, False), (1537, 64, 40, True), (2200, 128, 72, True)])
+def test_long_sequences_in_segments(cuda, T, dk, dv, ragged, dtype):
+    """Sequences whose chunks are cut into segments that run side by side: their
+    entering states, the lengths that end in any of them, and the gradients behind."""
+    from thetascan_amd._core.ops import delta
+    from thetascan_amd import _lib
+    import ctypes
+
+    s = inputs(4 if ragged else 1, 1, 2, T, dk, dv, dtype, seed=T, state=True)
+    s["decay"] = s["decay"] * 0.05  # (a memory that reaches over the segments)
+    lengths = torch.tensor([T, 0, T // 2 + 3, 64]) if ragged else None
+    one = delta._desc(*(s[n][:1] for n in ("q", "k", "v", "beta", "decay")), False)
+    n, short = ctypes.c_size_t(), ctypes.c_size_t()
+    _lib.load().ts_delta_workspace_bytes(ctypes.byref(one), ctypes.byref(n))
+    per_chunk = n.value / (2 * -(-T // 64))
+    one.T = 64
+    _lib.load().ts_delta_workspace_bytes(ctypes.byref(one), ctypes.byref(short))
+    assert per_chunk > short.value / 2  # segments' states beside the chunks' records
+    if ragged:
+        for b, m in enumerate(lengths.tolist()):
+            for name in ("q", "k", "v", "beta", "decay"):
+                s[name][b, :, m:] = 0.0
+    check(s, cuda, lengths=lengths)

@@ -55,6 +55,10 @@ struct DeltaP {
   const float* state;      // [B,H,dk,dv] or null (zero)
   float* state_out;        // or null
   char* prep;              // [B*H*nc] of prep_bytes
+  int nseg, seg_chunks;    // segments of the chain, chunks of each
+  float* seg_x;            // [B*H*nseg][DK + dvp][DK], by column: X, then N of the transfers
+  float* seg_state;        // [B*H*nseg][dvp][DK], by column: states entering the segments
+                           // (backward: gradients behind them)
   void* u;                 // kept: [B*H*nc][dvp][64]
   void* s0;                // kept: [B*H*nc][dvp][DK]
   // backward
@@ -66,6 +70,7 @@ struct DeltaP {
   float* dstate;            // gradient of the entering state or null
   void* dr;                 // [B*H*nc][dvp][64]
   void* ds;                 // [B*H*nc][dvp][DK]
+  float* seg_n;             // [B*H*nseg][dvp][DK]: N of the backward's transfers
 };
 
 __device__ __forceinline__ int delta_len(const DeltaP& p, int b) {
@@ -252,8 +257,10 @@ __device__ __forceinline__ floatx4 col4<float>(const float* rows, int pitch, int
   return floatx4{a[0], a[pitch], a[2 * pitch], a[3 * pitch]};
 }
 
-constexpr int kLdsBytes = 160 * 1024;
+template <int DK, bool BACK>
+__global__ void delta_segments_kernel(DeltaP p);
 
+int delta_segments(const ts_delta_desc* d);
 int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const char* what);
 
 }  // namespace ts

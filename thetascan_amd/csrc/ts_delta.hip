@@ -212,31 +212,40 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
     }
 }
 
-// What the waves of a workgroup read of one chunk.
-template <typename E, int DK>
+// What the waves of a workgroup read of one chunk (a transfer: no queries).
+template <typename E, int DK, bool TRANSFER>
 struct ForwardChunk {
-  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD;
-  E k[kChunk * PITCH], q[kChunk * PITCH], v[kChunk * VP];
-  __align__(16) char prep[Linear<E, 256, prep_bytes<E>()>::LDS];
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD, SET = TriSets<E>::N * kTriElems;
+  E k[kChunk * PITCH], v[kChunk * VP], t[SET], p[TRANSFER ? 8 : SET], q[TRANSFER ? 8 : kChunk * PITCH];
+  float vec[256];
 };
-template <typename E, int DK>
-constexpr int kForwardBufs = 2 * sizeof(ForwardChunk<E, DK>) <= kLdsBytes ? 2 : 1;
 
-template <typename E, int DK, bool KEEP>
+// kForward: outputs.  kKeep: also U and S0 of every chunk, for the backward.
+// kTransfer: what a segment of chunks makes of its entering state, S -> X S + N:
+// no outputs; column blocks of X (the identity's columns, without values), then of
+// N (a zero state).
+enum { kForward = 0, kKeep = 1, kTransfer = 2 };
+
+template <typename E, int DK, int MODE>
 __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
-  typedef ForwardChunk<E, DK> Chunk;
-  constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32, BUFS = kForwardBufs<E, DK>;
+  constexpr bool TRANSFER = MODE == kTransfer, KEEP = MODE == kKeep;
+  typedef ForwardChunk<E, DK, TRANSFER> Chunk;
+  constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32;
   extern __shared__ __align__(16) char smem[];
-  Chunk* lds = (Chunk*)smem;
+  Chunk& ch = *(Chunk*)smem;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-  const int base = (int)blockIdx.y * 64, col0 = base + w * 16, col = col0 + l16;
-  const bool mine = col0 < p.dvp, on = col < p.dv;  // (a wave past the columns only helps staging)
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, seg = blockIdx.z;
+  const bool unit = TRANSFER && blockIdx.y < DK / 64;  // columns of the identity
+  const int base = ((int)blockIdx.y - (TRANSFER && !unit ? DK / 64 : 0)) * 64, col0 = base + w * 16, col = col0 + l16;
+  const bool mine = unit || col0 < p.dvp, on = unit || col < p.dv;  // (a wave past the columns only helps staging)
   const int len = delta_len(p, b), chunks = (len + kChunk - 1) / kChunk;
+  const int c0 = seg * p.seg_chunks, c1 = min(c0 + p.seg_chunks, chunks);
+  // (no segment enters behind the last; its X is the backward's all the same)
+  if (TRANSFER && (unit && p.u ? c0 >= chunks : c1 >= chunks)) return;
   const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
-  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh + base;
+  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh + (unit ? 0 : base);
   E* ob = (E*)p.out.ptr + b * p.out.sb + h * p.out.sh + col0 + 4 * g;
   const bool out_on = col0 + 4 * g < p.dv;
 
@@ -244,7 +253,13 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
 #pragma unroll
   for (int d = 0; d < KB; ++d) {
     S[d] = zero4();
-    if (p.state && on) {
+    if (TRANSFER) {
+      if (unit)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[d][i] = 16 * d + 4 * g + i == col ? 1.f : 0.f;
+    } else if (seg) {
+      if (mine && c0 < chunks) S[d] = *(const floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 16 * d + 4 * g);
+    } else if (p.state && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = 16 * d + 4 * g + i;
@@ -254,36 +269,44 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
   }
   ChunkTile<E, DK, 256> kt, qt;
   ChunkTile<E, 64, 256> vt;
+  Linear<E, 256, Chunk::SET * sizeof(E)> tt, tp;
+  const int vcols = unit ? 0 : p.dv - base;
+  float vv = 0.f;
   kt.init(p.k.st, p.dk, tid);
   qt.init(p.q.st, p.dk, tid);
-  vt.init(p.v.st, p.dv - base, tid);
-  Linear<E, 256, prep_bytes<E>()> pt;
+  vt.init(p.v.st, vcols, tid);
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
+    const E* prep = (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>());
     kt.fetch(kb, p.k.st, t0, len);
-    qt.fetch(qb, p.q.st, t0, len);
     vt.fetch(vb, p.v.st, t0, len);
-    pt.fetch(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>(), tid);
+    tt.fetch(prep, tid);
+    vv = ((const float*)(prep + 2 * Chunk::SET))[min(tid, kVec - 1)];
+    if (!TRANSFER) {
+      qt.fetch(qb, p.q.st, t0, len);
+      tp.fetch(prep + Chunk::SET, tid);
+    }
   };
-  if (chunks) fetch(0);
+  if (c0 < c1) fetch(c0);
   loads_landed();
-  for (int c = 0; c < chunks; ++c) {
+  for (int c = c0; c < c1; ++c) {
     const int t0 = c * kChunk;
-    Chunk& ch = lds[BUFS == 2 ? c & 1 : 0];
-    if (BUFS == 1) __syncthreads();  // the last chunk has been read
+    __syncthreads();  // the last chunk has been read
     kt.store(ch.k, PITCH, p.dk, tid);
-    qt.store(ch.q, PITCH, p.dk, tid);
-    vt.store(ch.v, VP, p.dv - base, tid);
-    pt.store(ch.prep, tid);
-    fetch(min(c + 1, chunks - 1));
-    // this chunk is staged; the other buffer was last read before this barrier
+    vt.store(ch.v, VP, vcols, tid);
+    tt.store(ch.t, tid);
+    ch.vec[tid] = vv;
+    if (!TRANSFER) {
+      qt.store(ch.q, PITCH, p.dk, tid);
+      tp.store(ch.p, tid);
+    }
+    fetch(min(c + 1, c1 - 1));
     __syncthreads();
     if (!mine) continue;
     const E *ks = ch.k, *qs = ch.q;
     const int64_t n = (int64_t)bh * p.nc + c;
-    const E* tri_t = (const E*)ch.prep;
-    const E* tri_p = tri_t + TriSets<E>::N * kTriElems;
-    const float* vec = (const float*)(tri_p + TriSets<E>::N * kTriElems);
+    const E *tri_t = ch.t, *tri_p = ch.p;
+    const float* vec = ch.vec;
 
     if constexpr (KEEP) {
       E* s0 = (E*)p.s0 + (n * p.dvp + col) * DK + 4 * g;
@@ -326,7 +349,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
       for (int r = 0; r < 4; ++r) IO::st4(u + 16 * r, U[r][0], U[r][1], U[r][2], U[r][3]);
     }
     // O^T = S0^T Q^T e^G + U^T P^T: lane l16 a token, four columns
-    {
+    if constexpr (!TRANSFER) {
       floatx4 O[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) O[r] = zero4();
@@ -377,10 +400,19 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
     }
   }
   if (!mine) return;
-  // tokens behind the length, chunk by chunk (those of its own chunk are written above)
-  for (int t = chunks * kChunk + l16; t < p.T; t += 16)
+  if constexpr (TRANSFER) {
+    float* x = p.seg_x + (((int64_t)bh * p.nseg + seg) * (DK + p.dvp) + (unit ? 0 : DK) + col) * DK + 4 * g;
+#pragma unroll
+    for (int d = 0; d < KB; ++d) *(floatx4*)(x + 16 * d) = S[d];
+    return;
+  }
+  // tokens behind the length (those of its own chunk are written above), by the segment of each
+  const int last = min(p.T, (c0 + p.seg_chunks) * kChunk);
+  for (int t = max(c0, chunks) * kChunk + l16; t < last; t += 16)
     if (out_on) IO::st4(ob + (int64_t)t * p.out.st, 0.f, 0.f, 0.f, 0.f);
-  if (p.state_out && on) {
+  // the segment that holds the last token (the first, where there is none) has the final state
+  const bool final = chunks ? c0 < chunks && c0 + p.seg_chunks >= chunks : seg == 0;
+  if (p.state_out && on && final) {
 #pragma unroll
     for (int d = 0; d < KB; ++d)
 #pragma unroll
@@ -389,6 +421,77 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
         if (row < p.dk) p.state_out[((int64_t)bh * p.dk + row) * p.dv + col] = S[d][i];
       }
   }
+}
+
+// The states entering the segments: S_{s+1} = X_s S_s + N_s, a wave for 16 value
+// columns, on fp32 MFMA.  BACK: dS_s = X_s^T dS_{s+1} + N_s from the last segment
+// that any token reaches.
+template <int DK, bool BACK>
+__global__ __launch_bounds__(64) void delta_segments_kernel(DeltaP p) {
+  constexpr int KB = DK / 16, KS = DK / 32;
+  const int lane = threadIdx.x, l16 = lane & 15, g = lane >> 4;
+  const int bh = blockIdx.x, b = bh / p.H, col = (int)blockIdx.y * 16 + l16;
+  const int chunks = (delta_len(p, b) + kChunk - 1) / kChunk, segs = (chunks + p.seg_chunks - 1) / p.seg_chunks;
+  const float* first = BACK ? p.dstate_out : p.state;
+  floatx4 S[KB];
+#pragma unroll
+  for (int d = 0; d < KB; ++d) {
+    S[d] = zero4();
+    if (first && col < p.dv) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * d + 4 * g + i;
+        if (row < p.dk) S[d][i] = first[((int64_t)bh * p.dk + row) * p.dv + col];
+      }
+    }
+  }
+  for (int k = 0; k + 1 < segs; ++k) {
+    const int s = BACK ? segs - 1 - k : k, to = BACK ? s - 1 : s + 1;
+    const int64_t at = (int64_t)bh * p.nseg + s;
+    const float* x = p.seg_x + at * (DK + p.dvp) * DK;
+    const float* nn = (BACK ? p.seg_n + at * p.dvp * DK : x + DK * DK) + col * DK + 4 * g;
+    floatx4 R[KB];
+#pragma unroll
+    for (int d = 0; d < KB; ++d) R[d] = *(const floatx4*)(nn + 16 * d);
+#pragma unroll
+    for (int e = 0; e < KS; ++e) {
+      const floatx8 sf = __builtin_shufflevector(S[2 * e], S[2 * e + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int d = 0; d < KB; ++d) {
+        floatx8 xf;  // rows 16d + l16, columns in accumulator order; x is [column][row]
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = 16 * d + l16, c = 32 * e + 16 * (j >> 2) + 4 * g + (j & 3);
+          xf[j] = BACK ? x[r * DK + c] : x[c * DK + r];
+        }
+        R[d] = mma32(xf, sf, R[d]);
+      }
+    }
+    float* out = p.seg_state + (((int64_t)bh * p.nseg + to) * p.dvp + col) * DK + 4 * g;
+#pragma unroll
+    for (int d = 0; d < KB; ++d) {
+      S[d] = R[d];
+      *(floatx4*)(out + 16 * d) = R[d];
+    }
+  }
+}
+
+template __global__ void delta_segments_kernel<64, true>(DeltaP);
+template __global__ void delta_segments_kernel<128, true>(DeltaP);
+
+// Segments of a sequence's chunks, one chain each.  A chain's chunks follow one
+// another (about 2.7 us each), so where heads and value columns alone leave CUs
+// without a workgroup, the sequence is cut: every segment but the last first forms
+// what it makes of its entering state (the transfer: dk more columns, no outputs),
+// then the segments run side by side.  Two workgroups a CU, no segment under eight
+// chunks (the cut costs about 12 us and 1.5 us a segment), 32 at most.
+int delta_segments(const ts_delta_desc* d) {
+  const int64_t chains = (int64_t)d->B * d->H * ((d->dv + 63) / 64);
+  const int nc = (d->T + kChunk - 1) / kChunk;
+  int64_t n = 512 / chains;
+  if (n > nc / 8) n = nc / 8;
+  if (n > 32) n = 32;
+  return n < 2 ? 1 : (int)n;
 }
 
 int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const char* what) {
@@ -406,6 +509,8 @@ int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const 
   p->B = d->B; p->Hk = d->Hk; p->H = d->H; p->rep = d->H / d->Hk; p->T = d->T; p->dk = d->dk; p->dv = d->dv;
   p->nc = (d->T + kChunk - 1) / kChunk;
   p->dvp = (d->dv + 15) / 16 * 16;
+  p->nseg = delta_segments(d);
+  p->seg_chunks = (p->nc + p->nseg - 1) / p->nseg;
   p->beta_bf16 = d->beta_dtype == TS_BF16;
   p->decay_bf16 = d->decay_dtype == TS_BF16;
   if (!io) return TS_OK;
@@ -434,32 +539,47 @@ using ts::fail;
 int padded_keys(int dk) { return dk <= 64 ? 64 : 128; }
 
 struct Sizes {
-  size_t prep, u, s0;  // bytes of each part; u and s0 only where kept
+  size_t prep, seg_x, seg_state, u, s0;  // bytes of each part; u and s0 only where kept
+  size_t all(const ts_delta_desc* d) const { return prep + seg_x + seg_state + (d->keep ? u + s0 : 0); }
 };
 Sizes sizes(const ts_delta_desc* d) {
   const size_t es = d->dtype == TS_BF16 ? 2 : 4;
   const size_t n = (size_t)d->B * d->H * ((d->T + 63) / 64), dvp = (d->dv + 15) / 16 * 16;
   Sizes s;
   s.prep = n * (d->dtype == TS_BF16 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>());
+  const size_t seg = (size_t)d->B * d->H * ts::delta_segments(d), dkp = padded_keys(d->dk);
+  s.seg_x = s.seg_state = 0;
+  if (ts::delta_segments(d) > 1) {
+    s.seg_x = seg * (dkp + dvp) * dkp * sizeof(float);
+    s.seg_state = seg * dvp * dkp * sizeof(float);
+  }
   s.u = n * dvp * 64 * es;
   s.s0 = n * dvp * padded_keys(d->dk) * es;
   return s;
 }
 
+template <typename E, int DK, int MODE>
+int launch(const DeltaP& p, unsigned columns, hipStream_t stream) {
+  const int lds = (int)sizeof(ts::ForwardChunk<E, DK, MODE == ts::kTransfer>);
+  if (ts::ensure_lds_limit((const void*)ts::delta_forward_kernel<E, DK, MODE>, lds) != hipSuccess)
+    return fail(TS_ERR_RUNTIME, "delta: LDS of %d bytes", lds);
+  hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, MODE>), dim3((unsigned)(p.B * p.H), columns, (unsigned)p.nseg),
+                     dim3(256), lds, stream, p);
+  return TS_OK;
+}
+
 template <typename E, int DK>
 int forward(const DeltaP& p, hipStream_t stream) {
   const int64_t n = (int64_t)p.B * p.H * p.nc;
-  const int lds = (int)sizeof(ts::ForwardChunk<E, DK>) * ts::kForwardBufs<E, DK>;
-  const void* fn = p.u ? (const void*)ts::delta_forward_kernel<E, DK, true>
-                       : (const void*)ts::delta_forward_kernel<E, DK, false>;
-  if (ts::ensure_lds_limit(fn, lds) != hipSuccess) return fail(TS_ERR_RUNTIME, "delta: LDS of %d bytes", lds);
   hipLaunchKernelGGL((ts::delta_prepare_kernel<E, DK>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, p);
-  const dim3 grid((unsigned)(p.B * p.H), (unsigned)((p.dvp + 63) / 64));
-  if (p.u)
-    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, true>), grid, dim3(256), lds, stream, p);
-  else
-    hipLaunchKernelGGL((ts::delta_forward_kernel<E, DK, false>), grid, dim3(256), lds, stream, p);
-  return TS_OK;
+  const unsigned columns = (unsigned)((p.dvp + 63) / 64);
+  if (p.nseg > 1) {
+    const int rc = launch<E, DK, ts::kTransfer>(p, columns + DK / 64, stream);
+    if (rc) return rc;
+    hipLaunchKernelGGL((ts::delta_segments_kernel<DK, false>), dim3((unsigned)(p.B * p.H), (unsigned)(p.dvp / 16)),
+                       dim3(64), 0, stream, p);
+  }
+  return p.u ? launch<E, DK, ts::kKeep>(p, columns, stream) : launch<E, DK, ts::kForward>(p, columns, stream);
 }
 
 }  // namespace
@@ -470,7 +590,7 @@ int ts_delta_workspace_bytes(const ts_delta_desc* d, size_t* bytes) {
   const int rc = ts::delta_check(d, nullptr, nullptr, "delta");
   if (rc) return rc;
   const Sizes s = sizes(d);
-  if (bytes) *bytes = s.prep + (d->keep ? s.u + s.s0 : 0);
+  if (bytes) *bytes = s.all(d);
   return TS_OK;
 }
 
@@ -482,13 +602,15 @@ int ts_delta_fwd(const ts_delta_desc* d, const ts_delta_io* io, void* workspace,
   if (rc) return rc;
   if (d->T == 0) return TS_OK;
   const Sizes s = sizes(d);
-  if (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < s.prep + (d->keep ? s.u + s.s0 : 0))
+  if (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < s.all(d))
     return fail(TS_ERR_VALUE, "delta: the workspace is missing, misaligned or too small");
   if (((int64_t)p.B * p.H * p.nc + 3) / 4 > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta: grid too large");
   p.prep = (char*)workspace;
+  p.seg_x = (float*)(p.prep + s.prep);
+  p.seg_state = (float*)(p.prep + s.prep + s.seg_x);
   if (d->keep) {
-    p.u = p.prep + s.prep;
-    p.s0 = p.prep + s.prep + s.u;
+    p.u = p.prep + s.prep + s.seg_x + s.seg_state;
+    p.s0 = (char*)p.u + s.u;
   }
   const bool narrow = d->dk <= 64;
   int rc2;

@@ -30,22 +30,26 @@ struct ChainChunk {
   __align__(16) char p[Linear<E, 256, kTriElems * sizeof(E)>::LDS];
   float vec[256];
 };
-template <typename E, int DK>
-constexpr int kChainBufs = 2 * sizeof(ChainChunk<E, DK>) <= kLdsBytes ? 2 : 1;
-
-template <typename E, int DK>
+// TRANSFER: what a segment of chunks adds to the gradient behind it, from its
+// tokens alone (X^T of the forward's transfer makes the rest): nothing is stored
+// but that.
+template <typename E, int DK, bool TRANSFER>
 __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef typename Frag<E>::f8 f8;
   typedef ChainChunk<E, DK> Chunk;
-  constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32, BUFS = kChainBufs<E, DK>;
+  constexpr int PITCH = Chunk::PITCH, VP = Chunk::VP, KB = DK / 16, KS = DK / 32;
   extern __shared__ __align__(16) char smem[];
-  Chunk* bufs = (Chunk*)smem;
+  Chunk& lds = *(Chunk*)smem;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, seg = blockIdx.z;
   const int base = (int)blockIdx.y * 64, col0 = base + w * 16, col = col0 + l16;
   const bool mine = col0 < p.dvp, on = col < p.dv;
   const int len = delta_len(p, b), chunks = (len + kChunk - 1) / kChunk;
+  const int c0 = seg * p.seg_chunks, c1 = min(c0 + p.seg_chunks, chunks);
+  if (TRANSFER && (seg == 0 || c0 >= chunks)) return;  // (nothing is behind it to hand it on to)
+  // the segment of the last token (the first, where there is none) starts from the final state's gradient
+  const bool final = chunks ? c0 < chunks && c0 + p.seg_chunks >= chunks : seg == 0;
   const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
   const E* db = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh + base;
@@ -55,7 +59,11 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
 #pragma unroll
   for (int d = 0; d < KB; ++d) {
     S[d] = zero4();
-    if (p.dstate_out && on) {
+    if (TRANSFER) continue;
+    if (!final) {
+      if (mine && c0 < chunks)
+        S[d] = *(const floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 16 * d + 4 * g);
+    } else if (p.dstate_out && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = 16 * d + 4 * g + i;
@@ -80,21 +88,19 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
     tp.fetch(prep + TriSets<E>::N * kTriElems, tid);
     vv = ((const float*)(prep + 2 * TriSets<E>::N * kTriElems))[min(tid, kVec - 1)];
   };
-  if (chunks) fetch(chunks - 1);
+  if (c0 < c1) fetch(c1 - 1);
   loads_landed();
-  for (int c = chunks - 1; c >= 0; --c) {
+  for (int c = c1 - 1; c >= c0; --c) {
     const int t0 = c * kChunk;
     const int64_t n = (int64_t)bh * p.nc + c;
-    Chunk& lds = bufs[BUFS == 2 ? c & 1 : 0];
-    if (BUFS == 1) __syncthreads();  // the last chunk has been read
+    __syncthreads();  // the last chunk has been read
     kt.store(lds.k, PITCH, p.dk, tid);
     qt.store(lds.q, PITCH, p.dk, tid);
     ot.store(lds.o, VP, p.dv - base, tid);
     tt.store(lds.t, tid);
     tp.store(lds.p, tid);
     lds.vec[tid] = vv;
-    fetch(max(c - 1, 0));
-    // this chunk is staged; the other buffer was last read before this barrier
+    fetch(max(c - 1, c0));
     __syncthreads();
     if (!mine) continue;
     const float* vec = lds.vec;
@@ -102,9 +108,11 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) of[s] = TokFrag<E>::get(lds.o, VP, 16 * w, s, lane);
 
-    E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 4 * g;
+    if constexpr (!TRANSFER) {
+      E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 4 * g;
 #pragma unroll
-    for (int d = 0; d < KB; ++d) IO::st4(ds + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
+      for (int d = 0; d < KB; ++d) IO::st4(ds + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
+    }
     // dU = P^T dO + e^{G_63 - G} K dS
     floatx4 X[4];
 #pragma unroll
@@ -138,14 +146,14 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
     float od[16];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      IO::st4(dro + 16 * r, R[r][0], R[r][1], R[r][2], R[r][3]);
+      if constexpr (!TRANSFER) IO::st4(dro + 16 * r, R[r][0], R[r][1], R[r][2], R[r][3]);
       const floatx4 eg = *(const floatx4*)(vec + 16 * r + 4 * g);
       const floatx4 be = *(const floatx4*)(vec + 2 * kChunk + 16 * r + 4 * g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = t0 + 16 * r + 4 * g + i;
         const float dv = be[i] * R[r][i];
-        if (t < p.T && on) vb[(int64_t)t * p.dval.st] = cvt<E>(t < len ? dv : 0.f);
+        if (!TRANSFER && t < p.T && on) vb[(int64_t)t * p.dval.st] = cvt<E>(t < len ? dv : 0.f);
         R[r][i] = -eg[i] * dv;
         od[4 * r + i] = eg[i] * tof(of[r / 2][4 * (r & 1) + i]);
       }
@@ -168,9 +176,16 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
     }
   }
   if (!mine) return;
+  if constexpr (TRANSFER) {
+    float* nn = p.seg_n + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 4 * g;
+#pragma unroll
+    for (int d = 0; d < KB; ++d) *(floatx4*)(nn + 16 * d) = S[d];
+    return;
+  }
+  const int last = min(p.T, (c0 + p.seg_chunks) * kChunk);
   if (on)
-    for (int t = chunks * kChunk + g; t < p.T; t += 4) vb[(int64_t)t * p.dval.st] = (E)0.0f;
-  if (p.dstate && on) {
+    for (int t = max(c0, chunks) * kChunk + g; t < last; t += 4) vb[(int64_t)t * p.dval.st] = (E)0.0f;
+  if (p.dstate && on && seg == 0) {
 #pragma unroll
     for (int d = 0; d < KB; ++d)
 #pragma unroll
@@ -528,13 +543,18 @@ using ts::fail;
 
 template <typename E, int DK>
 int backward(const DeltaP& p, hipStream_t stream) {
-  const int chain = (int)sizeof(ts::ChainChunk<E, DK>) * ts::kChainBufs<E, DK>;
-  const int grads = (int)sizeof(ts::GradsLds<E, DK>);
-  if (ts::ensure_lds_limit((const void*)ts::delta_chain_kernel<E, DK>, chain) != hipSuccess ||
+  const int chain = (int)sizeof(ts::ChainChunk<E, DK>), grads = (int)sizeof(ts::GradsLds<E, DK>);
+  if (ts::ensure_lds_limit((const void*)ts::delta_chain_kernel<E, DK, false>, chain) != hipSuccess ||
+      ts::ensure_lds_limit((const void*)ts::delta_chain_kernel<E, DK, true>, chain) != hipSuccess ||
       ts::ensure_lds_limit((const void*)ts::delta_grads_kernel<E, DK>, grads) != hipSuccess)
     return fail(TS_ERR_RUNTIME, "delta bwd: LDS of %d bytes", grads);
-  hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK>), dim3((unsigned)(p.B * p.H), (unsigned)((p.dvp + 63) / 64)),
-                     dim3(256), chain, stream, p);
+  const dim3 grid((unsigned)(p.B * p.H), (unsigned)((p.dvp + 63) / 64), (unsigned)p.nseg);
+  if (p.nseg > 1) {
+    hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK, true>), grid, dim3(256), chain, stream, p);
+    hipLaunchKernelGGL((ts::delta_segments_kernel<DK, true>), dim3((unsigned)(p.B * p.H), (unsigned)(p.dvp / 16)),
+                       dim3(64), 0, stream, p);
+  }
+  hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK, false>), grid, dim3(256), chain, stream, p);
   hipLaunchKernelGGL((ts::delta_grads_kernel<E, DK>), dim3((unsigned)((int64_t)p.B * p.H * p.nc)), dim3(256), grads,
                      stream, p);
   return TS_OK;
@@ -559,7 +579,9 @@ int ts_delta_bwd_workspace_bytes(const ts_delta_desc* d, size_t* bytes) {
   if (rc) return rc;
   const size_t es = d->dtype == TS_BF16 ? 2 : 4;
   const size_t n = (size_t)d->B * d->H * ((d->T + 63) / 64), dvp = (d->dv + 15) / 16 * 16;
-  size_t total = n * dvp * (64 + (d->dk <= 64 ? 64 : 128)) * es;
+  const size_t dkp = d->dk <= 64 ? 64 : 128, nseg = ts::delta_segments(d);
+  size_t total = n * dvp * (64 + dkp) * es;
+  if (nseg > 1) total += 2 * (size_t)d->B * d->H * nseg * dvp * dkp * sizeof(float);
   if (d->H != d->Hk) total += align16(2 * (size_t)d->B * d->H * d->T * d->dk * sizeof(float));
   if (bytes) *bytes = total + align16((size_t)d->B * d->H * d->T * sizeof(float));
   return TS_OK;
@@ -601,6 +623,14 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
   p.dr = ws;
   p.ds = ws + u;
   ws += u + s0;
+  if (p.nseg > 1) {
+    // X of the forward's transfers, which follow its chunks' records
+    const size_t states = (size_t)p.B * p.H * p.nseg * p.dvp * dkp * sizeof(float);
+    p.seg_x = (float*)((char*)saved + chunks * (int64_t)(es == 2 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>()));
+    p.seg_state = (float*)ws;
+    p.seg_n = (float*)(ws + states);
+    ws += 2 * states;
+  }
   p.dout = gr->dout; p.dval = gr->dv; p.dq = gr->dq; p.dkey = gr->dk;
   p.dbeta = gr->dbeta; p.ddecay = gr->ddecay; p.ddecay_bf16 = p.decay_bf16;
   p.dstate_out = gr->dstate_out; p.dstate = gr->dstate;
