@@ -423,56 +423,61 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
   }
 }
 
-// The states entering the segments: S_{s+1} = X_s S_s + N_s, a wave for 16 value
-// columns, on fp32 MFMA.  BACK: dS_s = X_s^T dS_{s+1} + N_s from the last segment
-// that any token reaches.
+// The states entering the segments: S_{s+1} = X_s S_s + N_s for 16 value columns,
+// a wave for every 16 rows, on fp32 MFMA.  BACK: dS_s = X_s^T dS_{s+1} + N_s from
+// the last segment that any token reaches.  A step needs the whole state of the one
+// before (through LDS); its matrices are loaded a step ahead.
 template <int DK, bool BACK>
-__global__ __launch_bounds__(64) void delta_segments_kernel(DeltaP p) {
-  constexpr int KB = DK / 16, KS = DK / 32;
-  const int lane = threadIdx.x, l16 = lane & 15, g = lane >> 4;
+__global__ __launch_bounds__(4 * DK, 1) void delta_segments_kernel(DeltaP p) {
+  constexpr int KS = DK / 32, PITCH = DK + 4;
+  __shared__ __align__(16) float state[2][16 * PITCH];  // [column][row]
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.H, col = (int)blockIdx.y * 16 + l16;
   const int chunks = (delta_len(p, b) + kChunk - 1) / kChunk, segs = (chunks + p.seg_chunks - 1) / p.seg_chunks;
   const float* first = BACK ? p.dstate_out : p.state;
-  floatx4 S[KB];
+  floatx4 S = zero4();  // rows 16w + 4g ..
+  if (first && col < p.dv) {
 #pragma unroll
-  for (int d = 0; d < KB; ++d) {
-    S[d] = zero4();
-    if (first && col < p.dv) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * d + 4 * g + i;
-        if (row < p.dk) S[d][i] = first[((int64_t)bh * p.dk + row) * p.dv + col];
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * w + 4 * g + i;
+      if (row < p.dk) S[i] = first[((int64_t)bh * p.dk + row) * p.dv + col];
     }
   }
-  for (int k = 0; k + 1 < segs; ++k) {
-    const int s = BACK ? segs - 1 - k : k, to = BACK ? s - 1 : s + 1;
+  const int steps = segs - 1, r = 16 * w + l16;
+  floatx8 xf[KS], xn[KS];  // row r, columns in accumulator order; X is stored [column][row]
+  floatx4 nf, nn;
+  auto load = [&](int k, floatx8* x8, floatx4& n4) {
+    const int s = BACK ? segs - 1 - k : k;
     const int64_t at = (int64_t)bh * p.nseg + s;
     const float* x = p.seg_x + at * (DK + p.dvp) * DK;
-    const float* nn = (BACK ? p.seg_n + at * p.dvp * DK : x + DK * DK) + col * DK + 4 * g;
-    floatx4 R[KB];
-#pragma unroll
-    for (int d = 0; d < KB; ++d) R[d] = *(const floatx4*)(nn + 16 * d);
+    n4 = *(const floatx4*)((BACK ? p.seg_n + at * p.dvp * DK : x + DK * DK) + col * DK + 16 * w + 4 * g);
 #pragma unroll
     for (int e = 0; e < KS; ++e) {
-      const floatx8 sf = __builtin_shufflevector(S[2 * e], S[2 * e + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+      if (BACK) {
+        const floatx4 lo = *(const floatx4*)(x + r * DK + 32 * e + 4 * g);
+        const floatx4 hi = *(const floatx4*)(x + r * DK + 32 * e + 16 + 4 * g);
+        x8[e] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
 #pragma unroll
-      for (int d = 0; d < KB; ++d) {
-        floatx8 xf;  // rows 16d + l16, columns in accumulator order; x is [column][row]
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = 16 * d + l16, c = 32 * e + 16 * (j >> 2) + 4 * g + (j & 3);
-          xf[j] = BACK ? x[r * DK + c] : x[c * DK + r];
-        }
-        R[d] = mma32(xf, sf, R[d]);
+        for (int j = 0; j < 8; ++j) x8[e][j] = x[(32 * e + 16 * (j >> 2) + 4 * g + (j & 3)) * DK + r];
       }
     }
-    float* out = p.seg_state + (((int64_t)bh * p.nseg + to) * p.dvp + col) * DK + 4 * g;
+  };
+  if (steps > 0) load(0, xf, nf);
+  loads_landed();
+  for (int k = 0; k < steps; ++k) {
+    load(min(k + 1, steps - 1), xn, nn);
+    float* st = state[k & 1];
+    *(floatx4*)(st + l16 * PITCH + 16 * w + 4 * g) = S;
+    __syncthreads();
+    S = nf;
 #pragma unroll
-    for (int d = 0; d < KB; ++d) {
-      S[d] = R[d];
-      *(floatx4*)(out + 16 * d) = R[d];
-    }
+    for (int e = 0; e < KS; ++e) S = mma32(xf[e], row_perm<float>(st + l16 * PITCH, e, g), S);
+    const int to = BACK ? segs - 2 - k : k + 1;
+    *(floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + to) * p.dvp + col) * DK + 16 * w + 4 * g) = S;
+    nf = nn;
+#pragma unroll
+    for (int e = 0; e < KS; ++e) xf[e] = xn[e];
   }
 }
 
@@ -577,7 +582,7 @@ int forward(const DeltaP& p, hipStream_t stream) {
     const int rc = launch<E, DK, ts::kTransfer>(p, columns + DK / 64, stream);
     if (rc) return rc;
     hipLaunchKernelGGL((ts::delta_segments_kernel<DK, false>), dim3((unsigned)(p.B * p.H), (unsigned)(p.dvp / 16)),
-                       dim3(64), 0, stream, p);
+                       dim3(4 * DK), 0, stream, p);
   }
   return p.u ? launch<E, DK, ts::kKeep>(p, columns, stream) : launch<E, DK, ts::kForward>(p, columns, stream);
 }

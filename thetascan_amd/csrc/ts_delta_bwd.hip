@@ -217,21 +217,47 @@ struct GradsLds {
   float cols[4][kChunk], base[kChunk], f[kChunk], red[4];
 };
 
-// [rows x W] contiguous rows -> LDS; rows at or past `rows` are zero.
+// [ROWS x W] contiguous rows on their way to LDS; rows at or past `rows` are zero.
 template <typename E, int ROWS, int W>
-__device__ __forceinline__ void stage_rows(const E* src, int rows, E* dst, int pitch, int tid) {
-  constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC;
+struct Block {
+  static constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC, SLOTS = ROWS * PER / 256;
+  uint4 r[SLOTS];
+  __device__ __forceinline__ void fetch(const E* src, int rows, int tid) {
 #pragma unroll
-  for (int i = 0; i < ROWS * PER / 256; ++i) {
-    const int idx = tid + i * 256, row = idx / PER, c = (idx % PER) * VEC;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (row < rows) v = *(const uint4*)(src + row * W + c);
-    *(uint4*)(dst + row * pitch + c) = v;
+    for (int i = 0; i < SLOTS; ++i) {
+      const int idx = tid + i * 256;
+      r[i] = *(const uint4*)(src + min(idx / PER, rows - 1) * W + (idx % PER) * VEC);
+    }
   }
-}
+  __device__ __forceinline__ void store(E* dst, int rows, int pitch, int tid) {
+    if (rows < ROWS) {  // uniform
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i)
+        if ((tid + i * 256) / PER >= rows) r[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int idx = tid + i * 256;
+      *(uint4*)(dst + (idx / PER) * pitch + (idx % PER) * VEC) = r[i];
+    }
+  }
+  // Sum of the products with another block's entries of the same places.
+  __device__ __forceinline__ float dot(const Block& o) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      Vec16<E> a, b;
+      a.raw = r[i];
+      b.raw = o.r[i];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum = fmaf(tof(a.e[j]), tof(b.e[j]), sum);
+    }
+    return sum;
+  }
+};
 
 template <typename E, int DK>
-__global__ __launch_bounds__(256) void delta_grads_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef TokFrag<E> TF;
   typedef typename Frag<E>::f8 f8;
@@ -275,17 +301,27 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaP p) {
   }
   const E* kb = (const E*)p.k.ptr + b * p.k.sb + (h / p.rep) * p.k.sh;
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
-  {
-    ChunkTile<E, DK, 256> kt, qt;
-    kt.init(p.k.st, p.dk, tid);
-    qt.init(p.q.st, p.dk, tid);
-    kt.fetch(kb, p.k.st, t0, len);
-    qt.fetch(qb, p.q.st, t0, len);
-    kt.clear(t0, len, tid);
-    qt.clear(t0, len, tid);
-    kt.store(lds.k, PITCH, p.dk, tid);
-    qt.store(lds.q, PITCH, p.dk, tid);
-  }
+  // every row of the first pass on its way at once
+  ChunkTile<E, DK, 256> kt, qt;
+  ChunkTile<E, VB, 256> ot;
+  Block<E, VB, kChunk> ut, rt;
+  Block<E, VB, DK> st, dt;
+  const E* ob = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh;
+  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh;
+  auto fetch = [&](int v0) {
+    const int rows = p.dvp - v0;
+    ot.init(p.dout.st, p.dv - v0, tid);
+    ot.fetch(ob + v0, p.dout.st, t0, len);
+    ut.fetch((const E*)p.u + (n * p.dvp + v0) * kChunk, rows, tid);
+    rt.fetch((const E*)p.dr + (n * p.dvp + v0) * kChunk, rows, tid);
+    st.fetch((const E*)p.s0 + (n * p.dvp + v0) * DK, rows, tid);
+    dt.fetch((const E*)p.ds + (n * p.dvp + v0) * DK, rows, tid);
+  };
+  kt.init(p.k.st, p.dk, tid);
+  qt.init(p.q.st, p.dk, tid);
+  kt.fetch(kb, p.k.st, t0, len);
+  qt.fetch(qb, p.q.st, t0, len);
+  fetch(0);
   const float* vec =
       (const float*)((const E*)(p.prep + n * (int64_t)prep_bytes<E>()) + 2 * TriSets<E>::N * kTriElems);
   const float eg = vec[t], tail = vec[kChunk + t], be = vec[2 * kChunk + t], whole = vec[3 * kChunk];
@@ -313,31 +349,24 @@ __global__ __launch_bounds__(256) void delta_grads_kernel(DeltaP p) {
 #pragma unroll
   for (int d = 0; d < KB; ++d) z[d] = y[d] = fu[d] = zero4();
   float inner = 0.f;  // this thread's part of <S0, dS>
-  const E* ob = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh;
-  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh;
+  kt.clear(t0, len, tid);
+  qt.clear(t0, len, tid);
+  kt.store(lds.k, PITCH, p.dk, tid);
+  qt.store(lds.q, PITCH, p.dk, tid);
   for (int v0 = 0; v0 < p.dvp; v0 += VB) {
-    __syncthreads();
-    {
-      ChunkTile<E, VB, 256> ot;
-      ot.init(p.dout.st, p.dv - v0, tid);
-      ot.fetch(ob + v0, p.dout.st, t0, len);
-      ot.clear(t0, len, tid);
-      ot.store(lds.pass.dout, VP, p.dv - v0, tid);
+    if (v0) {
+      __syncthreads();  // the last pass has been read
+      fetch(v0);
     }
     const int rows = p.dvp - v0;
-    stage_rows<E, VB, kChunk>((const E*)p.u + (n * p.dvp + v0) * kChunk, rows, lds.pass.u, TP, tid);
-    stage_rows<E, VB, kChunk>((const E*)p.dr + (n * p.dvp + v0) * kChunk, rows, lds.pass.dr, TP, tid);
-    stage_rows<E, VB, DK>((const E*)p.s0 + (n * p.dvp + v0) * DK, rows, lds.pass.s0, PITCH, tid);
-    stage_rows<E, VB, DK>((const E*)p.ds + (n * p.dvp + v0) * DK, rows, lds.pass.ds, PITCH, tid);
+    ot.clear(t0, len, tid);
+    ot.store(lds.pass.dout, VP, p.dv - v0, tid);
+    ut.store(lds.pass.u, rows, TP, tid);
+    rt.store(lds.pass.dr, rows, TP, tid);
+    st.store(lds.pass.s0, rows, PITCH, tid);
+    dt.store(lds.pass.ds, rows, PITCH, tid);
+    inner += st.dot(dt);
     __syncthreads();
-    for (int i = tid; i < VB * DK / 4; i += 256) {
-      const int row = i / (DK / 4), cc = (i % (DK / 4)) * 4;
-      float a[4], bb[4];
-      ld4f<E>(lds.pass.s0 + row * PITCH + cc, a);
-      ld4f<E>(lds.pass.ds + row * PITCH + cc, bb);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) inner = fmaf(a[e], bb[e], inner);
-    }
 #pragma unroll
     for (int s = 0; s < VB / 32; ++s) {
       const f8 of = row_perm<E>(lds.pass.dout + t * VP, s, g);
@@ -552,7 +581,7 @@ int backward(const DeltaP& p, hipStream_t stream) {
   if (p.nseg > 1) {
     hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK, true>), grid, dim3(256), chain, stream, p);
     hipLaunchKernelGGL((ts::delta_segments_kernel<DK, true>), dim3((unsigned)(p.B * p.H), (unsigned)(p.dvp / 16)),
-                       dim3(64), 0, stream, p);
+                       dim3(4 * DK), 0, stream, p);
   }
   hipLaunchKernelGGL((ts::delta_chain_kernel<E, DK, false>), grid, dim3(256), chain, stream, p);
   hipLaunchKernelGGL((ts::delta_grads_kernel<E, DK>), dim3((unsigned)((int64_t)p.B * p.H * p.nc)), dim3(256), grads,
