@@ -201,21 +201,36 @@ template <typename E> constexpr int kGradCols = sizeof(E) == 2 ? 64 : 32;
 
 template <typename E, int DK>
 struct GradsLds {
-  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VB = kGradCols<E>, VP = VB + PAD, TP = kChunk + PAD;
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VB = kGradCols<E>, TP = kChunk + PAD;
   struct Pass {
-    E dout[kChunk * VP], u[VB * TP], dr[VB * TP], s0[VB * PITCH], ds[VB * PITCH];
+    E u[VB * TP], dr[VB * TP], s0[VB * PITCH], ds[VB * PITCH];
   };
   struct Pairs {
-    E a[kChunk * TP], m[kChunk * TP];
+    E k[kChunk * PITCH], q[kChunk * PITCH], a[kChunk * TP], m[kChunk * TP];
   };
-  E k[kChunk * PITCH], q[kChunk * PITCH];
-  union {
+  union {  // the passes over the value columns, then the pairs of tokens
     Pass pass;
     Pairs pairs;
   };
   double G[kChunk];
   float cols[4][kChunk], base[kChunk], f[kChunk], red[4];
 };
+
+// Eight columns of a global row in accumulator order (c.., c + 16..), zero at or
+// past `width` and where the row is none.
+template <typename E>
+__device__ __forceinline__ typename Frag<E>::f8 row_global(const E* row, int c, int width, bool on) {
+  typename Frag<E>::f4 part[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool in = c + 16 * i < width;
+    part[i] = LdsIO<E>::ld4(row + (in ? c + 16 * i : 0));
+    if (!(in && on))
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[i][j] = (E)0.0f;
+  }
+  return LdsIO<E>::cat(part[0], part[1]);
+}
 
 // [ROWS x W] contiguous rows on their way to LDS; rows at or past `rows` are zero.
 template <typename E, int ROWS, int W>
@@ -257,12 +272,12 @@ struct Block {
 };
 
 template <typename E, int DK>
-__global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void delta_grads_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef TokFrag<E> TF;
   typedef typename Frag<E>::f8 f8;
   typedef GradsLds<E, DK> Lds;
-  constexpr int PITCH = Lds::PITCH, VB = Lds::VB, VP = Lds::VP, TP = Lds::TP, KB = DK / 16, KS = DK / 32;
+  constexpr int PITCH = Lds::PITCH, VB = Lds::VB, TP = Lds::TP, KB = DK / 16, KS = DK / 32;
   extern __shared__ __align__(16) char smem[];
   Lds& lds = *(Lds*)smem;
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -303,15 +318,15 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
   const E* qb = (const E*)p.q.ptr + b * p.q.sb + (h / p.rep) * p.q.sh;
   // every row of the first pass on its way at once
   ChunkTile<E, DK, 256> kt, qt;
-  ChunkTile<E, VB, 256> ot;
   Block<E, VB, kChunk> ut, rt;
   Block<E, VB, DK> st, dt;
-  const E* ob = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh;
-  const E* vb = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh;
+  f8 of[VB / 32];  // this wave's rows of dO
+  const E* orow = (const E*)p.dout.ptr + b * p.dout.sb + h * p.dout.sh + (int64_t)min(t0 + t, len - 1) * p.dout.st;
+  const E* vrow = (const E*)p.v.ptr + b * p.v.sb + h * p.v.sh + (int64_t)min(t0 + t, len - 1) * p.v.st;
   auto fetch = [&](int v0) {
     const int rows = p.dvp - v0;
-    ot.init(p.dout.st, p.dv - v0, tid);
-    ot.fetch(ob + v0, p.dout.st, t0, len);
+#pragma unroll
+    for (int s = 0; s < VB / 32; ++s) of[s] = row_global<E>(orow, v0 + 32 * s + 4 * g, p.dv, t0 + t < len);
     ut.fetch((const E*)p.u + (n * p.dvp + v0) * kChunk, rows, tid);
     rt.fetch((const E*)p.dr + (n * p.dvp + v0) * kChunk, rows, tid);
     st.fetch((const E*)p.s0 + (n * p.dvp + v0) * DK, rows, tid);
@@ -351,16 +366,12 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
   float inner = 0.f;  // this thread's part of <S0, dS>
   kt.clear(t0, len, tid);
   qt.clear(t0, len, tid);
-  kt.store(lds.k, PITCH, p.dk, tid);
-  qt.store(lds.q, PITCH, p.dk, tid);
   for (int v0 = 0; v0 < p.dvp; v0 += VB) {
     if (v0) {
       __syncthreads();  // the last pass has been read
       fetch(v0);
     }
     const int rows = p.dvp - v0;
-    ot.clear(t0, len, tid);
-    ot.store(lds.pass.dout, VP, p.dv - v0, tid);
     ut.store(lds.pass.u, rows, TP, tid);
     rt.store(lds.pass.dr, rows, TP, tid);
     st.store(lds.pass.s0, rows, PITCH, tid);
@@ -369,37 +380,31 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < VB / 32; ++s) {
-      const f8 of = row_perm<E>(lds.pass.dout + t * VP, s, g);
       const f8 rf = TF::get(lds.pass.dr, TP, 16 * w, s, lane), uw = TF::get(lds.pass.u, TP, 16 * w, s, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (r <= w) {
           const f8 uf = TF::get(lds.pass.u, TP, 16 * r, s, lane);
-          dp[r] = mma32(uf, of, dp[r]);
+          dp[r] = mma32(uf, of[s], dp[r]);
           ru[r] = mma32(uf, rf, ru[r]);
         }
 #pragma unroll
       for (int d = 0; d < KB; ++d) {
         const f8 sf = TF::get(lds.pass.s0, PITCH, 16 * d, s, lane);
-        z[d] = mma32(sf, of, z[d]);
+        z[d] = mma32(sf, of[s], z[d]);
         y[d] = mma32(sf, rf, y[d]);
         fu[d] = mma32(TF::get(lds.pass.ds, PITCH, 16 * d, s, lane), uw, fu[d]);
       }
       if (any_zero) {
-        E v8[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int cc = v0 + 32 * s + 16 * (j >> 2) + 4 * g + (j & 3);
-          v8[j] = (E)0.0f;
-          if (cc < p.dv && t0 + t < len) v8[j] = vb[(int64_t)(t0 + t) * p.v.st + cc];
-        }
-        f8 vf;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vf[j] = v8[j];
+        const f8 vf = row_global<E>(vrow, v0 + 32 * s + 4 * g, p.dv, t0 + t < len);
         rv = mma32(vf, rf, rv);
       }
     }
   }
+  __syncthreads();  // the last pass has been read: keys, queries and pairs take its place
+  kt.store(lds.pairs.k, PITCH, p.dk, tid);
+  qt.store(lds.pairs.q, PITCH, p.dk, tid);
+  __syncthreads();
   // pairs (i, t): rows i = 16r + 4g + j, column t
   const double gt = lds.G[t];
   float rows_x = 0.f, rows_n = 0.f;
@@ -413,9 +418,9 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
       floatx4 kk = zero4(), qk = zero4();
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const f8 ki = IO::ld8(lds.k + (16 * r + l16) * PITCH + 32 * s + 8 * g);
-        kk = mma32(ki, IO::ld8(lds.k + t * PITCH + 32 * s + 8 * g), kk);
-        qk = mma32(ki, IO::ld8(lds.q + t * PITCH + 32 * s + 8 * g), qk);
+        const f8 ki = IO::ld8(lds.pairs.k + (16 * r + l16) * PITCH + 32 * s + 8 * g);
+        kk = mma32(ki, IO::ld8(lds.pairs.k + t * PITCH + 32 * s + 8 * g), kk);
+        qk = mma32(ki, IO::ld8(lds.pairs.q + t * PITCH + 32 * s + 8 * g), qk);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -442,7 +447,6 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
     for (int o = 1; o < 16; o <<= 1) cx[i] += __shfl_xor(cx[i], o, 64);
     if (l16 == 0) lds.cols[w][16 * (i >> 2) + 4 * g + (i & 3)] = cx[i];
   }
-  __syncthreads();  // the last pass has been read: the pair matrices take its place
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     IO::st4(lds.pairs.a + t * TP + 16 * r + 4 * g, dp[r][0], dp[r][1], dp[r][2], dp[r][3]);
@@ -453,8 +457,8 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
 #pragma unroll
   for (int d = 0; d < KB; ++d) {
     float qv[4], kv[4];
-    ld4f<E>(lds.q + t * PITCH + 16 * d + 4 * g, qv);
-    ld4f<E>(lds.k + t * PITCH + 16 * d + 4 * g, kv);
+    ld4f<E>(lds.pairs.q + t * PITCH + 16 * d + 4 * g, qv);
+    ld4f<E>(lds.pairs.k + t * PITCH + 16 * d + 4 * g, kv);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       zq = fmaf(z[d][i], qv[i], zq);
@@ -488,14 +492,14 @@ __global__ __launch_bounds__(256, 2) void delta_grads_kernel(DeltaP p) {
     const f8 at = TF::get(lds.pairs.a, TP, 16 * w, s, lane), mt = TF::get(lds.pairs.m, TP, 16 * w, s, lane);
 #pragma unroll
     for (int d = 0; d < KB; ++d) {
-      const f8 kf = TF::get(lds.k, PITCH, 16 * d, s, lane);
+      const f8 kf = TF::get(lds.pairs.k, PITCH, 16 * d, s, lane);
       if (2 * s <= w) {
         z[d] = mma32(kf, af, z[d]);
         fu[d] = mma32(kf, mf, fu[d]);
       }
       if (2 * s + 1 >= w) {
         fu[d] = mma32(kf, mt, fu[d]);
-        fu[d] = mma32(TF::get(lds.q, PITCH, 16 * d, s, lane), at, fu[d]);
+        fu[d] = mma32(TF::get(lds.pairs.q, PITCH, 16 * d, s, lane), at, fu[d]);
       }
     }
   }
