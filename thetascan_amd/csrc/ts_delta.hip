@@ -313,18 +313,20 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
 #pragma unroll
       for (int d = 0; d < KB; ++d) IO::st4(s0 + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
     }
-    // R = b (V - e^G K S0)
-    floatx4 R[4];
-    {
+    // K S0 and S0^T Q^T (lane l16 a token, four columns): independent products side by side
+    floatx4 R[4], O[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) R[r] = zero4();
+    for (int r = 0; r < 4; ++r) R[r] = O[r] = zero4();
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const Split<E> sf(S[2 * s], S[2 * s + 1]);
+    for (int s = 0; s < KS; ++s) {
+      const Split<E> sf(S[2 * s], S[2 * s + 1]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) R[r] = mma_split(row_perm<E>(ks + (16 * r + l16) * PITCH, s, g), sf, R[r]);
+      for (int r = 0; r < 4; ++r) {
+        R[r] = mma_split(row_perm<E>(ks + (16 * r + l16) * PITCH, s, g), sf, R[r]);
+        if constexpr (!TRANSFER) O[r] = mma_split(sf, row_perm<E>(qs + (16 * r + l16) * PITCH, s, g), O[r]);
       }
     }
+    // R = b (V - e^G K S0)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const floatx4 eg = *(const floatx4*)(vec + 16 * r + 4 * g);
@@ -348,29 +350,38 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) IO::st4(u + 16 * r, U[r][0], U[r][1], U[r][2], U[r][3]);
     }
-    // O^T = S0^T Q^T e^G + U^T P^T: lane l16 a token, four columns
+    // S = e^{G_63} S0 + K^T (e^{G_63 - G} U), and beside it O^T = e^G S0^T Q^T + U^T P^T
+    const float whole = vec[3 * kChunk];
+#pragma unroll
+    for (int d = 0; d < KB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[d][i] *= whole;
     if constexpr (!TRANSFER) {
-      floatx4 O[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) O[r] = zero4();
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const Split<E> sf(S[2 * s], S[2 * s + 1]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) O[r] = mma_split(sf, row_perm<E>(qs + (16 * r + l16) * PITCH, s, g), O[r]);
-      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float eg = vec[16 * r + l16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) O[r][i] *= eg;
       }
+    }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const Split<E> uf(U[2 * s], U[2 * s + 1]);
+    for (int s = 0; s < 2; ++s) {
+      floatx4 f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const floatx4 tail = *(const floatx4*)(vec + kChunk + 16 * (2 * s + e) + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[e][i] = U[2 * s + e][i] * tail[i];
+      }
+      const Split<E> ff(f[0], f[1]), uf(U[2 * s], U[2 * s + 1]);
+#pragma unroll
+      for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(ks, PITCH, 16 * d, s, lane), ff, S[d]);
+      if constexpr (!TRANSFER) {
 #pragma unroll
         for (int r = 2 * s; r < 4; ++r) O[r] = mma_tri_t(tri_p, r, s, lane, uf, O[r]);
       }
+    }
+    if constexpr (!TRANSFER) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int t = t0 + 16 * r + l16;
@@ -379,24 +390,6 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
           IO::st4(ob + (int64_t)t * p.out.st, in ? O[r][0] : 0.f, in ? O[r][1] : 0.f, in ? O[r][2] : 0.f,
                   in ? O[r][3] : 0.f);
       }
-    }
-    // S = e^{G_63} S0 + K^T (e^{G_63 - G} U)
-    const float whole = vec[3 * kChunk];
-#pragma unroll
-    for (int d = 0; d < KB; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) S[d][i] *= whole;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const floatx4 tail = *(const floatx4*)(vec + kChunk + 16 * r + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) U[r][i] *= tail[i];
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const Split<E> uf(U[2 * s], U[2 * s + 1]);
-#pragma unroll
-      for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(ks, PITCH, 16 * d, s, lane), uf, S[d]);
     }
   }
   if (!mine) return;

@@ -113,10 +113,12 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
 #pragma unroll
       for (int d = 0; d < KB; ++d) IO::st4(ds + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
     }
-    // dU = P^T dO + e^{G_63 - G} K dS
-    floatx4 X[4];
+    // dU = P^T dO + e^{G_63 - G} K dS, and beside it Q^T (e^G dO): independent products
+    floatx4 X[4], Y[4], Z[KB];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) X[r] = zero4();
+    for (int r = 0; r < 4; ++r) X[r] = Y[r] = zero4();
+#pragma unroll
+    for (int d = 0; d < KB; ++d) Z[d] = zero4();
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const Split<E> sf(S[2 * s], S[2 * s + 1]);
@@ -124,12 +126,25 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
       for (int r = 0; r < 4; ++r) X[r] = mma_split(row_perm<E>(lds.k + (16 * r + l16) * PITCH, s, g), sf, X[r]);
     }
 #pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      floatx4 f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const floatx4 eg = *(const floatx4*)(vec + 16 * (2 * s + e) + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[e][i] = eg[i] * tof(of[s][4 * e + i]);
+      }
+      const f8 qf = IO::from_acc(f[0], f[1]);
+#pragma unroll
+      for (int r = 0; r < 2 * s + 2; ++r) Y[r] = mma32(TriT<E>::get((const E*)lds.p, r, s, lane), of[s], Y[r]);
+#pragma unroll
+      for (int d = 0; d < KB; ++d) Z[d] = mma32(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, Z[d]);
+    }
+#pragma unroll
     for (int r = 0; r < 4; ++r) {
       const floatx4 tail = *(const floatx4*)(vec + kChunk + 16 * r + 4 * g);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) X[r][i] *= tail[i];
-#pragma unroll
-      for (int s = r / 2; s < 2; ++s) X[r] = mma32(TriT<E>::get((const E*)lds.p, r, s, lane), of[s], X[r]);
+      for (int i = 0; i < 4; ++i) X[r][i] = fmaf(tail[i], X[r][i], Y[r][i]);
     }
     // dR = Ti^T dU
     floatx4 R[4];
@@ -143,7 +158,6 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
     }
     E* dro = (E*)p.dr + (n * p.dvp + col) * kChunk + 4 * g;
     const float whole = vec[3 * kChunk];
-    float od[16];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       if constexpr (!TRANSFER) IO::st4(dro + 16 * r, R[r][0], R[r][1], R[r][2], R[r][3]);
@@ -155,24 +169,18 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
         const float dv = be[i] * R[r][i];
         if (!TRANSFER && t < p.T && on) vb[(int64_t)t * p.dval.st] = cvt<E>(t < len ? dv : 0.f);
         R[r][i] = -eg[i] * dv;
-        od[4 * r + i] = eg[i] * tof(of[r / 2][4 * (r & 1) + i]);
       }
     }
     // dS0
 #pragma unroll
     for (int d = 0; d < KB; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) S[d][i] *= whole;
+      for (int i = 0; i < 4; ++i) S[d][i] = fmaf(whole, S[d][i], Z[d][i]);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const Split<E> rf(R[2 * s], R[2 * s + 1]);
-      const Split<E> qf(floatx4{od[8 * s], od[8 * s + 1], od[8 * s + 2], od[8 * s + 3]},
-                        floatx4{od[8 * s + 4], od[8 * s + 5], od[8 * s + 6], od[8 * s + 7]});
+      const f8 rf = IO::from_acc(R[2 * s], R[2 * s + 1]);
 #pragma unroll
-      for (int d = 0; d < KB; ++d) {
-        S[d] = mma_split(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, S[d]);
-        S[d] = mma_split(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
-      }
+      for (int d = 0; d < KB; ++d) S[d] = mma32(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
     }
   }
   if (!mine) return;
