@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -37,10 +38,13 @@ MAX_KEYS, MAX_VALUES = 128, 512
 STEP_TOKENS = 8
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """The device a launch needs as the current one (a no-op where it is)."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -59,9 +63,25 @@ def _gate(t: torch.Tensor | None, heads: bool = False) -> _lib.Strided:
 
 def _desc(q, k, v, beta, decay, keep: bool) -> _lib.DeltaDesc:
     B, Hk, T, dk = q.shape
-    return _lib.DeltaDesc(B, Hk, v.shape[1], T, _width(q.dtype, dk), _width(q.dtype, v.shape[-1]),
-                          _lib.dtype_code(q.dtype), _lib.dtype_code(beta.dtype),
-                          _lib.TS_F32 if decay is None else _lib.dtype_code(decay.dtype), int(keep))
+    _, H, _, dv = v.shape
+    dt = q.dtype
+    return _lib.DeltaDesc(B, Hk, H, T, _width(dt, dk), _width(dt, dv), _lib.dtype_code(dt),
+                          _lib.dtype_code(beta.dtype), _lib.TS_F32 if decay is None else _lib.dtype_code(decay.dtype),
+                          int(keep))
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes(backward: bool, *shape) -> int:
+    """Bytes of a call's workspace, by the descriptor's entries."""
+    lib, n = _lib.load(), ctypes.c_size_t()
+    size = lib.ts_delta_bwd_workspace_bytes if backward else lib.ts_delta_workspace_bytes
+    _lib.check(size(ctypes.byref(_lib.DeltaDesc(*shape)), ctypes.byref(n)), "ts_delta_workspace_bytes")
+    return n.value
+
+
+def _workspace(d: _lib.DeltaDesc, device, backward: bool = False) -> torch.Tensor:
+    n = _bytes(backward, d.B, d.Hk, d.H, d.T, d.dk, d.dv, d.dtype, d.beta_dtype, d.decay_dtype, d.keep)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _padded_state(state: torch.Tensor | None, dk: int, dv: int) -> torch.Tensor | None:
@@ -112,7 +132,7 @@ def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, 
                 status = lib.ts_delta_step(ctypes.byref(desc), ctypes.byref(io), stream)
             _lib.check(status, "ts_delta_step")
         else:
-            work = torch.empty(_workspace_bytes(desc), dtype=torch.uint8, device=q.device)
+            work = _workspace(desc, q.device)
             with _lib.timed("ts_delta_fwd", lambda: _lib.nbytes(q, k, v4, beta, decay, out, given, final)):
                 status = lib.ts_delta_fwd(ctypes.byref(desc), ctypes.byref(io), work.data_ptr(), work.numel(), stream)
             _lib.check(status, "ts_delta_fwd")
@@ -122,13 +142,7 @@ def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, 
             final = final.contiguous()
         if state_out is not None:
             final = state_out.copy_(final)
-    return out[..., :dv], final, work
-
-
-def _workspace_bytes(desc: _lib.DeltaDesc) -> int:
-    n = ctypes.c_size_t()
-    _lib.check(_lib.load().ts_delta_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), "ts_delta_workspace_bytes")
-    return n.value
+    return out if dvp == dv else out[..., :dv], final, work
 
 
 def _forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor | None,
@@ -142,7 +156,7 @@ def _forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tens
 def _forward_fake(q, k, v, beta, decay, state, lengths, want_state, keep, step):
     B, H, _, dv = v.shape
     out = _rows_like(v, q.dtype, _width(q.dtype, dv))[..., :dv]
-    nbytes = _workspace_bytes(_desc(q, k, v, beta, decay, True)) if keep else 0
+    nbytes = _workspace(_desc(q, k, v, beta, decay, True), "meta").numel() if keep else 0
     return [out, q.new_empty((B, H, q.shape[-1], dv) if want_state else (0,), dtype=torch.float32),
             q.new_empty(nbytes, dtype=torch.uint8)]
 
@@ -157,7 +171,7 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
     q4, k4, v4 = (_kernel_view(x) for x in (q, k, v))
     if dout is None:
         dout = torch.zeros(B, H, T, dvp, dtype=q.dtype, device=q.device)
-    do4 = _kernel_view(dout.to(q.dtype))
+    do4 = _kernel_view(dout if dout.dtype == q.dtype else dout.to(q.dtype))
     given = None if dfinal is None else _padded_state(dfinal.to(torch.float32), dkp, dvp)
     dq, dk_, dv_ = _rows_like(q, q.dtype, dkp), _rows_like(k, q.dtype, dkp), _rows_like(v, q.dtype, dvp)
     dbeta = torch.empty(B, H, T, dtype=beta.dtype, device=q.device)
@@ -171,15 +185,16 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
     grads = _lib.DeltaGrads(_lib.strided(do4), _lib.strided(dq), _lib.strided(dk_), _lib.strided(dv_), dbeta.data_ptr(),
                             None if per_head else _lib.ptr(ddecay), _lib.ptr(ddecay) if per_head else None,
                             _lib.ptr(given), _lib.ptr(dstate))
-    n = ctypes.c_size_t()
-    _lib.check(lib.ts_delta_bwd_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)), "ts_delta_bwd_workspace_bytes")
-    work = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+    work = _workspace(desc, q.device, backward=True)
     with _on(q.device), _lib.timed("ts_delta_bwd", lambda: _lib.nbytes(q4, k4, v4, do4, dq, dk_, dv_, dbeta, ddecay)):
         status = lib.ts_delta_bwd(ctypes.byref(desc), ctypes.byref(io), ctypes.byref(grads), saved.data_ptr(),
                                   saved.numel(), work.data_ptr(), work.numel(), _lib.stream_handle(q.device))
     _lib.check(status, "ts_delta_bwd")
-    return [dq[..., :dk], dk_[..., :dk], dv_[..., :dv], dbeta, q.new_empty(0) if ddecay is None else ddecay,
-            q.new_empty(0) if dstate is None else dstate[..., :dk, :dv]]
+    if (dkp, dvp) != (dk, dv):
+        dq, dk_, dv_ = dq[..., :dk], dk_[..., :dk], dv_[..., :dv]
+        dstate = None if dstate is None else dstate[..., :dk, :dv]
+    return [dq, dk_, dv_, dbeta, q.new_empty(0) if ddecay is None else ddecay,
+            q.new_empty(0) if dstate is None else dstate]
 
 
 def _backward_fake(dout, dfinal, q, k, v, beta, decay, state, lengths, saved, need_state):
@@ -244,15 +259,13 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
 
     Differentiable in q, k, v, beta, the retention and the state.
     """
-    tensors = (q, k, v, beta)
-    for name, x in zip(("q", "k", "v"), tensors):
+    for name, x in (("q", q), ("k", k), ("v", v)):
         if x.ndim != 4:
             raise ValueError(f"gated_delta_rule: {name} must be [B,H,T,D], got {tuple(x.shape)}")
-    B, Hk, T, dk = q.shape
-    H, dv = v.shape[1], v.shape[3]
-    if tuple(k.shape) != (B, Hk, T, dk) or v.shape[0] != B or v.shape[2] != T:
+    (B, Hk, T, dk), (Bv, H, Tv, dv) = q.shape, v.shape
+    if k.shape != q.shape or Bv != B or Tv != T:
         raise ValueError(f"gated_delta_rule: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    if B < 1 or Hk < 1 or dk < 1 or dv < 1 or H < 1 or H % Hk:
+    if min(B, Hk, dk, dv, H) < 1 or H % Hk:
         raise ValueError(f"gated_delta_rule: {H} value heads over {Hk} key heads, {B} sequences, widths {dk} and {dv}")
     if dk > MAX_KEYS or dv > MAX_VALUES:
         raise NotImplementedError(f"gated_delta_rule: at most {MAX_KEYS} keys and {MAX_VALUES} values, got {dk} and {dv}")
@@ -267,21 +280,26 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
         if retention.ndim == 4 and retention.shape[-1] != 1:
             raise NotImplementedError("gated_delta_rule: one retention per token and head (no per-channel decay)")
         retention = _token_gate(retention, "retention", B, H, T)
-    for x in (q, beta) if retention is None else (q, beta, retention):
-        _lib.dtype_code(x.dtype)
+    for x in (q, beta, retention):
+        if x is not None:
+            _lib.dtype_code(x.dtype)
     for name, s in (("state", state), ("state_out", state_out)):
         if s is not None and (tuple(s.shape) != (B, H, dk, dv) or s.dtype != torch.float32):
             raise ValueError(f"gated_delta_rule: {name} must be fp32 {(B, H, dk, dv)}, got {s.dtype} {tuple(s.shape)}")
     if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"gated_delta_rule: lengths must be integers [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
-    everything = [x for x in (*tensors, retention, state, lengths, state_out) if x is not None]
-    if not all(x.is_cuda for x in everything):
+    device, record = q.get_device(), torch.is_grad_enabled() and q.requires_grad
+    if device < 0:
         raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")
-    if any(x.device != q.device for x in everything):
-        raise ValueError("gated_delta_rule: tensors on several devices")
+    for x in (k, v, beta, retention, state, lengths, state_out):
+        if x is not None:
+            if x.get_device() != device:
+                if not x.is_cuda:
+                    raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")
+                raise ValueError("gated_delta_rule: tensors on several devices")
+            record = record or (x.requires_grad and torch.is_grad_enabled())
     if lengths is not None:
         lengths = lengths.to(torch.int64).contiguous()
-    record = torch.is_grad_enabled() and any(x.requires_grad for x in everything)
     if state_out is not None:
         if record or state_out.requires_grad:
             raise ValueError("gated_delta_rule: state_out takes no part in gradients: call it without them")

@@ -43,31 +43,35 @@ def _forward(z: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, adv: torc
     _lib.check(lib.ts_policy_loss_parts(ctypes.byref(desc), ctypes.byref(n)), "ts_policy_loss_parts")
     loss = torch.empty((), dtype=torch.float32, device=z.device)
     lp = torch.empty(rows, dtype=torch.float32, device=z.device)
-    coef = torch.empty_like(lp)
-    lse = torch.empty(2, rows, dtype=torch.float32, device=z.device)
-    parts = torch.empty(max(n.value, 1), dtype=torch.float64, device=z.device)
+    # dloss/dlp, the maximum and the logarithm of the sum of each row; the parts of the loss (fp64) before them
+    saved = torch.empty(max(2 * n.value + 3 * rows, 2), dtype=torch.float32, device=z.device)
+    at = saved.data_ptr()
+    coef = at + 8 * n.value
     io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), old.data_ptr(), _lib.ptr(ref), adv.data_ptr(),
-                       _lib.ptr(weights), lp.data_ptr(), coef.data_ptr(), lse.data_ptr(), parts.data_ptr(),
-                       loss.data_ptr())
+                       _lib.ptr(weights), lp.data_ptr(), coef, coef + 4 * rows, at, loss.data_ptr())
     with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tokens, old, adv, ref, weights, lp)):
         status = lib.ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
     _lib.check(status, "ts_policy_loss_fwd")
-    return [loss, lp, coef, lse]
+    return [loss, lp, saved]
 
 
 def _forward_fake(z, tokens, old, adv, ref, weights, low, high, kl, cap):
-    row = z.new_empty(z.shape[0], dtype=torch.float32)
-    return [z.new_empty((), dtype=torch.float32), row, torch.empty_like(row), row.new_empty(2, z.shape[0])]
+    n = ctypes.c_int64()
+    _lib.check(_lib.load().ts_policy_loss_parts(ctypes.byref(_desc(z, cap)), ctypes.byref(n)), "ts_policy_loss_parts")
+    return [z.new_empty((), dtype=torch.float32), z.new_empty(z.shape[0], dtype=torch.float32),
+            z.new_empty(max(2 * n.value + 3 * z.shape[0], 2), dtype=torch.float32)]
 
 
 def _backward_impl(g: torch.Tensor, z: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | None,
-                   coef: torch.Tensor, lse: torch.Tensor, cap: float) -> torch.Tensor:
+                   saved: torch.Tensor, cap: float) -> torch.Tensor:
     lib = _lib.load()
     z = _rows(z)
+    rows = z.shape[0]
     dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    g32 = g.detach().to(torch.float32).reshape(1).contiguous()
-    io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), None, None, None, _lib.ptr(weights), None, coef.data_ptr(),
-                       lse.data_ptr(), None, None)
+    g32 = g if g.dtype == torch.float32 else g.to(torch.float32)
+    coef = saved.data_ptr() + 4 * (saved.numel() - 3 * rows)
+    io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), None, None, None, _lib.ptr(weights), None, coef,
+                       coef + 4 * rows, None, None)
     desc = _desc(z, cap)
     with _on(z.device), _lib.timed("ts_policy_loss_bwd", lambda: _lib.nbytes(z, tokens, dz)):
         status = lib.ts_policy_loss_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(),
@@ -76,24 +80,31 @@ def _backward_impl(g: torch.Tensor, z: torch.Tensor, tokens: torch.Tensor, weigh
     return dz
 
 
-def _backward_fake(g, z, tokens, weights, coef, lse, cap):
+def _backward_fake(g, z, tokens, weights, saved, cap):
     return z.new_empty(z.shape)
 
 
 def _setup(ctx, inputs, output):
     z, tokens, weights, ctx.cap = inputs[0], inputs[1], inputs[5], inputs[9]
-    ctx.save_for_backward(z, tokens, weights, output[2], output[3])
+    ctx.save_for_backward(z, tokens, weights, output[2])
 
 
 def _backward(ctx, grads, bwd):
     if grads[0] is None:
         return (None,) * 10
-    z, tokens, weights, coef, lse = ctx.saved_tensors
-    return (bwd(grads[0], z, tokens, weights, coef, lse, ctx.cap), *(None,) * 9)
+    z, tokens, weights, saved = ctx.saved_tensors
+    return (bwd(grads[0], z, tokens, weights, saved, ctx.cap), *(None,) * 9)
 
 
 _policy_op = HipOp("policy_loss", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,
                    backward_fake=_backward_fake, setup=_setup, backward=_backward)
+
+
+def _row_values(x: torch.Tensor | None) -> torch.Tensor | None:
+    """One fp32 value a row, contiguous, without its gradient."""
+    if x is None or (x.dtype == torch.float32 and x.ndim == 1 and not x.requires_grad and x.is_contiguous()):
+        return x
+    return x.detach().to(torch.float32).reshape(-1).contiguous()
 
 
 def _flat(what: str, logits: torch.Tensor, tokens: torch.Tensor, softcap: float | None,
@@ -111,14 +122,16 @@ def _flat(what: str, logits: torch.Tensor, tokens: torch.Tensor, softcap: float 
     if softcap is not None and not 0.0 < cap < float("inf"):
         raise ValueError(f"{what}: softcap must be positive (None: no cap), got {softcap}")
     _lib.dtype_code(logits.dtype)
-    given = [logits, tokens, *(x for x in rows.values() if x is not None)]
-    if not all(x.is_cuda for x in given):
-        raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")
-    if any(x.device != logits.device for x in given):
-        raise ValueError(f"{what}: tensors on several devices")
-    flat = {name: None if x is None else x.detach().to(torch.float32).reshape(-1).contiguous()
-            for name, x in rows.items()}
-    return logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1).contiguous(), cap, flat
+    device = logits.get_device()
+    for x in (logits, tokens, *rows.values()):
+        if x is not None and (x.get_device() != device or device < 0):
+            if not (x.is_cuda and logits.is_cuda):
+                raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")
+            raise ValueError(f"{what}: tensors on several devices")
+    flat = {name: _row_values(x) for name, x in rows.items()}
+    if len(shape) != 1:
+        logits, tokens = logits.reshape(-1, logits.shape[-1]), tokens.reshape(-1)
+    return logits, tokens if tokens.is_contiguous() else tokens.contiguous(), cap, flat
 
 
 def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor, *,
@@ -148,9 +161,10 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch
     z, tok, cap, r = _flat("policy_loss", logits, tokens, softcap,
                            {"old_log_probs": old_log_probs, "advantages": advantages,
                             "ref_log_probs": ref_log_probs if kl else None, "weights": weights})
-    loss, lp, _, _ = _policy_op(z, tok, r["old_log_probs"], r["advantages"], r["ref_log_probs"], r["weights"], low, high,
+    loss, lp, _ = _policy_op(z, tok, r["old_log_probs"], r["advantages"], r["ref_log_probs"], r["weights"], low, high,
                                 kl, cap)
-    return loss, lp.detach().view(tokens.shape)
+    lp = lp.detach()
+    return loss, lp if tokens.ndim == 1 else lp.view(tokens.shape)
 
 
 @torch.no_grad()
