@@ -312,9 +312,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
         out = v.new_empty(B, H, 0, dv)
         return (out, final) if return_state else out
     step = not record and T <= STEP_TOKENS
-    if state_out is not None:
-        with torch.no_grad():
-            out, final, _ = _launch(q, k, v, beta, retention, state, lengths, True, False, step, state_out)
+    if state_out is not None or not (record or torch.compiler.is_compiling()):
+        out, final, _ = _launch(q, k, v, beta, retention, state, lengths, return_state or state_out is not None, False,
+                                step, state_out)
         return (out, final) if return_state else out
     out, final, _ = _delta_op(q, k, v, beta, retention, state, lengths, bool(return_state), record, step)
     return (out, final) if return_state else out

@@ -17,6 +17,10 @@ the parameter count follows the count contract of
 tests/test_projection_layouts.py:101-113 (baseline 17,059,912 parameters,
 attention mixer 786,440, FFN hidden 1024).
 
+``HybridLM(memory="delta")`` has gated delta memories
+(:class:`thetascan_amd.delta.GatedDelta`) in those two layers instead, and
+``policy_loss`` trains either on rollouts.
+
 The upstream script is not available, so this model is defined here from
 those facts; its int8 round trip has no reference numbers to match.
 """
@@ -28,9 +32,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._core.ops import attention as hip_attention, rowglue, rownorm
+from ._core.ops import attention as hip_attention, policy, rowglue, rownorm
 from .api import ThetaScan
 from .config import ThetaScanConfig
+from .delta import GatedDelta, GatedDeltaConfig
 
 VOCAB = 1024
 D_MODEL = 512
@@ -156,15 +161,25 @@ class MLP(nn.Module):
         return self.proj(rowglue.relu2(self.fc(x)))
 
 
+def delta_config() -> GatedDeltaConfig:
+    """The gated delta layer: the attention layers' head layout (key and query
+    heads shared by two value heads each)."""
+    return GatedDeltaConfig(d_model=D_MODEL, n_heads=HEADS, key_heads=KV_HEADS)
+
+
 class Block(nn.Module):
-    def __init__(self, theta: bool):
+    def __init__(self, theta: bool, memory: str = "theta"):
         super().__init__()
         self.theta = theta
-        self.attn = ThetaScan(theta_config()) if theta else CausalSelfAttention()
-        if theta:
-            # the recipe's memory starts near identity; its projections start
-            # like attention's (the output projection at zero)
-            nn.init.zeros_(self.attn._core.proj_out.weight)
+        if theta and memory == "delta":
+            self.attn = GatedDelta(delta_config())
+            nn.init.zeros_(self.attn.proj_out.weight)
+        else:
+            self.attn = ThetaScan(theta_config()) if theta else CausalSelfAttention()
+            if theta:
+                # the recipe's memory starts near identity; its projections start
+                # like attention's (the output projection at zero)
+                nn.init.zeros_(self.attn._core.proj_out.weight)
         self.mlp = MLP(D_MODEL, THETA_FFN_HIDDEN if theta else FFN_HIDDEN)
         self.attn_scale = nn.Parameter(torch.ones(D_MODEL))
         self.mlp_scale = nn.Parameter(torch.ones(D_MODEL))
@@ -179,17 +194,23 @@ class Block(nn.Module):
 
 
 class HybridLM(nn.Module):
-    """Token ids [B,T] -> mean next-token cross-entropy (or logits)."""
+    """Token ids [B,T] -> mean next-token cross-entropy (or logits).
 
-    def __init__(self):
+    ``memory`` names the mixers of layers 4 and 5: "theta" (ThetaScan-Kernel) or
+    "delta" (gated delta rule)."""
+
+    def __init__(self, memory: str = "theta"):
         super().__init__()
+        if memory not in ("theta", "delta"):
+            raise ValueError(f"memory must be 'theta' or 'delta', got {memory!r}")
         self.tok_emb = nn.Embedding(VOCAB, D_MODEL)
         nn.init.normal_(self.tok_emb.weight, std=0.005)
-        self.blocks = nn.ModuleList([Block(i in THETA_LAYERS) for i in range(LAYERS)])
+        self.blocks = nn.ModuleList([Block(i in THETA_LAYERS, memory) for i in range(LAYERS)])
         self.n_enc = LAYERS // 2
         self.skip_weights = nn.Parameter(torch.ones(min(self.n_enc, LAYERS - self.n_enc), D_MODEL))
 
-    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None) -> torch.Tensor:
+    def _logits(self, idx: torch.Tensor) -> torch.Tensor:
+        """The logits [B,T,V] before the soft cap, in the weights' dtype."""
         x = _rms(self.tok_emb(idx))
         x0 = x
         skips = []
@@ -200,12 +221,29 @@ class HybridLM(nn.Module):
             if i < self.n_enc:
                 skips.append(x)
         x = _rms(x)
-        logits = F.linear(x, self.tok_emb.weight.to(x.dtype))
+        return F.linear(x, self.tok_emb.weight.to(x.dtype))
+
+    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None) -> torch.Tensor:
+        logits = self._logits(idx)
         if targets is None:
             return LOGIT_SOFTCAP * torch.tanh(logits.float() / LOGIT_SOFTCAP)
         # the soft-capped logits' cross entropy: one HIP launch per direction
         # on the GPU (the fp32 capped logits are never stored)
         return rowglue.softcap_cross_entropy(logits.reshape(-1, VOCAB), targets.reshape(-1), LOGIT_SOFTCAP)
+
+    def log_probs(self, idx: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+        """Log-probabilities [B,T] (fp32, without a gradient) of ``tokens`` as the
+        successors of ``idx``: a rollout's ``old_log_probs`` and a reference
+        model's ``ref_log_probs``."""
+        with torch.no_grad():
+            return policy.token_log_probs(self._logits(idx), tokens, softcap=LOGIT_SOFTCAP)
+
+    def policy_loss(self, idx: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch.Tensor,
+                    advantages: torch.Tensor, **options) -> tuple[torch.Tensor, torch.Tensor]:
+        """``(loss, log_probs)`` of :func:`thetascan_amd.policy_loss` for the
+        sampled successors ``tokens`` [B,T] of ``idx`` [B,T] (``options``: its
+        keywords but the soft cap)."""
+        return policy.policy_loss(self._logits(idx), tokens, old_log_probs, advantages, softcap=LOGIT_SOFTCAP, **options)
 
 
 # ---------------------------------------------------------------- int8 round trip
