@@ -19,6 +19,8 @@
 
 #include <string.h>
 
+#include <type_traits>
+
 namespace ts {
 
 // What the waves of a workgroup read of one chunk: the triangles in one rounding.
@@ -223,6 +225,18 @@ struct GradsLds {
   double G[kChunk];
   float cols[4][kChunk], base[kChunk], f[kChunk], red[4];
 };
+
+// The sum over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ float row_sum(float x) {
+  auto add = [&](auto ctrl) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  add(std::integral_constant<int, 0xb1>());   // lanes 1, 0, 3, 2
+  add(std::integral_constant<int, 0x4e>());   // lanes 2, 3, 0, 1
+  add(std::integral_constant<int, 0x141>());  // the half row mirrored
+  add(std::integral_constant<int, 0x140>());  // the row mirrored
+  return x;
+}
 
 // Eight columns of a global row in accumulator order (c.., c + 16..), zero at or
 // past `width` and where the row is none.
@@ -451,8 +465,7 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void del
     }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) cx[i] += __shfl_xor(cx[i], o, 64);
+    cx[i] = row_sum(cx[i]);
     if (l16 == 0) lds.cols[w][16 * (i >> 2) + 4 * g + (i & 3)] = cx[i];
   }
 #pragma unroll
