@@ -56,7 +56,7 @@ extern "C" {
  *     stride of 32 Mi elements and more was taken before).
  * 19: ts_delta_fwd / ts_delta_bwd / ts_delta_step (with their workspace sizes)
  *     and ts_policy_loss_fwd / ts_policy_loss_bwd /
- *     ts_policy_loss_parts; nothing earlier changed. */
+ *     ts_policy_loss_parts / ts_policy_one_pass / ts_policy_scale; nothing earlier changed. */
 #define TS_ABI_VERSION 19
 
 enum ts_status {
@@ -1326,10 +1326,19 @@ typedef struct ts_policy_io {
                                            backward                              */
   double *parts;                        /* scratch, ts_policy_loss_parts of them */
   float *loss;                          /* out [1], or NULL: log_probs only      */
+  void *dlogits;                        /* out [rows, V] contiguous, 16-byte
+                                           aligned: the logits' gradient for a
+                                           unit gradient of the loss, in the same
+                                           pass (where ts_policy_one_pass), or
+                                           NULL                                  */
 } ts_policy_io;
 
 int ts_policy_loss_parts(const ts_policy_desc* desc, int64_t* parts);
 int ts_policy_loss_fwd(const ts_policy_desc* desc, const ts_policy_io* io, hipStream_t stream);
+/* Whether loss and gradient of rows of this length are formed in one pass. */
+int ts_policy_one_pass(const ts_policy_desc* desc, int32_t* one_pass);
+/* x[i] *= g[0] (n elements of ts_dtype `dtype`, 16-byte aligned); nothing where it is one. */
+int ts_policy_scale(void* x, int64_t n, int32_t dtype, const float* g, hipStream_t stream);
 /* dlogits [rows, V] contiguous from the forward's coef and lse and the loss's
  * gradient dloss (fp32, on the device). */
 int ts_policy_loss_bwd(const ts_policy_desc* desc, const ts_policy_io* io, const float* dloss, void* dlogits,

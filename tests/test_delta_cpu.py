@@ -143,7 +143,7 @@ def test_policy_entry_points_check_on_the_host():
     for bad, code in ((dict(rows=-1), 1), (dict(V=0), 1), (dict(cap=-1.0), 1), (dict(low=1.5), 1), (dict(kl=-0.1), 1),
                       (dict(high=float("nan")), 1), (dict(dtype=5), 2), (dict(rows=1 << 32), 2)):
         assert lib.ts_policy_loss_parts(ctypes.byref(d(**bad)), ctypes.byref(n)) == code, bad
-    full = _lib.PolicyIO(*[FAKE] * 11)
+    full = _lib.PolicyIO(*[FAKE] * 12)
     for name in ("logits", "tokens", "old_log_probs", "advantages", "log_probs", "coef", "lse", "parts"):
         missing = _lib.PolicyIO(*[None if f[0] == name else FAKE for f in _lib.PolicyIO._fields_])
         assert lib.ts_policy_loss_fwd(ctypes.byref(d()), ctypes.byref(missing), None) == _lib.TS_ERR_VALUE, name

@@ -170,6 +170,39 @@ def test_strided_rows_layouts_and_dtypes(cuda):
     assert float(empty[0]) == 0.0 and empty[1].shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [100, 1000, 5000, 70000])
+def test_second_backward_and_two_pass_rows(cuda, V, dtype):
+    """The gradient of the first backward, of a second one of the same loss with
+    another upstream gradient, of rows that take one pass and of rows that take two."""
+    import thetascan_amd as ts
+    from thetascan_amd import _lib
+
+    z, tokens, old, ref, adv = inputs(21, V, dtype, seed=V)
+    want, lp_want, _ = reference(z.double().requires_grad_(), tokens, old, adv, cap=30.0)
+    zr = z.double().requires_grad_()
+    want, lp_want, _ = reference(zr, tokens, old, adv, cap=30.0)
+    dz_want, dlp = torch.autograd.grad(want, (zr, lp_want))
+    zd = z.to(cuda).requires_grad_()
+    with _lib.record_launches() as recs:
+        loss, _ = ts.policy_loss(zd, tokens.to(cuda), old.to(cuda), adv.to(cuda), softcap=30.0)
+        first = torch.autograd.grad(loss, zd, retain_graph=True)[0]
+        held = first.clone()
+        second = torch.autograd.grad(loss, zd, torch.tensor(-3.0, device=cuda), retain_graph=True)[0]
+        third = torch.autograd.grad(loss, zd)[0]
+    names = [r[0] for r in recs]
+    assert names.count("ts_policy_loss_bwd") == (3 if V <= 2048 else 2)
+    assert torch.equal(first, held)
+    for x, g in ((first, 1.0), (second, -3.0), (third, 1.0)):
+        err = float((x.double().cpu() / g - dz_want).norm())
+        assert err <= (2.0 ** -8 if dtype == BF else 0.0) * float(dz_want.norm()) + 2.0 ** -16 * float(dlp.norm())
+    # an upstream gradient other than one: rounded to bf16 before and after
+    loss, _ = ts.policy_loss(zd, tokens.to(cuda), old.to(cuda), adv.to(cuda), softcap=30.0)
+    x = torch.autograd.grad(loss * 0.3, zd)[0]
+    err = float((x.double().cpu() / 0.3 - dz_want).norm())
+    assert err <= (2 * 2.0 ** -8 if dtype == BF else 0.0) * float(dz_want.norm()) + 2.0 ** -15 * float(dlp.norm())
+
+
 def test_a_token_outside_the_vocabulary_gives_nan(cuda):
     import thetascan_amd as ts
 

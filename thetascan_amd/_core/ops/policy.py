@@ -8,24 +8,41 @@ logits, with ``y = cap tanh(z / cap)`` (or z), ``lp = log softmax(y)[token]`` an
     loss = sum_n w_n [ -min(r A, clip(r, 1 - low, 1 + high) A)
                        + kl (exp(ref - lp) - (ref - lp) - 1) ]
 
-One pass over the logits a direction (ts_policy_loss_fwd, ts_policy_loss_bwd):
-neither the capped logits nor the probabilities are stored.  A row of weight zero
+One pass over the logits a direction (ts_policy_loss_fwd, ts_policy_loss_bwd);
+where a gradient is recorded and rows are long, the forward gives the gradient for a
+unit upstream gradient too, which the backward scales where it is another (a second
+backward of the same loss forms it again).  Neither the capped logits nor the
+probabilities are stored.  A row of weight zero
 (a prompt's, a padding's) is not read.
 """
 from __future__ import annotations
 
 import ctypes
+import functools
+import threading
 
 import torch
 
 from ... import _lib
 from .delta import _on
-from .dispatch import HipOp
+from .dispatch import HipOp, eager_forward
+
+_GRADIENT = threading.local()  # the gradient that an eager forward leaves for its setup
 
 
 def _desc(z: torch.Tensor, cap: float, kl: float = 0.0, low: float = 0.0, high: float = 0.0) -> _lib.PolicyDesc:
     return _lib.PolicyDesc(z.shape[0], z.stride(0) if z.shape[0] > 1 else z.shape[1], z.shape[1],
                            _lib.dtype_code(z.dtype), cap, 0, kl, low, high)
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(rows: int, V: int, dtype: int, cap: bool) -> tuple[int, bool]:
+    """Partial sums of a call, and whether one pass gives the gradient too."""
+    lib, n, one = _lib.load(), ctypes.c_int64(), ctypes.c_int32()
+    desc = _lib.PolicyDesc(rows, V, V, dtype, 1.0 if cap else 0.0, 0, 0.0, 0.0, 0.0)
+    _lib.check(lib.ts_policy_loss_parts(ctypes.byref(desc), ctypes.byref(n)), "ts_policy_loss_parts")
+    _lib.check(lib.ts_policy_one_pass(ctypes.byref(desc), ctypes.byref(one)), "ts_policy_one_pass")
+    return n.value, bool(one.value)
 
 
 def _rows(z: torch.Tensor) -> torch.Tensor:
@@ -39,27 +56,29 @@ def _forward(z: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, adv: torc
     z = _rows(z)
     rows = z.shape[0]
     desc = _desc(z, cap, kl, low, high)
-    n = ctypes.c_int64()
-    _lib.check(lib.ts_policy_loss_parts(ctypes.byref(desc), ctypes.byref(n)), "ts_policy_loss_parts")
+    parts, one_pass = _plan(rows, z.shape[1], desc.dtype, cap > 0.0)
     loss = torch.empty((), dtype=torch.float32, device=z.device)
     lp = torch.empty(rows, dtype=torch.float32, device=z.device)
     # dloss/dlp, the maximum and the logarithm of the sum of each row; the parts of the loss (fp64) before them
-    saved = torch.empty(max(2 * n.value + 3 * rows, 2), dtype=torch.float32, device=z.device)
+    saved = torch.empty(max(2 * parts + 3 * rows, 2), dtype=torch.float32, device=z.device)
     at = saved.data_ptr()
-    coef = at + 8 * n.value
+    coef = at + 8 * parts
+    dz = None
+    if one_pass and rows and eager_forward():
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        _GRADIENT.of = (loss, dz)
     io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), old.data_ptr(), _lib.ptr(ref), adv.data_ptr(),
-                       _lib.ptr(weights), lp.data_ptr(), coef, coef + 4 * rows, at, loss.data_ptr())
-    with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tokens, old, adv, ref, weights, lp)):
+                       _lib.ptr(weights), lp.data_ptr(), coef, coef + 4 * rows, at, loss.data_ptr(), _lib.ptr(dz))
+    with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tokens, old, adv, ref, weights, lp, dz)):
         status = lib.ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
     _lib.check(status, "ts_policy_loss_fwd")
     return [loss, lp, saved]
 
 
 def _forward_fake(z, tokens, old, adv, ref, weights, low, high, kl, cap):
-    n = ctypes.c_int64()
-    _lib.check(_lib.load().ts_policy_loss_parts(ctypes.byref(_desc(z, cap)), ctypes.byref(n)), "ts_policy_loss_parts")
+    parts = _plan(z.shape[0], z.shape[1], _lib.dtype_code(z.dtype), cap > 0.0)[0]
     return [z.new_empty((), dtype=torch.float32), z.new_empty(z.shape[0], dtype=torch.float32),
-            z.new_empty(max(2 * n.value + 3 * z.shape[0], 2), dtype=torch.float32)]
+            z.new_empty(max(2 * parts + 3 * z.shape[0], 2), dtype=torch.float32)]
 
 
 def _backward_impl(g: torch.Tensor, z: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | None,
@@ -71,7 +90,7 @@ def _backward_impl(g: torch.Tensor, z: torch.Tensor, tokens: torch.Tensor, weigh
     g32 = g if g.dtype == torch.float32 else g.to(torch.float32)
     coef = saved.data_ptr() + 4 * (saved.numel() - 3 * rows)
     io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), None, None, None, _lib.ptr(weights), None, coef,
-                       coef + 4 * rows, None, None)
+                       coef + 4 * rows, None, None, None)
     desc = _desc(z, cap)
     with _on(z.device), _lib.timed("ts_policy_loss_bwd", lambda: _lib.nbytes(z, tokens, dz)):
         status = lib.ts_policy_loss_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(),
@@ -87,13 +106,29 @@ def _backward_fake(g, z, tokens, weights, saved, cap):
 def _setup(ctx, inputs, output):
     z, tokens, weights, ctx.cap = inputs[0], inputs[1], inputs[5], inputs[9]
     ctx.save_for_backward(z, tokens, weights, output[2])
+    left, _GRADIENT.of = getattr(_GRADIENT, "of", None), None
+    if left is not None and left[0] is output[0]:
+        ctx.dz = left[1]
 
 
 def _backward(ctx, grads, bwd):
     if grads[0] is None:
         return (None,) * 10
     z, tokens, weights, saved = ctx.saved_tensors
+    dz = ctx.__dict__.pop("dz", None)
+    if dz is not None:
+        return (_scaled(dz, grads[0]), *(None,) * 9)
     return (bwd(grads[0], z, tokens, weights, saved, ctx.cap), *(None,) * 9)
+
+
+def _scaled(dz: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
+    """The forward's gradient times the loss's, in place (each is handed out once)."""
+    g32 = g if g.dtype == torch.float32 else g.to(torch.float32)
+    with _on(dz.device), _lib.timed("ts_policy_scale", 0):
+        status = _lib.load().ts_policy_scale(dz.data_ptr(), dz.numel(), _lib.dtype_code(dz.dtype), g32.data_ptr(),
+                                             _lib.stream_handle(dz.device))
+    _lib.check(status, "ts_policy_scale")
+    return dz
 
 
 _policy_op = HipOp("policy_loss", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,
@@ -175,7 +210,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, softcap: floa
     z, tok, cap, _ = _flat("token_log_probs", logits.detach(), tokens, softcap, {})
     z = _rows(z)
     lp = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-    io = _lib.PolicyIO(z.data_ptr(), tok.data_ptr(), None, None, None, None, lp.data_ptr(), None, None, None, None)
+    io = _lib.PolicyIO(z.data_ptr(), tok.data_ptr(), None, None, None, None, lp.data_ptr(), None, None, None, None,
+                       None)
     desc = _desc(z, cap)
     with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tok, lp)):
         status = _lib.load().ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))

@@ -568,7 +568,7 @@ class PolicyDesc(ctypes.Structure):
 
 class PolicyIO(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "tokens", "old_log_probs", "ref_log_probs", "advantages",
-                                               "weights", "log_probs", "coef", "lse", "parts", "loss")]
+                                               "weights", "log_probs", "coef", "lse", "parts", "loss", "dlogits")]
 
 
 ABI_VERSION = 19  # the include/thetascan_hip.h these bindings are written for
@@ -729,6 +729,8 @@ def load() -> ctypes.CDLL:
         lib.ts_delta_bwd.argtypes = [P(DeltaDesc), P(DeltaIO), P(DeltaGrads), ctypes.c_void_p, ctypes.c_size_t,
                                      ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.ts_policy_loss_parts.argtypes = [P(PolicyDesc), P(ctypes.c_int64)]
+        lib.ts_policy_one_pass.argtypes = [P(PolicyDesc), P(ctypes.c_int32)]
+        lib.ts_policy_scale.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_policy_loss_fwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p]
         lib.ts_policy_loss_bwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_scale_add_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 6

@@ -6,8 +6,9 @@
 //   dloss/dlp = w [ -r A where not clipped + kl (1 - e^{ref - lp}) ]
 //   dz_v = dloss/dlp (1[v = tok] - e^{y_v - lse}) (1 - (y_v / cap)^2)
 //
-// Bound by the logits' bytes: a row is read once a direction, by one wave (or by
-// a workgroup where it is long), with a running maximum and sum.  The sums of
+// Bound by the logits' bytes: a row is scanned by one wave (or by a workgroup where
+// it is long) with a running maximum and sum, and its gradient is formed by the same
+// workgroup right after (long rows in training) or by a kernel of its own.  The sums of
 // exponentials are fp32; a row's own terms are formed in fp64, for several rows
 // at once (a lane each, after the rows of its wave), and the rows are added in
 // fp64 in a fixed order: normalized advantages all but cancel in the sum.  A row
@@ -68,156 +69,84 @@ struct RowSpan {
   }
 };
 
-// WPR waves a row, R rows one after the other whose terms are formed together.
-template <typename E, bool CAP, int WPR, int R>
-__global__ __launch_bounds__(WPR <= 4 ? 256 : 64 * WPR) void policy_fwd_kernel(PolicyP p) {
-  constexpr int N = Vec16<E>::N, THREADS = WPR <= 4 ? 256 : 64 * WPR, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
-  constexpr int U = 4;
-  __shared__ float sm[WPR == 1 ? 1 : THREADS / 64], ss[WPR == 1 ? 1 : THREADS / 64];
-  __shared__ double sums[THREADS / 64];
-  const int tid = threadIdx.x, lane = tid & 63, gi = tid / LANES, li = tid % LANES;
-  const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + gi) * R;
-  const Logit<CAP> f(p.cap);
-  float mine_m = 0.f, mine_s = 1.f;  // of the row this lane finishes
-  for (int k = 0; k < R; ++k) {
-    const int64_t n = row0 + k;
-    // (uniform over the row's threads; with several waves a row over the workgroup)
-    if (n >= p.rows) break;
-    if (p.w && p.w[n] == 0.f) continue;
-    const E* row = (const E*)p.z + n * p.stride;
-    const RowSpan<E> span(row, p.V);
-    const Vec16<E>* vec = (const Vec16<E>*)(row + span.head);
-    float m = kLowest, s = 0.f;
-    auto one = [&](float x) {
-      const float top = fmaxf(m, x);
-      s = fmaf(s, ex<CAP>(m - top), ex<CAP>(x - top));
-      m = top;
-    };
-    for (int i = li; i < span.vecs; i += LANES * U) {
-      Vec16<E> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * LANES < span.vecs) v[u].raw = vec[i + u * LANES].raw;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * LANES < span.vecs) {
-          float x[N], top = m;
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            x[j] = f(tof(v[u].e[j]));
-            top = fmaxf(top, x[j]);
-          }
-          s *= ex<CAP>(m - top);
-#pragma unroll
-          for (int j = 0; j < N; ++j) s += ex<CAP>(x[j] - top);
-          m = top;
-        }
-    }
-    if (li < span.head) one(f(tof(row[li])));
-    for (int i = span.head + span.vecs * N + li; i < p.V; i += LANES) one(f(tof(row[i])));
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2);
-      s = s * ex<CAP>(m - top) + s2 * ex<CAP>(m2 - top);
-      m = top;
-    }
-    if constexpr (WPR > 1) {
-      const int w0 = gi * WPR;
-      if (lane == 0) {
-        sm[tid >> 6] = m;
-        ss[tid >> 6] = s;
-      }
-      __syncthreads();
-      m = kLowest;
-#pragma unroll
-      for (int w = 0; w < WPR; ++w) m = fmaxf(m, sm[w0 + w]);
-      s = 0.f;
-#pragma unroll
-      for (int w = 0; w < WPR; ++w) s = fmaf(ss[w0 + w], ex<CAP>(sm[w0 + w] - m), s);
-      __syncthreads();
-    }
-    if (li == k) {
-      mine_m = m;
-      mine_s = s;
-    }
-  }
-  // the rows' own terms, a lane each
-  double term = 0.0;
-  const int64_t n = row0 + li;
-  if (li < R && n < p.rows) {
-    const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
-    float coef = 0.f, logs = 0.f, lpf = 0.f;
-    if (w != 0.f) {
-      const double l2 = log2((double)mine_s), top = CAP ? (double)mine_m * kLn2 : (double)mine_m;
-      const int64_t tok = p.tokens[n];
-      double y = (double)NAN;  // a token that is none of the row's
-      if (tok >= 0 && tok < p.V) {
-        y = (double)tof(((const E*)p.z)[n * p.stride + tok]);
-        if (CAP) y = (double)p.cap * tanh(y / (double)p.cap);
-      }
-      const double lp = (y - top) - l2 * kLn2;
-      logs = (float)l2;
-      lpf = (float)lp;
-      if (p.adv) {
-        const double A = (double)p.adv[n], r = exp(lp - (double)p.old[n]);
-        const double edge = A > 0.0 ? 1.0 + p.high : 1.0 - p.low;
-        const bool flat = (A > 0.0 && r > edge) || (A < 0.0 && r < edge);
-        term = -(flat ? edge : r) * A;
-        double slope = flat ? 0.0 : -r * A;
-        if (p.ref) {
-          const double d = (double)p.ref[n] - lp, e = expm1(d);
-          term += p.kl * (e - d);
-          slope -= p.kl * e;
-        }
-        term *= (double)w;
-        coef = (float)(slope * (double)w);
-      }
-    }
-    p.lp[n] = lpf;
-    if (p.coef) {
-      p.coef[n] = coef;
-      p.lse[n] = mine_m;
-      p.lse[p.rows + n] = logs;
-    }
-  }
-  if (!p.part) return;
-#pragma unroll
-  for (int o = R / 2; o >= 1; o >>= 1) term += __shfl_xor(term, o, 64);
-  if (lane == 0) sums[tid >> 6] = term;
-  __syncthreads();
-  if (tid == 0) {
-    double total = 0.0;
-    for (int i = 0; i < GROUPS; ++i) total += sums[i * WPR];
-    p.part[blockIdx.x] = total;
-  }
-}
-
-__global__ __launch_bounds__(256) void policy_sum_kernel(const double* part, int64_t n, float* loss) {
-  __shared__ double s[256];
-  const int tid = threadIdx.x;
-  double sum = 0.0;
-  for (int64_t i = tid; i < n; i += 256) sum += part[i];
-  s[tid] = sum;
-  __syncthreads();
-  for (int o = 128; o >= 1; o >>= 1) {
-    if (tid < o) s[tid] += s[tid + o];
-    __syncthreads();
-  }
-  if (tid == 0) loss[0] = (float)s[0];
-}
-
-template <typename E, bool CAP, int WPR>
-__global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
-  constexpr int N = Vec16<E>::N, LANES = 64 * WPR, GROUPS = 256 / LANES, U = 4;
-  const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
-  const int64_t n = (int64_t)blockIdx.x * GROUPS + gi;
-  if (n >= p.rows) return;
-  const float c = p.coef[n] * p.g[0], top = p.lse[n], logs = p.lse[p.rows + n];
+// One row's terms from its maximum and sum, in fp64.
+template <typename E, bool CAP>
+__device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, float m, float s, float& lpf, float& coef,
+                                          float& logs, double& term) {
+  const double l2 = log2((double)s), top = CAP ? (double)m * kLn2 : (double)m;
   const int64_t tok = p.tokens[n];
-  const bool read = !p.w || p.w[n] != 0.f;
-  const Logit<CAP> f(p.cap);
-  const E* row = (const E*)p.z + n * p.stride;
-  E* out = (E*)p.dz + n * (int64_t)p.V;
+  double y = (double)NAN;  // a token that is none of the row's
+  if (tok >= 0 && tok < p.V) {
+    y = (double)tof(((const E*)p.z)[n * p.stride + tok]);
+    if (CAP) y = (double)p.cap * (1.0 - 2.0 / (1.0 + exp(2.0 * y / (double)p.cap)));
+  }
+  const double lp = (y - top) - l2 * kLn2;
+  logs = (float)l2;
+  lpf = (float)lp;
+  if (!p.adv) return;
+  const double A = (double)p.adv[n], r = exp(lp - (double)p.old[n]);
+  const double edge = A > 0.0 ? 1.0 + p.high : 1.0 - p.low;
+  const bool flat = (A > 0.0 && r > edge) || (A < 0.0 && r < edge);
+  term = -(flat ? edge : r) * A;
+  double slope = flat ? 0.0 : -r * A;
+  if (p.ref) {
+    const double d = (double)p.ref[n] - lp, e = expm1(d);
+    term += p.kl * (e - d);
+    slope -= p.kl * e;
+  }
+  term *= (double)w;
+  coef = (float)(slope * (double)w);
+}
+
+// This thread's share (of LANES) of a row's running maximum and sum.
+template <typename E, bool CAP, int LANES>
+__device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& f, int li, float& m, float& s) {
+  constexpr int N = Vec16<E>::N, U = 4;
+  const RowSpan<E> span(row, V);
+  const Vec16<E>* vec = (const Vec16<E>*)(row + span.head);
+  m = kLowest;
+  s = 0.f;
+  auto one = [&](float x) {
+    const float top = fmaxf(m, x);
+    s = fmaf(s, ex<CAP>(m - top), ex<CAP>(x - top));
+    m = top;
+  };
+  for (int i = li; i < span.vecs; i += LANES * U) {
+    Vec16<E> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * LANES < span.vecs) v[u].raw = vec[i + u * LANES].raw;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u * LANES < span.vecs) {
+        float x[N], top = m;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          x[j] = f(tof(v[u].e[j]));
+          top = fmaxf(top, x[j]);
+        }
+        s *= ex<CAP>(m - top);
+#pragma unroll
+        for (int j = 0; j < N; ++j) s += ex<CAP>(x[j] - top);
+        m = top;
+      }
+  }
+  if (li < span.head) one(f(tof(row[li])));
+  for (int i = span.head + span.vecs * N + li; i < V; i += LANES) one(f(tof(row[i])));
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2);
+    s = s * ex<CAP>(m - top) + s2 * ex<CAP>(m2 - top);
+    m = top;
+  }
+}
+
+// This thread's share of a row's gradient c dlp/dz: parts of the row's vectors
+// (part of parts), and its ends with the first part.
+template <typename E, bool CAP, int LANES>
+__device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read, const Logit<CAP>& f, float c, float top,
+                                         float logs, int64_t tok, int li, int part, int parts) {
+  constexpr int N = Vec16<E>::N, U = 4;
   auto grad = [&](float z, int v) {
     float x = z, slope = 1.f;
     if (CAP) {
@@ -229,9 +158,9 @@ __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
     return c * ((v == tok ? 1.f : 0.f) - prob) * slope;
   };
   // the output's vectors; where the logits' do not start with them, they are read element by element
-  const RowSpan<E> span(out, p.V);
+  const RowSpan<E> span(out, V);
   const bool together = (((uintptr_t)(row + span.head)) & 15) == 0;
-  for (int i = li + (int)blockIdx.y * LANES * U; i < span.vecs; i += (int)gridDim.y * LANES * U) {
+  for (int i = li + part * LANES * U; i < span.vecs; i += parts * LANES * U) {
     Vec16<E> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -258,10 +187,169 @@ __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
       }
     }
   }
-  if (blockIdx.y) return;
+  if (part) return;
   if (li < span.head) out[li] = read ? cvt<E>(grad(tof(row[li]), li)) : (E)0.0f;
-  for (int i = span.head + span.vecs * N + li; i < p.V; i += LANES)
-    out[i] = read ? cvt<E>(grad(tof(row[i]), i)) : (E)0.0f;
+  for (int i = span.head + span.vecs * N + li; i < V; i += LANES) out[i] = read ? cvt<E>(grad(tof(row[i]), i)) : (E)0.0f;
+}
+
+// WPR waves a row, R rows one after the other whose terms are formed together.
+template <typename E, bool CAP, int WPR, int R>
+__global__ __launch_bounds__(WPR <= 4 ? 256 : 64 * WPR) void policy_fwd_kernel(PolicyP p) {
+  constexpr int THREADS = WPR <= 4 ? 256 : 64 * WPR, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
+  __shared__ float sm[WPR == 1 ? 1 : THREADS / 64], ss[WPR == 1 ? 1 : THREADS / 64];
+  __shared__ double sums[THREADS / 64];
+  const int tid = threadIdx.x, lane = tid & 63, gi = tid / LANES, li = tid % LANES;
+  const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + gi) * R;
+  const Logit<CAP> f(p.cap);
+  float mine_m = 0.f, mine_s = 1.f;  // of the row this lane finishes
+  for (int k = 0; k < R; ++k) {
+    const int64_t n = row0 + k;
+    // (uniform over the row's threads; with several waves a row over the workgroup)
+    if (n >= p.rows) break;
+    if (p.w && p.w[n] == 0.f) continue;
+    const E* row = (const E*)p.z + n * p.stride;
+    float m, s;
+    row_scan<E, CAP, LANES>(row, p.V, f, li, m, s);
+    if constexpr (WPR > 1) {
+      const int w0 = gi * WPR;
+      if (lane == 0) {
+        sm[tid >> 6] = m;
+        ss[tid >> 6] = s;
+      }
+      __syncthreads();
+      m = kLowest;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) m = fmaxf(m, sm[w0 + w]);
+      s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) s = fmaf(ss[w0 + w], ex<CAP>(sm[w0 + w] - m), s);
+      __syncthreads();
+    }
+    if (li == k) {
+      mine_m = m;
+      mine_s = s;
+    }
+  }
+  // the rows' own terms, a lane each
+  double term = 0.0;
+  const int64_t n = row0 + li;
+  if (li < R && n < p.rows) {
+    const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
+    float coef = 0.f, logs = 0.f, lpf = 0.f;
+    if (w != 0.f) row_terms<E, CAP>(p, n, w, mine_m, mine_s, lpf, coef, logs, term);
+    p.lp[n] = lpf;
+    if (p.coef) {
+      p.coef[n] = coef;
+      p.lse[n] = mine_m;
+      p.lse[p.rows + n] = logs;
+    }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int o = R / 2; o >= 1; o >>= 1) term += __shfl_xor(term, o, 64);
+  if (lane == 0) sums[tid >> 6] = term;
+  __syncthreads();
+  if (tid == 0) {
+    double total = 0.0;
+    for (int i = 0; i < GROUPS; ++i) total += sums[i * WPR];
+    p.part[blockIdx.x] = total;
+  }
+}
+
+// The sum of the workgroups' parts, in a fixed order.
+__global__ __launch_bounds__(1024) void policy_sum_kernel(const double* part, int64_t n, float* loss) {
+  __shared__ double s[1024];
+  const int tid = threadIdx.x;
+  double sum = 0.0;
+  for (int64_t i = tid; i < n; i += 8 * 1024) {  // eight loads on their way at once
+    double v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i + u * 1024 < n ? part[i + u * 1024] : 0.0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += v[u];
+  }
+  s[tid] = sum;
+  __syncthreads();
+  for (int o = 512; o >= 1; o >>= 1) {
+    if (tid < o) s[tid] += s[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) loss[0] = (float)s[0];
+}
+
+template <typename E, bool CAP, int WPR>
+__global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
+  constexpr int LANES = 64 * WPR, GROUPS = 256 / LANES;
+  const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
+  const int64_t n = (int64_t)blockIdx.x * GROUPS + gi;
+  if (n >= p.rows) return;
+  const float c = p.coef[n] * p.g[0], top = p.lse[n], logs = p.lse[p.rows + n];
+  const int64_t tok = p.tokens[n];
+  const bool read = !p.w || p.w[n] != 0.f;
+  row_grad<E, CAP, LANES>((const E*)p.z + n * p.stride, (E*)p.dz + n * (int64_t)p.V, p.V, read, Logit<CAP>(p.cap), c, top,
+                          logs, tok, li, (int)blockIdx.y, (int)gridDim.y);
+}
+
+// Long rows in training: a workgroup scans a row and forms its gradient (for an
+// upstream gradient of one) at once, so that the second reading finds the row in
+// the caches: 8192 rows of 32768 bf16 logits 236 us, against 118 and 169 of the two kernels.
+template <typename E, bool CAP>
+__global__ __launch_bounds__(256) void policy_fused_kernel(PolicyP p) {
+  __shared__ float sm[4], ss[4], sc[3];
+  const int tid = threadIdx.x;
+  const int64_t n = blockIdx.x;
+  const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
+  const bool read = w != 0.f;  // uniform
+  const Logit<CAP> f(p.cap);
+  const E* row = (const E*)p.z + n * p.stride;
+  float m = 0.f, s = 1.f;
+  if (read) {
+    row_scan<E, CAP, 256>(row, p.V, f, tid, m, s);
+    if ((tid & 63) == 0) {
+      sm[tid >> 6] = m;
+      ss[tid >> 6] = s;
+    }
+    __syncthreads();
+    m = kLowest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, sm[i]);
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = fmaf(ss[i], ex<CAP>(sm[i] - m), s);
+  }
+  if (tid == 0) {
+    double term = 0.0;
+    float coef = 0.f, logs = 0.f, lpf = 0.f;
+    if (read) row_terms<E, CAP>(p, n, w, m, s, lpf, coef, logs, term);
+    p.lp[n] = lpf;
+    p.coef[n] = coef;
+    p.lse[n] = m;
+    p.lse[p.rows + n] = logs;
+    p.part[n] = term;
+    sc[0] = coef;
+    sc[1] = logs;
+  }
+  __syncthreads();
+  row_grad<E, CAP, 256>(row, (E*)p.dz + n * (int64_t)p.V, p.V, read, f, sc[0], m, sc[1], p.tokens[n], tid, 0, 1);
+}
+
+// x *= g, where g is not one.
+template <typename E>
+__global__ __launch_bounds__(256) void policy_scale_kernel(E* x, int64_t n, const float* g) {
+  constexpr int N = Vec16<E>::N;
+  const float scale = g[0];
+  if (scale == 1.f) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i * N < n; i += (int64_t)gridDim.x * 256) {
+    if (i * N + N <= n) {
+      Vec16<E> v;
+      v.raw = ((const Vec16<E>*)x)[i].raw;
+#pragma unroll
+      for (int j = 0; j < N; ++j) v.e[j] = cvt<E>(scale * tof(v.e[j]));
+      ((Vec16<E>*)x)[i].raw = v.raw;
+    } else {
+      for (int64_t j = i * N; j < n; ++j) x[j] = cvt<E>(scale * tof(x[j]));
+    }
+  }
 }
 
 }  // namespace ts
@@ -271,10 +359,15 @@ namespace {
 using ts::fail;
 using ts::PolicyP;
 
-// Rows of up to 2048 logits take a wave each (no barrier); longer ones a
-// workgroup of four, or of sixteen waves where the rows alone leave most of the
-// CUs without one.
-int waves_of(const PolicyP& p) { return p.V <= 2048 ? 1 : (p.rows < 256 && p.V > 8192 ? 16 : 4); }
+// Rows of up to 2048 logits take a wave each (no barrier), longer ones a workgroup
+// of four.
+int waves_of(const PolicyP& p) { return p.V <= 2048 ? 1 : 4; }
+
+// Whether training forms loss and gradient in one kernel: rows of a workgroup each.
+// (Of a wave's rows the fp64 terms are shared, and 65536 rows of 1024 fit the last
+// cache between two kernels: one kernel that held them in registers took 113 us
+// against 99.)
+bool one_pass(const PolicyP& p) { return waves_of(p) == 4; }
 
 // A row's fp64 terms cost a wave about as much as 1500 of its logits: where there
 // are rows enough to keep every CU busy all the same, eight rows share one pass.
@@ -295,11 +388,12 @@ void forward(const PolicyP& p, hipStream_t stream) {
 }
 template <typename E, bool CAP>
 void forward(const PolicyP& p, hipStream_t stream) {
-  switch (waves_of(p)) {
-    case 1: return forward<E, CAP, 1>(p, stream);
-    case 4: return forward<E, CAP, 4>(p, stream);
-    default: return forward<E, CAP, 16>(p, stream);
-  }
+  if (p.dz)
+    hipLaunchKernelGGL((ts::policy_fused_kernel<E, CAP>), dim3((unsigned)p.rows), dim3(256), 0, stream, p);
+  else if (waves_of(p) == 1)
+    forward<E, CAP, 1>(p, stream);
+  else
+    forward<E, CAP, 4>(p, stream);
 }
 template <typename E, bool CAP>
 void backward(const PolicyP& p, hipStream_t stream) {
@@ -344,8 +438,31 @@ int ts_policy_loss_parts(const ts_policy_desc* d, int64_t* parts) {
   PolicyP p;
   const int rc = setup(d, (const void*)16, (const int64_t*)16, &p);
   if (rc) return rc;
-  if (parts) *parts = forward_blocks(p);
+  const int64_t split = forward_blocks(p);
+  if (parts) *parts = one_pass(p) && p.rows > split ? p.rows : split;
   return TS_OK;
+}
+
+int ts_policy_one_pass(const ts_policy_desc* d, int32_t* yes) {
+  PolicyP p;
+  const int rc = setup(d, (const void*)16, (const int64_t*)16, &p);
+  if (rc) return rc;
+  if (yes) *yes = one_pass(p);
+  return TS_OK;
+}
+
+int ts_policy_scale(void* x, int64_t n, int32_t dtype, const float* g, hipStream_t stream) {
+  if (n < 0 || (n && (!x || ((uintptr_t)x & 15u) || !g)))
+    return fail(TS_ERR_VALUE, "policy_scale: missing or misaligned tensors");
+  if (dtype != TS_BF16 && dtype != TS_F32) return fail(TS_ERR_NOT_IMPLEMENTED, "policy_scale: bf16 or fp32 only");
+  if (n == 0) return TS_OK;
+  const int64_t blocks = (n / (dtype == TS_BF16 ? 8 : 4) + 256) / 256;
+  const dim3 grid((unsigned)(blocks < 2048 ? blocks : 2048));
+  if (dtype == TS_BF16)
+    hipLaunchKernelGGL(ts::policy_scale_kernel<ts::bf16>, grid, dim3(256), 0, stream, (ts::bf16*)x, n, g);
+  else
+    hipLaunchKernelGGL(ts::policy_scale_kernel<float>, grid, dim3(256), 0, stream, (float*)x, n, g);
+  return finish("policy_scale");
 }
 
 int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStream_t stream) {
@@ -359,6 +476,10 @@ int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStrea
   p.old = io->old_log_probs; p.ref = io->ref_log_probs; p.adv = io->loss ? io->advantages : nullptr; p.w = io->weights;
   p.lp = io->log_probs; p.coef = io->loss ? io->coef : nullptr; p.lse = io->lse;
   p.part = io->loss ? io->parts : nullptr;
+  p.dz = io->loss ? io->dlogits : nullptr;
+  if ((uintptr_t)p.dz & 15u) return fail(TS_ERR_VALUE, "policy_loss: misaligned gradient");
+  if (p.dz && !one_pass(p))
+    return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: rows of %d take two passes", p.V);
   if (d->rows) {
     if (d->dtype == TS_BF16)
       p.cap > 0.f ? forward<ts::bf16, true>(p, stream) : forward<ts::bf16, false>(p, stream);
@@ -366,8 +487,8 @@ int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStrea
       p.cap > 0.f ? forward<float, true>(p, stream) : forward<float, false>(p, stream);
   }
   if (io->loss)
-    hipLaunchKernelGGL(ts::policy_sum_kernel, dim3(1), dim3(256), 0, stream, (const double*)io->parts,
-                       d->rows ? forward_blocks(p) : 0, io->loss);
+    hipLaunchKernelGGL(ts::policy_sum_kernel, dim3(1), dim3(1024), 0, stream, (const double*)io->parts,
+                       !d->rows ? 0 : (p.dz ? p.rows : forward_blocks(p)), io->loss);
   return finish("policy_loss");
 }
 
