@@ -403,3 +403,23 @@ def test_long_sequences_in_segments(cuda, T, dk, dv, ragged, dtype):
             for name in ("q", "k", "v", "beta", "decay"):
                 s[name][b, :, m:] = 0.0
     check(s, cuda, lengths=lengths)
+
+
+@pytest.mark.parametrize("T", [100, 2100])
+def test_new_state_in_place_of_the_old(cuda, T):
+    """state_out = state, also where segments of the sequence run side by side:
+    the numbers of a call with a tensor of its own, whatever the lengths."""
+    import thetascan_amd as ts
+
+    s = on_gpu(inputs(5, 1, 2, T, 64, 64, BF, seed=T, state=True), cuda, False)
+    args = [s[n] for n in ("q", "k", "v", "beta", "decay")]
+    lengths = torch.tensor([T, 0, 1, T - 1, T // 2], device=cuda)
+    want, S = ts.gated_delta_rule(*args, state=s["state"], lengths=lengths, return_state=True)
+    for _ in range(3):
+        held = s["state"].clone()
+        out, got = ts.gated_delta_rule(*args, state=held, state_out=held, lengths=lengths, return_state=True)
+        assert got is held and torch.equal(held, S) and torch.equal(out, want)
+    # into a tensor of its own, without the state's being asked for
+    other = torch.full_like(S, float("nan"))
+    assert torch.equal(ts.gated_delta_rule(*args, state=s["state"], lengths=lengths, state_out=other), want)
+    assert torch.equal(other, S)

@@ -98,6 +98,17 @@ def test_states_steps_and_captured_steps(cuda, dtype):
         assert rel(a, b) <= (4 * 2.0 ** -8 if dtype == BF else 0.0)
 
 
+def test_compiled_mixer_is_the_eager_one(cuda):
+    m = mixer(cuda, BF)
+    x = torch.randn(2, 70, 256, device=cuda, dtype=BF)
+    y = m(x)
+    z = torch.compile(m, backend="aot_eager", fullgraph=True)(x)
+    assert torch.equal(y, z)
+    grads = [torch.autograd.grad(t, list(m.parameters()), torch.ones_like(t)) for t in (y, z)]
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
 def test_refused_states(cuda):
     m = mixer(cuda, F32)
     x = torch.randn(2, 4, 256, device=cuda)

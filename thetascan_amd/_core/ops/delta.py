@@ -305,6 +305,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
             raise ValueError("gated_delta_rule: state_out takes no part in gradients: call it without them")
         if not state_out.is_contiguous():
             raise ValueError("gated_delta_rule: state_out must be contiguous")
+        if torch.compiler.is_compiling():
+            raise NotImplementedError("gated_delta_rule: a traced call writes into no tensor it is given (state_out)")
     if T == 0:
         final = torch.zeros(B, H, dk, dv, dtype=torch.float32, device=q.device) if state is None else state.clone()
         if state_out is not None:

@@ -66,12 +66,13 @@ def _forward(z: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, adv: torc
     dz = None
     if one_pass and rows and eager_forward():
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        _GRADIENT.of = (loss, dz)
     io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), old.data_ptr(), _lib.ptr(ref), adv.data_ptr(),
                        _lib.ptr(weights), lp.data_ptr(), coef, coef + 4 * rows, at, loss.data_ptr(), _lib.ptr(dz))
     with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tokens, old, adv, ref, weights, lp, dz)):
         status = lib.ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
     _lib.check(status, "ts_policy_loss_fwd")
+    if dz is not None:
+        _GRADIENT.of = (loss, dz)
     return [loss, lp, saved]
 
 

@@ -257,8 +257,8 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
       if (unit)
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[d][i] = 16 * d + 4 * g + i == col ? 1.f : 0.f;
-    } else if (seg) {
-      if (mine && c0 < chunks) S[d] = *(const floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 16 * d + 4 * g);
+    } else if (p.nseg > 1) {
+      if (mine && (c0 < chunks || seg == 0)) S[d] = *(const floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 16 * d + 4 * g);
     } else if (p.state && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -436,6 +436,9 @@ __global__ __launch_bounds__(4 * DK, 1) void delta_segments_kernel(DeltaP p) {
       if (row < p.dk) S[i] = first[((int64_t)bh * p.dk + row) * p.dv + col];
     }
   }
+  // the forward's first segment too enters from here: its own reading of the state
+  // could meet the last segment's writing of its successor in place
+  if (!BACK) *(floatx4*)(p.seg_state + ((int64_t)bh * p.nseg * p.dvp + col) * DK + 16 * w + 4 * g) = S;
   const int steps = segs - 1, r = 16 * w + l16;
   floatx8 xf[KS], xn[KS];  // row r, columns in accumulator order; X is stored [column][row]
   floatx4 nf, nn;
