@@ -56,7 +56,8 @@ extern "C" {
  *     stride of 32 Mi elements and more was taken before).
  * 19: ts_delta_fwd / ts_delta_bwd / ts_delta_step (with their workspace sizes)
  *     and ts_policy_loss_fwd / ts_policy_loss_bwd /
- *     ts_policy_loss_parts / ts_policy_one_pass / ts_policy_scale; nothing earlier changed. */
+ *     ts_policy_loss_parts / ts_policy_one_pass / ts_policy_scale and ts_capture_id; nothing
+ *     earlier changed. */
 #define TS_ABI_VERSION 19
 
 enum ts_status {
@@ -1339,6 +1340,9 @@ int ts_policy_loss_fwd(const ts_policy_desc* desc, const ts_policy_io* io, hipSt
 int ts_policy_one_pass(const ts_policy_desc* desc, int32_t* one_pass);
 /* x[i] *= g[0] (n elements of ts_dtype `dtype`, 16-byte aligned); nothing where it is one. */
 int ts_policy_scale(void* x, int64_t n, int32_t dtype, const float* g, hipStream_t stream);
+/* The graph that `stream` is being captured into (0: none): what a forward leaves for
+ * its backward to change in place is only the backward's of the same graph. */
+int ts_capture_id(hipStream_t stream, uint64_t* id);
 /* dlogits [rows, V] contiguous from the forward's coef and lse and the loss's
  * gradient dloss (fp32, on the device). */
 int ts_policy_loss_bwd(const ts_policy_desc* desc, const ts_policy_io* io, const float* dloss, void* dlogits,

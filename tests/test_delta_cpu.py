@@ -149,3 +149,13 @@ def test_policy_entry_points_check_on_the_host():
         assert lib.ts_policy_loss_fwd(ctypes.byref(d()), ctypes.byref(missing), None) == _lib.TS_ERR_VALUE, name
     assert lib.ts_policy_loss_bwd(ctypes.byref(d()), ctypes.byref(full), None, FAKE, None) == _lib.TS_ERR_VALUE
     assert lib.ts_policy_loss_bwd(ctypes.byref(d()), ctypes.byref(full), FAKE, FAKE + 1, None) == _lib.TS_ERR_VALUE
+
+
+def test_sizes_past_a_launch_are_refused():
+    lib, n, m = _lib.load(), ctypes.c_size_t(), ctypes.c_int64()
+    for B, code in (((1 << 22) - 1, _lib.TS_OK), (1 << 22, _lib.TS_ERR_NOT_IMPLEMENTED)):
+        assert lib.ts_delta_workspace_bytes(ctypes.byref(desc(B=B, T=1)), ctypes.byref(n)) == code
+    for V, rows in ((2048, 1 << 26), (2049, 1 << 24)):
+        for less, code in ((1, _lib.TS_OK), (0, _lib.TS_ERR_NOT_IMPLEMENTED)):
+            d = _lib.PolicyDesc(rows - less, V, V, _lib.TS_BF16, 0.0, 0, 0.0, 0.0, 0.0)
+            assert lib.ts_policy_loss_parts(ctypes.byref(d), ctypes.byref(m)) == code

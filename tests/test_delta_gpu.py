@@ -423,3 +423,23 @@ def test_new_state_in_place_of_the_old(cuda, T):
     other = torch.full_like(S, float("nan"))
     assert torch.equal(ts.gated_delta_rule(*args, state=s["state"], lengths=lengths, state_out=other), want)
     assert torch.equal(other, S)
+
+
+def test_traced_calls_of_changing_lengths(cuda):
+    import thetascan_amd as ts
+
+    fn = torch.compile(lambda *x: ts.gated_delta_rule(*x, return_state=True), backend="aot_eager", dynamic=True,
+                       fullgraph=True)
+    for T in (70, 129, 5):
+        gen = torch.Generator(cuda).manual_seed(T)
+        args = [torch.randn(2, h, T, d, device=cuda, generator=gen).mul(d ** -0.5).requires_grad_()
+                for h, d in ((2, 16), (2, 16), (4, 24))]
+        args.append(torch.rand(2, 4, T, device=cuda, generator=gen).requires_grad_())
+        want, got = ts.gated_delta_rule(*args, return_state=True), fn(*args)
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+        for a, b in zip(*(torch.autograd.grad(x[0].sum() + x[1].sum(), args) for x in (want, got))):
+            assert torch.equal(a, b)
+        with torch.no_grad():
+            for a, b in zip(ts.gated_delta_rule(*args, return_state=True), fn(*args)):
+                assert torch.equal(a, b)

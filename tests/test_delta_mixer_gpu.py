@@ -183,3 +183,32 @@ def test_language_model_with_delta_memories_trains(cuda):
     assert all(x is not None and bool(torch.isfinite(x).all()) for x in grads)
     with pytest.raises(ValueError, match="memory must be"):
         lm.HybridLM(memory="gn")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_padding_is_not_read(cuda, dtype):
+    """Whatever the padding holds: outputs, the input's and the weights' gradients as
+    with zeros there."""
+    m = mixer(cuda, dtype)
+    x = torch.randn(3, 70, 256, device=cuda, dtype=dtype, generator=torch.Generator(cuda).manual_seed(1))
+    lengths = torch.tensor([70, 33, 0], device=cuda)
+    past = (torch.arange(70, device=cuda) >= lengths[:, None])[..., None]
+
+    def run(fill):
+        xi = x.masked_fill(past, fill).requires_grad_()
+        y = m(xi, lengths=lengths)
+        return [y, *torch.autograd.grad(y.float().square().sum(), (xi, *m.parameters()))]
+
+    for a, b in zip(run(0.0), run(float("nan"))):
+        assert torch.equal(a, b)
+    assert not run(float("nan"))[0].masked_select(past).any()
+    with pytest.raises(ValueError, match="lengths"):
+        m(x, lengths=lengths[:2])
+
+
+def test_no_tokens(cuda):
+    m = mixer(cuda, F32)
+    assert m(torch.zeros(2, 0, 256, device=cuda)).shape == (2, 0, 256)
+    with torch.no_grad():
+        y, s = m(torch.zeros(2, 0, 256, device=cuda), m.initial_state())
+    assert y.shape == (2, 0, 256) and s.position == 0

@@ -251,3 +251,48 @@ def test_compiled_call_is_the_eager_one(cuda):
     a, b = f(z), torch.compile(f, backend="aot_eager", fullgraph=True)(z)
     assert torch.equal(a, b)
     assert torch.equal(torch.autograd.grad(a, z)[0], torch.autograd.grad(b, z)[0])
+
+
+def test_a_captured_backward_replayed_more_often_than_its_forward(cuda):
+    """Forward and backward in graphs of their own, the backward replayed twice: the
+    second gives what the first gave (rows long enough to form loss and gradient in
+    one pass, an upstream gradient that is not one)."""
+    import thetascan_amd as ts
+
+    z, tokens, old, ref, adv = (x.to(cuda) for x in inputs(5, 2056, BF))
+
+    def loss_of(x):
+        return ts.policy_loss(x, tokens, old, adv, ref_log_probs=ref, kl=0.1)[0]
+
+    graphed = torch.cuda.make_graphed_callables(loss_of, (z.clone().requires_grad_(),))
+    for seed in (1, 2):
+        zr = inputs(5, 2056, BF, seed)[0].to(cuda).requires_grad_()
+        loss = graphed(zr)
+        got = [torch.autograd.grad(3.0 * loss, zr, retain_graph=True)[0].clone() for _ in range(2)]
+        assert torch.equal(got[0], got[1])
+        want = torch.autograd.grad(3.0 * loss_of(zr), zr)[0]
+        # (one rounding of the row's gradient here, the scaling's second one there)
+        assert (got[0].float() - want.float()).abs().max() <= 2 * 2.0 ** -8 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("V", [64, 2056])
+def test_traced_log_probs(cuda, V):
+    import thetascan_amd as ts
+
+    z, tokens = (x.to(cuda) for x in inputs(6, V, BF)[:2])
+    fn = torch.compile(lambda x, t: ts.token_log_probs(x.view(2, 3, -1), t, softcap=30.0), backend="eager", fullgraph=True)
+    got = fn(z, tokens.view(2, 3))
+    assert torch.equal(got, ts.token_log_probs(z, tokens, softcap=30.0).view(2, 3)) and not got.requires_grad
+
+
+def test_traced_loss_of_changing_sizes(cuda):
+    import thetascan_amd as ts
+
+    fn = torch.compile(lambda x, t, o, a: ts.policy_loss(x, t, o, a, softcap=30.0), backend="aot_eager", dynamic=True,
+                       fullgraph=True)
+    for N, V in ((6, 64), (9, 64), (9, 2056)):
+        z, tokens, old, _, adv = (x.to(cuda) for x in inputs(N, V, F32))
+        z.requires_grad_()
+        want, got = ts.policy_loss(z, tokens, old, adv, softcap=30.0), fn(z, tokens, old, adv)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(*(torch.autograd.grad(x[0], z)[0] for x in (want, got)))

@@ -65,9 +65,10 @@ def _desc(q, k, v, beta, decay, keep: bool) -> _lib.DeltaDesc:
     B, Hk, T, dk = q.shape
     _, H, _, dv = v.shape
     dt = q.dtype
-    return _lib.DeltaDesc(B, Hk, H, T, _width(dt, dk), _width(dt, dv), _lib.dtype_code(dt),
-                          _lib.dtype_code(beta.dtype), _lib.TS_F32 if decay is None else _lib.dtype_code(decay.dtype),
-                          int(keep))
+    # (int: a traced size becomes a number here)
+    return _lib.DeltaDesc(int(B), int(Hk), int(H), int(T), int(_width(dt, dk)), int(_width(dt, dv)),
+                          _lib.dtype_code(dt), _lib.dtype_code(beta.dtype),
+                          _lib.TS_F32 if decay is None else _lib.dtype_code(decay.dtype), int(keep))
 
 
 @functools.lru_cache(maxsize=256)

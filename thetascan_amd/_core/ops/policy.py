@@ -45,6 +45,15 @@ def _plan(rows: int, V: int, dtype: int, cap: bool) -> tuple[int, bool]:
     return n.value, bool(one.value)
 
 
+def _capture(device: torch.device) -> int:
+    """The graph that the device's current stream is captured into (0: none)."""
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    n = ctypes.c_uint64()
+    _lib.check(_lib.load().ts_capture_id(_lib.stream_handle(device), ctypes.byref(n)), "ts_capture_id")
+    return n.value
+
+
 def _rows(z: torch.Tensor) -> torch.Tensor:
     """Logits [rows, V] with contiguous rows (any distance apart)."""
     return z if z.stride(1) == 1 or z.shape[1] == 1 else z.contiguous()
@@ -70,14 +79,16 @@ def _forward(z: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, adv: torc
                        _lib.ptr(weights), lp.data_ptr(), coef, coef + 4 * rows, at, loss.data_ptr(), _lib.ptr(dz))
     with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tokens, old, adv, ref, weights, lp, dz)):
         status = lib.ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
+        graph = 0 if dz is None else _capture(z.device)
     _lib.check(status, "ts_policy_loss_fwd")
     if dz is not None:
-        _GRADIENT.of = (loss, dz)
+        _GRADIENT.of = (loss, dz, graph)
     return [loss, lp, saved]
 
 
 def _forward_fake(z, tokens, old, adv, ref, weights, low, high, kl, cap):
-    parts = _plan(z.shape[0], z.shape[1], _lib.dtype_code(z.dtype), cap > 0.0)[0]
+    # (a traced size becomes a number here: the parts follow no formula of it)
+    parts = _plan(int(z.shape[0]), int(z.shape[1]), _lib.dtype_code(z.dtype), cap > 0.0)[0]
     return [z.new_empty((), dtype=torch.float32), z.new_empty(z.shape[0], dtype=torch.float32),
             z.new_empty(max(2 * parts + 3 * z.shape[0], 2), dtype=torch.float32)]
 
@@ -109,16 +120,21 @@ def _setup(ctx, inputs, output):
     ctx.save_for_backward(z, tokens, weights, output[2])
     left, _GRADIENT.of = getattr(_GRADIENT, "of", None), None
     if left is not None and left[0] is output[0]:
-        ctx.dz = left[1]
+        ctx.dz = left[1:]
 
 
 def _backward(ctx, grads, bwd):
     if grads[0] is None:
         return (None,) * 10
     z, tokens, weights, saved = ctx.saved_tensors
-    dz = ctx.__dict__.pop("dz", None)
+    dz, graph = ctx.__dict__.pop("dz", (None, 0))
     if dz is not None:
-        return (_scaled(dz, grads[0]), *(None,) * 9)
+        # (a backward in a graph of its own may be replayed more often than the
+        # forward, and would scale what it has scaled)
+        with _on(dz.device):
+            same = _capture(dz.device) == graph
+        if same:
+            return (_scaled(dz, grads[0]), *(None,) * 9)
     return (bwd(grads[0], z, tokens, weights, saved, ctx.cap), *(None,) * 9)
 
 
@@ -184,7 +200,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch
     distance of the clipping borders from 1, below and above.  ``weights`` [...]
     multiplies each row's loss (default: the mean over all rows); a row of weight
     zero may hold anything in any input, and gives a log-probability of zero and a
-    gradient of zero.  ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.
+    gradient of zero.  At most 2^24 rows (2^26 of up to 2048 logits) a call.
+    ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.
     """
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl = float(low), float(high), float(kl)
@@ -209,6 +226,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, softcap: floa
     (soft-capped) logits [..., V]: what :func:`policy_loss` takes as
     ``old_log_probs`` and ``ref_log_probs``, in the same arithmetic."""
     z, tok, cap, _ = _flat("token_log_probs", logits.detach(), tokens, softcap, {})
+    if torch.compiler.is_compiling():  # (one opaque call, as the loss is)
+        none = torch.zeros(z.shape[0], dtype=torch.float32, device=z.device)
+        return _policy_op(z, tok, none, none, None, None, 0.0, 0.0, 0.0, cap)[1].view(tokens.shape)
     z = _rows(z)
     lp = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
     io = _lib.PolicyIO(z.data_ptr(), tok.data_ptr(), None, None, None, None, lp.data_ptr(), None, None, None, None,

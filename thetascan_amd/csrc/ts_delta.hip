@@ -503,7 +503,8 @@ int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const 
   if (d->dk > 128 || d->dv > 512)
     return fail(TS_ERR_NOT_IMPLEMENTED, "%s: at most 128 keys and 512 values, got %d and %d", what, d->dk, d->dv);
   if (d->dk % vec || d->dv % vec) return fail(TS_ERR_VALUE, "%s: widths must be multiples of 16 bytes", what);
-  if ((int64_t)d->B * d->H > 0x7fffffff || d->T > 0x7fffffff - 64)
+  // (a launch counts its threads in 32 bits: 256 to a head)
+  if ((int64_t)d->B * d->H >= 1 << 24 || d->T > 0x7fffffff - 64)
     return fail(TS_ERR_NOT_IMPLEMENTED, "%s: too many heads or tokens", what);
   if (!p) return TS_OK;
   memset(p, 0, sizeof(*p));

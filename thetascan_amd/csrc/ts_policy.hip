@@ -421,6 +421,9 @@ int setup(const ts_policy_desc* d, const void* z, const int64_t* tokens, PolicyP
   p->rows = d->rows; p->V = d->V; p->stride = d->stride; p->cap = d->cap;
   p->kl = d->kl; p->low = d->low; p->high = d->high;
   p->z = z; p->tokens = tokens;
+  // (a launch counts its threads in 32 bits)
+  if (d->rows * 64 * waves_of(*p) >= (int64_t)1 << 32)
+    return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: too many rows");
   return TS_OK;
 }
 
@@ -433,6 +436,15 @@ int finish(const char* what) {
 }  // namespace
 
 extern "C" {
+
+int ts_capture_id(hipStream_t stream, uint64_t* id) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  const hipError_t e = hipStreamGetCaptureInfo(stream, &status, &n);
+  if (e != hipSuccess) return fail(TS_ERR_RUNTIME, "capture id: %s", hipGetErrorString(e));
+  if (id) *id = status == hipStreamCaptureStatusNone ? 0 : n;
+  return TS_OK;
+}
 
 int ts_policy_loss_parts(const ts_policy_desc* d, int64_t* parts) {
   PolicyP p;

@@ -84,10 +84,16 @@ class GatedDelta(nn.Module):
     def forward(self, x: torch.Tensor, state: ThetaScanState | None = None, *, lengths: torch.Tensor | None = None):
         """``y`` [B,T,D]; with ``state`` the sequence continues from it (without
         autograd) and ``(y, new_state)`` is returned.  ``lengths`` [B] makes a
-        padded batch: tokens at or past a sequence's length write nothing, and their
-        outputs are zero."""
+        padded batch: tokens at or past a sequence's length are not read (whatever they
+        hold), write nothing, and their outputs are zero."""
         if state is None:
-            return self._mix(x, None, None, lengths)[0]
+            if lengths is not None:
+                if tuple(lengths.shape) != x.shape[:1]:
+                    raise ValueError(f"lengths must be [{x.shape[0]}], got {tuple(lengths.shape)}")
+                # (what the padding holds must not meet the projections, nor their gradients)
+                past = torch.arange(x.shape[1], device=x.device) >= lengths.unsqueeze(1)
+                x = x.masked_fill(past.unsqueeze(-1), 0.0)
+            return self._mix(x, None, None, lengths)[0] if x.shape[1] else torch.zeros_like(x)
         if lengths is not None:
             raise ValueError("a state counts one position for every sequence: a continued call takes no lengths")
         if state.fingerprint != config_fingerprint(self.cfg):
