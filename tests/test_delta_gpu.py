@@ -443,3 +443,23 @@ def test_traced_calls_of_changing_lengths(cuda):
         with torch.no_grad():
             for a, b in zip(ts.gated_delta_rule(*args, return_state=True), fn(*args)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,launch", [(12, "ts_delta_step"), (13, "ts_delta_fwd")])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dk,dv", [(64, 96), (72, 40)])
+def test_a_ragged_batch_of_few_tokens(cuda, T, launch, dk, dv, dtype):
+    """Both forms at the border between them, with sequences that end before T."""
+    import thetascan_amd as ts
+    from thetascan_amd import _lib
+
+    s = inputs(3, 2, 4, T, dk, dv, dtype, seed=T + dk, state=True)
+    lengths = torch.tensor([T, 5, 0])
+    dev = on_gpu(s, cuda, False)
+    ref, ref_S = reference(**s, lengths=lengths)
+    with torch.no_grad(), _lib.record_launches() as recs:
+        out, S = ts.gated_delta_rule(dev["q"], dev["k"], dev["v"], dev["beta"], dev["decay"], state=dev["state"],
+                                     lengths=lengths.to(cuda), return_state=True)
+    assert [r[0] for r in recs] == [launch]
+    assert rel(S, ref_S) <= STATE[dtype] and rel(out, ref) <= OUT[dtype]
+    assert torch.equal(S[2], dev["state"][2]) and not out[1, :, 5:].any() and not out[2].any()
