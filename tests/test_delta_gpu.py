@@ -463,3 +463,17 @@ def test_a_ragged_batch_of_few_tokens(cuda, T, launch, dk, dv, dtype):
     assert [r[0] for r in recs] == [launch]
     assert rel(S, ref_S) <= STATE[dtype] and rel(out, ref) <= OUT[dtype]
     assert torch.equal(S[2], dev["state"][2]) and not out[1, :, 5:].any() and not out[2].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,dk,dv,ragged", [(1, 385, 64, 64, False), (3, 700, 40, 72, True), (1, 517, 128, 128, False),
+                                              (2, 2111, 128, 24, True)])
+def test_short_sequences_in_uneven_segments(cuda, B, T, dk, dv, ragged, dtype):
+    s = inputs(B, 1, 2, T, dk, dv, dtype, seed=T, state=True)
+    s["decay"] = s["decay"] * 0.05
+    lengths = torch.tensor([T, T // 2, 129][:B]) if ragged else None
+    if ragged:
+        for b, m in enumerate(lengths.tolist()):
+            for name in ("q", "k", "v", "beta", "decay"):
+                s[name][b, :, m:] = 0.0
+    check(s, cuda, lengths=lengths)

@@ -481,18 +481,33 @@ template __global__ void delta_segments_kernel<64, true>(DeltaP);
 template __global__ void delta_segments_kernel<128, true>(DeltaP);
 
 // Segments of a sequence's chunks, one chain each.  A chain's chunks follow one
-// another (about 2.7 us each), so where heads and value columns alone leave CUs
-// without a workgroup, the sequence is cut: every segment but the last first forms
-// what it makes of its entering state (the transfer: dk more columns, no outputs),
-// then the segments run side by side.  Two workgroups a CU, no segment under eight
-// chunks (the cut costs about 12 us and 1.5 us a segment), 32 at most.
+// another, so where heads and value columns alone leave CUs without a workgroup, the
+// sequence is cut: every segment but the last first forms what it makes of its entering
+// state (the transfer: dk more columns, no outputs), then the segments run side by side.
+// n segments of nc / n chunks take n steps between them and 2 nc / n chunks of a chain:
+// best near n^2 = c nc.  Measured (forward, 64 keys): 8 heads of 1024 tokens 53 us
+// whole, 38 at four segments, 32 at eight, of 4096 65 at eight, 55 at 16, 61 at 32:
+// c = 4.  Where that is more than a workgroup a CU, chains side by side slow each other
+// and c = 2: 64 heads of 1024 tokens 61 whole, 51 at four, 53 at eight; 8 of 32768 170
+// at 16, 123 at 32, 129 at 64.  Two workgroups a CU at most.  Whole stay: five chunks and fewer
+// (four: 23.5 us, in two segments 25.9); with more than 64 chains, under 32 chunks (128
+// heads of 512 tokens 42 us, 47 in two, of 1024 68 and 70, of 2048 125 and in four 118);
+// more than 128 chains (160 heads of 2048 tokens 143, 152 in three).
 int delta_segments(const ts_delta_desc* d) {
   const int64_t chains = (int64_t)d->B * d->H * ((d->dv + 63) / 64);
-  const int nc = (d->T + kChunk - 1) / kChunk;
-  int64_t n = 512 / chains;
-  if (n > nc / 8) n = nc / 8;
-  if (n > 32) n = 32;
-  return n < 2 ? 1 : (int)n;
+  const int64_t nc = (d->T + kChunk - 1) / kChunk;
+  if (nc < 6 || chains > 128 || (chains > 64 && nc < 32)) return 1;
+  auto root = [](int64_t x) {
+    int64_t n = 1;
+    while ((n + 1) * (n + 1) <= x) ++n;
+    return n;
+  };
+  int64_t n = root(4 * nc);
+  if (n * chains > 256) n = root(2 * nc);
+  if (n > 512 / chains) n = 512 / chains;
+  if (n > nc / 2) n = nc / 2;
+  const int64_t each = (nc + n - 1) / n;
+  return (int)((nc + each - 1) / each);
 }
 
 int delta_check(const ts_delta_desc* d, const ts_delta_io* io, DeltaP* p, const char* what) {
