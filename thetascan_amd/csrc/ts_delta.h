@@ -56,9 +56,10 @@ struct DeltaP {
   float* state_out;        // or null
   char* prep;              // [B*H*nc] of prep_bytes
   int nseg, seg_chunks;    // segments of the chain, chunks of each
-  float* seg_x;            // [B*H*nseg][DK + dvp][DK], by column: X, then N of the transfers
-  float* seg_state;        // [B*H*nseg][dvp][DK], by column: states entering the segments
-                           // (backward: gradients behind them)
+  float* seg_x;            // [B*H*nseg][seg_stride]: X as rows, N, and (kept) X as columns
+  int64_t seg_stride;
+  float* seg_state;        // [B*H*nseg][dvp][DK]: states entering the segments (backward:
+                           // gradients behind them)
   void* u;                 // kept: [B*H*nc][dvp][64]
   void* s0;                // kept: [B*H*nc][dvp][DK]
   // backward
@@ -71,6 +72,7 @@ struct DeltaP {
   void* dr;                 // [B*H*nc][dvp][64]
   void* ds;                 // [B*H*nc][dvp][DK]
   float* seg_n;             // [B*H*nseg][dvp][DK]: N of the backward's transfers
+  // (of the segments' matrices a wave's accumulators follow one another: block_at)
 };
 
 __device__ __forceinline__ int delta_len(const DeltaP& p, int b) {
@@ -256,6 +258,14 @@ __device__ __forceinline__ floatx4 col4<float>(const float* rows, int pitch, int
   const float* a = rows + (r0 + 4 * (lane >> 4)) * pitch + c0 + (lane & 15);
   return floatx4{a[0], a[pitch], a[2 * pitch], a[3 * pitch]};
 }
+
+// Where a lane's part of the 16 x 16 block (rows 16d.., columns 16cb..) of a [DK x W]
+// fp32 matrix stands: blocks of a column block follow one another, in a block the
+// lanes' accumulators.
+template <int DK>
+__device__ __forceinline__ int block_at(int cb, int d, int lane) { return ((cb * (DK / 16) + d) * 64 + lane) * 4; }
+// Floats of a segment's transfer.
+inline int64_t seg_floats(int dkp, int dvp, bool kept) { return (int64_t)(dkp * (kept ? 2 : 1) + dvp) * dkp; }
 
 template <int DK, bool BACK>
 __global__ void delta_segments_kernel(DeltaP p);

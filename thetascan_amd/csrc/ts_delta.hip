@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[d][i] = 16 * d + 4 * g + i == col ? 1.f : 0.f;
     } else if (p.nseg > 1) {
-      if (mine && (c0 < chunks || seg == 0)) S[d] = *(const floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 16 * d + 4 * g);
+      if (mine && (c0 < chunks || seg == 0)) S[d] = *(const floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + seg) * p.dvp * DK + block_at<DK>(col0 / 16, d, lane));
     } else if (p.state && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -394,9 +394,34 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
   }
   if (!mine) return;
   if constexpr (TRANSFER) {
-    float* x = p.seg_x + (((int64_t)bh * p.nseg + seg) * (DK + p.dvp) + (unit ? 0 : DK) + col) * DK + 4 * g;
+    float* x = p.seg_x + ((int64_t)bh * p.nseg + seg) * p.seg_stride;
+    const int cb = col0 / 16;
+    if (!unit) {
 #pragma unroll
-    for (int d = 0; d < KB; ++d) *(floatx4*)(x + 16 * d) = S[d];
+      for (int d = 0; d < KB; ++d) *(floatx4*)(x + DK * DK + block_at<DK>(cb, d, lane)) = S[d];
+      return;
+    }
+    // as operands of the segments' products: a row's columns in accumulator order (over
+    // LDS, a wave its own columns'), and a column's rows
+    constexpr int TP = DK + 4;
+    static_assert(sizeof(Chunk) >= 4 * 16 * TP * sizeof(float), "columns of four waves");
+    float* t = (float*)smem + w * 16 * TP;
+    __syncthreads();  // the last chunk has been read
+#pragma unroll
+    for (int d = 0; d < KB; ++d) *(floatx4*)(t + l16 * TP + 16 * d + 4 * g) = S[d];
+    wave_lds_sync();
+#pragma unroll
+    for (int d = 0; d < KB; ++d) {
+      floatx4 r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = t[(4 * g + j) * TP + 16 * d + l16];
+      *(floatx4*)(x + ((d * KS + (cb >> 1)) * 64 + lane) * 8 + 4 * (cb & 1)) = r;
+    }
+    if (p.u)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        *(floatx8*)(x + (DK + p.dvp) * DK + ((cb * KS + s) * 64 + lane) * 8) =
+            __builtin_shufflevector(S[2 * s], S[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7);
     return;
   }
   // tokens behind the length (those of its own chunk are written above), by the segment of each
@@ -419,9 +444,9 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
 // The states entering the segments: S_{s+1} = X_s S_s + N_s for 16 value columns,
 // a wave for every 16 rows, on fp32 MFMA.  BACK: dS_s = X_s^T dS_{s+1} + N_s from
 // the last segment that any token reaches.  A step needs the whole state of the one
-// before (through LDS); its matrices are loaded a step ahead.
+// before (through LDS); its matrices are loaded a step ahead, whole lines at a time.
 template <int DK, bool BACK>
-__global__ __launch_bounds__(4 * DK, 1) void delta_segments_kernel(DeltaP p) {
+__global__ __launch_bounds__(4 * DK, 4) void delta_segments_kernel(DeltaP p) {
   constexpr int KS = DK / 32, PITCH = DK + 4;
   __shared__ __align__(16) float state[2][16 * PITCH];  // [column][row]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
@@ -438,26 +463,19 @@ __global__ __launch_bounds__(4 * DK, 1) void delta_segments_kernel(DeltaP p) {
   }
   // the forward's first segment too enters from here: its own reading of the state
   // could meet the last segment's writing of its successor in place
-  if (!BACK) *(floatx4*)(p.seg_state + ((int64_t)bh * p.nseg * p.dvp + col) * DK + 16 * w + 4 * g) = S;
-  const int steps = segs - 1, r = 16 * w + l16;
-  floatx8 xf[KS], xn[KS];  // row r, columns in accumulator order; X is stored [column][row]
+  const int at_block = block_at<DK>((int)blockIdx.y, w, lane);
+  if (!BACK) *(floatx4*)(p.seg_state + (int64_t)bh * p.nseg * p.dvp * DK + at_block) = S;
+  const int steps = segs - 1;
+  floatx8 xf[KS], xn[KS];  // row 16w + l16 of X (BACK: of X^T), columns in accumulator order
   floatx4 nf, nn;
   auto load = [&](int k, floatx8* x8, floatx4& n4) {
     const int s = BACK ? segs - 1 - k : k;
     const int64_t at = (int64_t)bh * p.nseg + s;
-    const float* x = p.seg_x + at * (DK + p.dvp) * DK;
-    n4 = *(const floatx4*)((BACK ? p.seg_n + at * p.dvp * DK : x + DK * DK) + col * DK + 16 * w + 4 * g);
+    const float* x = p.seg_x + at * p.seg_stride;
+    n4 = *(const floatx4*)((BACK ? p.seg_n + at * p.dvp * DK : x + DK * DK) + at_block);
+    if (BACK) x += (DK + p.dvp) * DK;
 #pragma unroll
-    for (int e = 0; e < KS; ++e) {
-      if (BACK) {
-        const floatx4 lo = *(const floatx4*)(x + r * DK + 32 * e + 4 * g);
-        const floatx4 hi = *(const floatx4*)(x + r * DK + 32 * e + 16 + 4 * g);
-        x8[e] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x8[e][j] = x[(32 * e + 16 * (j >> 2) + 4 * g + (j & 3)) * DK + r];
-      }
-    }
+    for (int e = 0; e < KS; ++e) x8[e] = *(const floatx8*)(x + ((w * KS + e) * 64 + lane) * 8);
   };
   if (steps > 0) load(0, xf, nf);
   loads_landed();
@@ -470,7 +488,7 @@ __global__ __launch_bounds__(4 * DK, 1) void delta_segments_kernel(DeltaP p) {
 #pragma unroll
     for (int e = 0; e < KS; ++e) S = mma32(xf[e], row_perm<float>(st + l16 * PITCH, e, g), S);
     const int to = BACK ? segs - 2 - k : k + 1;
-    *(floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + to) * p.dvp + col) * DK + 16 * w + 4 * g) = S;
+    *(floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + to) * p.dvp * DK + at_block) = S;
     nf = nn;
 #pragma unroll
     for (int e = 0; e < KS; ++e) xf[e] = xn[e];
@@ -567,7 +585,7 @@ Sizes sizes(const ts_delta_desc* d) {
   const size_t seg = (size_t)d->B * d->H * ts::delta_segments(d), dkp = padded_keys(d->dk);
   s.seg_x = s.seg_state = 0;
   if (ts::delta_segments(d) > 1) {
-    s.seg_x = seg * (dkp + dvp) * dkp * sizeof(float);
+    s.seg_x = seg * ts::seg_floats((int)dkp, (int)dvp, d->keep) * sizeof(float);
     s.seg_state = seg * dvp * dkp * sizeof(float);
   }
   s.u = n * dvp * 64 * es;
@@ -624,6 +642,7 @@ int ts_delta_fwd(const ts_delta_desc* d, const ts_delta_io* io, void* workspace,
   if (((int64_t)p.B * p.H * p.nc + 3) / 4 > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta: grid too large");
   p.prep = (char*)workspace;
   p.seg_x = (float*)(p.prep + s.prep);
+  p.seg_stride = ts::seg_floats(padded_keys(p.dk), p.dvp, d->keep);
   p.seg_state = (float*)(p.prep + s.prep + s.seg_x);
   if (d->keep) {
     p.u = p.prep + s.prep + s.seg_x + s.seg_state;

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
     if (TRANSFER) continue;
     if (!final) {
       if (mine && c0 < chunks)
-        S[d] = *(const floatx4*)(p.seg_state + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 16 * d + 4 * g);
+        S[d] = *(const floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + seg) * p.dvp * DK + block_at<DK>(col0 / 16, d, lane));
     } else if (p.dstate_out && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -187,9 +187,9 @@ __global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
   }
   if (!mine) return;
   if constexpr (TRANSFER) {
-    float* nn = p.seg_n + (((int64_t)bh * p.nseg + seg) * p.dvp + col) * DK + 4 * g;
+    float* nn = p.seg_n + ((int64_t)bh * p.nseg + seg) * p.dvp * DK;
 #pragma unroll
-    for (int d = 0; d < KB; ++d) *(floatx4*)(nn + 16 * d) = S[d];
+    for (int d = 0; d < KB; ++d) *(floatx4*)(nn + block_at<DK>(col0 / 16, d, lane)) = S[d];
     return;
   }
   const int last = min(p.T, (c0 + p.seg_chunks) * kChunk);
@@ -681,6 +681,7 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
     // X of the forward's transfers, which follow its chunks' records
     const size_t states = (size_t)p.B * p.H * p.nseg * p.dvp * dkp * sizeof(float);
     p.seg_x = (float*)((char*)saved + chunks * (int64_t)(es == 2 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>()));
+    p.seg_stride = ts::seg_floats((int)dkp, p.dvp, true);
     p.seg_state = (float*)ws;
     p.seg_n = (float*)(ws + states);
     ws += 2 * states;
