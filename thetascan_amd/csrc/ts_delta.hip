@@ -14,6 +14,14 @@
 // contraction).  Every operand that is not an input is a bf16 pair hi + lo: the
 // state is the long sum here and keeps about 1e-5 over any length, and an output
 // is rounded once.
+//
+// Bound by the bytes where heads and tokens are many: 64 heads of 4096 tokens of 64 x 64
+// (bf16, training) prepare 39 us (175 MB, 4.5 TB/s), transfers 44 (134 MB), forward 66 (311
+// MB, 4.7 TB/s).  Where they are few, by the chain: a chunk takes 4.4 us (64 keys, a workgroup
+// a CU; 7 with two), of which a third is matrix instructions.  Workgroups of
+// eight waves (forward of 32 heads of 2048 x 128 65 us against 56) and three waves a SIMD (77
+// against 65) were slower; P formed here again, not stored, 0.8 us more a chunk for 6 % less time
+// where bytes bind.
 
 #include "ts_delta.h"
 
@@ -444,7 +452,9 @@ __global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
 // The states entering the segments: S_{s+1} = X_s S_s + N_s for 16 value columns,
 // a wave for every 16 rows, on fp32 MFMA.  BACK: dS_s = X_s^T dS_{s+1} + N_s from
 // the last segment that any token reaches.  A step needs the whole state of the one
-// before (through LDS); its matrices are loaded a step ahead, whole lines at a time.
+// before (through LDS); its matrices are loaded a step ahead, whole lines at a time
+// (31 steps of 64 keys 20.6 us, 26.7 with X by column; four steps ahead gained nothing: a
+// step is 16 dependent fp32 MFMA and an exchange over LDS).
 template <int DK, bool BACK>
 __global__ __launch_bounds__(4 * DK, 4) void delta_segments_kernel(DeltaP p) {
   constexpr int KS = DK / 32, PITCH = DK + 4;

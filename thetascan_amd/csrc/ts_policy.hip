@@ -6,7 +6,8 @@
 //   dloss/dlp = w [ -r A where not clipped + kl (1 - e^{ref - lp}) ]
 //   dz_v = dloss/dlp (1[v = tok] - e^{y_v - lse}) (1 - (y_v / cap)^2)
 //
-// Bound by the logits' bytes: a row is scanned by one wave (or by a workgroup where
+// Bound by the logits' bytes (65536 rows of 1024 bf16: scan 46 us, gradient 50 us at 5.4
+// TB/s; 8192 rows of 32768 scan and gradient 236 us, 4.6 TB/s of what has to move): a row is scanned by one wave (or by a workgroup where
 // it is long) with a running maximum and sum, and its gradient is formed by the same
 // workgroup right after (long rows in training) or by a kernel of its own.  The sums of
 // exponentials are fp32; a row's own terms are formed in fp64, for several rows
@@ -194,8 +195,8 @@ __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read,
 
 // WPR waves a row, R rows one after the other whose terms are formed together.
 template <typename E, bool CAP, int WPR, int R>
-__global__ __launch_bounds__(WPR <= 4 ? 256 : 64 * WPR) void policy_fwd_kernel(PolicyP p) {
-  constexpr int THREADS = WPR <= 4 ? 256 : 64 * WPR, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
+__global__ __launch_bounds__(256) void policy_fwd_kernel(PolicyP p) {
+  constexpr int THREADS = 256, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
   __shared__ float sm[WPR == 1 ? 1 : THREADS / 64], ss[WPR == 1 ? 1 : THREADS / 64];
   __shared__ double sums[THREADS / 64];
   const int tid = threadIdx.x, lane = tid & 63, gi = tid / LANES, li = tid % LANES;
@@ -359,8 +360,9 @@ namespace {
 using ts::fail;
 using ts::PolicyP;
 
-// Rows of up to 2048 logits take a wave each (no barrier), longer ones a workgroup
-// of four.
+// Rows of up to 2048 logits take a wave each (no barrier), longer ones a workgroup of
+// four.  Forward, bf16: 65536 rows of 1024 51 us with a wave a row, 96 with four; 32768 of
+// 2048 46 and 66; 64 of 4096 10 and 7.
 int waves_of(const PolicyP& p) { return p.V <= 2048 ? 1 : 4; }
 
 // Whether training forms loss and gradient in one kernel: rows of a workgroup each.
@@ -369,35 +371,33 @@ int waves_of(const PolicyP& p) { return p.V <= 2048 ? 1 : 4; }
 // against 99.)
 bool one_pass(const PolicyP& p) { return waves_of(p) == 4; }
 
-// A row's fp64 terms cost a wave about as much as 1500 of its logits: where there
-// are rows enough to keep every CU busy all the same, eight rows share one pass.
-bool shares_terms(const PolicyP& p) { return p.rows * waves_of(p) >= 8 * 8192; }
+// A row's fp64 terms cost a wave about as much as 1500 of its logits: where there are
+// rows enough to keep every CU busy all the same, eight rows of a wave share one pass
+// (forward, rows of 1024: 8192 rows 15.4 us, shared 18.1; 16384 25.2 and 21.5; 65536 79
+// and 52).  Rows of a workgroup do not (8192 of 32768: 133 us, shared 155).
+bool shares_terms(const PolicyP& p) { return waves_of(p) == 1 && p.rows >= 16384; }
 
 int64_t forward_blocks(const PolicyP& p) {
   const int64_t per = (waves_of(p) == 1 ? 4 : 1) * (shares_terms(p) ? 8 : 1);
   return (p.rows + per - 1) / per;
 }
 
-template <typename E, bool CAP, int WPR>
-void forward(const PolicyP& p, hipStream_t stream) {
-  const dim3 grid((unsigned)forward_blocks(p)), block(WPR <= 4 ? 256 : 64 * WPR);
-  if (shares_terms(p))
-    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, WPR, 8>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, WPR, 1>), grid, block, 0, stream, p);
-}
 template <typename E, bool CAP>
 void forward(const PolicyP& p, hipStream_t stream) {
+  const dim3 grid((unsigned)forward_blocks(p));
   if (p.dz)
     hipLaunchKernelGGL((ts::policy_fused_kernel<E, CAP>), dim3((unsigned)p.rows), dim3(256), 0, stream, p);
+  else if (shares_terms(p))
+    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 1, 8>), grid, dim3(256), 0, stream, p);
   else if (waves_of(p) == 1)
-    forward<E, CAP, 1>(p, stream);
+    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 1, 1>), grid, dim3(256), 0, stream, p);
   else
-    forward<E, CAP, 4>(p, stream);
+    hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 4, 1>), grid, dim3(256), 0, stream, p);
 }
 template <typename E, bool CAP>
 void backward(const PolicyP& p, hipStream_t stream) {
-  // a row's vectors split over workgroups where the rows are few
+  // a long row's vectors over several workgroups where the rows are few (16 rows of 131072:
+  // 5.5 us against 37, 128 of 32768: 7.1 and 12.3)
   const int64_t rows = p.V <= 2048 ? (p.rows + 3) / 4 : p.rows;
   int parts = 1;
   if (p.V > 2048)
