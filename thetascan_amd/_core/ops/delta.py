@@ -75,17 +75,25 @@ def _desc(q, k, v, beta, decay, keep: bool) -> _lib.DeltaDesc:
 
 
 @functools.lru_cache(maxsize=256)
-def _bytes(backward: bool, *shape) -> int:
-    """Bytes of a call's workspace, by the descriptor's entries."""
-    lib, n = _lib.load(), ctypes.c_size_t()
-    size = lib.ts_delta_bwd_workspace_bytes if backward else lib.ts_delta_workspace_bytes
-    _lib.check(size(ctypes.byref(_lib.DeltaDesc(*shape)), ctypes.byref(n)), "ts_delta_workspace_bytes")
-    return n.value
+def _plan(q, v, dtype, beta, decay, keep) -> tuple[_lib.DeltaDesc, int, int]:
+    """A call's descriptor and the bytes of its forward's and backward's
+    workspaces, by shapes and dtypes."""
+    B, Hk, T, dk = q
+    desc = _lib.DeltaDesc(B, Hk, v[1], T, _width(dtype, dk), _width(dtype, v[3]), _lib.dtype_code(dtype),
+                          _lib.dtype_code(beta), _lib.TS_F32 if decay is None else _lib.dtype_code(decay), int(keep))
+    lib, fwd, bwd = _lib.load(), ctypes.c_size_t(), ctypes.c_size_t()
+    _lib.check(lib.ts_delta_workspace_bytes(ctypes.byref(desc), ctypes.byref(fwd)), "ts_delta_workspace_bytes")
+    _lib.check(lib.ts_delta_bwd_workspace_bytes(ctypes.byref(desc), ctypes.byref(bwd)), "ts_delta_bwd_workspace_bytes")
+    return desc, fwd.value, bwd.value
 
 
-def _workspace(d: _lib.DeltaDesc, device, backward: bool = False) -> torch.Tensor:
-    n = _bytes(backward, d.B, d.Hk, d.H, d.T, d.dk, d.dv, d.dtype, d.beta_dtype, d.decay_dtype, d.keep)
-    return torch.empty(n, dtype=torch.uint8, device=device)
+def _rows(x: torch.Tensor, vec: int) -> tuple[torch.Tensor, _lib.Strided]:
+    """``x`` (or its copy) as the kernels read it, and its description."""
+    s = x.stride()
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % vec or x.shape[3] % vec or x.data_ptr() % 16:
+        x = _kernel_view(x)
+        s = x.stride()
+    return x, _lib.Strided(x.data_ptr(), s[0], s[1], s[2])
 
 
 def _padded_state(state: torch.Tensor | None, dk: int, dv: int) -> torch.Tensor | None:
@@ -107,18 +115,18 @@ def _rows_like(x: torch.Tensor, dtype: torch.dtype, width: int) -> torch.Tensor:
 
 
 def _io(q, k, v, beta, decay, lengths, out, state, state_out) -> _lib.DeltaIO:
-    return _lib.DeltaIO(_lib.strided(q), _lib.strided(k), _lib.strided(v), _gate(beta),
-                        _gate(decay, decay is not None and decay.ndim == 1), _lib.strided(out), _lib.ptr(lengths),
-                        _lib.ptr(state), _lib.ptr(state_out))
+    """(q, k, v and out by their descriptions)"""
+    return _lib.DeltaIO(q, k, v, _gate(beta), _gate(decay, decay is not None and decay.ndim == 1), out,
+                        _lib.ptr(lengths), _lib.ptr(state), _lib.ptr(state_out))
 
 
 def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, step: bool, state_out=None):
     """``(out, state or None, workspace or None)`` at the padded widths' slices."""
     lib = _lib.load()
-    desc = _desc(q, k, v, beta, decay, keep)
+    desc, nbytes, _ = _plan(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, keep)
     B, H, T, dv = v.shape
-    dk, dkp, dvp = q.shape[-1], desc.dk, desc.dv
-    q, k, v4 = (_kernel_view(x) for x in (q, k, v))
+    dk, dkp, dvp, vec = q.shape[-1], desc.dk, desc.dv, _vec(q.dtype)
+    (q, sq), (k, sk), (v4, sv) = _rows(q, vec), _rows(k, vec), _rows(v, vec)
     out = _rows_like(v, q.dtype, dvp)
     given = _padded_state(state, dkp, dvp)
     final = None
@@ -127,7 +135,7 @@ def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, 
             final = state_out
         else:
             final = torch.empty(B, H, dkp, dvp, dtype=torch.float32, device=q.device)
-    io = _io(q, k, v4, beta, decay, lengths, out, given, final)
+    io = _io(sq, sk, sv, beta, decay, lengths, _lib.strided(out), given, final)
     work = None
     with _on(q.device):
         stream = _lib.stream_handle(q.device)
@@ -136,7 +144,7 @@ def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, 
                 status = lib.ts_delta_step(ctypes.byref(desc), ctypes.byref(io), stream)
             _lib.check(status, "ts_delta_step")
         else:
-            work = _workspace(desc, q.device)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             with _lib.timed("ts_delta_fwd", lambda: _lib.nbytes(q, k, v4, beta, decay, out, given, final)):
                 status = lib.ts_delta_fwd(ctypes.byref(desc), ctypes.byref(io), work.data_ptr(), work.numel(), stream)
             _lib.check(status, "ts_delta_fwd")
@@ -160,7 +168,10 @@ def _forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tens
 def _forward_fake(q, k, v, beta, decay, state, lengths, want_state, keep, step):
     B, H, _, dv = v.shape
     out = _rows_like(v, q.dtype, _width(q.dtype, dv))[..., :dv]
-    nbytes = _workspace(_desc(q, k, v, beta, decay, True), "meta").numel() if keep else 0
+    nbytes = 0
+    if keep:  # (a traced size becomes a number here)
+        nbytes = _plan(tuple(map(int, q.shape)), tuple(map(int, v.shape)), q.dtype, beta.dtype,
+                       None if decay is None else decay.dtype, True)[1]
     return [out, q.new_empty((B, H, q.shape[-1], dv) if want_state else (0,), dtype=torch.float32),
             q.new_empty(nbytes, dtype=torch.uint8)]
 
@@ -169,13 +180,13 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
                    v: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor | None, state: torch.Tensor | None,
                    lengths: torch.Tensor | None, saved: torch.Tensor, need_state: bool) -> list[torch.Tensor]:
     lib = _lib.load()
-    desc = _desc(q, k, v, beta, decay, True)
+    desc, _, nbytes = _plan(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, True)
     B, H, T, dv = v.shape
-    Hk, dk, dkp, dvp = q.shape[1], q.shape[-1], desc.dk, desc.dv
-    q4, k4, v4 = (_kernel_view(x) for x in (q, k, v))
+    dk, dkp, dvp, vec = q.shape[-1], desc.dk, desc.dv, _vec(q.dtype)
+    (q4, sq), (k4, sk), (v4, sv) = _rows(q, vec), _rows(k, vec), _rows(v, vec)
     if dout is None:
         dout = torch.zeros(B, H, T, dvp, dtype=q.dtype, device=q.device)
-    do4 = _kernel_view(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+    do4, so = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype), vec)
     given = None if dfinal is None else _padded_state(dfinal.to(torch.float32), dkp, dvp)
     dq, dk_, dv_ = _rows_like(q, q.dtype, dkp), _rows_like(k, q.dtype, dkp), _rows_like(v, q.dtype, dvp)
     dbeta = torch.empty(B, H, T, dtype=beta.dtype, device=q.device)
@@ -185,11 +196,11 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
         ddecay = torch.empty((H,) if per_head else (B, H, T), dtype=decay.dtype, device=q.device)
     dstate = torch.empty(B, H, dkp, dvp, dtype=torch.float32, device=q.device) if need_state else None
     # (the forward's output and states play no part here: out takes dout's rows)
-    io = _io(q4, k4, v4, beta, decay, lengths, do4, None, None)
-    grads = _lib.DeltaGrads(_lib.strided(do4), _lib.strided(dq), _lib.strided(dk_), _lib.strided(dv_), dbeta.data_ptr(),
+    io = _io(sq, sk, sv, beta, decay, lengths, so, None, None)
+    grads = _lib.DeltaGrads(so, _lib.strided(dq), _lib.strided(dk_), _lib.strided(dv_), dbeta.data_ptr(),
                             None if per_head else _lib.ptr(ddecay), _lib.ptr(ddecay) if per_head else None,
                             _lib.ptr(given), _lib.ptr(dstate))
-    work = _workspace(desc, q.device, backward=True)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     with _on(q.device), _lib.timed("ts_delta_bwd", lambda: _lib.nbytes(q4, k4, v4, do4, dq, dk_, dv_, dbeta, ddecay)):
         status = lib.ts_delta_bwd(ctypes.byref(desc), ctypes.byref(io), ctypes.byref(grads), saved.data_ptr(),
                                   saved.numel(), work.data_ptr(), work.numel(), _lib.stream_handle(q.device))
@@ -263,9 +274,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
 
     Differentiable in q, k, v, beta, the retention and the state.
     """
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        if x.ndim != 4:
-            raise ValueError(f"gated_delta_rule: {name} must be [B,H,T,D], got {tuple(x.shape)}")
+    if not q.ndim == k.ndim == v.ndim == 4:
+        name, x = next(i for i in (("q", q), ("k", k), ("v", v)) if i[1].ndim != 4)
+        raise ValueError(f"gated_delta_rule: {name} must be [B,H,T,D], got {tuple(x.shape)}")
     (B, Hk, T, dk), (Bv, H, Tv, dv) = q.shape, v.shape
     if k.shape != q.shape or Bv != B or Tv != T:
         raise ValueError(f"gated_delta_rule: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")

@@ -49,7 +49,7 @@ def _tensor_slots(args):
 
 class _Eager(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hip_op, args, *tensors):
+    def forward(ctx, hip_op, slots, args, *tensors):
         ctx.set_materialize_grads(False)
         _EAGER.active = True
         try:
@@ -58,7 +58,7 @@ class _Eager(torch.autograd.Function):
             _EAGER.active = False
         hip_op.setup(ctx, args, out)
         ctx.hip_op = hip_op
-        ctx.slots = _tensor_slots(args)
+        ctx.slots = slots
         ctx.multi = isinstance(out, (list, tuple))
         return tuple(out) if ctx.multi else out
 
@@ -70,7 +70,7 @@ class _Eager(torch.autograd.Function):
         for i, j in ctx.slots:
             g = res[i]
             flat.append(g if j is None else (None if g is None else g[j]))
-        return (None, None, *flat)
+        return (None, None, None, *flat)
 
 
 class HipOp:
@@ -89,10 +89,11 @@ class HipOp:
     def __call__(self, *args):
         if torch.compiler.is_compiling():
             return self.op(*args)
-        tensors = [args[i] if j is None else args[i][j] for i, j in _tensor_slots(args)]
+        slots = _tensor_slots(args)
+        tensors = [args[i] if j is None else args[i][j] for i, j in slots]
         if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
             # nothing to record (inference, streaming continuation): the
             # forward alone, without an autograd node around it
             return self.forward(*args)
-        out = _Eager.apply(self, args, *tensors)
+        out = _Eager.apply(self, slots, args, *tensors)
         return list(out) if isinstance(out, tuple) else out
