@@ -235,7 +235,7 @@ struct ForwardChunk {
 enum { kForward = 0, kKeep = 1, kTransfer = 2 };
 
 template <typename E, int DK, int MODE>
-__global__ __launch_bounds__(256, 2) void delta_forward_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   constexpr bool TRANSFER = MODE == kTransfer, KEEP = MODE == kKeep;
   typedef ForwardChunk<E, DK, TRANSFER> Chunk;

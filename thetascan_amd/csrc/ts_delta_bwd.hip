@@ -23,7 +23,7 @@
 // gradients over a chunk fp64.
 //
 // 64 heads of 4096 tokens of 64 x 64, bf16: transfers 33 us, chain 60 (262 MB, 4.4 TB/s),
-// gradients 86 (349 MB, 4.1 TB/s; its loads and its products take turns in a workgroup, three
+// gradients 80 (349 MB, 4.4 TB/s; its loads and its products take turns in a workgroup, three
 // of which share a CU: two took 102).  A persistent workgroup that loads a chunk ahead spilled (111).
 
 #include "ts_delta.h"
@@ -47,7 +47,7 @@ struct ChainChunk {
 // tokens alone (X^T of the forward's transfer makes the rest): nothing is stored
 // but that.
 template <typename E, int DK, bool TRANSFER>
-__global__ __launch_bounds__(256, 2) void delta_chain_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef typename Frag<E>::f8 f8;
   typedef ChainChunk<E, DK> Chunk;
@@ -227,8 +227,9 @@ struct GradsLds {
     E u[VB * TP], dr[VB * TP], s0[VB * PITCH], ds[VB * PITCH];
   };
   struct Pairs {
-    E k[kChunk * PITCH], q[kChunk * PITCH], a[kChunk * TP], m[kChunk * TP];
+    E q[kChunk * PITCH], a[kChunk * TP], m[kChunk * TP];
   };
+  E k[kChunk * PITCH];
   union {  // the passes over the value columns, then the pairs of tokens
     Pass pass;
     Pairs pairs;
@@ -304,9 +305,10 @@ struct Block {
   }
 };
 
-// (three waves a SIMD where the registers allow it: 102 us with two, 86 with three)
+// (three waves a SIMD where registers and LDS allow it: 102 us with two, 87 with three; the
+// keys have a place of their own, in LDS from the first pass on and out of registers: 80)
 template <typename E, int DK>
-__global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void delta_grads_kernel(DeltaP p) {
+__global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK>)) void delta_grads_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef TokFrag<E> TF;
   typedef typename Frag<E>::f8 f8;
@@ -406,6 +408,7 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void del
       fetch(v0);
     }
     const int rows = p.dvp - v0;
+    if (v0 == 0) kt.store(lds.k, PITCH, p.dk, tid);
     ut.store(lds.pass.u, rows, TP, tid);
     rt.store(lds.pass.dr, rows, TP, tid);
     st.store(lds.pass.s0, rows, PITCH, tid);
@@ -436,7 +439,6 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void del
     }
   }
   __syncthreads();  // the last pass has been read: keys, queries and pairs take its place
-  kt.store(lds.pairs.k, PITCH, p.dk, tid);
   qt.store(lds.pairs.q, PITCH, p.dk, tid);
   __syncthreads();
   // pairs (i, t): rows i = 16r + 4g + j, column t
@@ -452,8 +454,8 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void del
       floatx4 kk = zero4(), qk = zero4();
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const f8 ki = IO::ld8(lds.pairs.k + (16 * r + l16) * PITCH + 32 * s + 8 * g);
-        kk = mma32(ki, IO::ld8(lds.pairs.k + t * PITCH + 32 * s + 8 * g), kk);
+        const f8 ki = IO::ld8(lds.k + (16 * r + l16) * PITCH + 32 * s + 8 * g);
+        kk = mma32(ki, IO::ld8(lds.k + t * PITCH + 32 * s + 8 * g), kk);
         qk = mma32(ki, IO::ld8(lds.pairs.q + t * PITCH + 32 * s + 8 * g), qk);
       }
 #pragma unroll
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void del
   for (int d = 0; d < KB; ++d) {
     float qv[4], kv[4];
     ld4f<E>(lds.pairs.q + t * PITCH + 16 * d + 4 * g, qv);
-    ld4f<E>(lds.pairs.k + t * PITCH + 16 * d + 4 * g, kv);
+    ld4f<E>(lds.k + t * PITCH + 16 * d + 4 * g, kv);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       zq = fmaf(z[d][i], qv[i], zq);
@@ -525,7 +527,7 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : 2)) void del
     const f8 at = TF::get(lds.pairs.a, TP, 16 * w, s, lane), mt = TF::get(lds.pairs.m, TP, 16 * w, s, lane);
 #pragma unroll
     for (int d = 0; d < KB; ++d) {
-      const f8 kf = TF::get(lds.pairs.k, PITCH, 16 * d, s, lane);
+      const f8 kf = TF::get(lds.k, PITCH, 16 * d, s, lane);
       if (2 * s <= w) {
         z[d] = mma32(kf, af, z[d]);
         fu[d] = mma32(kf, mf, fu[d]);
