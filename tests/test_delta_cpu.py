@@ -159,3 +159,16 @@ def test_sizes_past_a_launch_are_refused():
         for less, code in ((1, _lib.TS_OK), (0, _lib.TS_ERR_NOT_IMPLEMENTED)):
             d = _lib.PolicyDesc(rows - less, V, V, _lib.TS_BF16, 0.0, 0, 0.0, 0.0, 0.0)
             assert lib.ts_policy_loss_parts(ctypes.byref(d), ctypes.byref(m)) == code
+
+
+def test_caps_that_fp32_does_not_hold_are_refused():
+    z = torch.zeros
+    for cap in (1e-50, 1e-40, 1e39):
+        with pytest.raises(ValueError, match="softcap"):
+            ts.policy_loss(z(5, 7), z(5, dtype=torch.int64), z(5), z(5), softcap=cap)
+        with pytest.raises(ValueError, match="softcap"):
+            ts.token_log_probs(z(5, 7), z(5, dtype=torch.int64), softcap=cap)
+    n = ctypes.c_int64()
+    for cap, code in ((1e-40, 1), (1e39, 1), (1e-30, 0), (1e30, 0)):
+        d = _lib.PolicyDesc(5, 7, 7, _lib.TS_F32, cap, 0, 0.0, 0.0, 0.0)
+        assert _lib.load().ts_policy_loss_parts(ctypes.byref(d), ctypes.byref(n)) == code

@@ -296,3 +296,15 @@ def test_traced_loss_of_changing_sizes(cuda):
         want, got = ts.policy_loss(z, tokens, old, adv, softcap=30.0), fn(z, tokens, old, adv)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert torch.equal(*(torch.autograd.grad(x[0], z)[0] for x in (want, got)))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V", [77, 2500])
+@pytest.mark.parametrize("cap", [0.5, 64.0, 64.5, 1000.0, 1e6, 1e20])
+def test_caps_of_any_size(cuda, cap, V, dtype):
+    """A cap far above the logits leaves them as they are (to fp32's rounding of logits
+    up to 16, 2^-20: within the bars above), one below them binds."""
+    z, tokens, old, ref, adv = inputs(9, V, dtype, seed=V)
+    y = cap * torch.tanh(z.double() / cap)
+    old = (torch.log_softmax(y, -1).gather(-1, tokens[:, None])[:, 0] + 0.4 * (old - ref)).float()
+    compare(cuda, z, tokens, old, adv, ref, None, (0.2, 0.28), 0.1, cap)

@@ -171,8 +171,8 @@ def _flat(what: str, logits: torch.Tensor, tokens: torch.Tensor, softcap: float 
         if x is not None and (x.shape != shape or not (x.is_floating_point() or name == "weights")):
             raise ValueError(f"{what}: {name} must be floating-point {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
     cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not 0.0 < cap < float("inf"):
-        raise ValueError(f"{what}: softcap must be positive (None: no cap), got {softcap}")
+    if softcap is not None and not 1e-29 <= cap <= 1e29:
+        raise ValueError(f"{what}: softcap must be positive, in [1e-29, 1e29] (None: no cap), got {softcap}")
     _lib.dtype_code(logits.dtype)
     device = logits.get_device()
     for x in (logits, tokens, *rows.values()):

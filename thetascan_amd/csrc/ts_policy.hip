@@ -40,21 +40,41 @@ struct PolicyP {
   void* dz;
 };
 
-// A logit as the softmax takes it, x, and e^x relative to a maximum.  Without a
-// cap x is the logit itself (the lowest finite one too, whose multiple by log2 e
-// is none); with a cap, x = log2 e cap tanh(z / cap) = log2 e (cap - 2 cap r) with
-// r = 1 / (1 + e^{2 z / cap}).
-template <bool CAP>
+// A logit as the softmax takes it, x, and e^x relative to a maximum.  kPlain: x is the
+// logit itself (the lowest finite one too, whose multiple by log2 e is none).  kCap: x =
+// log2 e cap tanh(z / cap) = log2 e (cap - 2 cap r) with r = 1 / (1 + e^{2 z / cap}), off by
+// cap 2^-23.  kWide (caps of 64 and more, where that is too much): x = cap tanh(z / cap), by
+// the series of tanh(t) / t to t^14 (its next term 2^-26) for |t| < 1/2.
+enum { kPlain = 0, kCap = 1, kWide = 2 };
+template <int CAP>
 struct Logit {
-  float in, mul, add;
-  __device__ __forceinline__ explicit Logit(float cap)
-      : in(CAP ? 2.f * kLog2eF / cap : 0.f), mul(-2.f * cap * kLog2eF), add(cap * kLog2eF) {}
+  float in, mul, add, inv;
+  __device__ __forceinline__ explicit Logit(float cap) {
+    const float unit = CAP == kCap ? kLog2eF : 1.f;
+    in = CAP ? 2.f * kLog2eF / cap : 0.f;
+    mul = -2.f * cap * unit;
+    add = cap * unit;
+    inv = CAP == kWide ? 1.f / cap : 0.f;
+  }
   __device__ __forceinline__ float sig(float z) const { return rcp(1.f + __builtin_amdgcn_exp2f(z * in)); }
-  __device__ __forceinline__ float operator()(float z) const { return CAP ? fmaf(sig(z), mul, add) : z; }
+  __device__ __forceinline__ float of(float z, float r) const {
+    const float x = fmaf(r, mul, add);
+    if (CAP != kWide) return x;
+    const float t = z * inv, u = t * t;
+    float y = -929569.f / 638512875.f;
+    y = fmaf(y, u, 21844.f / 6081075.f);
+    y = fmaf(y, u, -1382.f / 155925.f);
+    y = fmaf(y, u, 62.f / 2835.f);
+    y = fmaf(y, u, -17.f / 315.f);
+    y = fmaf(y, u, 2.f / 15.f);
+    y = fmaf(y, u, -1.f / 3.f);
+    return fabsf(t) < 0.5f ? fmaf(z * u, y, z) : x;
+  }
+  __device__ __forceinline__ float operator()(float z) const { return CAP ? of(z, sig(z)) : z; }
 };
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ float ex(float d) {
-  return __builtin_amdgcn_exp2f(CAP ? d : d * kLog2eF);
+  return __builtin_amdgcn_exp2f(CAP == kCap ? d : d * kLog2eF);
 }
 constexpr float kLowest = -3.402823466e38f;
 
@@ -71,15 +91,16 @@ struct RowSpan {
 };
 
 // One row's terms from its maximum and sum, in fp64.
-template <typename E, bool CAP>
+template <typename E, int CAP>
 __device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, float m, float s, float& lpf, float& coef,
                                           float& logs, double& term) {
-  const double l2 = log2((double)s), top = CAP ? (double)m * kLn2 : (double)m;
+  const double l2 = log2((double)s), top = CAP == kCap ? (double)m * kLn2 : (double)m;
   const int64_t tok = p.tokens[n];
   double y = (double)NAN;  // a token that is none of the row's
   if (tok >= 0 && tok < p.V) {
     y = (double)tof(((const E*)p.z)[n * p.stride + tok]);
-    if (CAP) y = (double)p.cap * (1.0 - 2.0 / (1.0 + exp(2.0 * y / (double)p.cap)));
+    if (CAP == kCap) y = (double)p.cap * (1.0 - 2.0 / (1.0 + exp(2.0 * y / (double)p.cap)));
+    if (CAP == kWide) y = (double)p.cap * tanh(y / (double)p.cap);
   }
   const double lp = (y - top) - l2 * kLn2;
   logs = (float)l2;
@@ -100,7 +121,7 @@ __device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, 
 }
 
 // This thread's share (of LANES) of a row's running maximum and sum.
-template <typename E, bool CAP, int LANES>
+template <typename E, int CAP, int LANES>
 __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& f, int li, float& m, float& s) {
   constexpr int N = Vec16<E>::N, U = 4;
   const RowSpan<E> span(row, V);
@@ -144,7 +165,7 @@ __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& 
 
 // This thread's share of a row's gradient c dlp/dz: parts of the row's vectors
 // (part of parts), and its ends with the first part.
-template <typename E, bool CAP, int LANES>
+template <typename E, int CAP, int LANES>
 __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read, const Logit<CAP>& f, float c, float top,
                                          float logs, int64_t tok, int li, int part, int parts) {
   constexpr int N = Vec16<E>::N, U = 4;
@@ -152,10 +173,10 @@ __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read,
     float x = z, slope = 1.f;
     if (CAP) {
       const float r = f.sig(z);
-      x = fmaf(r, f.mul, f.add);
+      x = f.of(z, r);
       slope = 4.f * r * (1.f - r);
     }
-    const float prob = __builtin_amdgcn_exp2f(CAP ? (x - top) - logs : fmaf(x - top, kLog2eF, -logs));
+    const float prob = __builtin_amdgcn_exp2f(CAP == kCap ? (x - top) - logs : fmaf(x - top, kLog2eF, -logs));
     return c * ((v == tok ? 1.f : 0.f) - prob) * slope;
   };
   // the output's vectors; where the logits' do not start with them, they are read element by element
@@ -194,7 +215,7 @@ __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read,
 }
 
 // WPR waves a row, R rows one after the other whose terms are formed together.
-template <typename E, bool CAP, int WPR, int R>
+template <typename E, int CAP, int WPR, int R>
 __global__ __launch_bounds__(256) void policy_fwd_kernel(PolicyP p) {
   constexpr int THREADS = 256, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
   __shared__ float sm[WPR == 1 ? 1 : THREADS / 64], ss[WPR == 1 ? 1 : THREADS / 64];
@@ -278,7 +299,7 @@ __global__ __launch_bounds__(1024) void policy_sum_kernel(const double* part, in
   if (tid == 0) loss[0] = (float)s[0];
 }
 
-template <typename E, bool CAP, int WPR>
+template <typename E, int CAP, int WPR>
 __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
   constexpr int LANES = 64 * WPR, GROUPS = 256 / LANES;
   const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
@@ -294,7 +315,7 @@ __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
 // Long rows in training: a workgroup scans a row and forms its gradient (for an
 // upstream gradient of one) at once, so that the second reading finds the row in
 // the caches: 8192 rows of 32768 bf16 logits 236 us, against 118 and 169 of the two kernels.
-template <typename E, bool CAP>
+template <typename E, int CAP>
 __global__ __launch_bounds__(256) void policy_fused_kernel(PolicyP p) {
   __shared__ float sm[4], ss[4], sc[3];
   const int tid = threadIdx.x;
@@ -382,7 +403,7 @@ int64_t forward_blocks(const PolicyP& p) {
   return (p.rows + per - 1) / per;
 }
 
-template <typename E, bool CAP>
+template <typename E, int CAP>
 void forward(const PolicyP& p, hipStream_t stream) {
   const dim3 grid((unsigned)forward_blocks(p));
   if (p.dz)
@@ -394,7 +415,7 @@ void forward(const PolicyP& p, hipStream_t stream) {
   else
     hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 4, 1>), grid, dim3(256), 0, stream, p);
 }
-template <typename E, bool CAP>
+template <typename E, int CAP>
 void backward(const PolicyP& p, hipStream_t stream) {
   // a long row's vectors over several workgroups where the rows are few (16 rows of 131072:
   // 5.5 us against 37, 128 of 32768: 7.1 and 12.3)
@@ -409,8 +430,27 @@ void backward(const PolicyP& p, hipStream_t stream) {
     hipLaunchKernelGGL((ts::policy_bwd_kernel<E, CAP, 4>), grid, dim3(256), 0, stream, p);
 }
 
+// The form of the cap (without one, up to 64, and above).
+int cap_of(const PolicyP& p) { return p.cap == 0.f ? ts::kPlain : (p.cap <= 64.f ? ts::kCap : ts::kWide); }
+template <typename E>
+void forward(const PolicyP& p, hipStream_t stream) {
+  switch (cap_of(p)) {
+    case ts::kPlain: return forward<E, ts::kPlain>(p, stream);
+    case ts::kCap: return forward<E, ts::kCap>(p, stream);
+    default: return forward<E, ts::kWide>(p, stream);
+  }
+}
+template <typename E>
+void backward(const PolicyP& p, hipStream_t stream) {
+  switch (cap_of(p)) {
+    case ts::kPlain: return backward<E, ts::kPlain>(p, stream);
+    case ts::kCap: return backward<E, ts::kCap>(p, stream);
+    default: return backward<E, ts::kWide>(p, stream);
+  }
+}
+
 int setup(const ts_policy_desc* d, const void* z, const int64_t* tokens, PolicyP* p) {
-  if (!d || d->rows < 0 || d->V < 1 || d->stride < 0 || !(d->cap >= 0.f) || !(d->low >= 0.0 && d->low <= 1.0) ||
+  if (!d || d->rows < 0 || d->V < 1 || d->stride < 0 || !(d->cap == 0.f || (d->cap >= 1e-30f && d->cap <= 1e30f)) || !(d->low >= 0.0 && d->low <= 1.0) ||
       !(d->high >= 0.0) || !(d->kl >= 0.0))
     return fail(TS_ERR_VALUE, "policy_loss: bad shape, cap, clip range or KL coefficient");
   if (d->dtype != TS_BF16 && d->dtype != TS_F32) return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: bf16 or fp32 only");
@@ -494,9 +534,9 @@ int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStrea
     return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: rows of %d take two passes", p.V);
   if (d->rows) {
     if (d->dtype == TS_BF16)
-      p.cap > 0.f ? forward<ts::bf16, true>(p, stream) : forward<ts::bf16, false>(p, stream);
+      forward<ts::bf16>(p, stream);
     else
-      p.cap > 0.f ? forward<float, true>(p, stream) : forward<float, false>(p, stream);
+      forward<float>(p, stream);
   }
   if (io->loss)
     hipLaunchKernelGGL(ts::policy_sum_kernel, dim3(1), dim3(1024), 0, stream, (const double*)io->parts,
@@ -515,9 +555,9 @@ int ts_policy_loss_bwd(const ts_policy_desc* d, const ts_policy_io* io, const fl
     return fail(TS_ERR_VALUE, "policy_loss bwd: missing or misaligned tensors");
   p.w = io->weights; p.coef = io->coef; p.lse = io->lse; p.g = dloss; p.dz = dlogits;
   if (d->dtype == TS_BF16)
-    p.cap > 0.f ? backward<ts::bf16, true>(p, stream) : backward<ts::bf16, false>(p, stream);
+    backward<ts::bf16>(p, stream);
   else
-    p.cap > 0.f ? backward<float, true>(p, stream) : backward<float, false>(p, stream);
+    backward<float>(p, stream);
   return finish("policy_loss bwd");
 }
 
