@@ -264,7 +264,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
     ``beta`` [B,H,T] or [B,H,T,1] the write strengths; ``retention`` the log
     retentions (at most zero, -inf a reset): None, one per value head [H], or one
     per token [B,H,T] or [B,H,T,1].  Keys are taken as given: the memory is stable
-    where ``beta_t |k_t|^2`` is at most 2.  dk is at most 128, dv at most 512.
+    where ``beta_t |k_t|^2`` is at most 2, and keeps its digits to about 1 (at 2, with
+    alike keys and no retention, bf16 gradients are off by 5 %, fp32's by 2e-5).  dk is at
+    most 128, dv at most 512.
 
     ``state`` continues from the fp32 state of an earlier call (None: zero).
     ``lengths`` [B] (integers, on the GPU, clamped to [0, T]) makes a padded batch:
