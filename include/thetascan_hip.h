@@ -1325,7 +1325,8 @@ typedef struct ts_policy_io {
   float *log_probs;                     /* out [rows], zero where not read       */
   float *coef, *lse;                    /* out [rows] and [2, rows], kept for the
                                            backward                              */
-  double *parts;                        /* scratch, ts_policy_loss_parts of them */
+  double *parts;                        /* scratch, ts_policy_loss_parts of them (few long rows
+                                           need them without a loss too) */
   float *loss;                          /* out [1], or NULL: log_probs only      */
   void *dlogits;                        /* out [rows, V] contiguous, 16-byte
                                            aligned: the logits' gradient for a

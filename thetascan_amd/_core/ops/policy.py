@@ -9,7 +9,7 @@ logits, with ``y = cap tanh(z / cap)`` (or z), ``lp = log softmax(y)[token]`` an
                        + kl (exp(ref - lp) - (ref - lp) - 1) ]
 
 One pass over the logits a direction (ts_policy_loss_fwd, ts_policy_loss_bwd);
-where a gradient is recorded and rows are long, the forward gives the gradient for a
+where a gradient is recorded and rows are long (and not few), the forward gives the gradient for a
 unit upstream gradient too, which the backward scales where it is another (a second
 backward of the same loss forms it again).  Neither the capped logits nor the
 probabilities are stored.  A row of weight zero
@@ -231,9 +231,10 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, softcap: floa
         return _policy_op(z, tok, none, none, None, None, 0.0, 0.0, 0.0, cap)[1].view(tokens.shape)
     z = _rows(z)
     lp = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-    io = _lib.PolicyIO(z.data_ptr(), tok.data_ptr(), None, None, None, None, lp.data_ptr(), None, None, None, None,
-                       None)
     desc = _desc(z, cap)
+    parts = torch.empty(_plan(z.shape[0], z.shape[1], desc.dtype, cap > 0.0)[0], dtype=torch.float64, device=z.device)
+    io = _lib.PolicyIO(z.data_ptr(), tok.data_ptr(), None, None, None, None, lp.data_ptr(), None, None, parts.data_ptr(),
+                       None, None)
     with _on(z.device), _lib.timed("ts_policy_loss_fwd", lambda: _lib.nbytes(z, tok, lp)):
         status = _lib.load().ts_policy_loss_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
     _lib.check(status, "ts_policy_loss_fwd")

@@ -9,7 +9,8 @@
 // Bound by the logits' bytes (65536 rows of 1024 bf16: scan 46 us, gradient 50 us at 5.4
 // TB/s; 8192 rows of 32768 scan and gradient 236 us, 4.6 TB/s of what has to move): a row is scanned by one wave (or by a workgroup where
 // it is long) with a running maximum and sum, and its gradient is formed by the same
-// workgroup right after (long rows in training) or by a kernel of its own.  The sums of
+// workgroup right after (long rows in training) or by a kernel of its own; few long rows
+// are scanned by several workgroups each.  The sums of
 // exponentials are fp32; a row's own terms are formed in fp64, for several rows
 // at once (a lane each, after the rows of its wave), and the rows are added in
 // fp64 in a fixed order: normalized advantages all but cancel in the sum.  A row
@@ -36,6 +37,8 @@ struct PolicyP {
   float *lp, *coef;
   float* lse;  // [2][rows]: the maximum, and log2 of the sum of e^{x - maximum}
   double* part;
+  float2* scans;  // [rows][split], where split is not one
+  int split;
   const float* g;
   void* dz;
 };
@@ -120,10 +123,13 @@ __device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, 
   coef = (float)(slope * (double)w);
 }
 
-// This thread's share (of LANES) of a row's running maximum and sum.
+constexpr int kScan = 4;  // vectors a thread has on their way at once
+// This thread's share (of LANES) of a row's running maximum and sum: part `part` of
+// `parts` of its vectors, and its ends with the first.
 template <typename E, int CAP, int LANES>
-__device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& f, int li, float& m, float& s) {
-  constexpr int N = Vec16<E>::N, U = 4;
+__device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& f, int li, float& m, float& s,
+                                         int part = 0, int parts = 1) {
+  constexpr int N = Vec16<E>::N, U = kScan;
   const RowSpan<E> span(row, V);
   const Vec16<E>* vec = (const Vec16<E>*)(row + span.head);
   m = kLowest;
@@ -133,7 +139,7 @@ __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& 
     s = fmaf(s, ex<CAP>(m - top), ex<CAP>(x - top));
     m = top;
   };
-  for (int i = li; i < span.vecs; i += LANES * U) {
+  for (int i = li + part * LANES * U; i < span.vecs; i += parts * LANES * U) {
     Vec16<E> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -153,8 +159,10 @@ __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& 
         m = top;
       }
   }
-  if (li < span.head) one(f(tof(row[li])));
-  for (int i = span.head + span.vecs * N + li; i < V; i += LANES) one(f(tof(row[i])));
+  if (part == 0) {
+    if (li < span.head) one(f(tof(row[li])));
+    for (int i = span.head + span.vecs * N + li; i < V; i += LANES) one(f(tof(row[i])));
+  }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2);
@@ -278,6 +286,59 @@ __global__ __launch_bounds__(256) void policy_fwd_kernel(PolicyP p) {
   }
 }
 
+// Few long rows: a row's scan in `split` workgroups, each leaving its maximum and sum,
+template <typename E, int CAP>
+__global__ __launch_bounds__(256) void policy_scan_kernel(PolicyP p) {
+  __shared__ float sm[4], ss[4];
+  const int tid = threadIdx.x;
+  const int64_t n = blockIdx.x;
+  if (p.w && p.w[n] == 0.f) return;  // uniform
+  float m, s;
+  row_scan<E, CAP, 256>((const E*)p.z + n * p.stride, p.V, Logit<CAP>(p.cap), tid, m, s, (int)blockIdx.y, p.split);
+  if ((tid & 63) == 0) {
+    sm[tid >> 6] = m;
+    ss[tid >> 6] = s;
+  }
+  __syncthreads();
+  if (tid) return;
+  m = kLowest;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, sm[i]);
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = fmaf(ss[i], ex<CAP>(sm[i] - m), s);
+  p.scans[n * p.split + blockIdx.y] = make_float2(m, s);
+}
+// and the rows' own terms from those, a lane each.
+template <typename E, int CAP>
+__global__ __launch_bounds__(64) void policy_join_kernel(PolicyP p) {
+  const int64_t n = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  double term = 0.0;
+  if (n < p.rows) {
+    const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
+    float coef = 0.f, logs = 0.f, lpf = 0.f, m = 0.f, s = 0.f;
+    if (w != 0.f) {
+      m = kLowest;
+      for (int i = 0; i < p.split; ++i) m = fmaxf(m, p.scans[n * p.split + i].x);
+      for (int i = 0; i < p.split; ++i) {
+        const float2 one = p.scans[n * p.split + i];
+        s = fmaf(one.y, ex<CAP>(one.x - m), s);
+      }
+      row_terms<E, CAP>(p, n, w, m, s, lpf, coef, logs, term);
+    }
+    p.lp[n] = lpf;
+    if (p.coef) {
+      p.coef[n] = coef;
+      p.lse[n] = m;
+      p.lse[p.rows + n] = logs;
+    }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) term += __shfl_xor(term, o, 64);
+  if (threadIdx.x == 0) p.part[blockIdx.x] = term;
+}
+
 // The sum of the workgroups' parts, in a fixed order.
 __global__ __launch_bounds__(1024) void policy_sum_kernel(const double* part, int64_t n, float* loss) {
   __shared__ double s[1024];
@@ -386,11 +447,23 @@ using ts::PolicyP;
 // 2048 46 and 66; 64 of 4096 10 and 7.
 int waves_of(const PolicyP& p) { return p.V <= 2048 ? 1 : 4; }
 
+// Workgroups of a row's scan where rows are few and long: each a turn of its loop or
+// more (8192 bf16 logits), 1024 in all at most, four at least.  Log-probabilities of 16
+// rows of 131072 bf16 logits 8.7 us against 22.8 with a workgroup a row, loss and gradient
+// 16.0 against 60.9; 128 rows of 32768 8.2 and 8.7, 17.9 and 22.8; 256 of 32768 10.4 and 9.1,
+// 23.9 and 24.8.
+int split_of(const PolicyP& p, bool bf) {
+  const int64_t turn = 256 * ts::kScan * (bf ? 8 : 4);
+  const int64_t fit = p.rows ? 1024 / p.rows : 1, n = p.V / turn;
+  const int64_t split = fit < n ? fit : n;
+  return split < 4 ? 1 : (int)split;
+}
+
 // Whether training forms loss and gradient in one kernel: rows of a workgroup each.
 // (Of a wave's rows the fp64 terms are shared, and 65536 rows of 1024 fit the last
 // cache between two kernels: one kernel that held them in registers took 113 us
 // against 99.)
-bool one_pass(const PolicyP& p) { return waves_of(p) == 4; }
+bool one_pass(const PolicyP& p) { return waves_of(p) == 4 && p.split == 1; }
 
 // A row's fp64 terms cost a wave about as much as 1500 of its logits: where there are
 // rows enough to keep every CU busy all the same, eight rows of a wave share one pass
@@ -399,6 +472,7 @@ bool one_pass(const PolicyP& p) { return waves_of(p) == 4; }
 bool shares_terms(const PolicyP& p) { return waves_of(p) == 1 && p.rows >= 16384; }
 
 int64_t forward_blocks(const PolicyP& p) {
+  if (p.split > 1) return (p.rows + 63) / 64;
   const int64_t per = (waves_of(p) == 1 ? 4 : 1) * (shares_terms(p) ? 8 : 1);
   return (p.rows + per - 1) / per;
 }
@@ -408,7 +482,10 @@ void forward(const PolicyP& p, hipStream_t stream) {
   const dim3 grid((unsigned)forward_blocks(p));
   if (p.dz)
     hipLaunchKernelGGL((ts::policy_fused_kernel<E, CAP>), dim3((unsigned)p.rows), dim3(256), 0, stream, p);
-  else if (shares_terms(p))
+  else if (p.split > 1) {
+    hipLaunchKernelGGL((ts::policy_scan_kernel<E, CAP>), dim3((unsigned)p.rows, (unsigned)p.split), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((ts::policy_join_kernel<E, CAP>), grid, dim3(64), 0, stream, p);
+  } else if (shares_terms(p))
     hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 1, 8>), grid, dim3(256), 0, stream, p);
   else if (waves_of(p) == 1)
     hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 1, 1>), grid, dim3(256), 0, stream, p);
@@ -461,6 +538,7 @@ int setup(const ts_policy_desc* d, const void* z, const int64_t* tokens, PolicyP
   p->rows = d->rows; p->V = d->V; p->stride = d->stride; p->cap = d->cap;
   p->kl = d->kl; p->low = d->low; p->high = d->high;
   p->z = z; p->tokens = tokens;
+  p->split = split_of(*p, d->dtype == TS_BF16);
   // (a launch counts its threads in 32 bits)
   if (d->rows * 64 * waves_of(*p) >= (int64_t)1 << 32)
     return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: too many rows");
@@ -490,8 +568,9 @@ int ts_policy_loss_parts(const ts_policy_desc* d, int64_t* parts) {
   PolicyP p;
   const int rc = setup(d, (const void*)16, (const int64_t*)16, &p);
   if (rc) return rc;
-  const int64_t split = forward_blocks(p);
-  if (parts) *parts = one_pass(p) && p.rows > split ? p.rows : split;
+  // (the scans' results stand behind the sums)
+  const int64_t n = forward_blocks(p);
+  if (parts) *parts = p.split > 1 ? n + p.rows * p.split : (one_pass(p) && p.rows > n ? p.rows : n);
   return TS_OK;
 }
 
@@ -528,6 +607,10 @@ int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStrea
   p.old = io->old_log_probs; p.ref = io->ref_log_probs; p.adv = io->loss ? io->advantages : nullptr; p.w = io->weights;
   p.lp = io->log_probs; p.coef = io->loss ? io->coef : nullptr; p.lse = io->lse;
   p.part = io->loss ? io->parts : nullptr;
+  if (p.split > 1) {
+    if (!io->parts) return fail(TS_ERR_VALUE, "policy_loss: missing parts");
+    p.scans = (float2*)(io->parts + forward_blocks(p));
+  }
   p.dz = io->loss ? io->dlogits : nullptr;
   if ((uintptr_t)p.dz & 15u) return fail(TS_ERR_VALUE, "policy_loss: misaligned gradient");
   if (p.dz && !one_pass(p))
