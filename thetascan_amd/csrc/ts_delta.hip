@@ -266,7 +266,9 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[d][i] = 16 * d + 4 * g + i == col ? 1.f : 0.f;
     } else if (p.nseg > 1) {
-      if (mine && (c0 < chunks || seg == 0)) S[d] = *(const floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + seg) * p.dvp * DK + block_at<DK>(col0 / 16, d, lane));
+      if (mine && (c0 < chunks || seg == 0))
+        S[d] = *(const floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + seg) * p.dvp * DK +
+                                 block_at<DK>(col0 / 16, d, lane));
     } else if (p.state && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

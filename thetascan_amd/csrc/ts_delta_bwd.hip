@@ -75,7 +75,8 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
     if (TRANSFER) continue;
     if (!final) {
       if (mine && c0 < chunks)
-        S[d] = *(const floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + seg) * p.dvp * DK + block_at<DK>(col0 / 16, d, lane));
+        S[d] = *(const floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + seg) * p.dvp * DK +
+                                 block_at<DK>(col0 / 16, d, lane));
     } else if (p.dstate_out && on) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -695,7 +696,8 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
   if (p.nseg > 1) {
     // X of the forward's transfers, which follow its chunks' records
     const size_t states = (size_t)p.B * p.H * p.nseg * p.dvp * dkp * sizeof(float);
-    p.seg_x = (float*)((char*)saved + chunks * (int64_t)(es == 2 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>()));
+    const size_t rec = es == 2 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>();
+    p.seg_x = (float*)((char*)saved + (size_t)chunks * rec);
     p.seg_stride = ts::seg_floats((int)dkp, p.dvp, true);
     p.seg_state = (float*)ws;
     p.seg_n = (float*)(ws + states);

@@ -7,14 +7,14 @@
 //   dz_v = dloss/dlp (1[v = tok] - e^{y_v - lse}) (1 - (y_v / cap)^2)
 //
 // Bound by the logits' bytes (65536 rows of 1024 bf16: scan 46 us, gradient 50 us at 5.4
-// TB/s; 8192 rows of 32768 scan and gradient 236 us, 4.6 TB/s of what has to move): a row is scanned by one wave (or by a workgroup where
-// it is long) with a running maximum and sum, and its gradient is formed by the same
-// workgroup right after (long rows in training) or by a kernel of its own; few long rows
-// are scanned by several workgroups each.  The sums of
-// exponentials are fp32; a row's own terms are formed in fp64, for several rows
-// at once (a lane each, after the rows of its wave), and the rows are added in
-// fp64 in a fixed order: normalized advantages all but cancel in the sum.  A row
-// of weight zero is not read; its log-probability is given as zero, its gradient
+// TB/s; 8192 rows of 32768: both 236 us, 4.6 TB/s of what has to move): a row is
+// scanned by one wave (or by a workgroup where it is long) with a running maximum and
+// sum, and its gradient is formed by the same workgroup right after (long rows in
+// training) or by a kernel of its own; few long rows are scanned by several workgroups
+// each.  The sums of exponentials are fp32; a row's own terms are formed in fp64, for
+// several rows at once (a lane each, after the rows of its wave), and the rows are
+// added in fp64 in a fixed order: normalized advantages all but cancel in the sum.  A
+// row of weight zero is not read; its log-probability is given as zero, its gradient
 // too.
 
 #include "ts_common.h"
@@ -483,7 +483,8 @@ void forward(const PolicyP& p, hipStream_t stream) {
   if (p.dz)
     hipLaunchKernelGGL((ts::policy_fused_kernel<E, CAP>), dim3((unsigned)p.rows), dim3(256), 0, stream, p);
   else if (p.split > 1) {
-    hipLaunchKernelGGL((ts::policy_scan_kernel<E, CAP>), dim3((unsigned)p.rows, (unsigned)p.split), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((ts::policy_scan_kernel<E, CAP>), dim3((unsigned)p.rows, (unsigned)p.split), dim3(256), 0,
+                       stream, p);
     hipLaunchKernelGGL((ts::policy_join_kernel<E, CAP>), grid, dim3(64), 0, stream, p);
   } else if (shares_terms(p))
     hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 1, 8>), grid, dim3(256), 0, stream, p);
@@ -527,7 +528,8 @@ void backward(const PolicyP& p, hipStream_t stream) {
 }
 
 int setup(const ts_policy_desc* d, const void* z, const int64_t* tokens, PolicyP* p) {
-  if (!d || d->rows < 0 || d->V < 1 || d->stride < 0 || !(d->cap == 0.f || (d->cap >= 1e-30f && d->cap <= 1e30f)) || !(d->low >= 0.0 && d->low <= 1.0) ||
+  if (!d || d->rows < 0 || d->V < 1 || d->stride < 0 ||
+      !(d->cap == 0.f || (d->cap >= 1e-30f && d->cap <= 1e30f)) || !(d->low >= 0.0 && d->low <= 1.0) ||
       !(d->high >= 0.0) || !(d->kl >= 0.0))
     return fail(TS_ERR_VALUE, "policy_loss: bad shape, cap, clip range or KL coefficient");
   if (d->dtype != TS_BF16 && d->dtype != TS_F32) return fail(TS_ERR_NOT_IMPLEMENTED, "policy_loss: bf16 or fp32 only");
