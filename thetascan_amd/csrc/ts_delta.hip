@@ -454,12 +454,12 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
 // The states entering the segments: S_{s+1} = X_s S_s + N_s for 16 value columns,
 // a wave for every 16 rows, on fp32 MFMA.  BACK: dS_s = X_s^T dS_{s+1} + N_s from
 // the last segment that any token reaches.  A step needs the whole state of the one
-// before (through LDS); its matrices are loaded a step ahead, whole lines at a time
-// (31 steps of 64 keys 20.6 us, 26.7 with X by column; four steps ahead gained nothing: a
-// step is 16 dependent fp32 MFMA and an exchange over LDS).
+// before (through LDS); its matrices are loaded two steps ahead, whole lines at a time
+// (31 steps of 64 keys 18.8 us, a step ahead 20.7, with X by column 26.7; three ahead 18.1,
+// but spilled with 128 keys: seven steps 24 us against 17).
 template <int DK, bool BACK>
 __global__ __launch_bounds__(4 * DK, 4) void delta_segments_kernel(DeltaP p) {
-  constexpr int KS = DK / 32, PITCH = DK + 4;
+  constexpr int KS = DK / 32, PITCH = DK + 4, AHEAD = 2;
   __shared__ __align__(16) float state[2][16 * PITCH];  // [column][row]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
   const int bh = blockIdx.x, b = bh / p.H, col = (int)blockIdx.y * 16 + l16;
@@ -478,32 +478,35 @@ __global__ __launch_bounds__(4 * DK, 4) void delta_segments_kernel(DeltaP p) {
   const int at_block = block_at<DK>((int)blockIdx.y, w, lane);
   if (!BACK) *(floatx4*)(p.seg_state + (int64_t)bh * p.nseg * p.dvp * DK + at_block) = S;
   const int steps = segs - 1;
-  floatx8 xf[KS], xn[KS];  // row 16w + l16 of X (BACK: of X^T), columns in accumulator order
-  floatx4 nf, nn;
+  if (steps < 1) return;
+  floatx8 xf[AHEAD][KS];  // row 16w + l16 of X (BACK: of X^T), columns in accumulator order
+  floatx4 nf[AHEAD];
   auto load = [&](int k, floatx8* x8, floatx4& n4) {
-    const int s = BACK ? segs - 1 - k : k;
-    const int64_t at = (int64_t)bh * p.nseg + s;
+    k = min(k, steps - 1);
+    const int64_t at = (int64_t)bh * p.nseg + (BACK ? segs - 1 - k : k);
     const float* x = p.seg_x + at * p.seg_stride;
     n4 = *(const floatx4*)((BACK ? p.seg_n + at * p.dvp * DK : x + DK * DK) + at_block);
     if (BACK) x += (DK + p.dvp) * DK;
 #pragma unroll
     for (int e = 0; e < KS; ++e) x8[e] = *(const floatx8*)(x + ((w * KS + e) * 64 + lane) * 8);
   };
-  if (steps > 0) load(0, xf, nf);
-  loads_landed();
-  for (int k = 0; k < steps; ++k) {
-    load(min(k + 1, steps - 1), xn, nn);
-    float* st = state[k & 1];
-    *(floatx4*)(st + l16 * PITCH + 16 * w + 4 * g) = S;
-    __syncthreads();
-    S = nf;
 #pragma unroll
-    for (int e = 0; e < KS; ++e) S = mma32(xf[e], row_perm<float>(st + l16 * PITCH, e, g), S);
-    const int to = BACK ? segs - 2 - k : k + 1;
-    *(floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + to) * p.dvp * DK + at_block) = S;
-    nf = nn;
+  for (int i = 0; i < AHEAD; ++i) load(i, xf[i], nf[i]);
+  for (int k0 = 0; k0 < steps; k0 += AHEAD) {
 #pragma unroll
-    for (int e = 0; e < KS; ++e) xf[e] = xn[e];
+    for (int i = 0; i < AHEAD; ++i) {
+      const int k = k0 + i;
+      if (i && k >= steps) break;  // uniform
+      float* st = state[k & 1];
+      *(floatx4*)(st + l16 * PITCH + 16 * w + 4 * g) = S;
+      __syncthreads();
+      S = nf[i];
+#pragma unroll
+      for (int e = 0; e < KS; ++e) S = mma32(xf[i][e], row_perm<float>(st + l16 * PITCH, e, g), S);
+      load(k + AHEAD, xf[i], nf[i]);
+      const int to = BACK ? segs - 2 - k : k + 1;
+      *(floatx4*)(p.seg_state + ((int64_t)bh * p.nseg + to) * p.dvp * DK + at_block) = S;
+    }
   }
 }
 
