@@ -564,11 +564,13 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
 }
 
 // Rows of `rep` value heads added up, in head order: x [B,H,T,W] fp32
-// contiguous -> out [B,H/rep,T,W].  Bound by its bytes: 32 heads of 2048 tokens of 128,
-// two to a key, 42 MB in 8.8 us (4.8 TB/s).
+// contiguous -> out [B,H/rep,T,W], for the queries and (y = 1) the keys.  Bound by its
+// bytes: 32 heads of 2048 tokens of 128, two to a key, 84 MB in 14.8 us (two launches took 17.6).
 template <typename E>
-__global__ __launch_bounds__(256) void delta_group_sum_kernel(const float* x, ts_strided out, int Hk, int rep, int T,
-                                                              int W, int64_t total) {
+__global__ __launch_bounds__(256) void delta_group_sum_kernel(const float* x, ts_strided dq, ts_strided dkey, int Hk,
+                                                              int rep, int T, int W, int64_t total) {
+  const ts_strided& out = blockIdx.y ? dkey : dq;
+  if (blockIdx.y) x += total * rep * 4;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int cols = W / 4, c = (int)(i % cols) * 4;
     const int64_t row = i / cols;
@@ -632,10 +634,10 @@ int backward(const DeltaP& p, hipStream_t stream) {
 
 // The rows of value heads that share keys (fp32), added up.
 template <typename E>
-void group_sum(const DeltaP& p, const float* x, const ts_strided& out, hipStream_t stream) {
+void group_sum(const DeltaP& p, const float* x, const ts_strided& dq, const ts_strided& dkey, hipStream_t stream) {
   const int64_t total = (int64_t)p.B * p.Hk * p.T * (p.dk / 4), blocks = (total + 255) / 256;
-  hipLaunchKernelGGL((ts::delta_group_sum_kernel<E>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0,
-                     stream, x, out, p.Hk, p.rep, p.T, p.dk, total);
+  hipLaunchKernelGGL((ts::delta_group_sum_kernel<E>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2),
+                     dim3(256), 0, stream, x, dq, dkey, p.Hk, p.rep, p.T, p.dk, total);
 }
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
@@ -732,13 +734,10 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
     rc = narrow ? backward<float, 64>(p, stream) : backward<float, 128>(p, stream);
   if (rc) return rc;
   if (p.rep > 1) {
-    if (d->dtype == TS_BF16) {
-      group_sum<ts::bf16>(p, gq, gr->dq, stream);
-      group_sum<ts::bf16>(p, gk, gr->dk, stream);
-    } else {
-      group_sum<float>(p, gq, gr->dq, stream);
-      group_sum<float>(p, gk, gr->dk, stream);
-    }
+    if (d->dtype == TS_BF16)
+      group_sum<ts::bf16>(p, gq, gr->dq, gr->dk, stream);
+    else
+      group_sum<float>(p, gq, gr->dq, gr->dk, stream);
   }
   if (gr->ddecay_head) {
     if (d->decay_dtype == TS_BF16)
