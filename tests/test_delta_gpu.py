@@ -477,3 +477,20 @@ def test_short_sequences_in_uneven_segments(cuda, B, T, dk, dv, ragged, dtype):
             for name in ("q", "k", "v", "beta", "decay"):
                 s[name][b, :, m:] = 0.0
     check(s, cuda, lengths=lengths)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_first_token_forgets_nothing(cuda, dtype):
+    """Without an entering state the first token's retention acts on nothing: its
+    gradient is zero, not what rounding leaves of terms that cancel."""
+    import thetascan_amd as ts
+
+    for T in (1, 70):
+        s = on_gpu(inputs(2, 1, 2, T, 64, 40, dtype, seed=T), cuda, True)
+        args = [s[n] for n in ("q", "k", "v", "beta", "decay")]
+        out, S = ts.gated_delta_rule(*args, return_state=True)
+        (g,) = torch.autograd.grad(out.float().sum() + S.sum(), s["decay"])
+        if T == 1:
+            assert not g.any()
+        else:
+            assert g[..., 1:].any()

@@ -468,7 +468,8 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
           diag_v = rv[j];
         }
         const float a = i <= t ? dp[r][j] * d : 0.f, m = i < t ? ru[r][j] * d : 0.f;
-        const float xa = a * qk[j], xn = m * kk[j];
+        // (X_tt is in its row's sum and its column's: left out of both)
+        const float xa = i < t ? a * qk[j] : 0.f, xn = m * kk[j];
         rows_x += xa;
         rows_n += xn;
         cx[4 * r + j] = fmaf(-be, xn, xa);
