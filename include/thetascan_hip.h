@@ -57,8 +57,10 @@ extern "C" {
  * 19: ts_delta_fwd / ts_delta_bwd / ts_delta_step (with their workspace sizes)
  *     and ts_policy_loss_fwd / ts_policy_loss_bwd /
  *     ts_policy_loss_parts / ts_policy_one_pass / ts_policy_scale and ts_capture_id; nothing
- *     earlier changed. */
-#define TS_ABI_VERSION 19
+ *     earlier changed.
+ * 20: ts_delta_io has a buffer for the low halves of what a bf16 forward keeps (low,
+ *     ts_delta_low_bytes), which ts_delta_bwd reads. */
+#define TS_ABI_VERSION 20
 
 enum ts_status {
   TS_OK = 0,
@@ -1273,9 +1275,15 @@ typedef struct ts_delta_io {
                              it are not read, give zeros, and leave the state   */
   const float* state;     /* [B,H,dk,dv] contiguous, or NULL (zero)             */
   float* state_out;       /* the state after the last token, or NULL            */
+  void* low;              /* desc.keep and ts_delta_bwd: ts_delta_low_bytes, 16-byte
+                             aligned, kept beside the workspace (NULL where none)  */
 } ts_delta_io;
 
 int ts_delta_workspace_bytes(const ts_delta_desc* desc, size_t* bytes);
+
+/* Bytes of ts_delta_io.low: what rounding to bf16 leaves of the written values and of the
+ * chunks' states, kept for the gradients (none for fp32, nor without desc.keep). */
+int ts_delta_low_bytes(const ts_delta_desc* desc, size_t* bytes);
 
 /* The chunked form over T tokens.  workspace: 16-byte aligned; where desc.keep,
  * it is ts_delta_bwd's `saved`. */

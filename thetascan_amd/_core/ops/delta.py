@@ -16,8 +16,8 @@ are the same function of their inputs.
 
 bf16 inputs: products take bf16 operands and fp32 sums; everything that feeds the
 state in the forward (the state itself, what is written, the chunk's inverse)
-enters as a bf16 pair hi + lo, so the returned state is exact to about 1e-5; the
-outputs and the gradients carry bf16's rounding.  fp32 inputs compute in fp32.
+enters as a bf16 pair hi + lo, in the backward too, so the returned state is exact to
+about 1e-5, and outputs and gradients carry bf16's one rounding.  fp32 inputs compute in fp32.
 A non-finite value in a token that counts spreads over its chunk of 64 tokens
 and everything after it.
 """
@@ -75,16 +75,17 @@ def _desc(q, k, v, beta, decay, keep: bool) -> _lib.DeltaDesc:
 
 
 @functools.lru_cache(maxsize=256)
-def _plan(q, v, dtype, beta, decay, keep) -> tuple[_lib.DeltaDesc, int, int]:
-    """A call's descriptor and the bytes of its forward's and backward's
-    workspaces, by shapes and dtypes."""
+def _plan(q, v, dtype, beta, decay, keep) -> tuple[_lib.DeltaDesc, int, int, int]:
+    """A call's descriptor and the bytes of its forward's workspace, of the low
+    halves beside it and of the backward's workspace, by shapes and dtypes."""
     B, Hk, T, dk = q
     desc = _lib.DeltaDesc(B, Hk, v[1], T, _width(dtype, dk), _width(dtype, v[3]), _lib.dtype_code(dtype),
                           _lib.dtype_code(beta), _lib.TS_F32 if decay is None else _lib.dtype_code(decay), int(keep))
-    lib, fwd, bwd = _lib.load(), ctypes.c_size_t(), ctypes.c_size_t()
+    lib, fwd, low, bwd = _lib.load(), ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
     _lib.check(lib.ts_delta_workspace_bytes(ctypes.byref(desc), ctypes.byref(fwd)), "ts_delta_workspace_bytes")
+    _lib.check(lib.ts_delta_low_bytes(ctypes.byref(desc), ctypes.byref(low)), "ts_delta_low_bytes")
     _lib.check(lib.ts_delta_bwd_workspace_bytes(ctypes.byref(desc), ctypes.byref(bwd)), "ts_delta_bwd_workspace_bytes")
-    return desc, fwd.value, bwd.value
+    return desc, fwd.value, low.value, bwd.value
 
 
 def _rows(x: torch.Tensor, vec: int) -> tuple[torch.Tensor, _lib.Strided]:
@@ -114,16 +115,16 @@ def _rows_like(x: torch.Tensor, dtype: torch.dtype, width: int) -> torch.Tensor:
     return x.new_empty(B, H, T, width, dtype=dtype)
 
 
-def _io(q, k, v, beta, decay, lengths, out, state, state_out) -> _lib.DeltaIO:
+def _io(q, k, v, beta, decay, lengths, out, state, state_out, low=None) -> _lib.DeltaIO:
     """(q, k, v and out by their descriptions)"""
     return _lib.DeltaIO(q, k, v, _gate(beta), _gate(decay, decay is not None and decay.ndim == 1), out,
-                        _lib.ptr(lengths), _lib.ptr(state), _lib.ptr(state_out))
+                        _lib.ptr(lengths), _lib.ptr(state), _lib.ptr(state_out), low)
 
 
 def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, step: bool, state_out=None):
     """``(out, state or None, workspace or None)`` at the padded widths' slices."""
     lib = _lib.load()
-    desc, nbytes, _ = _plan(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, keep)
+    desc, nbytes, low, _ = _plan(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, keep)
     B, H, T, dv = v.shape
     dk, dkp, dvp, vec = q.shape[-1], desc.dk, desc.dv, _vec(q.dtype)
     (q, sq), (k, sk), (v4, sv) = _rows(q, vec), _rows(k, vec), _rows(v, vec)
@@ -144,9 +145,10 @@ def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, 
                 status = lib.ts_delta_step(ctypes.byref(desc), ctypes.byref(io), stream)
             _lib.check(status, "ts_delta_step")
         else:
-            work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            work = torch.empty(nbytes + low, dtype=torch.uint8, device=q.device)
+            io.low = work.data_ptr() + nbytes if low else None
             with _lib.timed("ts_delta_fwd", lambda: _lib.nbytes(q, k, v4, beta, decay, out, given, final)):
-                status = lib.ts_delta_fwd(ctypes.byref(desc), ctypes.byref(io), work.data_ptr(), work.numel(), stream)
+                status = lib.ts_delta_fwd(ctypes.byref(desc), ctypes.byref(io), work.data_ptr(), nbytes, stream)
             _lib.check(status, "ts_delta_fwd")
     if final is not None and final is not state_out:
         final = final[..., :dk, :dv]
@@ -170,8 +172,8 @@ def _forward_fake(q, k, v, beta, decay, state, lengths, want_state, keep, step):
     out = _rows_like(v, q.dtype, _width(q.dtype, dv))[..., :dv]
     nbytes = 0
     if keep:  # (a traced size becomes a number here)
-        nbytes = _plan(tuple(map(int, q.shape)), tuple(map(int, v.shape)), q.dtype, beta.dtype,
-                       None if decay is None else decay.dtype, True)[1]
+        nbytes = sum(_plan(tuple(map(int, q.shape)), tuple(map(int, v.shape)), q.dtype, beta.dtype,
+                           None if decay is None else decay.dtype, True)[1:3])
     return [out, q.new_empty((B, H, q.shape[-1], dv) if want_state else (0,), dtype=torch.float32),
             q.new_empty(nbytes, dtype=torch.uint8)]
 
@@ -180,7 +182,7 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
                    v: torch.Tensor, beta: torch.Tensor, decay: torch.Tensor | None, state: torch.Tensor | None,
                    lengths: torch.Tensor | None, saved: torch.Tensor, need_state: bool) -> list[torch.Tensor]:
     lib = _lib.load()
-    desc, _, nbytes = _plan(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, True)
+    desc, kept, low, nbytes = _plan(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, True)
     B, H, T, dv = v.shape
     dk, dkp, dvp, vec = q.shape[-1], desc.dk, desc.dv, _vec(q.dtype)
     (q4, sq), (k4, sk), (v4, sv) = _rows(q, vec), _rows(k, vec), _rows(v, vec)
@@ -196,14 +198,14 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
         ddecay = torch.empty((H,) if per_head else (B, H, T), dtype=decay.dtype, device=q.device)
     dstate = torch.empty(B, H, dkp, dvp, dtype=torch.float32, device=q.device) if need_state else None
     # (the forward's output and states play no part here: out takes dout's rows)
-    io = _io(sq, sk, sv, beta, decay, lengths, so, None, None)
+    io = _io(sq, sk, sv, beta, decay, lengths, so, None, None, saved.data_ptr() + kept if low else None)
     grads = _lib.DeltaGrads(so, _lib.strided(dq), _lib.strided(dk_), _lib.strided(dv_), dbeta.data_ptr(),
                             None if per_head else _lib.ptr(ddecay), _lib.ptr(ddecay) if per_head else None,
                             _lib.ptr(given), _lib.ptr(dstate))
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     with _on(q.device), _lib.timed("ts_delta_bwd", lambda: _lib.nbytes(q4, k4, v4, do4, dq, dk_, dv_, dbeta, ddecay)):
         status = lib.ts_delta_bwd(ctypes.byref(desc), ctypes.byref(io), ctypes.byref(grads), saved.data_ptr(),
-                                  saved.numel(), work.data_ptr(), work.numel(), _lib.stream_handle(q.device))
+                                  kept, work.data_ptr(), work.numel(), _lib.stream_handle(q.device))
     _lib.check(status, "ts_delta_bwd")
     if (dkp, dvp) != (dk, dv):
         dq, dk_, dv_ = dq[..., :dk], dk_[..., :dk], dv_[..., :dv]
@@ -264,8 +266,9 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
     ``beta`` [B,H,T] or [B,H,T,1] the write strengths; ``retention`` the log
     retentions (at most zero, -inf a reset): None, one per value head [H], or one
     per token [B,H,T] or [B,H,T,1].  Keys are taken as given: the memory is stable
-    where ``beta_t |k_t|^2`` is at most 2, and keeps its digits to about 1 (at 2, with
-    alike keys and no retention, bf16 gradients are off by 5 %, fp32's by 2e-5).  dk is at
+    where ``beta_t |k_t|^2`` is at most 2, and keeps its digits to there (with alike
+    keys and no retention, bf16 gradients are off by 3e-5 of their norm before their
+    rounding at 0.5 to 2, fp32's by 2e-5 at 2).  dk is at
     most 128, dv at most 512.
 
     ``state`` continues from the fp32 state of an earlier call (None: zero).

@@ -552,7 +552,7 @@ class DeltaDesc(ctypes.Structure):
 
 class DeltaIO(ctypes.Structure):
     _fields_ = [(n, Strided) for n in ("q", "k", "v", "beta", "decay", "out")] + [
-        (n, ctypes.c_void_p) for n in ("lengths", "state", "state_out")]
+        (n, ctypes.c_void_p) for n in ("lengths", "state", "state_out", "low")]
 
 
 class DeltaGrads(ctypes.Structure):
@@ -571,7 +571,7 @@ class PolicyIO(ctypes.Structure):
                                                "weights", "log_probs", "coef", "lse", "parts", "loss", "dlogits")]
 
 
-ABI_VERSION = 19  # the include/thetascan_hip.h these bindings are written for
+ABI_VERSION = 20  # the include/thetascan_hip.h these bindings are written for
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -723,6 +723,7 @@ def load() -> ctypes.CDLL:
         lib.ts_rotary_tables.argtypes = [ctypes.c_void_p] + [ctypes.c_int32] * 3 + [ctypes.c_void_p] * 3
         lib.ts_causal_attention_fwd.argtypes = [P(AttentionDesc), Strided, Strided, Strided, Strided, ctypes.c_void_p]
         lib.ts_delta_workspace_bytes.argtypes = [P(DeltaDesc), P(ctypes.c_size_t)]
+        lib.ts_delta_low_bytes.argtypes = [P(DeltaDesc), P(ctypes.c_size_t)]
         lib.ts_delta_fwd.argtypes = [P(DeltaDesc), P(DeltaIO), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.ts_delta_step.argtypes = [P(DeltaDesc), P(DeltaIO), ctypes.c_void_p]
         lib.ts_delta_bwd_workspace_bytes.argtypes = [P(DeltaDesc), P(ctypes.c_size_t)]

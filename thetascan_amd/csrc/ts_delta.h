@@ -62,6 +62,9 @@ struct DeltaP {
                            // gradients behind them)
   void* u;                 // kept: [B*H*nc][dvp][64]
   void* s0;                // kept: [B*H*nc][dvp][DK]
+  int64_t u_low, s0_low;   // elements from those to what their rounding to bf16 leaves, and from
+                           // dr and ds to theirs (fp32: none)
+  int64_t dr_low, ds_low;
   // backward
   ts_strided dout, dq, dkey, dval;
   void* dbeta;   // [B,H,T] of beta's dtype
@@ -114,6 +117,15 @@ template <> struct Split<bf16> {
     hi = __builtin_bit_cast(bf16x8, h);
     lo = __builtin_bit_cast(bf16x8, l);
   }
+  __device__ __forceinline__ Split(bf16x8 h, bf16x8 l) : hi(h), lo(l) {}
+  // The first block's four rows to a, the second's to b, what they leave `low` elements behind.
+  __device__ __forceinline__ void store(bf16* a, bf16* b, int64_t low) const {
+    const uint4 h = __builtin_bit_cast(uint4, hi), l = __builtin_bit_cast(uint4, lo);
+    *(uint2*)a = make_uint2(h.x, h.y);
+    *(uint2*)b = make_uint2(h.z, h.w);
+    *(uint2*)(a + low) = make_uint2(l.x, l.y);
+    *(uint2*)(b + low) = make_uint2(l.z, l.w);
+  }
   // (two elements to a conversion: one at a time takes a conversion each and their packing)
   static __device__ __forceinline__ void two(float x, float y, unsigned& h, unsigned& l) {
     h = pack2(x, y);
@@ -123,6 +135,11 @@ template <> struct Split<bf16> {
 template <> struct Split<float> {
   floatx8 hi;
   __device__ __forceinline__ Split(floatx4 a, floatx4 b) { hi = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+  __device__ __forceinline__ explicit Split(floatx8 h) : hi(h) {}
+  __device__ __forceinline__ void store(float* a, float* b, int64_t) const {
+    *(floatx4*)a = __builtin_shufflevector(hi, hi, 0, 1, 2, 3);
+    *(floatx4*)b = __builtin_shufflevector(hi, hi, 4, 5, 6, 7);
+  }
 };
 // c + x (y.hi + y.lo) and c + (y.hi + y.lo) x
 __device__ __forceinline__ floatx4 mma_split(bf16x8 x, const Split<bf16>& y, floatx4 c) {
@@ -133,6 +150,30 @@ __device__ __forceinline__ floatx4 mma_split(const Split<bf16>& y, bf16x8 x, flo
   return mma32(y.hi, x, mma32(y.lo, x, c));
 }
 __device__ __forceinline__ floatx4 mma_split(const Split<float>& y, floatx8 x, floatx4 c) { return mma32(y.hi, x, c); }
+// c + x y of a pair each: what the two remainders make together (2^-16) is left out.
+__device__ __forceinline__ floatx4 mma_split(const Split<bf16>& x, const Split<bf16>& y, floatx4 c) {
+  return mma32(x.hi, y.hi, mma32(x.hi, y.lo, mma32(x.lo, y.hi, c)));
+}
+__device__ __forceinline__ floatx4 mma_split(const Split<float>& x, const Split<float>& y, floatx4 c) {
+  return mma32(x.hi, y.hi, c);
+}
+
+// One fragment of a triangular matrix into its sets, and one read back.
+__device__ __forceinline__ void put_tri(bf16* m, int r, int s, int lane, const Split<bf16>& f) {
+  bf16* at = m + (tri(r, s) * 64 + lane) * 8;
+  *(bf16x8*)at = f.hi;
+  *(bf16x8*)(at + kTriElems) = f.lo;
+}
+__device__ __forceinline__ void put_tri(float* m, int r, int s, int lane, const Split<float>& f) {
+  *(floatx8*)(m + (tri(r, s) * 64 + lane) * 8) = f.hi;
+}
+__device__ __forceinline__ Split<bf16> get_tri(const bf16* m, int r, int s, int lane) {
+  const bf16* at = m + (tri(r, s) * 64 + lane) * 8;
+  return Split<bf16>(*(const bf16x8*)at, *(const bf16x8*)(at + kTriElems));
+}
+__device__ __forceinline__ Split<float> get_tri(const float* m, int r, int s, int lane) {
+  return Split<float>(*(const floatx8*)(m + (tri(r, s) * 64 + lane) * 8));
+}
 
 // Eight columns of an LDS row in accumulator order (32s + 4g.., 32s + 16 + 4g..).
 template <typename E>
@@ -169,6 +210,14 @@ template <> struct TriT<float> {
     return v;
   }
 };
+
+// The same of a matrix in its sets.
+__device__ __forceinline__ Split<bf16> get_tri_t(const bf16* t, int r, int s, int lane) {
+  return Split<bf16>(TriT<bf16>::get(t, r, s, lane), TriT<bf16>::get(t + kTriElems, r, s, lane));
+}
+__device__ __forceinline__ Split<float> get_tri_t(const float* t, int r, int s, int lane) {
+  return Split<float>(TriT<float>::get(t, r, s, lane));
+}
 
 // A [64 x W] token tile on its way from global memory to LDS rows: vector idx =
 // tid + i * THREADS.  Columns at or past `width` (a multiple of a vector) are

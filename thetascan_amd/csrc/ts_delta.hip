@@ -16,12 +16,12 @@
 // is rounded once.
 //
 // Bound by the bytes where heads and tokens are many: 64 heads of 4096 tokens of 64 x 64
-// (bf16, training) prepare 39 us (175 MB, 4.5 TB/s), transfers 44 (134 MB), forward 66 (311
-// MB, 4.7 TB/s).  Where they are few, by the chain: a chunk takes 4.4 us (64 keys, a workgroup
-// a CU; 7 with two), of which a third is matrix instructions.  Workgroups of
-// eight waves (forward of 32 heads of 2048 x 128 65 us against 56) and three waves a SIMD (77
-// against 65) were slower; P formed here again, not stored, 0.8 us more a chunk for 6 % less time
-// where bytes bind.
+// (bf16, training) prepare 42 us (175 MB, 4.2 TB/s), transfers 47 (134 MB), forward 91 (378
+// MB, 4.2 TB/s; four fifths of what it writes is kept for the gradients).  Where they are few,
+// by the chain: a chunk takes 4.4 us (64 keys, a workgroup a CU; 7 with two), of which a third
+// is matrix instructions.  Workgroups of eight waves (forward of 32 heads of 2048 x 128 65 us
+// against 56) and three waves a SIMD (77 against 65) were slower; P formed here again, not
+// stored, 0.8 us more a chunk for 6 % less time where bytes bind.
 
 #include "ts_delta.h"
 
@@ -42,34 +42,6 @@ __device__ __forceinline__ typename Frag<E>::f8 global8(const E* row, int c, int
 }
 
 constexpr int kDiagPitch = 20;
-
-// One fragment of a triangular matrix into its sets, and one read back.
-__device__ __forceinline__ void put_tri(bf16* m, int r, int s, int lane, const Split<bf16>& f) {
-  bf16* at = m + (tri(r, s) * 64 + lane) * 8;
-  *(bf16x8*)at = f.hi;
-  *(bf16x8*)(at + kTriElems) = f.lo;
-}
-__device__ __forceinline__ void put_tri(float* m, int r, int s, int lane, const Split<float>& f) {
-  *(floatx8*)(m + (tri(r, s) * 64 + lane) * 8) = f.hi;
-}
-// c + m x of a pair each: what the two remainders make together (2^-16) is left out.
-__device__ __forceinline__ floatx4 mma_tri(const bf16* m, int r, int s, int lane, const Split<bf16>& x, floatx4 c) {
-  const bf16* at = m + (tri(r, s) * 64 + lane) * 8;
-  const bf16x8 hi = *(const bf16x8*)at, lo = *(const bf16x8*)(at + kTriElems);
-  return mma32(hi, x.hi, mma32(hi, x.lo, mma32(lo, x.hi, c)));
-}
-__device__ __forceinline__ floatx4 mma_tri(const float* m, int r, int s, int lane, const Split<float>& x, floatx4 c) {
-  return mma32(*(const floatx8*)(m + (tri(r, s) * 64 + lane) * 8), x.hi, c);
-}
-// The same with the sides exchanged (the transposed result).
-__device__ __forceinline__ floatx4 mma_tri_t(const bf16* m, int r, int s, int lane, const Split<bf16>& x, floatx4 c) {
-  const bf16* at = m + (tri(r, s) * 64 + lane) * 8;
-  const bf16x8 hi = *(const bf16x8*)at, lo = *(const bf16x8*)(at + kTriElems);
-  return mma32(x.hi, hi, mma32(x.lo, hi, mma32(x.hi, lo, c)));
-}
-__device__ __forceinline__ floatx4 mma_tri_t(const float* m, int r, int s, int lane, const Split<float>& x, floatx4 c) {
-  return mma32(x.hi, *(const floatx8*)(m + (tri(r, s) * 64 + lane) * 8), c);
-}
 
 template <typename E, int DK>
 __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
@@ -318,11 +290,6 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
     const E *tri_t = ch.t, *tri_p = ch.p;
     const float* vec = ch.vec;
 
-    if constexpr (KEEP) {
-      E* s0 = (E*)p.s0 + (n * p.dvp + col) * DK + 4 * g;
-#pragma unroll
-      for (int d = 0; d < KB; ++d) IO::st4(s0 + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
-    }
     // K S0 and S0^T Q^T (lane l16 a token, four columns): independent products side by side
     floatx4 R[4], O[4];
 #pragma unroll
@@ -330,6 +297,10 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const Split<E> sf(S[2 * s], S[2 * s + 1]);
+      if constexpr (KEEP) {
+        E* s0 = (E*)p.s0 + (n * p.dvp + col) * DK + 32 * s + 4 * g;
+        sf.store(s0, s0 + 16, p.s0_low);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         R[r] = mma_split(row_perm<E>(ks + (16 * r + l16) * PITCH, s, g), sf, R[r]);
@@ -353,12 +324,7 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
     for (int s = 0; s < 2; ++s) {
       const Split<E> rf(R[2 * s], R[2 * s + 1]);
 #pragma unroll
-      for (int r = 2 * s; r < 4; ++r) U[r] = mma_tri(tri_t, r, s, lane, rf, U[r]);
-    }
-    if constexpr (KEEP) {
-      E* u = (E*)p.u + (n * p.dvp + col) * kChunk + 4 * g;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) IO::st4(u + 16 * r, U[r][0], U[r][1], U[r][2], U[r][3]);
+      for (int r = 2 * s; r < 4; ++r) U[r] = mma_split(get_tri(tri_t, r, s, lane), rf, U[r]);
     }
     // S = e^{G_63} S0 + K^T (e^{G_63 - G} U), and beside it O^T = e^G S0^T Q^T + U^T P^T
     const float whole = vec[3 * kChunk];
@@ -384,11 +350,15 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
         for (int i = 0; i < 4; ++i) f[e][i] = U[2 * s + e][i] * tail[i];
       }
       const Split<E> ff(f[0], f[1]), uf(U[2 * s], U[2 * s + 1]);
+      if constexpr (KEEP) {
+        E* u = (E*)p.u + (n * p.dvp + col) * kChunk + 32 * s + 4 * g;
+        uf.store(u, u + 16, p.u_low);
+      }
 #pragma unroll
       for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(ks, PITCH, 16 * d, s, lane), ff, S[d]);
       if constexpr (!TRANSFER) {
 #pragma unroll
-        for (int r = 2 * s; r < 4; ++r) O[r] = mma_tri_t(tri_p, r, s, lane, uf, O[r]);
+        for (int r = 2 * s; r < 4; ++r) O[r] = mma_split(uf, get_tri(tri_p, r, s, lane), O[r]);
       }
     }
     if constexpr (!TRANSFER) {
@@ -590,6 +560,7 @@ int padded_keys(int dk) { return dk <= 64 ? 64 : 128; }
 
 struct Sizes {
   size_t prep, seg_x, seg_state, u, s0;  // bytes of each part; u and s0 only where kept
+  size_t low;                            // bytes of ts_delta_io.low
   size_t all(const ts_delta_desc* d) const { return prep + seg_x + seg_state + (d->keep ? u + s0 : 0); }
 };
 Sizes sizes(const ts_delta_desc* d) {
@@ -605,6 +576,7 @@ Sizes sizes(const ts_delta_desc* d) {
   }
   s.u = n * dvp * 64 * es;
   s.s0 = n * dvp * padded_keys(d->dk) * es;
+  s.low = d->keep && d->dtype == TS_BF16 ? s.u + s.s0 : 0;
   return s;
 }
 
@@ -644,6 +616,13 @@ int ts_delta_workspace_bytes(const ts_delta_desc* d, size_t* bytes) {
   return TS_OK;
 }
 
+int ts_delta_low_bytes(const ts_delta_desc* d, size_t* bytes) {
+  const int rc = ts::delta_check(d, nullptr, nullptr, "delta");
+  if (rc) return rc;
+  if (bytes) *bytes = sizes(d).low;
+  return TS_OK;
+}
+
 int ts_delta_fwd(const ts_delta_desc* d, const ts_delta_io* io, void* workspace, size_t workspace_bytes,
                  hipStream_t stream) {
   DeltaP p;
@@ -662,6 +641,12 @@ int ts_delta_fwd(const ts_delta_desc* d, const ts_delta_io* io, void* workspace,
   if (d->keep) {
     p.u = p.prep + s.prep + s.seg_x + s.seg_state;
     p.s0 = (char*)p.u + s.u;
+    if (s.low) {
+      if (!io->low || ((uintptr_t)io->low & 15u))
+        return fail(TS_ERR_VALUE, "delta: the low halves' buffer is missing or misaligned");
+      p.u_low = ((char*)io->low - (char*)p.u) / 2;
+      p.s0_low = ((char*)io->low + s.u - (char*)p.s0) / 2;
+    }
   }
   const bool narrow = d->dk <= 64;
   int rc2;

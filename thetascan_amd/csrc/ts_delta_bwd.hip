@@ -15,16 +15,15 @@
 // forward; it leaves dR and dS per chunk and writes dV.  delta_grads takes the
 // chunks on their own: one workgroup each, a wave per 16 tokens.
 //
-// Roundings (bf16 inputs): dS and dU, which the chain carries on, enter products as pairs
-// hi + lo; everything that ends in one gradient (dR, dS, U and S0 as kept, A, M, e^G dO)
-// enters once rounded, 2^-9 of itself, beside the gradient's own rounding: the gradients
-// are within 0.0035 (2-norm) of float64, where one rounding alone is 0.0017.  Pairs there
-// would double what the chain leaves and delta_grads reads.  Sums are fp32, those of the gates'
-// gradients over a chunk fp64.
+// Roundings (bf16 inputs): every operand that is not an input is a pair hi + lo, also as kept
+// (U, S0, dR, dS, the triangles), since sums over alike keys cancel: with these rounded once
+// the gradients of 256 nearly alike keys were off by 0.8 % (dq), 0.5 (dv), 0.8 (db) and 1.0 (the
+// retentions'), of one key throughout up to 7 % (float64 emulation), with the pairs 1e-5, beside
+// the gradient's own rounding.  Sums are fp32, those of the gates' gradients over a chunk fp64.
 //
-// 64 heads of 4096 tokens of 64 x 64, bf16: transfers 33 us, chain 60 (262 MB, 4.4 TB/s),
-// gradients 80 (349 MB, 4.4 TB/s; its loads and its products take turns in a workgroup, three
-// of which share a CU: two took 102).  A persistent workgroup that loads a chunk ahead spilled (111).
+// 64 heads of 4096 tokens of 64 x 64, bf16: transfers 48 us, chain 95 (380 MB, 4.0 TB/s),
+// gradients 122 (483 MB, 4.0 TB/s; its loads and its products take turns in a workgroup, three
+// of which share a CU).  Without the low halves 33, 62 and 80 us.
 
 #include "ts_delta.h"
 
@@ -34,13 +33,11 @@
 
 namespace ts {
 
-// What the waves of a workgroup read of one chunk: the triangles in one rounding.
+// What the waves of a workgroup read of one chunk.
 template <typename E, int DK>
 struct ChainChunk {
-  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD;
-  E k[kChunk * PITCH], q[kChunk * PITCH], o[kChunk * VP];
-  __align__(16) char t[Linear<E, 256, kTriElems * sizeof(E)>::LDS];
-  __align__(16) char p[Linear<E, 256, kTriElems * sizeof(E)>::LDS];
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD, SET = TriSets<E>::N * kTriElems;
+  E k[kChunk * PITCH], q[kChunk * PITCH], o[kChunk * VP], t[SET], p[SET];
   float vec[256];
 };
 // TRANSFER: what a segment of chunks adds to the gradient behind it, from its
@@ -90,7 +87,8 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
   kt.init(p.k.st, p.dk, tid);
   qt.init(p.q.st, p.dk, tid);
   ot.init(p.dout.st, p.dv - base, tid);
-  Linear<E, 256, kTriElems * sizeof(E)> tt, tp;
+  Linear<E, 256, Chunk::SET * sizeof(E)> tt, tp;
+  static_assert(Linear<E, 256, Chunk::SET * sizeof(E)>::LDS == Chunk::SET * sizeof(E), "whole slots");
   float vv = 0.f;
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
@@ -99,8 +97,8 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
     ot.fetch(db, p.dout.st, t0, len);
     const E* prep = (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>());
     tt.fetch(prep, tid);
-    tp.fetch(prep + TriSets<E>::N * kTriElems, tid);
-    vv = ((const float*)(prep + 2 * TriSets<E>::N * kTriElems))[min(tid, kVec - 1)];
+    tp.fetch(prep + Chunk::SET, tid);
+    vv = ((const float*)(prep + 2 * Chunk::SET))[min(tid, kVec - 1)];
   };
   if (c0 < c1) fetch(c1 - 1);
   loads_landed();
@@ -122,11 +120,6 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
 #pragma unroll
     for (int s = 0; s < 2; ++s) of[s] = TokFrag<E>::get(lds.o, VP, 16 * w, s, lane);
 
-    if constexpr (!TRANSFER) {
-      E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 4 * g;
-#pragma unroll
-      for (int d = 0; d < KB; ++d) IO::st4(ds + 16 * d, S[d][0], S[d][1], S[d][2], S[d][3]);
-    }
     // dU = P^T dO + e^{G_63 - G} K dS, and beside it Q^T (e^G dO): independent products
     floatx4 X[4], Y[4], Z[KB];
 #pragma unroll
@@ -136,6 +129,10 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const Split<E> sf(S[2 * s], S[2 * s + 1]);
+      if constexpr (!TRANSFER) {
+        E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 32 * s + 4 * g;
+        sf.store(ds, ds + 16, p.ds_low);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[r] = mma_split(row_perm<E>(lds.k + (16 * r + l16) * PITCH, s, g), sf, X[r]);
     }
@@ -148,11 +145,11 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[e][i] = eg[i] * tof(of[s][4 * e + i]);
       }
-      const f8 qf = IO::from_acc(f[0], f[1]);
+      const Split<E> qf(f[0], f[1]);
 #pragma unroll
-      for (int r = 0; r < 2 * s + 2; ++r) Y[r] = mma32(TriT<E>::get((const E*)lds.p, r, s, lane), of[s], Y[r]);
+      for (int r = 0; r < 2 * s + 2; ++r) Y[r] = mma_split(get_tri_t(lds.p, r, s, lane), of[s], Y[r]);
 #pragma unroll
-      for (int d = 0; d < KB; ++d) Z[d] = mma32(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, Z[d]);
+      for (int d = 0; d < KB; ++d) Z[d] = mma_split(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, Z[d]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -166,15 +163,19 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
       const Split<E> u0(X[0], X[1]), u1(X[2], X[3]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        R[r] = mma_split(TriT<E>::get((const E*)lds.t, r, 1, lane), u1, zero4());
-        if (r < 2) R[r] = mma_split(TriT<E>::get((const E*)lds.t, r, 0, lane), u0, R[r]);
+        R[r] = mma_split(get_tri_t(lds.t, r, 1, lane), u1, zero4());
+        if (r < 2) R[r] = mma_split(get_tri_t(lds.t, r, 0, lane), u0, R[r]);
       }
     }
-    E* dro = (E*)p.dr + (n * p.dvp + col) * kChunk + 4 * g;
+    if constexpr (!TRANSFER) {
+      E* dro = (E*)p.dr + (n * p.dvp + col) * kChunk + 4 * g;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        Split<E>(R[2 * s], R[2 * s + 1]).store(dro + 32 * s, dro + 32 * s + 16, p.dr_low);
+    }
     const float whole = vec[3 * kChunk];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      if constexpr (!TRANSFER) IO::st4(dro + 16 * r, R[r][0], R[r][1], R[r][2], R[r][3]);
       const floatx4 eg = *(const floatx4*)(vec + 16 * r + 4 * g);
       const floatx4 be = *(const floatx4*)(vec + 2 * kChunk + 16 * r + 4 * g);
 #pragma unroll
@@ -192,9 +193,9 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
       for (int i = 0; i < 4; ++i) S[d][i] = fmaf(whole, S[d][i], Z[d][i]);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const f8 rf = IO::from_acc(R[2 * s], R[2 * s + 1]);
+      const Split<E> rf(R[2 * s], R[2 * s + 1]);
 #pragma unroll
-      for (int d = 0; d < KB; ++d) S[d] = mma32(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
+      for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
     }
   }
   if (!mine) return;
@@ -219,16 +220,17 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
 }
 
 // Value columns of a pass of delta_grads.
-template <typename E> constexpr int kGradCols = sizeof(E) == 2 ? 64 : 32;
+constexpr int kGradCols = 32;
 
 template <typename E, int DK>
 struct GradsLds {
-  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VB = kGradCols<E>, TP = kChunk + PAD;
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VB = kGradCols, TP = kChunk + PAD;
+  static constexpr int N = TriSets<E>::N, US = VB * TP, SS = VB * PITCH;  // elements of one of a pair's halves
   struct Pass {
-    E u[VB * TP], dr[VB * TP], s0[VB * PITCH], ds[VB * PITCH];
+    E u[N * US], dr[N * US], s0[N * SS], ds[N * SS];
   };
   struct Pairs {
-    E q[kChunk * PITCH], a[kChunk * TP], m[kChunk * TP];
+    E q[kChunk * PITCH], a[N * kTriElems], m[N * kTriElems];
   };
   E k[kChunk * PITCH];
   union {  // the passes over the value columns, then the pairs of tokens
@@ -267,54 +269,77 @@ __device__ __forceinline__ typename Frag<E>::f8 row_global(const E* row, int c, 
   return LdsIO<E>::cat(part[0], part[1]);
 }
 
-// [ROWS x W] contiguous rows on their way to LDS; rows at or past `rows` are zero.
+// [ROWS x W] contiguous rows (of pairs: `low` elements from one half to the other) on their
+// way to LDS; rows at or past `rows` are zero.
 template <typename E, int ROWS, int W>
 struct Block {
-  static constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC, SLOTS = ROWS * PER / 256;
-  uint4 r[SLOTS];
-  __device__ __forceinline__ void fetch(const E* src, int rows, int tid) {
+  static constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC, SLOTS = ROWS * PER / 256, N = TriSets<E>::N;
+  uint4 r[N][SLOTS];
+  __device__ __forceinline__ void fetch(const E* src, int64_t low, int rows, int tid) {
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      const int idx = tid + i * 256;
-      r[i] = *(const uint4*)(src + min(idx / PER, rows - 1) * W + (idx % PER) * VEC);
-    }
+    for (int h = 0; h < N; ++h)
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) {
+        const int idx = tid + i * 256;
+        r[h][i] = *(const uint4*)(src + h * low + min(idx / PER, rows - 1) * W + (idx % PER) * VEC);
+      }
   }
   __device__ __forceinline__ void store(E* dst, int rows, int pitch, int tid) {
     if (rows < ROWS) {  // uniform
 #pragma unroll
-      for (int i = 0; i < SLOTS; ++i)
-        if ((tid + i * 256) / PER >= rows) r[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int h = 0; h < N; ++h)
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i)
+          if ((tid + i * 256) / PER >= rows) r[h][i] = make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      const int idx = tid + i * 256;
-      *(uint4*)(dst + (idx / PER) * pitch + (idx % PER) * VEC) = r[i];
-    }
+    for (int h = 0; h < N; ++h)
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) {
+        const int idx = tid + i * 256;
+        *(uint4*)(dst + (h * ROWS + idx / PER) * pitch + (idx % PER) * VEC) = r[h][i];
+      }
   }
   // Sum of the products with another block's entries of the same places.
   __device__ __forceinline__ float dot(const Block& o) const {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
-      Vec16<E> a, b;
-      a.raw = r[i];
-      b.raw = o.r[i];
+      Vec16<E> a[N], b[N];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum = fmaf(tof(a.e[j]), tof(b.e[j]), sum);
+      for (int h = 0; h < N; ++h) {
+        a[h].raw = r[h][i];
+        b[h].raw = o.r[h][i];
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum = fmaf(whole(a, j), whole(b, j), sum);
     }
     return sum;
   }
+  static __device__ __forceinline__ float whole(const Vec16<E>* v, int j) {
+    return N == 2 ? tof(v[0].e[j]) + tof(v[N - 1].e[j]) : tof(v[0].e[j]);
+  }
 };
 
-// (three waves a SIMD where registers and LDS allow it: 102 us with two, 87 with three; the
-// keys have a place of their own, in LDS from the first pass on and out of registers: 80)
+// TokFrag of a tile of pairs, `half` elements from one half to the other.
+__device__ __forceinline__ Split<bf16> pair_frag(const bf16* rows, int half, int pitch, int c0, int kp, int lane) {
+  return Split<bf16>(TokFrag<bf16>::get(rows, pitch, c0, kp, lane), TokFrag<bf16>::get(rows + half, pitch, c0, kp, lane));
+}
+__device__ __forceinline__ Split<float> pair_frag(const float* rows, int, int pitch, int c0, int kp, int lane) {
+  return Split<float>(TokFrag<float>::get(rows, pitch, c0, kp, lane));
+}
+
+// (three waves a SIMD where registers and LDS allow it: without the low halves 102 us with two,
+// 87 with three; the keys have a place of their own, in LDS from the first pass on and out of
+// registers: 80)
 template <typename E, int DK>
 __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK>)) void delta_grads_kernel(DeltaP p) {
   typedef LdsIO<E> IO;
   typedef TokFrag<E> TF;
   typedef typename Frag<E>::f8 f8;
   typedef GradsLds<E, DK> Lds;
-  constexpr int PITCH = Lds::PITCH, VB = Lds::VB, TP = Lds::TP, KB = DK / 16, KS = DK / 32;
+  constexpr int PITCH = Lds::PITCH, VB = Lds::VB, TP = Lds::TP, US = Lds::US, SS = Lds::SS;
+  constexpr int KB = DK / 16, KS = DK / 32;
   extern __shared__ __align__(16) char smem[];
   Lds& lds = *(Lds*)smem;
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -364,10 +389,10 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
     const int rows = p.dvp - v0;
 #pragma unroll
     for (int s = 0; s < VB / 32; ++s) of[s] = row_global<E>(orow, v0 + 32 * s + 4 * g, p.dv, t0 + t < len);
-    ut.fetch((const E*)p.u + (n * p.dvp + v0) * kChunk, rows, tid);
-    rt.fetch((const E*)p.dr + (n * p.dvp + v0) * kChunk, rows, tid);
-    st.fetch((const E*)p.s0 + (n * p.dvp + v0) * DK, rows, tid);
-    dt.fetch((const E*)p.ds + (n * p.dvp + v0) * DK, rows, tid);
+    ut.fetch((const E*)p.u + (n * p.dvp + v0) * kChunk, p.u_low, rows, tid);
+    rt.fetch((const E*)p.dr + (n * p.dvp + v0) * kChunk, p.dr_low, rows, tid);
+    st.fetch((const E*)p.s0 + (n * p.dvp + v0) * DK, p.s0_low, rows, tid);
+    dt.fetch((const E*)p.ds + (n * p.dvp + v0) * DK, p.ds_low, rows, tid);
   };
   kt.init(p.k.st, p.dk, tid);
   qt.init(p.q.st, p.dk, tid);
@@ -418,24 +443,25 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < VB / 32; ++s) {
-      const f8 rf = TF::get(lds.pass.dr, TP, 16 * w, s, lane), uw = TF::get(lds.pass.u, TP, 16 * w, s, lane);
+      const Split<E> rf = pair_frag(lds.pass.dr, US, TP, 16 * w, s, lane);
+      const Split<E> uw = pair_frag(lds.pass.u, US, TP, 16 * w, s, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (r <= w) {
-          const f8 uf = TF::get(lds.pass.u, TP, 16 * r, s, lane);
-          dp[r] = mma32(uf, of[s], dp[r]);
-          ru[r] = mma32(uf, rf, ru[r]);
+          const Split<E> uf = pair_frag(lds.pass.u, US, TP, 16 * r, s, lane);
+          dp[r] = mma_split(uf, of[s], dp[r]);
+          ru[r] = mma_split(uf, rf, ru[r]);
         }
 #pragma unroll
       for (int d = 0; d < KB; ++d) {
-        const f8 sf = TF::get(lds.pass.s0, PITCH, 16 * d, s, lane);
-        z[d] = mma32(sf, of[s], z[d]);
-        y[d] = mma32(sf, rf, y[d]);
-        fu[d] = mma32(TF::get(lds.pass.ds, PITCH, 16 * d, s, lane), uw, fu[d]);
+        const Split<E> sf = pair_frag(lds.pass.s0, SS, PITCH, 16 * d, s, lane);
+        z[d] = mma_split(sf, of[s], z[d]);
+        y[d] = mma_split(sf, rf, y[d]);
+        fu[d] = mma_split(pair_frag(lds.pass.ds, SS, PITCH, 16 * d, s, lane), uw, fu[d]);
       }
       if (any_zero) {
         const f8 vf = row_global<E>(vrow, v0 + 32 * s + 4 * g, p.dv, t0 + t < len);
-        rv = mma32(vf, rf, rv);
+        rv = mma_split(vf, rf, rv);
       }
     }
   }
@@ -485,10 +511,11 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
     if (l16 == 0) lds.cols[w][16 * (i >> 2) + 4 * g + (i & 3)] = cx[i];
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    IO::st4(lds.pairs.a + t * TP + 16 * r + 4 * g, dp[r][0], dp[r][1], dp[r][2], dp[r][3]);
-    IO::st4(lds.pairs.m + t * TP + 16 * r + 4 * g, ru[r][0], ru[r][1], ru[r][2], ru[r][3]);
-  }
+  for (int s = 0; s < 2; ++s)
+    if (2 * s <= w) {
+      put_tri(lds.pairs.a, w, s, lane, Split<E>(dp[2 * s], dp[2 * s + 1]));
+      put_tri(lds.pairs.m, w, s, lane, Split<E>(ru[2 * s], ru[2 * s + 1]));
+    }
   // state terms of the gates, and of the rows
   float zq = 0.f, yk = 0.f, fk = 0.f;
 #pragma unroll
@@ -525,18 +552,21 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
   // dQ^T = K^T A^T + .., dK^T = Q^T A + K^T (M + M^T)^T + ..
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const f8 af = IO::from_acc(dp[2 * s], dp[2 * s + 1]), mf = IO::from_acc(ru[2 * s], ru[2 * s + 1]);
-    const f8 at = TF::get(lds.pairs.a, TP, 16 * w, s, lane), mt = TF::get(lds.pairs.m, TP, 16 * w, s, lane);
+    if (2 * s <= w) {
+      const Split<E> af(dp[2 * s], dp[2 * s + 1]), mf(ru[2 * s], ru[2 * s + 1]);
 #pragma unroll
-    for (int d = 0; d < KB; ++d) {
-      const f8 kf = TF::get(lds.k, PITCH, 16 * d, s, lane);
-      if (2 * s <= w) {
-        z[d] = mma32(kf, af, z[d]);
-        fu[d] = mma32(kf, mf, fu[d]);
+      for (int d = 0; d < KB; ++d) {
+        const f8 kf = TF::get(lds.k, PITCH, 16 * d, s, lane);
+        z[d] = mma_split(kf, af, z[d]);
+        fu[d] = mma_split(kf, mf, fu[d]);
       }
-      if (2 * s + 1 >= w) {
-        fu[d] = mma32(kf, mt, fu[d]);
-        fu[d] = mma32(TF::get(lds.pairs.q, PITCH, 16 * d, s, lane), at, fu[d]);
+    }
+    if (2 * s + 1 >= w) {
+      const Split<E> at = get_tri_t(lds.pairs.a, w, s, lane), mt = get_tri_t(lds.pairs.m, w, s, lane);
+#pragma unroll
+      for (int d = 0; d < KB; ++d) {
+        fu[d] = mma_split(TF::get(lds.k, PITCH, 16 * d, s, lane), mt, fu[d]);
+        fu[d] = mma_split(TF::get(lds.pairs.q, PITCH, 16 * d, s, lane), at, fu[d]);
       }
     }
   }
@@ -650,10 +680,9 @@ extern "C" {
 int ts_delta_bwd_workspace_bytes(const ts_delta_desc* d, size_t* bytes) {
   const int rc = ts::delta_check(d, nullptr, nullptr, "delta bwd");
   if (rc) return rc;
-  const size_t es = d->dtype == TS_BF16 ? 2 : 4;
   const size_t n = (size_t)d->B * d->H * ((d->T + 63) / 64), dvp = (d->dv + 15) / 16 * 16;
   const size_t dkp = d->dk <= 64 ? 64 : 128, nseg = ts::delta_segments(d);
-  size_t total = n * dvp * (64 + dkp) * es;
+  size_t total = n * dvp * (64 + dkp) * sizeof(float);  // (dR and dS, fp32 or two bf16 each)
   if (nseg > 1) total += 2 * (size_t)d->B * d->H * nseg * dvp * dkp * sizeof(float);
   if (d->H != d->Hk) total += align16(2 * (size_t)d->B * d->H * d->T * d->dk * sizeof(float));
   if (bytes) *bytes = total + align16((size_t)d->B * d->H * d->T * sizeof(float));
@@ -696,6 +725,14 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
   p.dr = ws;
   p.ds = ws + u;
   ws += u + s0;
+  if (es == 2) {
+    if (!io->low || ((uintptr_t)io->low & 15u))
+      return fail(TS_ERR_VALUE, "delta bwd: the low halves' buffer is missing or misaligned");
+    p.u_low = ((char*)io->low - (char*)p.u) / 2;
+    p.s0_low = ((char*)io->low + u - (char*)p.s0) / 2;
+    p.dr_low = p.ds_low = (int64_t)(u + s0) / 2;
+    ws += u + s0;
+  }
   if (p.nseg > 1) {
     // X of the forward's transfers, which follow its chunks' records
     const size_t states = (size_t)p.B * p.H * p.nseg * p.dvp * dkp * sizeof(float);
