@@ -88,3 +88,31 @@ def test_rows_of_ordinary_keys(cuda, Hk, T, dk, lengths):
                 s[name][b, :, n:] = 0.0
         lengths = torch.tensor(lengths)
     hold(s, cuda, lengths)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("H,T", [(2, 2), (2, 70), (1, 200)])
+def test_retentions_that_act_on_nothing_have_no_gradient(cuda, H, T, dtype):
+    """A first token's without an entering state, and a reset's (-inf, or a factor that
+    fp32 does not hold): exactly zero, not what rounding leaves of terms that cancel.
+    The others' are as their definition has them."""
+    import thetascan_amd as ts
+
+    s = inputs(2, 1, H, T, 64, 40, dtype, seed=T)
+    s["beta"], s["decay"] = s["beta"].float(), s["decay"].float()
+    resets = [t for t in (1, 40, 64, 65, 130, T - 1) if t < T]
+    s["decay"][..., resets] = -float("inf")
+    s["decay"][..., resets[-1:]] = -200.0
+    del s["state"]
+    ref_in = {n: x.double().requires_grad_() for n, x in s.items()}
+    ref = sum((x * (i + 1)).sum() for i, x in enumerate(reference(**ref_in)))
+    (want,) = torch.autograd.grad(ref, ref_in["decay"])
+    dev = on_gpu(s, cuda, True)
+    got = ts.gated_delta_rule(*dev.values(), return_state=True)
+    (grad,) = torch.autograd.grad(sum((x.float() * (i + 1)).sum() for i, x in enumerate(got)), dev["decay"])
+    zero = torch.zeros(T, dtype=torch.bool)
+    zero[[0, *resets]] = True
+    assert not bool(grad[..., zero].any())
+    if T > 2:
+        rest = want[..., ~zero]
+        assert float((grad.double().cpu()[..., ~zero] - rest).norm()) <= HELD * float(rest.norm())

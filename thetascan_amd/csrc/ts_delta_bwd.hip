@@ -7,9 +7,11 @@
 //   dQ = A K + e^G dO S0^T
 //   dK = A^T Q + (M + M^T) K + e^{G_63 - G} U dS^T - b e^G dR S0^T
 //   db_t = dR_t.U_t / b_t,   or dR_t.(v_t - e^{G_t} S0^T k_t - sum_i e^{G_t - G_i} k_t.k_i U_i) where b_t = 0
-//   dG_t = sum_i X_ti - sum_i X_it + e^{G_t} q_t.(S0 dO_t) - b e^{G_t} k_t.(S0 dR_t) - f_t,
-//     X = A (Q K^T) + M (K K^T) elementwise,  f_t = e^{G_63 - G_t} k_t.(dS U_t)
-//   dG_63 += sum_t f_t + e^{G_63} <S0, dS>;   dlog a_t = sum_{s >= t} dG_s
+//   dlog a_t = sum_{i < t <= s} X_si + sum_{s >= t} h_s + sum_{i < t} f_i + e^{G_63} <S0, dS>,
+//     X = A (Q K^T) + M (K K^T) elementwise,  h_s = e^{G_s} q_s.(S0 dO_s) - b e^{G_s} k_s.(S0 dR_s),
+//     f_i = e^{G_63 - G_i} k_i.(dS U_i)
+// (what token t's retention acts on, and nothing that would have to cancel: every term of a
+// reset holds its zero, and a first token's without an entering state are none.)
 //
 // delta_chain walks the chunks backwards, a wave per 16 value columns as in the
 // forward; it leaves dR and dS per chunk and writes dV.  delta_grads takes the
@@ -22,7 +24,7 @@
 // the gradient's own rounding.  Sums are fp32, those of the gates' gradients over a chunk fp64.
 //
 // 64 heads of 4096 tokens of 64 x 64, bf16: transfers 48 us, chain 95 (380 MB, 4.0 TB/s),
-// gradients 122 (483 MB, 4.0 TB/s; its loads and its products take turns in a workgroup, three
+// gradients 117 (483 MB, 4.1 TB/s; its loads and its products take turns in a workgroup, three
 // of which share a CU).  Without the low halves 33, 62 and 80 us.
 
 #include "ts_delta.h"
@@ -470,8 +472,8 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
   __syncthreads();
   // pairs (i, t): rows i = 16r + 4g + j, column t
   const double gt = lds.G[t];
-  float rows_x = 0.f, rows_n = 0.f;
-  float cx[16];
+  float rows_n = 0.f, before = 0.f;  // before: row t of X up to block r
+  float cx[16];                      // X_t0 + .. + X_ti, i < t
 #pragma unroll
   for (int i = 0; i < 16; ++i) cx[i] = 0.f;
   float diag = 0.f, diag_v = 0.f;
@@ -485,6 +487,7 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
         kk = mma32(ki, IO::ld8(lds.k + t * PITCH + 32 * s + 8 * g), kk);
         qk = mma32(ki, IO::ld8(lds.pairs.q + t * PITCH + 32 * s + 8 * g), qk);
       }
+      float own = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = 16 * r + 4 * g + j;
@@ -494,14 +497,19 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
           diag_v = rv[j];
         }
         const float a = i <= t ? dp[r][j] * d : 0.f, m = i < t ? ru[r][j] * d : 0.f;
-        // (X_tt is in its row's sum and its column's: left out of both)
-        const float xa = i < t ? a * qk[j] : 0.f, xn = m * kk[j];
-        rows_x += xa;
+        const float xn = m * kk[j];
         rows_n += xn;
-        cx[4 * r + j] = fmaf(-be, xn, xa);
+        own += fmaf(-be, xn, i < t ? a * qk[j] : 0.f);
+        cx[4 * r + j] = own;
         dp[r][j] = a;
         ru[r][j] = -be * m;
       }
+      // the lanes of lower columns: pairs give the even row's value first, then the lower half's
+      const LanePair near = xor16_pair(own), far = xor32_pair(near.a + near.b);
+      const float below = before + ((g & 1 ? near.a : 0.f) + (g & 2 ? far.a : 0.f));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cx[4 * r + j] = 16 * r + 4 * g + j < t ? below + cx[4 * r + j] : 0.f;
+      before += far.a + far.b;
     } else {
       dp[r] = ru[r] = zero4();
     }
@@ -535,10 +543,9 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
   zq = sum_g(zq) * eg;
   yk = sum_g(yk) * eg;
   fk = sum_g(fk) * tail;
-  rows_x = sum_g(rows_x);
   rows_n = sum_g(rows_n);
   if (g == 0) {
-    lds.base[t] = rows_x - be * rows_n + zq - be * yk - fk;
+    lds.base[t] = zq - be * yk;
     lds.f[t] = fk;
   }
   if (g == (l16 >> 2) && t0 + t < p.T) {  // the lane that holds (t, t)
@@ -577,19 +584,17 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
     put_row(p.dkey, d, in ? fu[d] : zero4());
   }
   if (w == 0 && p.ddecay) {
-    double dg = (double)lds.base[lane];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) dg -= (double)lds.cols[r][lane];
-    double total = (double)lds.f[lane];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
-    total += (double)whole * ((double)lds.red[0] + lds.red[1] + lds.red[2] + lds.red[3]);
-    if (lane == 63) dg += total;
+    double behind = (double)lds.base[lane], ahead = lane ? (double)lds.f[lane - 1] : 0.0;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const double above = __shfl_down(dg, o, 64);
-      if (lane + o < 64) dg += above;
+      const double above = __shfl_down(behind, o, 64), below = __shfl_up(ahead, o, 64);
+      if (lane + o < 64) behind += above;
+      if (lane >= o) ahead += below;
     }
+    double dg = behind + ahead + (double)whole * ((double)lds.red[0] + lds.red[1] + lds.red[2] + lds.red[3]);
+    if (lane)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dg += (double)lds.cols[r][lane - 1];
     if (t0 + lane < p.T) put_gate(p.ddecay, p.ddecay_bf16, gate0 + lane, t0 + lane < len ? (float)dg : 0.f);
   }
 }
