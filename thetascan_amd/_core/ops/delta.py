@@ -150,6 +150,9 @@ def _launch(q, k, v, beta, decay, state, lengths, want_state: bool, keep: bool, 
             with _lib.timed("ts_delta_fwd", lambda: _lib.nbytes(q, k, v4, beta, decay, out, given, final)):
                 status = lib.ts_delta_fwd(ctypes.byref(desc), ctypes.byref(io), work.data_ptr(), nbytes, stream)
             _lib.check(status, "ts_delta_fwd")
+    if final is not None and final is state_out and not final.is_inference():
+        # (the kernel's writing is autograd's in-place change: what saved the old values says so)
+        torch.autograd.graph.increment_version(final)
     if final is not None and final is not state_out:
         final = final[..., :dk, :dv]
         if (dkp, dvp) != (dk, dv):
