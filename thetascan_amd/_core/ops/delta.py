@@ -212,9 +212,9 @@ def _backward_impl(dout: torch.Tensor | None, dfinal: torch.Tensor | None, q: to
     _lib.check(status, "ts_delta_bwd")
     if (dkp, dvp) != (dk, dv):
         dq, dk_, dv_ = dq[..., :dk], dk_[..., :dk], dv_[..., :dv]
-        dstate = None if dstate is None else dstate[..., :dk, :dv]
+        dstate = None if dstate is None else dstate[..., :dk, :dv].contiguous()
     return [dq, dk_, dv_, dbeta, q.new_empty(0) if ddecay is None else ddecay,
-            q.new_empty(0) if dstate is None else dstate]
+            q.new_empty(0, dtype=torch.float32) if dstate is None else dstate]
 
 
 def _backward_fake(dout, dfinal, q, k, v, beta, decay, state, lengths, saved, need_state):
