@@ -93,19 +93,23 @@ struct RowSpan {
   }
 };
 
-// One row's terms from its maximum and sum, in fp64.
+// One row's terms from its maximum and sum, in fp64.  Where the token is the maximum, its
+// distance from it is zero: the capped maximum is off by up to cap 2^-23, and a difference from
+// the token's exact value gave log-probabilities above zero (of up to 3e-6 at a cap of 30).
 template <typename E, int CAP>
 __device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, float m, float s, float& lpf, float& coef,
                                           float& logs, double& term) {
   const double l2 = log2((double)s), top = CAP == kCap ? (double)m * kLn2 : (double)m;
   const int64_t tok = p.tokens[n];
-  double y = (double)NAN;  // a token that is none of the row's
+  double off = (double)NAN;  // the token's logit from the maximum; of a token that is none of the row's
   if (tok >= 0 && tok < p.V) {
-    y = (double)tof(((const E*)p.z)[n * p.stride + tok]);
+    const float z = tof(((const E*)p.z)[n * p.stride + tok]);
+    double y = (double)z;
     if (CAP == kCap) y = (double)p.cap * (1.0 - 2.0 / (1.0 + exp(2.0 * y / (double)p.cap)));
     if (CAP == kWide) y = (double)p.cap * tanh(y / (double)p.cap);
+    off = CAP && Logit<CAP>(p.cap)(z) >= m ? 0.0 : y - top;
   }
-  const double lp = (y - top) - l2 * kLn2;
+  const double lp = off - l2 * kLn2;
   logs = (float)l2;
   lpf = (float)lp;
   if (!p.adv) return;
