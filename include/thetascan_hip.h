@@ -59,7 +59,8 @@ extern "C" {
  *     ts_policy_loss_parts / ts_policy_one_pass / ts_policy_scale and ts_capture_id; nothing
  *     earlier changed.
  * 20: ts_delta_io has a buffer for the low halves of what a bf16 forward keeps (low,
- *     ts_delta_low_bytes), which ts_delta_bwd reads. */
+ *     ts_delta_low_bytes), which ts_delta_bwd reads; ts_policy_loss_scale in place of
+ *     ts_policy_scale. */
 #define TS_ABI_VERSION 20
 
 enum ts_status {
@@ -1347,8 +1348,9 @@ int ts_policy_loss_parts(const ts_policy_desc* desc, int64_t* parts);
 int ts_policy_loss_fwd(const ts_policy_desc* desc, const ts_policy_io* io, hipStream_t stream);
 /* Whether loss and gradient of rows of this length are formed in one pass. */
 int ts_policy_one_pass(const ts_policy_desc* desc, int32_t* one_pass);
-/* x[i] *= g[0] (n elements of ts_dtype `dtype`, 16-byte aligned); nothing where it is one. */
-int ts_policy_scale(void* x, int64_t n, int32_t dtype, const float* g, hipStream_t stream);
+/* io.dlogits, as such a forward left it, for the loss's gradient dloss: formed again from the
+ * logits (one rounding, zero in rows of weight zero) where that is not one.  Once a forward. */
+int ts_policy_loss_scale(const ts_policy_desc* desc, const ts_policy_io* io, const float* dloss, hipStream_t stream);
 /* The graph that `stream` is being captured into (0: none): what a forward leaves for
  * its backward to change in place is only the backward's of the same graph. */
 int ts_capture_id(hipStream_t stream, uint64_t* id);

@@ -10,8 +10,8 @@ logits, with ``y = cap tanh(z / cap)`` (or z), ``lp = log softmax(y)[token]`` an
 
 One pass over the logits a direction (ts_policy_loss_fwd, ts_policy_loss_bwd);
 where a gradient is recorded and rows are long (and not few), the forward gives the gradient for a
-unit upstream gradient too, which the backward scales where it is another (a second
-backward of the same loss forms it again).  Neither the capped logits nor the
+unit upstream gradient too, which the backward forms again where it is another (as does a
+second backward of the same loss).  Neither the capped logits nor the
 probabilities are stored.  A row of weight zero
 (a prompt's, a padding's) is not read.
 """
@@ -95,19 +95,28 @@ def _forward_fake(z, tokens, old, adv, ref, weights, low, high, kl, cap):
 
 def _backward_impl(g: torch.Tensor, z: torch.Tensor, tokens: torch.Tensor, weights: torch.Tensor | None,
                    saved: torch.Tensor, cap: float) -> torch.Tensor:
+    return _gradient(g, z, tokens, weights, saved, cap, None)
+
+
+def _gradient(g, z, tokens, weights, saved, cap, formed: torch.Tensor | None) -> torch.Tensor:
+    """The logits' gradient; ``formed`` is the forward's, for a unit ``g``, which
+    becomes it."""
     lib = _lib.load()
     z = _rows(z)
     rows = z.shape[0]
-    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if formed is None else formed
     g32 = g if g.dtype == torch.float32 else g.to(torch.float32)
     coef = saved.data_ptr() + 4 * (saved.numel() - 3 * rows)
     io = _lib.PolicyIO(z.data_ptr(), tokens.data_ptr(), None, None, None, _lib.ptr(weights), None, coef,
-                       coef + 4 * rows, None, None, None)
-    desc = _desc(z, cap)
-    with _on(z.device), _lib.timed("ts_policy_loss_bwd", lambda: _lib.nbytes(z, tokens, dz)):
-        status = lib.ts_policy_loss_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(),
-                                        _lib.stream_handle(z.device))
-    _lib.check(status, "ts_policy_loss_bwd")
+                       coef + 4 * rows, None, None, dz.data_ptr())
+    desc, name = _desc(z, cap), "ts_policy_loss_bwd" if formed is None else "ts_policy_loss_scale"
+    with _on(z.device), _lib.timed(name, lambda: _lib.nbytes(z, tokens, dz)):
+        stream = _lib.stream_handle(z.device)
+        if formed is None:
+            status = lib.ts_policy_loss_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(), stream)
+        else:
+            status = lib.ts_policy_loss_scale(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), stream)
+    _lib.check(status, name)
     return dz
 
 
@@ -130,22 +139,12 @@ def _backward(ctx, grads, bwd):
     dz, graph = ctx.__dict__.pop("dz", (None, 0))
     if dz is not None:
         # (a backward in a graph of its own may be replayed more often than the
-        # forward, and would scale what it has scaled)
+        # forward, and would take another gradient's for the unit one's; each is handed out once)
         with _on(dz.device):
             same = _capture(dz.device) == graph
         if same:
-            return (_scaled(dz, grads[0]), *(None,) * 9)
+            return (_gradient(grads[0], z, tokens, weights, saved, ctx.cap, dz), *(None,) * 9)
     return (bwd(grads[0], z, tokens, weights, saved, ctx.cap), *(None,) * 9)
-
-
-def _scaled(dz: torch.Tensor, g: torch.Tensor) -> torch.Tensor:
-    """The forward's gradient times the loss's, in place (each is handed out once)."""
-    g32 = g if g.dtype == torch.float32 else g.to(torch.float32)
-    with _on(dz.device), _lib.timed("ts_policy_scale", 0):
-        status = _lib.load().ts_policy_scale(dz.data_ptr(), dz.numel(), _lib.dtype_code(dz.dtype), g32.data_ptr(),
-                                             _lib.stream_handle(dz.device))
-    _lib.check(status, "ts_policy_scale")
-    return dz
 
 
 _policy_op = HipOp("policy_loss", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,

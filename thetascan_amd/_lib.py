@@ -731,7 +731,7 @@ def load() -> ctypes.CDLL:
                                      ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         lib.ts_policy_loss_parts.argtypes = [P(PolicyDesc), P(ctypes.c_int64)]
         lib.ts_policy_one_pass.argtypes = [P(PolicyDesc), P(ctypes.c_int32)]
-        lib.ts_policy_scale.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
+        lib.ts_policy_loss_scale.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_capture_id.argtypes = [ctypes.c_void_p, P(ctypes.c_uint64)]
         lib.ts_policy_loss_fwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p]
         lib.ts_policy_loss_bwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]

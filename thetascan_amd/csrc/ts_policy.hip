@@ -41,6 +41,7 @@ struct PolicyP {
   int split;
   const float* g;
   void* dz;
+  int formed;  // dz holds the gradient for g = 1: nothing is left to do there
 };
 
 // A logit as the softmax takes it, x, and e^x relative to a maximum.  kPlain: x is the
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
   constexpr int LANES = 64 * WPR, GROUPS = 256 / LANES;
   const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
   const int64_t n = (int64_t)blockIdx.x * GROUPS + gi;
-  if (n >= p.rows) return;
+  if (n >= p.rows || (p.formed && p.g[0] == 1.f)) return;
   const float c = p.coef[n] * p.g[0], top = p.lse[n], logs = p.lse[p.rows + n];
   const int64_t tok = p.tokens[n];
   const bool read = !p.w || p.w[n] != 0.f;
@@ -418,25 +419,6 @@ __global__ __launch_bounds__(256) void policy_fused_kernel(PolicyP p) {
   }
   __syncthreads();
   row_grad<E, CAP, 256>(row, (E*)p.dz + n * (int64_t)p.V, p.V, read, f, sc[0], m, sc[1], p.tokens[n], tid, 0, 1);
-}
-
-// x *= g, where g is not one.
-template <typename E>
-__global__ __launch_bounds__(256) void policy_scale_kernel(E* x, int64_t n, const float* g) {
-  constexpr int N = Vec16<E>::N;
-  const float scale = g[0];
-  if (scale == 1.f) return;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i * N < n; i += (int64_t)gridDim.x * 256) {
-    if (i * N + N <= n) {
-      Vec16<E> v;
-      v.raw = ((const Vec16<E>*)x)[i].raw;
-#pragma unroll
-      for (int j = 0; j < N; ++j) v.e[j] = cvt<E>(scale * tof(v.e[j]));
-      ((Vec16<E>*)x)[i].raw = v.raw;
-    } else {
-      for (int64_t j = i * N; j < n; ++j) x[j] = cvt<E>(scale * tof(x[j]));
-    }
-  }
 }
 
 }  // namespace ts
@@ -588,20 +570,6 @@ int ts_policy_one_pass(const ts_policy_desc* d, int32_t* yes) {
   return TS_OK;
 }
 
-int ts_policy_scale(void* x, int64_t n, int32_t dtype, const float* g, hipStream_t stream) {
-  if (n < 0 || (n && (!x || ((uintptr_t)x & 15u) || !g)))
-    return fail(TS_ERR_VALUE, "policy_scale: missing or misaligned tensors");
-  if (dtype != TS_BF16 && dtype != TS_F32) return fail(TS_ERR_NOT_IMPLEMENTED, "policy_scale: bf16 or fp32 only");
-  if (n == 0) return TS_OK;
-  const int64_t blocks = (n / (dtype == TS_BF16 ? 8 : 4) + 256) / 256;
-  const dim3 grid((unsigned)(blocks < 2048 ? blocks : 2048));
-  if (dtype == TS_BF16)
-    hipLaunchKernelGGL(ts::policy_scale_kernel<ts::bf16>, grid, dim3(256), 0, stream, (ts::bf16*)x, n, g);
-  else
-    hipLaunchKernelGGL(ts::policy_scale_kernel<float>, grid, dim3(256), 0, stream, (float*)x, n, g);
-  return finish("policy_scale");
-}
-
 int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStream_t stream) {
   PolicyP p;
   if (!io) return fail(TS_ERR_VALUE, "policy_loss: missing tensors");
@@ -633,8 +601,8 @@ int ts_policy_loss_fwd(const ts_policy_desc* d, const ts_policy_io* io, hipStrea
   return finish("policy_loss");
 }
 
-int ts_policy_loss_bwd(const ts_policy_desc* d, const ts_policy_io* io, const float* dloss, void* dlogits,
-                       hipStream_t stream) {
+static int policy_bwd(const ts_policy_desc* d, const ts_policy_io* io, const float* dloss, void* dlogits, bool formed,
+                      hipStream_t stream) {
   PolicyP p;
   if (!io) return fail(TS_ERR_VALUE, "policy_loss bwd: missing tensors");
   const int rc = setup(d, io->logits, io->tokens, &p);
@@ -642,12 +610,21 @@ int ts_policy_loss_bwd(const ts_policy_desc* d, const ts_policy_io* io, const fl
   if (d->rows == 0) return TS_OK;
   if (!io->coef || !io->lse || !dloss || !dlogits || ((uintptr_t)dlogits & (d->dtype == TS_BF16 ? 1u : 3u)))
     return fail(TS_ERR_VALUE, "policy_loss bwd: missing or misaligned tensors");
-  p.w = io->weights; p.coef = io->coef; p.lse = io->lse; p.g = dloss; p.dz = dlogits;
+  p.w = io->weights; p.coef = io->coef; p.lse = io->lse; p.g = dloss; p.dz = dlogits; p.formed = formed;
   if (d->dtype == TS_BF16)
     backward<ts::bf16>(p, stream);
   else
     backward<float>(p, stream);
   return finish("policy_loss bwd");
+}
+
+int ts_policy_loss_bwd(const ts_policy_desc* d, const ts_policy_io* io, const float* dloss, void* dlogits,
+                       hipStream_t stream) {
+  return policy_bwd(d, io, dloss, dlogits, false, stream);
+}
+
+int ts_policy_loss_scale(const ts_policy_desc* d, const ts_policy_io* io, const float* dloss, hipStream_t stream) {
+  return policy_bwd(d, io, dloss, io ? io->dlogits : nullptr, true, stream);
 }
 
 }  // extern "C"
