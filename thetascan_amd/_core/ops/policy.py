@@ -11,7 +11,9 @@ logits, with ``y = cap tanh(z / cap)`` (or z), ``lp = log softmax(y)[token]`` an
 One pass over the logits a direction (ts_policy_loss_fwd, ts_policy_loss_bwd);
 where a gradient is recorded and rows are long (and not few), the forward gives the gradient for a
 unit upstream gradient too, which the backward forms again where it is another (as does a
-second backward of the same loss).  Neither the capped logits nor the
+second backward of the same loss).  It is as large as the logits and held from the
+forward to the backward, as a saved tensor: offloading hooks and (non-reentrant)
+activation checkpointing see it.  Neither the capped logits nor the
 probabilities are stored.  A row of weight zero
 (a prompt's, a padding's) is not read.
 """
@@ -126,24 +128,24 @@ def _backward_fake(g, z, tokens, weights, saved, cap):
 
 def _setup(ctx, inputs, output):
     z, tokens, weights, ctx.cap = inputs[0], inputs[1], inputs[5], inputs[9]
-    ctx.save_for_backward(z, tokens, weights, output[2])
     left, _GRADIENT.of = getattr(_GRADIENT, "of", None), None
-    if left is not None and left[0] is output[0]:
-        ctx.dz = left[1:]
+    dz, ctx.graph = left[1:] if left is not None and left[0] is output[0] else (None, None)
+    ctx.save_for_backward(z, tokens, weights, output[2], dz)
 
 
 def _backward(ctx, grads, bwd):
     if grads[0] is None:
         return (None,) * 10
-    z, tokens, weights, saved = ctx.saved_tensors
-    dz, graph = ctx.__dict__.pop("dz", (None, 0))
-    if dz is not None:
+    z, tokens, weights, saved, dz = ctx.saved_tensors
+    graph, ctx.graph = ctx.graph, None
+    if dz is not None and graph is not None:
         # (a backward in a graph of its own may be replayed more often than the
         # forward, and would take another gradient's for the unit one's; each is handed out once)
         with _on(dz.device):
             same = _capture(dz.device) == graph
         if same:
-            return (_gradient(grads[0], z, tokens, weights, saved, ctx.cap, dz), *(None,) * 9)
+            # (.data: what the caller does with it is no change of the saved tensor)
+            return (_gradient(grads[0], z, tokens, weights, saved, ctx.cap, dz.data), *(None,) * 9)
     return (bwd(grads[0], z, tokens, weights, saved, ctx.cap), *(None,) * 9)
 
 
