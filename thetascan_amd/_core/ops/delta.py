@@ -30,7 +30,7 @@ import functools
 import torch
 
 from ... import _lib
-from .dispatch import HipOp
+from .dispatch import HipOp, refuse_tangents
 from .scan_hip import _kernel_view, _vec
 
 MAX_KEYS, MAX_VALUES = 128, 512
@@ -280,7 +280,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
     zero, and leave its state as it was.  ``state_out`` (without gradients only) is
     the contiguous fp32 tensor to write the new state into; it may be ``state``.
 
-    Differentiable in q, k, v, beta, the retention and the state.
+    Differentiable in q, k, v, beta, the retention and the state (backwards; forward-mode
+    derivatives are refused).
     """
     if not q.ndim == k.ndim == v.ndim == 4:
         name, x = next(i for i in (("q", q), ("k", k), ("v", v)) if i[1].ndim != 4)
@@ -311,6 +312,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
             raise ValueError(f"gated_delta_rule: {name} must be fp32 {(B, H, dk, dv)}, got {s.dtype} {tuple(s.shape)}")
     if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"gated_delta_rule: lengths must be integers [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
+    if not torch.compiler.is_compiling():
+        refuse_tangents("gated_delta_rule", q, k, v, beta, retention, state)
     device, record = q.get_device(), torch.is_grad_enabled() and q.requires_grad
     if device < 0:
         raise RuntimeError("hip backend: tensors must live on the GPU (no CPU fallback)")

@@ -26,6 +26,7 @@ from __future__ import annotations
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _EAGER = threading.local()
 
@@ -34,6 +35,15 @@ def eager_forward() -> bool:
     """True inside a forward that the eager autograd.Function runs (its setup
     follows on the same thread), False under the custom-op dispatcher."""
     return getattr(_EAGER, "active", False)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raise where a tensor has a forward-mode tangent: where autograd records nothing,
+    a launch would drop it without a word."""
+    if forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivatives")
 
 
 def _tensor_slots(args):

@@ -27,7 +27,7 @@ import torch
 
 from ... import _lib
 from .delta import _on
-from .dispatch import HipOp, eager_forward
+from .dispatch import HipOp, eager_forward, refuse_tangents
 
 _GRADIENT = threading.local()  # the gradient that an eager forward leaves for its setup
 
@@ -202,7 +202,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch
     multiplies each row's loss (default: the mean over all rows); a row of weight
     zero may hold anything in any input, and gives a log-probability of zero and a
     gradient of zero.  At most 2^24 rows (2^26 of up to 2048 logits) a call.
-    ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.
+    ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.  Forward-mode
+    derivatives are refused.
     """
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl = float(low), float(high), float(kl)
@@ -212,6 +213,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch
         raise ValueError(f"policy_loss: kl must be at least 0, got {kl}")
     if kl and ref_log_probs is None:
         raise ValueError("policy_loss: the KL term needs ref_log_probs")
+    if not torch.compiler.is_compiling():
+        refuse_tangents("policy_loss", logits)
     z, tok, cap, r = _flat("policy_loss", logits, tokens, softcap,
                            {"old_log_probs": old_log_probs, "advantages": advantages,
                             "ref_log_probs": ref_log_probs if kl else None, "weights": weights})
