@@ -246,7 +246,7 @@ def _backward(ctx, grads, bwd):
 
 
 _delta_op = HipOp("gated_delta", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,
-                  backward_fake=_backward_fake, setup=_setup, backward=_backward)
+                  backward_fake=_backward_fake, setup=_setup, backward=_backward, once=True)
 
 
 def _token_gate(t: torch.Tensor, name: str, B: int, H: int, T: int) -> torch.Tensor:
@@ -280,8 +280,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
     zero, and leave its state as it was.  ``state_out`` (without gradients only) is
     the contiguous fp32 tensor to write the new state into; it may be ``state``.
 
-    Differentiable in q, k, v, beta, the retention and the state (backwards; forward-mode
-    derivatives are refused).
+    Differentiable in q, k, v, beta, the retention and the state (once, backwards:
+    forward-mode and second derivatives are refused).
     """
     if not q.ndim == k.ndim == v.ndim == 4:
         name, x = next(i for i in (("q", q), ("k", k), ("v", v)) if i[1].ndim != 4)

@@ -83,11 +83,37 @@ class _Eager(torch.autograd.Function):
         return (None, None, None, *flat)
 
 
-class HipOp:
-    """One HIP operation with its backward (see the module docstring)."""
+class _Final(torch.autograd.Function):
+    """Its argument, with a derivative that raises."""
 
-    def __init__(self, name: str, *, forward, forward_fake, backward_impl, backward_fake, setup, backward):
+    @staticmethod
+    def forward(ctx, grad):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("trying to differentiate twice a HIP operation that has first derivatives only")
+
+
+class _EagerOnce(_Eager):
+    @staticmethod
+    def backward(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return _Eager.backward(ctx, *grads)
+        # with create_graph: a second derivative would take the first for a constant
+        with torch.no_grad():
+            flat = _Eager.backward(ctx, *grads)
+        return tuple(None if g is None else _Final.apply(g.detach().requires_grad_()) for g in flat)
+
+
+class HipOp:
+    """One HIP operation with its backward (see the module docstring); ``once``:
+    its gradients refuse to be differentiated again."""
+
+    def __init__(self, name: str, *, forward, forward_fake, backward_impl, backward_fake, setup, backward,
+                 once: bool = False):
         self.name = name
+        self.node = _EagerOnce if once else _Eager
         self.forward, self.backward_impl = forward, backward_impl
         self.setup, self.backward = setup, backward
         self.op = torch.library.custom_op(f"thetascan_hip::{name}", forward, mutates_args=())
@@ -105,5 +131,5 @@ class HipOp:
             # nothing to record (inference, streaming continuation): the
             # forward alone, without an autograd node around it
             return self.forward(*args)
-        out = _Eager.apply(self, slots, args, *tensors)
+        out = self.node.apply(self, slots, args, *tensors)
         return list(out) if isinstance(out, tuple) else out

@@ -150,7 +150,7 @@ def _backward(ctx, grads, bwd):
 
 
 _policy_op = HipOp("policy_loss", forward=_forward, forward_fake=_forward_fake, backward_impl=_backward_impl,
-                   backward_fake=_backward_fake, setup=_setup, backward=_backward)
+                   backward_fake=_backward_fake, setup=_setup, backward=_backward, once=True)
 
 
 def _row_values(x: torch.Tensor | None) -> torch.Tensor | None:
@@ -202,8 +202,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_log_probs: torch
     multiplies each row's loss (default: the mean over all rows); a row of weight
     zero may hold anything in any input, and gives a log-probability of zero and a
     gradient of zero.  At most 2^24 rows (2^26 of up to 2048 logits) a call.
-    ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.  Forward-mode
-    derivatives are refused.
+    ``softcap`` caps the logits at ``softcap tanh(z / softcap)``.  Forward-mode and
+    second derivatives are refused.
     """
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl = float(low), float(high), float(kl)
