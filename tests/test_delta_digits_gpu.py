@@ -116,3 +116,29 @@ def test_retentions_that_act_on_nothing_have_no_gradient(cuda, H, T, dtype):
     if T > 2:
         rest = want[..., ~zero]
         assert float((grad.double().cpu()[..., ~zero] - rest).norm()) <= HELD * float(rest.norm())
+
+
+@pytest.mark.parametrize("Hk,T,dk,dv,lengths", [(2, 200, 64, 64, None), (1, 130, 40, 72, [130, 64]),
+                                                (1, 2200, 64, 64, [2200, 1283]), (1, 1100, 128, 128, None)])
+def test_states_of_bf16_streams_are_fp32_ones(cuda, Hk, T, dk, dv, lengths):
+    """The fp32 state of a bf16 call: operands in three parts hold 24 bits, and what is
+    left out of their products is less; some 16 roundings of 2^-24 (the sums of a chunk,
+    of the inverse, of what is written and of the state) do not cancel for ordinary keys."""
+    import thetascan_amd as ts
+
+    s = inputs(2, Hk, 2, T, dk, dv, BF, seed=T, state=True)
+    s["beta"], s["decay"] = s["beta"].float(), s["decay"].float() * 0.1
+    if lengths:
+        for b, n in enumerate(lengths):
+            for name in ("q", "k", "v", "beta", "decay"):
+                s[name][b, :, n:] = 0.0
+        lengths = torch.tensor(lengths)
+    _, want = reference(**s, lengths=lengths)
+    dev = on_gpu(s, cuda, False)
+    for grad in (False, True):
+        q = dev["q"].detach().requires_grad_(grad)
+        _, got = ts.gated_delta_rule(q, *(dev[n] for n in ("k", "v", "beta", "decay")), state=dev["state"],
+                                     lengths=None if lengths is None else lengths.to(cuda), return_state=True)
+        off = float((got.detach().double().cpu() - want).norm() / want.norm())
+        print(f"{off:.1e}", flush=True)
+        assert off <= 16 * 2.0 ** -24

@@ -14,10 +14,10 @@ ts_delta_bwd for the gradients); a few tokens against a carried state, without
 gradients, run token by token in one pass over the state (ts_delta_step).  Both
 are the same function of their inputs.
 
-bf16 inputs: products take bf16 operands and fp32 sums; everything that feeds the
-state in the forward (the state itself, what is written, the chunk's inverse)
-enters as a bf16 pair hi + lo, in the backward too, so the returned state is exact to
-about 1e-5, and outputs and gradients carry bf16's one rounding.  fp32 inputs compute in fp32.
+bf16 inputs: products take bf16 operands and fp32 sums; what is not an input enters in
+three bf16 parts in the forward, so the returned state is one of fp32 arithmetic, and in
+two in the backward: bf16 outputs and gradients carry bf16's one rounding, fp32 gradients
+(of states and of fp32 gates) 16 bits.  fp32 inputs compute in fp32.
 A non-finite value in a token that counts spreads over its chunk of 64 tokens
 and everything after it.
 """

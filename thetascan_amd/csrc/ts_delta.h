@@ -33,18 +33,16 @@ __device__ __forceinline__ constexpr int tri(int r, int s) { return r < 2 ? r : 
 // Elements of one fragment set in the workspace.
 constexpr int kTriElems = kTri * 64 * 8;
 
-// The inverse and P are kept as bf16 pairs hi + lo (fp32: once): where keys are
-// alike, sums over the chunk cancel, and what one rounding leaves does not.
-template <typename E> struct TriSets { static constexpr int N = 1; };
-template <> struct TriSets<bf16> { static constexpr int N = 2; };
+// Parts that a value enters products in: bf16 ones whose sum it is (fp32: itself).  Where
+// keys are alike, sums over a chunk cancel, and what one rounding leaves does not.  Three
+// hold fp32's 24 bits, for what the state and the outputs come of; two hold 16, for the
+// gradients, which are rounded to 8.
+template <typename E, int N> constexpr int kParts = sizeof(E) == 2 ? N : 1;
 
-// Per chunk, in bytes: the inverse, P, and e^G, e^{G_63 - G}, b (fp32 x 64 each,
-// zero past the length) and e^{G_63}.
+// Per chunk, fp32: the inverse, P, and e^G, e^{G_63 - G}, b (64 each, zero past the
+// length) and e^{G_63}.
 constexpr int kVec = 3 * kChunk + 4;
-constexpr size_t kVecBytes = kVec * sizeof(float);
-template <typename E> __host__ __device__ constexpr size_t prep_bytes() {
-  return (size_t)2 * TriSets<E>::N * kTriElems * sizeof(E) + kVecBytes;
-}
+constexpr int kRecord = 2 * kTriElems + kVec;
 
 struct DeltaP {
   int B, Hk, H, rep, T, dk, dv, nc;  // nc: chunks of T
@@ -54,7 +52,7 @@ struct DeltaP {
   const int64_t* lengths;  // [B] or null
   const float* state;      // [B,H,dk,dv] or null (zero)
   float* state_out;        // or null
-  char* prep;              // [B*H*nc] of prep_bytes
+  float* prep;             // [B*H*nc] of kRecord
   int nseg, seg_chunks;    // segments of the chain, chunks of each
   float* seg_x;            // [B*H*nseg][seg_stride]: X as rows, N, and (kept) X as columns
   int64_t seg_stride;
@@ -102,77 +100,95 @@ __device__ __forceinline__ unsigned pack2(float x, float y) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2{x, y}), bf16x2));
 }
 
-// Accumulators of two 16-row blocks as an operand, in one rounding (hi) and
-// what that leaves (lo): hi + lo holds 16 bits and more.  fp32 keeps everything
-// in hi.
-template <typename E> struct Split;
-template <> struct Split<bf16> {
-  bf16x8 hi, lo;
-  __device__ __forceinline__ Split(floatx4 a, floatx4 b) {
-    uint4 h, l;
-    two(a[0], a[1], h.x, l.x);
-    two(a[2], a[3], h.y, l.y);
-    two(b[0], b[1], h.z, l.z);
-    two(b[2], b[3], h.w, l.w);
-    hi = __builtin_bit_cast(bf16x8, h);
-    lo = __builtin_bit_cast(bf16x8, l);
+// Two values' leading bf16 parts, packed, and what they leave.
+// (two to a conversion: one at a time takes a conversion each and their packing)
+__device__ __forceinline__ unsigned lead2(float& x, float& y) {
+  const unsigned h = pack2(x, y);
+  x -= __uint_as_float(h << 16);
+  y -= __uint_as_float(h & 0xffff0000u);
+  return h;
+}
+
+// An operand in N parts (fp32: in one), from the accumulators of two 16-row blocks or
+// from parts in memory.
+template <typename E, int N> struct Parts;
+template <int N> struct Parts<bf16, N> {
+  bf16x8 p[N];
+  __device__ __forceinline__ Parts() {}
+  __device__ __forceinline__ Parts(floatx4 a, floatx4 b) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint4 u;
+      u.x = lead2(v[0], v[1]);
+      u.y = lead2(v[2], v[3]);
+      u.z = lead2(v[4], v[5]);
+      u.w = lead2(v[6], v[7]);
+      p[i] = __builtin_bit_cast(bf16x8, u);
+    }
   }
-  __device__ __forceinline__ Split(bf16x8 h, bf16x8 l) : hi(h), lo(l) {}
-  // The first block's four rows to a, the second's to b, what they leave `low` elements behind.
-  __device__ __forceinline__ void store(bf16* a, bf16* b, int64_t low) const {
-    const uint4 h = __builtin_bit_cast(uint4, hi), l = __builtin_bit_cast(uint4, lo);
+  // The first block's four rows to a, the second's to b, of the second part `low` elements behind.
+  __device__ __forceinline__ void store2(bf16* a, bf16* b, int64_t low) const {
+    const uint4 h = __builtin_bit_cast(uint4, p[0]), l = __builtin_bit_cast(uint4, p[1]);
     *(uint2*)a = make_uint2(h.x, h.y);
     *(uint2*)b = make_uint2(h.z, h.w);
     *(uint2*)(a + low) = make_uint2(l.x, l.y);
     *(uint2*)(b + low) = make_uint2(l.z, l.w);
   }
-  // (two elements to a conversion: one at a time takes a conversion each and their packing)
-  static __device__ __forceinline__ void two(float x, float y, unsigned& h, unsigned& l) {
-    h = pack2(x, y);
-    l = pack2(x - __uint_as_float(h << 16), y - __uint_as_float(h & 0xffff0000u));
+};
+template <int N> struct Parts<float, N> {
+  floatx8 p[1];
+  __device__ __forceinline__ Parts() {}
+  __device__ __forceinline__ Parts(floatx4 a, floatx4 b) {
+    p[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  __device__ __forceinline__ void store2(float* a, float* b, int64_t) const {
+    *(floatx4*)a = __builtin_shufflevector(p[0], p[0], 0, 1, 2, 3);
+    *(floatx4*)b = __builtin_shufflevector(p[0], p[0], 4, 5, 6, 7);
   }
 };
-template <> struct Split<float> {
-  floatx8 hi;
-  __device__ __forceinline__ Split(floatx4 a, floatx4 b) { hi = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
-  __device__ __forceinline__ explicit Split(floatx8 h) : hi(h) {}
-  __device__ __forceinline__ void store(float* a, float* b, int64_t) const {
-    *(floatx4*)a = __builtin_shufflevector(hi, hi, 0, 1, 2, 3);
-    *(floatx4*)b = __builtin_shufflevector(hi, hi, 4, 5, 6, 7);
-  }
-};
-// c + x (y.hi + y.lo) and c + (y.hi + y.lo) x
-__device__ __forceinline__ floatx4 mma_split(bf16x8 x, const Split<bf16>& y, floatx4 c) {
-  return mma32(x, y.hi, mma32(x, y.lo, c));
+// c + x y, the smallest products first; of two operands in parts, those that reach the
+// last part's place.
+template <typename E, int N>
+__device__ __forceinline__ floatx4 mma_parts(typename Frag<E>::f8 x, const Parts<E, N>& y, floatx4 c) {
+#pragma unroll
+  for (int i = kParts<E, N> - 1; i >= 0; --i) c = mma32(x, y.p[i], c);
+  return c;
 }
-__device__ __forceinline__ floatx4 mma_split(floatx8 x, const Split<float>& y, floatx4 c) { return mma32(x, y.hi, c); }
-__device__ __forceinline__ floatx4 mma_split(const Split<bf16>& y, bf16x8 x, floatx4 c) {
-  return mma32(y.hi, x, mma32(y.lo, x, c));
+template <typename E, int N>
+__device__ __forceinline__ floatx4 mma_parts(const Parts<E, N>& y, typename Frag<E>::f8 x, floatx4 c) {
+#pragma unroll
+  for (int i = kParts<E, N> - 1; i >= 0; --i) c = mma32(y.p[i], x, c);
+  return c;
 }
-__device__ __forceinline__ floatx4 mma_split(const Split<float>& y, floatx8 x, floatx4 c) { return mma32(y.hi, x, c); }
-// c + x y of a pair each: what the two remainders make together (2^-16) is left out.
-__device__ __forceinline__ floatx4 mma_split(const Split<bf16>& x, const Split<bf16>& y, floatx4 c) {
-  return mma32(x.hi, y.hi, mma32(x.hi, y.lo, mma32(x.lo, y.hi, c)));
-}
-__device__ __forceinline__ floatx4 mma_split(const Split<float>& x, const Split<float>& y, floatx4 c) {
-  return mma32(x.hi, y.hi, c);
+template <typename E, int N>
+__device__ __forceinline__ floatx4 mma_parts(const Parts<E, N>& x, const Parts<E, N>& y, floatx4 c) {
+#pragma unroll
+  for (int sum = kParts<E, N> - 1; sum >= 0; --sum)
+#pragma unroll
+    for (int i = sum; i >= 0; --i) c = mma32(x.p[i], y.p[sum - i], c);
+  return c;
 }
 
-// One fragment of a triangular matrix into its sets, and one read back.
-__device__ __forceinline__ void put_tri(bf16* m, int r, int s, int lane, const Split<bf16>& f) {
-  bf16* at = m + (tri(r, s) * 64 + lane) * 8;
-  *(bf16x8*)at = f.hi;
-  *(bf16x8*)(at + kTriElems) = f.lo;
+// One fragment of a triangular matrix of N parts in LDS, kTriElems from one to the next.
+template <int N, typename E>
+__device__ __forceinline__ Parts<E, N> get_tri(const E* m, int r, int s, int lane) {
+  Parts<E, N> f;
+#pragma unroll
+  for (int i = 0; i < kParts<E, N>; ++i)
+    f.p[i] = *(const typename Frag<E>::f8*)(m + i * kTriElems + (tri(r, s) * 64 + lane) * 8);
+  return f;
 }
-__device__ __forceinline__ void put_tri(float* m, int r, int s, int lane, const Split<float>& f) {
-  *(floatx8*)(m + (tri(r, s) * 64 + lane) * 8) = f.hi;
-}
-__device__ __forceinline__ Split<bf16> get_tri(const bf16* m, int r, int s, int lane) {
-  const bf16* at = m + (tri(r, s) * 64 + lane) * 8;
-  return Split<bf16>(*(const bf16x8*)at, *(const bf16x8*)(at + kTriElems));
-}
-__device__ __forceinline__ Split<float> get_tri(const float* m, int r, int s, int lane) {
-  return Split<float>(*(const floatx8*)(m + (tri(r, s) * 64 + lane) * 8));
+template <int N, typename E>
+__device__ __forceinline__ void put_tri(E* m, int r, int s, int lane, const Parts<E, N>& f) {
+#pragma unroll
+  for (int i = 0; i < kParts<E, N>; ++i)
+    *(typename Frag<E>::f8*)(m + i * kTriElems + (tri(r, s) * 64 + lane) * 8) = f.p[i];
 }
 
 // Eight columns of an LDS row in accumulator order (32s + 4g.., 32s + 16 + 4g..).
@@ -211,12 +227,13 @@ template <> struct TriT<float> {
   }
 };
 
-// The same of a matrix in its sets.
-__device__ __forceinline__ Split<bf16> get_tri_t(const bf16* t, int r, int s, int lane) {
-  return Split<bf16>(TriT<bf16>::get(t, r, s, lane), TriT<bf16>::get(t + kTriElems, r, s, lane));
-}
-__device__ __forceinline__ Split<float> get_tri_t(const float* t, int r, int s, int lane) {
-  return Split<float>(TriT<float>::get(t, r, s, lane));
+// The same of a matrix in N parts.
+template <int N, typename E>
+__device__ __forceinline__ Parts<E, N> get_tri_t(const E* t, int r, int s, int lane) {
+  Parts<E, N> f;
+#pragma unroll
+  for (int i = 0; i < kParts<E, N>; ++i) f.p[i] = TriT<E>::get(t + i * kTriElems, r, s, lane);
+  return f;
 }
 
 // A [64 x W] token tile on its way from global memory to LDS rows: vector idx =
@@ -271,19 +288,30 @@ struct ChunkTile {
   }
 };
 
-// A chunk's record of delta_prepare, copied as it stands (to whole slots).
-template <typename E, int THREADS, size_t BYTES>
-struct Linear {
-  static constexpr int VECS = (int)(BYTES / 16), SLOTS = (VECS + THREADS - 1) / THREADS;
-  static constexpr size_t LDS = (size_t)SLOTS * THREADS * 16;
+// A triangular matrix of a chunk's record on its way to LDS, where it stands in N parts.
+template <int N>
+struct TriTile {
+  static constexpr int SLOTS = kTriElems / 4 / 256;
+  static_assert(SLOTS * 4 * 256 == kTriElems, "whole slots of 256 threads");
   floatx4 r[SLOTS];
-  __device__ __forceinline__ void fetch(const void* src, int tid) {
+  __device__ __forceinline__ void fetch(const float* src, int tid) {
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) r[i] = ((const floatx4*)src)[min(tid + i * THREADS, VECS - 1)];
+    for (int i = 0; i < SLOTS; ++i) r[i] = ((const floatx4*)src)[tid + i * 256];
   }
-  __device__ __forceinline__ void store(void* dst, int tid) const {
+  __device__ __forceinline__ void store(float* dst, int tid) const {
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) ((floatx4*)dst)[tid + i * THREADS] = r[i];
+    for (int i = 0; i < SLOTS; ++i) ((floatx4*)dst)[tid + i * 256] = r[i];
+  }
+  __device__ __forceinline__ void store(bf16* dst, int tid) const {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      float x = r[i][0], y = r[i][1], z = r[i][2], w = r[i][3];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const unsigned a = lead2(x, y), b = lead2(z, w);
+        ((uint2*)(dst + k * kTriElems))[tid + i * 256] = make_uint2(a, b);
+      }
+    }
   }
 };
 

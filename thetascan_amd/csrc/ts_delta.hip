@@ -11,17 +11,19 @@
 // other column, so a wave owns 16 value columns of one head for the whole
 // sequence, its state in accumulators, and an accumulator is the next product's
 // operand without leaving the registers (rows of the accumulator are the
-// contraction).  Every operand that is not an input is a bf16 pair hi + lo: the
-// state is the long sum here and keeps about 1e-5 over any length, and an output
-// is rounded once.
+// contraction).  Every operand that is not an input enters in three bf16 parts, which
+// hold fp32's 24 bits (six products of two such operands, three with an input): the
+// state, the long sum here, is off by 1.4e-7 to 2e-7 over any length, as of fp32 inputs, and
+// an output is rounded once.  In two parts it is off by 4e-6, for 16 % (prompts) to 7 %
+// (training) less time.
 //
 // Bound by the bytes where heads and tokens are many: 64 heads of 4096 tokens of 64 x 64
-// (bf16, training) prepare 42 us (175 MB, 4.2 TB/s), transfers 47 (134 MB), forward 91 (378
-// MB, 4.2 TB/s; four fifths of what it writes is kept for the gradients).  Where they are few,
-// by the chain: a chunk takes 4.4 us (64 keys, a workgroup a CU; 7 with two), of which a third
-// is matrix instructions.  Workgroups of eight waves (forward of 32 heads of 2048 x 128 65 us
-// against 56) and three waves a SIMD (77 against 65) were slower; P formed here again, not
-// stored, 0.8 us more a chunk for 6 % less time where bytes bind.
+// (bf16, training) prepare 42 us (175 MB, 4.2 TB/s), transfers 62 (134 MB), forward 99 (378
+// MB, 3.8 TB/s; four fifths of what it writes is kept for the gradients).  Where they are few,
+// by the chain: 16 chunks of 64 keys 73 us, 4.5 a chunk, a workgroup a CU.  In two parts:
+// workgroups of eight waves (forward of 32 heads of 2048 x 128 65 us against 56) and three waves
+// a SIMD (77 against 65) were slower; P formed here again, not stored, 0.8 us more a chunk for
+// 6 % less time where bytes bind.
 
 #include "ts_delta.h"
 
@@ -75,10 +77,8 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
     if (lane >= o) sum += below;
   }
   G[lane] = sum;
-  char* prep = p.prep + n * (int64_t)prep_bytes<E>();
-  E* tri_t = (E*)prep;
-  E* tri_p = tri_t + TriSets<E>::N * kTriElems;
-  float* vec = (float*)(tri_p + TriSets<E>::N * kTriElems);
+  float* tri_t = p.prep + n * kRecord;
+  float *tri_p = tri_t + kTriElems, *vec = tri_p + kTriElems;
   const double last = __shfl(sum, 63, 64);
   const float eg = __builtin_amdgcn_exp2f((float)(sum * kLog2e));
   const float tail = __builtin_amdgcn_exp2f((float)((last - sum) * kLog2e));
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
 #pragma unroll
     for (int s = 0; s <= rt / 2; ++s) {
       const int at = rt * (rt + 1) / 2 + 2 * s;
-      put_tri(tri_p, rt, s, lane, Split<E>(qk[at], 2 * s + 1 <= rt ? qk[2 * s + 1 <= rt ? at + 1 : at] : z4));
+      put_tri(tri_p, rt, s, lane, Parts<float, 1>(qk[at], 2 * s + 1 <= rt ? qk[2 * s + 1 <= rt ? at + 1 : at] : z4));
     }
   }
   // diagonal blocks: block g, row l16 of it per lane.  L_gg^T in LDS, [column][row]
@@ -188,14 +188,14 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
 #pragma unroll
     for (int s = 0; s <= rt / 2; ++s) {
       const int at = rt * (rt + 1) / 2 + 2 * s;
-      put_tri(tri_t, rt, s, lane, Split<E>(tr[at], 2 * s + 1 <= rt ? tr[2 * s + 1 <= rt ? at + 1 : at] : z4));
+      put_tri(tri_t, rt, s, lane, Parts<float, 1>(tr[at], 2 * s + 1 <= rt ? tr[2 * s + 1 <= rt ? at + 1 : at] : z4));
     }
 }
 
 // What the waves of a workgroup read of one chunk (a transfer: no queries).
 template <typename E, int DK, bool TRANSFER>
 struct ForwardChunk {
-  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD, SET = TriSets<E>::N * kTriElems;
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD, SET = kParts<E, 3> * kTriElems;
   E k[kChunk * PITCH], v[kChunk * VP], t[SET], p[TRANSFER ? 8 : SET], q[TRANSFER ? 8 : kChunk * PITCH];
   float vec[256];
 };
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
   }
   ChunkTile<E, DK, 256> kt, qt;
   ChunkTile<E, 64, 256> vt;
-  Linear<E, 256, Chunk::SET * sizeof(E)> tt, tp;
+  TriTile<3> tt, tp;
   const int vcols = unit ? 0 : p.dv - base;
   float vv = 0.f;
   kt.init(p.k.st, p.dk, tid);
@@ -259,14 +259,14 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
   vt.init(p.v.st, vcols, tid);
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
-    const E* prep = (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>());
+    const float* prep = p.prep + ((int64_t)bh * p.nc + c) * kRecord;
     kt.fetch(kb, p.k.st, t0, len);
     vt.fetch(vb, p.v.st, t0, len);
     tt.fetch(prep, tid);
-    vv = ((const float*)(prep + 2 * Chunk::SET))[min(tid, kVec - 1)];
+    vv = prep[2 * kTriElems + min(tid, kVec - 1)];
     if (!TRANSFER) {
       qt.fetch(qb, p.q.st, t0, len);
-      tp.fetch(prep + Chunk::SET, tid);
+      tp.fetch(prep + kTriElems, tid);
     }
   };
   if (c0 < c1) fetch(c0);
@@ -296,15 +296,15 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
     for (int r = 0; r < 4; ++r) R[r] = O[r] = zero4();
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const Split<E> sf(S[2 * s], S[2 * s + 1]);
+      const Parts<E, 3> sf(S[2 * s], S[2 * s + 1]);
       if constexpr (KEEP) {
         E* s0 = (E*)p.s0 + (n * p.dvp + col) * DK + 32 * s + 4 * g;
-        sf.store(s0, s0 + 16, p.s0_low);
+        sf.store2(s0, s0 + 16, p.s0_low);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        R[r] = mma_split(row_perm<E>(ks + (16 * r + l16) * PITCH, s, g), sf, R[r]);
-        if constexpr (!TRANSFER) O[r] = mma_split(sf, row_perm<E>(qs + (16 * r + l16) * PITCH, s, g), O[r]);
+        R[r] = mma_parts(row_perm<E>(ks + (16 * r + l16) * PITCH, s, g), sf, R[r]);
+        if constexpr (!TRANSFER) O[r] = mma_parts(sf, row_perm<E>(qs + (16 * r + l16) * PITCH, s, g), O[r]);
       }
     }
     // R = b (V - e^G K S0)
@@ -322,9 +322,9 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
     for (int r = 0; r < 4; ++r) U[r] = zero4();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const Split<E> rf(R[2 * s], R[2 * s + 1]);
+      const Parts<E, 3> rf(R[2 * s], R[2 * s + 1]);
 #pragma unroll
-      for (int r = 2 * s; r < 4; ++r) U[r] = mma_split(get_tri(tri_t, r, s, lane), rf, U[r]);
+      for (int r = 2 * s; r < 4; ++r) U[r] = mma_parts(get_tri<3>(tri_t, r, s, lane), rf, U[r]);
     }
     // S = e^{G_63} S0 + K^T (e^{G_63 - G} U), and beside it O^T = e^G S0^T Q^T + U^T P^T
     const float whole = vec[3 * kChunk];
@@ -349,16 +349,16 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[e][i] = U[2 * s + e][i] * tail[i];
       }
-      const Split<E> ff(f[0], f[1]), uf(U[2 * s], U[2 * s + 1]);
+      const Parts<E, 3> ff(f[0], f[1]), uf(U[2 * s], U[2 * s + 1]);
       if constexpr (KEEP) {
         E* u = (E*)p.u + (n * p.dvp + col) * kChunk + 32 * s + 4 * g;
-        uf.store(u, u + 16, p.u_low);
+        uf.store2(u, u + 16, p.u_low);
       }
 #pragma unroll
-      for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(ks, PITCH, 16 * d, s, lane), ff, S[d]);
+      for (int d = 0; d < KB; ++d) S[d] = mma_parts(TokFrag<E>::get(ks, PITCH, 16 * d, s, lane), ff, S[d]);
       if constexpr (!TRANSFER) {
 #pragma unroll
-        for (int r = 2 * s; r < 4; ++r) O[r] = mma_split(uf, get_tri(tri_p, r, s, lane), O[r]);
+        for (int r = 2 * s; r < 4; ++r) O[r] = mma_parts(uf, get_tri<3>(tri_p, r, s, lane), O[r]);
       }
     }
     if constexpr (!TRANSFER) {
@@ -567,7 +567,7 @@ Sizes sizes(const ts_delta_desc* d) {
   const size_t es = d->dtype == TS_BF16 ? 2 : 4;
   const size_t n = (size_t)d->B * d->H * ((d->T + 63) / 64), dvp = (d->dv + 15) / 16 * 16;
   Sizes s;
-  s.prep = n * (d->dtype == TS_BF16 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>());
+  s.prep = n * ts::kRecord * sizeof(float);
   const size_t seg = (size_t)d->B * d->H * ts::delta_segments(d), dkp = padded_keys(d->dk);
   s.seg_x = s.seg_state = 0;
   if (ts::delta_segments(d) > 1) {
@@ -634,12 +634,12 @@ int ts_delta_fwd(const ts_delta_desc* d, const ts_delta_io* io, void* workspace,
   if (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < s.all(d))
     return fail(TS_ERR_VALUE, "delta: the workspace is missing, misaligned or too small");
   if (((int64_t)p.B * p.H * p.nc + 3) / 4 > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta: grid too large");
-  p.prep = (char*)workspace;
-  p.seg_x = (float*)(p.prep + s.prep);
+  p.prep = (float*)workspace;
+  p.seg_x = (float*)((char*)workspace + s.prep);
   p.seg_stride = ts::seg_floats(padded_keys(p.dk), p.dvp, d->keep);
-  p.seg_state = (float*)(p.prep + s.prep + s.seg_x);
+  p.seg_state = (float*)((char*)workspace + s.prep + s.seg_x);
   if (d->keep) {
-    p.u = p.prep + s.prep + s.seg_x + s.seg_state;
+    p.u = (char*)workspace + s.prep + s.seg_x + s.seg_state;
     p.s0 = (char*)p.u + s.u;
     if (s.low) {
       if (!io->low || ((uintptr_t)io->low & 15u))

@@ -17,11 +17,12 @@
 // forward; it leaves dR and dS per chunk and writes dV.  delta_grads takes the
 // chunks on their own: one workgroup each, a wave per 16 tokens.
 //
-// Roundings (bf16 inputs): every operand that is not an input is a pair hi + lo, also as kept
-// (U, S0, dR, dS, the triangles), since sums over alike keys cancel: with these rounded once
+// Roundings (bf16 inputs): every operand that is not an input is a pair of bf16 parts, 16 bits,
+// also as kept (U, S0, dR, dS), since sums over alike keys cancel: with these rounded once
 // the gradients of 256 nearly alike keys were off by 0.8 % (dq), 0.5 (dv), 0.8 (db) and 1.0 (the
-// retentions'), of one key throughout up to 7 % (float64 emulation), with the pairs 1e-5, beside
-// the gradient's own rounding.  Sums are fp32, those of the gates' gradients over a chunk fp64.
+// retentions'), of one key throughout up to 7 % (float64 emulation), with the pairs 1e-5.  A
+// bf16 gradient's own rounding is 0.0017 of it; fp32 ones (of states and fp32 gates) hold
+// those 16 bits, 3e-6 to 5e-5.  Sums are fp32, those of the gates' gradients over a chunk fp64.
 //
 // 64 heads of 4096 tokens of 64 x 64, bf16: transfers 48 us, chain 95 (380 MB, 4.0 TB/s),
 // gradients 117 (483 MB, 4.1 TB/s; its loads and its products take turns in a workgroup, three
@@ -38,7 +39,7 @@ namespace ts {
 // What the waves of a workgroup read of one chunk.
 template <typename E, int DK>
 struct ChainChunk {
-  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD, SET = TriSets<E>::N * kTriElems;
+  static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VP = 64 + PAD, SET = kParts<E, 2> * kTriElems;
   E k[kChunk * PITCH], q[kChunk * PITCH], o[kChunk * VP], t[SET], p[SET];
   float vec[256];
 };
@@ -89,18 +90,17 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
   kt.init(p.k.st, p.dk, tid);
   qt.init(p.q.st, p.dk, tid);
   ot.init(p.dout.st, p.dv - base, tid);
-  Linear<E, 256, Chunk::SET * sizeof(E)> tt, tp;
-  static_assert(Linear<E, 256, Chunk::SET * sizeof(E)>::LDS == Chunk::SET * sizeof(E), "whole slots");
+  TriTile<2> tt, tp;
   float vv = 0.f;
   auto fetch = [&](int c) {
     const int t0 = c * kChunk;
     kt.fetch(kb, p.k.st, t0, len);
     qt.fetch(qb, p.q.st, t0, len);
     ot.fetch(db, p.dout.st, t0, len);
-    const E* prep = (const E*)(p.prep + ((int64_t)bh * p.nc + c) * (int64_t)prep_bytes<E>());
+    const float* prep = p.prep + ((int64_t)bh * p.nc + c) * kRecord;
     tt.fetch(prep, tid);
-    tp.fetch(prep + Chunk::SET, tid);
-    vv = ((const float*)(prep + 2 * Chunk::SET))[min(tid, kVec - 1)];
+    tp.fetch(prep + kTriElems, tid);
+    vv = prep[2 * kTriElems + min(tid, kVec - 1)];
   };
   if (c0 < c1) fetch(c1 - 1);
   loads_landed();
@@ -130,13 +130,13 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
     for (int d = 0; d < KB; ++d) Z[d] = zero4();
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const Split<E> sf(S[2 * s], S[2 * s + 1]);
+      const Parts<E, 2> sf(S[2 * s], S[2 * s + 1]);
       if constexpr (!TRANSFER) {
         E* ds = (E*)p.ds + (n * p.dvp + col) * DK + 32 * s + 4 * g;
-        sf.store(ds, ds + 16, p.ds_low);
+        sf.store2(ds, ds + 16, p.ds_low);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) X[r] = mma_split(row_perm<E>(lds.k + (16 * r + l16) * PITCH, s, g), sf, X[r]);
+      for (int r = 0; r < 4; ++r) X[r] = mma_parts(row_perm<E>(lds.k + (16 * r + l16) * PITCH, s, g), sf, X[r]);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -147,11 +147,11 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[e][i] = eg[i] * tof(of[s][4 * e + i]);
       }
-      const Split<E> qf(f[0], f[1]);
+      const Parts<E, 2> qf(f[0], f[1]);
 #pragma unroll
-      for (int r = 0; r < 2 * s + 2; ++r) Y[r] = mma_split(get_tri_t(lds.p, r, s, lane), of[s], Y[r]);
+      for (int r = 0; r < 2 * s + 2; ++r) Y[r] = mma_parts(get_tri_t<2>(lds.p, r, s, lane), of[s], Y[r]);
 #pragma unroll
-      for (int d = 0; d < KB; ++d) Z[d] = mma_split(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, Z[d]);
+      for (int d = 0; d < KB; ++d) Z[d] = mma_parts(TokFrag<E>::get(lds.q, PITCH, 16 * d, s, lane), qf, Z[d]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -162,18 +162,18 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
     // dR = Ti^T dU
     floatx4 R[4];
     {
-      const Split<E> u0(X[0], X[1]), u1(X[2], X[3]);
+      const Parts<E, 2> u0(X[0], X[1]), u1(X[2], X[3]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        R[r] = mma_split(get_tri_t(lds.t, r, 1, lane), u1, zero4());
-        if (r < 2) R[r] = mma_split(get_tri_t(lds.t, r, 0, lane), u0, R[r]);
+        R[r] = mma_parts(get_tri_t<2>(lds.t, r, 1, lane), u1, zero4());
+        if (r < 2) R[r] = mma_parts(get_tri_t<2>(lds.t, r, 0, lane), u0, R[r]);
       }
     }
     if constexpr (!TRANSFER) {
       E* dro = (E*)p.dr + (n * p.dvp + col) * kChunk + 4 * g;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        Split<E>(R[2 * s], R[2 * s + 1]).store(dro + 32 * s, dro + 32 * s + 16, p.dr_low);
+        Parts<E, 2>(R[2 * s], R[2 * s + 1]).store2(dro + 32 * s, dro + 32 * s + 16, p.dr_low);
     }
     const float whole = vec[3 * kChunk];
 #pragma unroll
@@ -195,9 +195,9 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_chain_kernel(Delta
       for (int i = 0; i < 4; ++i) S[d][i] = fmaf(whole, S[d][i], Z[d][i]);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const Split<E> rf(R[2 * s], R[2 * s + 1]);
+      const Parts<E, 2> rf(R[2 * s], R[2 * s + 1]);
 #pragma unroll
-      for (int d = 0; d < KB; ++d) S[d] = mma_split(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
+      for (int d = 0; d < KB; ++d) S[d] = mma_parts(TokFrag<E>::get(lds.k, PITCH, 16 * d, s, lane), rf, S[d]);
     }
   }
   if (!mine) return;
@@ -227,7 +227,7 @@ constexpr int kGradCols = 32;
 template <typename E, int DK>
 struct GradsLds {
   static constexpr int PAD = 16 / (int)sizeof(E), PITCH = DK + PAD, VB = kGradCols, TP = kChunk + PAD;
-  static constexpr int N = TriSets<E>::N, US = VB * TP, SS = VB * PITCH;  // elements of one of a pair's halves
+  static constexpr int N = kParts<E, 2>, US = VB * TP, SS = VB * PITCH;  // elements of one of a pair's halves
   struct Pass {
     E u[N * US], dr[N * US], s0[N * SS], ds[N * SS];
   };
@@ -275,7 +275,7 @@ __device__ __forceinline__ typename Frag<E>::f8 row_global(const E* row, int c, 
 // way to LDS; rows at or past `rows` are zero.
 template <typename E, int ROWS, int W>
 struct Block {
-  static constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC, SLOTS = ROWS * PER / 256, N = TriSets<E>::N;
+  static constexpr int VEC = 16 / (int)sizeof(E), PER = W / VEC, SLOTS = ROWS * PER / 256, N = kParts<E, 2>;
   uint4 r[N][SLOTS];
   __device__ __forceinline__ void fetch(const E* src, int64_t low, int rows, int tid) {
 #pragma unroll
@@ -324,11 +324,12 @@ struct Block {
 };
 
 // TokFrag of a tile of pairs, `half` elements from one half to the other.
-__device__ __forceinline__ Split<bf16> pair_frag(const bf16* rows, int half, int pitch, int c0, int kp, int lane) {
-  return Split<bf16>(TokFrag<bf16>::get(rows, pitch, c0, kp, lane), TokFrag<bf16>::get(rows + half, pitch, c0, kp, lane));
-}
-__device__ __forceinline__ Split<float> pair_frag(const float* rows, int, int pitch, int c0, int kp, int lane) {
-  return Split<float>(TokFrag<float>::get(rows, pitch, c0, kp, lane));
+template <typename E>
+__device__ __forceinline__ Parts<E, 2> pair_frag(const E* rows, int half, int pitch, int c0, int kp, int lane) {
+  Parts<E, 2> f;
+#pragma unroll
+  for (int i = 0; i < kParts<E, 2>; ++i) f.p[i] = TokFrag<E>::get(rows + i * half, pitch, c0, kp, lane);
+  return f;
 }
 
 // (three waves a SIMD where registers and LDS allow it: without the low halves 102 us with two,
@@ -401,8 +402,7 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
   kt.fetch(kb, p.k.st, t0, len);
   qt.fetch(qb, p.q.st, t0, len);
   fetch(0);
-  const float* vec =
-      (const float*)((const E*)(p.prep + n * (int64_t)prep_bytes<E>()) + 2 * TriSets<E>::N * kTriElems);
+  const float* vec = p.prep + n * kRecord + 2 * kTriElems;
   const float eg = vec[t], tail = vec[kChunk + t], be = vec[2 * kChunk + t], whole = vec[3 * kChunk];
   if (w == 0) {
     double sum = 0.0;
@@ -445,25 +445,25 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < VB / 32; ++s) {
-      const Split<E> rf = pair_frag(lds.pass.dr, US, TP, 16 * w, s, lane);
-      const Split<E> uw = pair_frag(lds.pass.u, US, TP, 16 * w, s, lane);
+      const Parts<E, 2> rf = pair_frag(lds.pass.dr, US, TP, 16 * w, s, lane);
+      const Parts<E, 2> uw = pair_frag(lds.pass.u, US, TP, 16 * w, s, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (r <= w) {
-          const Split<E> uf = pair_frag(lds.pass.u, US, TP, 16 * r, s, lane);
-          dp[r] = mma_split(uf, of[s], dp[r]);
-          ru[r] = mma_split(uf, rf, ru[r]);
+          const Parts<E, 2> uf = pair_frag(lds.pass.u, US, TP, 16 * r, s, lane);
+          dp[r] = mma_parts(uf, of[s], dp[r]);
+          ru[r] = mma_parts(uf, rf, ru[r]);
         }
 #pragma unroll
       for (int d = 0; d < KB; ++d) {
-        const Split<E> sf = pair_frag(lds.pass.s0, SS, PITCH, 16 * d, s, lane);
-        z[d] = mma_split(sf, of[s], z[d]);
-        y[d] = mma_split(sf, rf, y[d]);
-        fu[d] = mma_split(pair_frag(lds.pass.ds, SS, PITCH, 16 * d, s, lane), uw, fu[d]);
+        const Parts<E, 2> sf = pair_frag(lds.pass.s0, SS, PITCH, 16 * d, s, lane);
+        z[d] = mma_parts(sf, of[s], z[d]);
+        y[d] = mma_parts(sf, rf, y[d]);
+        fu[d] = mma_parts(pair_frag(lds.pass.ds, SS, PITCH, 16 * d, s, lane), uw, fu[d]);
       }
       if (any_zero) {
         const f8 vf = row_global<E>(vrow, v0 + 32 * s + 4 * g, p.dv, t0 + t < len);
-        rv = mma_split(vf, rf, rv);
+        rv = mma_parts(vf, rf, rv);
       }
     }
   }
@@ -521,8 +521,8 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
 #pragma unroll
   for (int s = 0; s < 2; ++s)
     if (2 * s <= w) {
-      put_tri(lds.pairs.a, w, s, lane, Split<E>(dp[2 * s], dp[2 * s + 1]));
-      put_tri(lds.pairs.m, w, s, lane, Split<E>(ru[2 * s], ru[2 * s + 1]));
+      put_tri(lds.pairs.a, w, s, lane, Parts<E, 2>(dp[2 * s], dp[2 * s + 1]));
+      put_tri(lds.pairs.m, w, s, lane, Parts<E, 2>(ru[2 * s], ru[2 * s + 1]));
     }
   // state terms of the gates, and of the rows
   float zq = 0.f, yk = 0.f, fk = 0.f;
@@ -560,20 +560,20 @@ __global__ __launch_bounds__(256, (DK == 64 && sizeof(E) == 2 ? 3 : kWaves<E, DK
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     if (2 * s <= w) {
-      const Split<E> af(dp[2 * s], dp[2 * s + 1]), mf(ru[2 * s], ru[2 * s + 1]);
+      const Parts<E, 2> af(dp[2 * s], dp[2 * s + 1]), mf(ru[2 * s], ru[2 * s + 1]);
 #pragma unroll
       for (int d = 0; d < KB; ++d) {
         const f8 kf = TF::get(lds.k, PITCH, 16 * d, s, lane);
-        z[d] = mma_split(kf, af, z[d]);
-        fu[d] = mma_split(kf, mf, fu[d]);
+        z[d] = mma_parts(kf, af, z[d]);
+        fu[d] = mma_parts(kf, mf, fu[d]);
       }
     }
     if (2 * s + 1 >= w) {
-      const Split<E> at = get_tri_t(lds.pairs.a, w, s, lane), mt = get_tri_t(lds.pairs.m, w, s, lane);
+      const Parts<E, 2> at = get_tri_t<2>(lds.pairs.a, w, s, lane), mt = get_tri_t<2>(lds.pairs.m, w, s, lane);
 #pragma unroll
       for (int d = 0; d < KB; ++d) {
-        fu[d] = mma_split(TF::get(lds.k, PITCH, 16 * d, s, lane), mt, fu[d]);
-        fu[d] = mma_split(TF::get(lds.pairs.q, PITCH, 16 * d, s, lane), at, fu[d]);
+        fu[d] = mma_parts(TF::get(lds.k, PITCH, 16 * d, s, lane), mt, fu[d]);
+        fu[d] = mma_parts(TF::get(lds.pairs.q, PITCH, 16 * d, s, lane), at, fu[d]);
       }
     }
   }
@@ -723,7 +723,7 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
   if (chunks > 0x7fffffff) return fail(TS_ERR_NOT_IMPLEMENTED, "delta bwd: grid too large");
   const size_t es = d->dtype == TS_BF16 ? 2 : 4, dkp = d->dk <= 64 ? 64 : 128;
   const size_t u = (size_t)chunks * p.dvp * 64 * es, s0 = (size_t)chunks * p.dvp * dkp * es;
-  p.prep = (char*)saved;
+  p.prep = (float*)saved;
   p.u = (char*)saved + (kept - u - s0);
   p.s0 = (char*)saved + (kept - s0);
   char* ws = (char*)workspace;
@@ -741,8 +741,7 @@ int ts_delta_bwd(const ts_delta_desc* d, const ts_delta_io* io, const ts_delta_g
   if (p.nseg > 1) {
     // X of the forward's transfers, which follow its chunks' records
     const size_t states = (size_t)p.B * p.H * p.nseg * p.dvp * dkp * sizeof(float);
-    const size_t rec = es == 2 ? ts::prep_bytes<ts::bf16>() : ts::prep_bytes<float>();
-    p.seg_x = (float*)((char*)saved + (size_t)chunks * rec);
+    p.seg_x = p.prep + chunks * ts::kRecord;
     p.seg_stride = ts::seg_floats((int)dkp, p.dvp, true);
     p.seg_state = (float*)ws;
     p.seg_n = (float*)(ws + states);
