@@ -64,23 +64,22 @@ def _gate(t: torch.Tensor | None, heads: bool = False) -> _lib.Strided:
     return _lib.Strided(t.data_ptr(), *t.stride())
 
 
+def _describe(q, v, dtype, beta, decay, keep) -> _lib.DeltaDesc:
+    B, Hk, T, dk = q
+    return _lib.DeltaDesc(B, Hk, v[1], T, _width(dtype, dk), _width(dtype, v[3]), _lib.dtype_code(dtype),
+                          _lib.dtype_code(beta), _lib.TS_F32 if decay is None else _lib.dtype_code(decay), int(keep))
+
+
 def _desc(q, k, v, beta, decay, keep: bool) -> _lib.DeltaDesc:
-    B, Hk, T, dk = q.shape
-    _, H, _, dv = v.shape
-    dt = q.dtype
-    # (int: a traced size becomes a number here)
-    return _lib.DeltaDesc(int(B), int(Hk), int(H), int(T), int(_width(dt, dk)), int(_width(dt, dv)),
-                          _lib.dtype_code(dt), _lib.dtype_code(beta.dtype),
-                          _lib.TS_F32 if decay is None else _lib.dtype_code(decay.dtype), int(keep))
+    """The descriptor of a call with these tensors, the caller's own."""
+    return _describe(q.shape, v.shape, q.dtype, beta.dtype, None if decay is None else decay.dtype, keep)
 
 
 @functools.lru_cache(maxsize=256)
 def _plan(q, v, dtype, beta, decay, keep) -> tuple[_lib.DeltaDesc, int, int, int]:
     """A call's descriptor and the bytes of its forward's workspace, of the low
     halves beside it and of the backward's workspace, by shapes and dtypes."""
-    B, Hk, T, dk = q
-    desc = _lib.DeltaDesc(B, Hk, v[1], T, _width(dtype, dk), _width(dtype, v[3]), _lib.dtype_code(dtype),
-                          _lib.dtype_code(beta), _lib.TS_F32 if decay is None else _lib.dtype_code(decay), int(keep))
+    desc = _describe(q, v, dtype, beta, decay, keep)
     lib, fwd, low, bwd = _lib.load(), ctypes.c_size_t(), ctypes.c_size_t(), ctypes.c_size_t()
     _lib.check(lib.ts_delta_workspace_bytes(ctypes.byref(desc), ctypes.byref(fwd)), "ts_delta_workspace_bytes")
     _lib.check(lib.ts_delta_low_bytes(ctypes.byref(desc), ctypes.byref(low)), "ts_delta_low_bytes")
