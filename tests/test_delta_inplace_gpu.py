@@ -43,3 +43,20 @@ def test_states_of_inference_mode(cuda):
         held = s["state"].clone()
         out, got = ts.gated_delta_rule(*args, state=held, state_out=held, return_state=True)
     assert got is held and torch.equal(held, S) and torch.equal(out, want)
+
+
+def test_a_new_state_that_overlaps_the_old_one_is_refused(cuda):
+    import thetascan_amd as ts
+
+    s = on_gpu(inputs(2, 1, 2, 3, 64, 64, BF, seed=1), cuda, False)
+    args = [s[n] for n in ("q", "k", "v", "beta", "decay")]
+    both = torch.zeros(5, 2, 64, 64, device=cuda)
+    for old, new in ((both[:2], both[1:3]), (both[2:4], both[1:3])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ts.gated_delta_rule(*args, state=old, state_out=new)
+    assert not bool(both.any())
+    # side by side, and the transpose of its own memory (read from a copy)
+    ts.gated_delta_rule(*args, state=both[:2], state_out=both[2:4])
+    want = ts.gated_delta_rule(*args, state=both[2:4].transpose(2, 3), return_state=True)[1]
+    got = ts.gated_delta_rule(*args, state=both[2:4].transpose(2, 3), state_out=both[2:4], return_state=True)[1]
+    assert torch.equal(got, want) and got.data_ptr() == both[2:4].data_ptr()

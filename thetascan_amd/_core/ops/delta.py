@@ -330,6 +330,10 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
             raise ValueError("gated_delta_rule: state_out takes no part in gradients: call it without them")
         if not state_out.is_contiguous():
             raise ValueError("gated_delta_rule: state_out must be contiguous")
+        # (a head's new state would meet another's old one; a state that is not contiguous is read from a copy)
+        if state is not None and state.is_contiguous() and (
+                0 < abs(state_out.data_ptr() - state.data_ptr()) < 4 * state.numel()):
+            raise ValueError("gated_delta_rule: state_out overlaps the state (it may be the state itself)")
         if torch.compiler.is_compiling():
             raise NotImplementedError("gated_delta_rule: a traced call writes into no tensor it is given (state_out)")
     if T == 0:
