@@ -35,9 +35,9 @@ from .scan_hip import _kernel_view, _vec
 
 MAX_KEYS, MAX_VALUES = 128, 512
 # Tokens that the recurrent form takes (without gradients).  Its time grows with the
-# tokens, the chunked form's does not (to 64): 16 heads of 64 x 64 4.3 us for one token, 11.4
-# for 12, 14.0 for 16 against 14.6; 128 of 128 x 128 7, 18.8 and 22.9 against 21; 2048 of
-# those 49, 96 and 116 against 144.
+# tokens, the chunked form's does not (to 64): 16 heads of 64 x 64 4.3 us for one token, 11.6
+# for 12, 14.2 for 16 against 15.4; 128 of 128 x 128 7, 18.9 and 23.0 against 22; 2048 of
+# those 49, 96 and 117 against 154.
 STEP_TOKENS = 12
 
 

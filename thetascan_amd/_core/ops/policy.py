@@ -13,7 +13,8 @@ where a gradient is recorded and rows are long (and not few), the forward gives 
 unit upstream gradient too, which the backward forms again where it is another (as does a
 second backward of the same loss).  It is as large as the logits and held from the
 forward to the backward, as a saved tensor: offloading hooks and (non-reentrant)
-activation checkpointing see it.  Neither the capped logits nor the
+activation checkpointing see it.  A loss whose value alone is wanted is called
+without gradients.  Neither the capped logits nor the
 probabilities are stored.  A row of weight zero
 (a prompt's, a padding's) is not read.
 """

@@ -18,8 +18,8 @@
 // 6 % (training) less time.
 //
 // Bound by the bytes where heads and tokens are many: 64 heads of 4096 tokens of 64 x 64
-// (bf16, training) prepare 42 us (175 MB, 4.2 TB/s), transfers 62 (134 MB), forward 99 (378
-// MB, 3.8 TB/s; four fifths of what it writes is kept for the gradients).  Where they are few,
+// (bf16, training; bytes by counters) prepare 42 us (180 MB, 4.3 TB/s), transfers 62 (145 MB),
+// forward 100 (394 MB, 3.9 TB/s; four fifths of what it writes is kept for the gradients).  Where they are few,
 // by the chain: 16 chunks of 64 keys 73 us, 4.5 a chunk, a workgroup a CU.  In two parts:
 // workgroups of eight waves (forward of 32 heads of 2048 x 128 65 us against 56) and three waves
 // a SIMD (77 against 65) were slower; P formed here again, not stored, 0.8 us more a chunk for
@@ -488,7 +488,7 @@ template __global__ void delta_segments_kernel<128, true>(DeltaP);
 // sequence is cut: every segment but the last first forms what it makes of its entering
 // state (the transfer: dk more columns, no outputs), then the segments run side by side.
 // n segments of nc / n chunks take n steps between them and 2 nc / n chunks of a chain:
-// best near n^2 = c nc.  Measured (forward, 64 keys): 8 heads of 1024 tokens 53 us
+// best near n^2 = c nc.  Measured (forward, 64 keys, operands in two parts): 8 heads of 1024 tokens 53 us
 // whole, 38 at four segments, 32 at eight, of 4096 65 at eight, 55 at 16, 61 at 32:
 // c = 4.  Where that is more than a workgroup a CU, chains side by side slow each other
 // and c = 2: 64 heads of 1024 tokens 61 whole, 51 at four, 53 at eight; 8 of 32768 170

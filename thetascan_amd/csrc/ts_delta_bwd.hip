@@ -24,9 +24,9 @@
 // bf16 gradient's own rounding is 0.0017 of it; fp32 ones (of states and fp32 gates) hold
 // those 16 bits, 3e-6 to 5e-5.  Sums are fp32, those of the gates' gradients over a chunk fp64.
 //
-// 64 heads of 4096 tokens of 64 x 64, bf16: transfers 48 us, chain 95 (380 MB, 4.0 TB/s),
-// gradients 117 (483 MB, 4.1 TB/s; its loads and its products take turns in a workgroup, three
-// of which share a CU).  Without the low halves 33, 62 and 80 us.
+// 64 heads of 4096 tokens of 64 x 64, bf16 (bytes by counters): transfers 48 us (187 MB), chain
+// 95 (390 MB, 4.1 TB/s), gradients 116 to 123 (495 MB, 4.0 to 4.3 TB/s; its loads and its products
+// take turns in a workgroup, three of which share a CU).  Without the low halves 33, 62 and 80 us.
 
 #include "ts_delta.h"
 
