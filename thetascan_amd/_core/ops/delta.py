@@ -18,8 +18,9 @@ bf16 inputs: products take bf16 operands and fp32 sums; what is not an input ent
 three bf16 parts in the forward, so the returned state is one of fp32 arithmetic, and in
 two in the backward: bf16 outputs and gradients carry bf16's one rounding, fp32 gradients
 (of states and of fp32 gates) 16 bits.  fp32 inputs compute in fp32.
-A non-finite value in a token that counts spreads over its chunk of 64 tokens
-and everything after it.
+A value that is not finite reaches no output before its own token; from there on outputs
+and the state are not finite (of its value column where it stands in v, of its own token
+where in q).  Gradients of its chunk of 64 tokens and of the tokens before are not either.
 """
 from __future__ import annotations
 

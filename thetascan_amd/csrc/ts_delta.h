@@ -320,6 +320,9 @@ struct TriTile {
 // forward 281 us against 230, backward 657 against 417).
 template <typename E, int DK> constexpr int kWaves = DK == 128 && sizeof(E) == 4 ? 1 : 2;
 
+// Whether a value is NaN or infinite, gathered over several: NaN then, zero otherwise.
+__device__ __forceinline__ float taint(float x, float sofar) { return fmaf(x, 0.f, sofar); }
+
 // Every load so far has landed (counted from here, a loop's waits are for its own).
 __device__ __forceinline__ void loads_landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 

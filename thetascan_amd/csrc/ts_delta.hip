@@ -135,6 +135,33 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(DeltaP p) {
       put_tri(tri_p, rt, s, lane, Parts<float, 1>(qk[at], 2 * s + 1 <= rt ? qk[2 * s + 1 <= rt ? at + 1 : at] : z4));
     }
   }
+  // A token that is not finite reaches none before it: the products' zeros above the diagonal
+  // would not keep it out (0 NaN), so rows of L from the first such one on are left out.  What
+  // is made of those rows is not finite by itself (delta_forward sees it in R).
+  float off = 0.f;
+#pragma unroll
+  for (int at = 0; at < 10; ++at)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) off = taint(kk[at][j], off);
+  if (__any(off != off)) {
+    int first = kChunk;
+#pragma unroll
+    for (int rt = 3; rt >= 0; --rt) {
+      float row = 0.f;
+#pragma unroll
+      for (int ri = 0; ri <= rt; ++ri)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row = taint(kk[rt * (rt + 1) / 2 + ri][j], row);
+      if (row != row) first = 16 * rt + l16;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+      if (16 * rt + l16 >= first)
+#pragma unroll
+        for (int ri = 0; ri <= rt; ++ri) kk[rt * (rt + 1) / 2 + ri] = zero4();
+  }
   // diagonal blocks: block g, row l16 of it per lane.  L_gg^T in LDS, [column][row]
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -316,6 +343,32 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
 #pragma unroll
       for (int i = 0; i < 4; ++i) R[r][i] = be[i] * fmaf(-eg[i], R[r][i], v[i]);
     }
+    // (from a column's first row that is not finite on, its rows are left out of the products,
+    // and what they would have reached is NaN: outputs behind, what is kept, and the state)
+    bool spoilt = false;
+    int first = kChunk;
+    if constexpr (!TRANSFER) {
+      float off = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) off = taint(R[r][i], off);
+      spoilt = __any(off != off);
+      if (spoilt) {
+#pragma unroll
+        for (int r = 3; r >= 0; --r)
+#pragma unroll
+          for (int i = 3; i >= 0; --i)
+            if (R[r][i] * 0.f != 0.f) first = 16 * r + 4 * g + i;
+        first = min(first, __shfl_xor(first, 16, 64));
+        first = min(first, __shfl_xor(first, 32, 64));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * r + 4 * g + i >= first) R[r][i] = 0.f;
+      }
+    }
     // U = Ti R
     floatx4 U[4];
 #pragma unroll
@@ -359,6 +412,27 @@ __global__ __launch_bounds__(256, (kWaves<E, DK>)) void delta_forward_kernel(Del
       if constexpr (!TRANSFER) {
 #pragma unroll
         for (int r = 2 * s; r < 4; ++r) O[r] = mma_parts(uf, get_tri<3>(tri_p, r, s, lane), O[r]);
+      }
+    }
+    if (spoilt) {
+      const float nan = __builtin_nanf("");
+      if (first < kChunk)
+#pragma unroll
+        for (int d = 0; d < KB; ++d) S[d] = floatx4{nan, nan, nan, nan};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int from = __shfl(first, 4 * g + i, 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * r + l16 >= from) O[r][i] = nan;
+      }
+      if constexpr (KEEP) {
+        E* u = (E*)p.u + (n * p.dvp + col) * kChunk + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * r + 4 * g + i >= first) u[16 * r + i] = (E)nan;
       }
     }
     if constexpr (!TRANSFER) {
