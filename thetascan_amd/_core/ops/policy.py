@@ -33,9 +33,14 @@ from .dispatch import HipOp, eager_forward, refuse_tangents
 _GRADIENT = threading.local()  # the gradient that an eager forward leaves for its setup
 
 
+@functools.lru_cache(maxsize=256)
+def _describe(rows, stride, V, dtype, cap, kl, low, high) -> _lib.PolicyDesc:
+    return _lib.PolicyDesc(rows, stride if rows > 1 else V, V, _lib.dtype_code(dtype), cap, 0, kl, low, high)
+
+
 def _desc(z: torch.Tensor, cap: float, kl: float = 0.0, low: float = 0.0, high: float = 0.0) -> _lib.PolicyDesc:
-    return _lib.PolicyDesc(z.shape[0], z.stride(0) if z.shape[0] > 1 else z.shape[1], z.shape[1],
-                           _lib.dtype_code(z.dtype), cap, 0, kl, low, high)
+    rows, V = z.shape
+    return _describe(rows, z.stride(0), V, z.dtype, cap, kl, low, high)
 
 
 @functools.lru_cache(maxsize=256)
