@@ -6,8 +6,9 @@
 //   dloss/dlp = w [ -r A where not clipped + kl (1 - e^{ref - lp}) ]
 //   dz_v = dloss/dlp (1[v = tok] - e^{y_v - lse}) (1 - (y_v / cap)^2)
 //
-// Bound by the logits' bytes (65536 rows of 1024 bf16: scan 46 us, gradient 50 us at 5.4
-// TB/s; 8192 rows of 32768: both 236 us, 4.6 TB/s of what has to move): a row is
+// Bound by the logits' bytes (65536 rows of 1024 bf16, capped: gradient 53 us at 5.1 TB/s; its
+// scan by its arithmetic, 57 us for 134 MB; 8192 rows of 32768: both 239 us, 4.5 TB/s of what
+// has to move): a row is
 // scanned by one wave (or by a workgroup where it is long) with a running maximum and
 // sum, and its gradient is formed by the same workgroup right after (long rows in
 // training) or by a kernel of its own; few long rows are scanned by several workgroups
@@ -44,26 +45,23 @@ struct PolicyP {
   int formed;  // dz holds the gradient for g = 1: nothing is left to do there
 };
 
-// A logit as the softmax takes it, x, and e^x relative to a maximum.  kPlain: x is the
-// logit itself (the lowest finite one too, whose multiple by log2 e is none).  kCap: x =
-// log2 e cap tanh(z / cap) = log2 e (cap - 2 cap r) with r = 1 / (1 + e^{2 z / cap}), off by
-// cap 2^-23.  kWide (caps of 64 and more, where that is too much): x = cap tanh(z / cap), by
-// the series of tanh(t) / t to t^14 (its next term 2^-26) for |t| < 1/2.
-enum { kPlain = 0, kCap = 1, kWide = 2 };
-template <int CAP>
+// A logit as the softmax takes it: itself, or y = cap tanh(z / cap).  near, for |z| < cap / 2: by
+// the series of tanh(t) / t to t^14 (its next term 2^-26 of it), one rounding of z and what the
+// cap takes off.  any: beyond that cap - 2 cap r of the size, r = 1 / (1 + e^{2 |z| / cap}), off by
+// some 2^-23 of itself.  (near costs what the exponential and the reciprocal do; a wave whose
+// logits are all near takes it alone.  By r alone, of z instead of its size, capped logits were
+// off by cap 2^-23.)
+template <bool CAP>
 struct Logit {
-  float in, mul, add, inv;
-  __device__ __forceinline__ explicit Logit(float cap) {
-    const float unit = CAP == kCap ? kLog2eF : 1.f;
-    in = CAP ? 2.f * kLog2eF / cap : 0.f;
-    mul = -2.f * cap * unit;
-    add = cap * unit;
-    inv = CAP == kWide ? 1.f / cap : 0.f;
+  float cap, inv, in, half;
+  __device__ __forceinline__ explicit Logit(float c) {
+    cap = c;
+    inv = CAP ? 1.f / c : 0.f;
+    in = CAP ? 2.f * kLog2eF / c : 0.f;
+    half = 0.5f * c;
   }
-  __device__ __forceinline__ float sig(float z) const { return rcp(1.f + __builtin_amdgcn_exp2f(z * in)); }
-  __device__ __forceinline__ float of(float z, float r) const {
-    const float x = fmaf(r, mul, add);
-    if (CAP != kWide) return x;
+  __device__ __forceinline__ float near(float z) const {
+    if (!CAP) return z;
     const float t = z * inv, u = t * t;
     float y = -929569.f / 638512875.f;
     y = fmaf(y, u, 21844.f / 6081075.f);
@@ -72,14 +70,41 @@ struct Logit {
     y = fmaf(y, u, -17.f / 315.f);
     y = fmaf(y, u, 2.f / 15.f);
     y = fmaf(y, u, -1.f / 3.f);
-    return fabsf(t) < 0.5f ? fmaf(z * u, y, z) : x;
+    return fmaf(z * u, y, z);
   }
-  __device__ __forceinline__ float operator()(float z) const { return CAP ? of(z, sig(z)) : z; }
+  __device__ __forceinline__ float sig(float z) const { return rcp(1.f + __builtin_amdgcn_exp2f(fabsf(z) * in)); }
+  __device__ __forceinline__ float far(float z, float r) const { return copysignf(fmaf(-2.f * cap, r, cap), z); }
+  __device__ __forceinline__ float any(float z) const {
+    return CAP && !(fabsf(z) < half) ? far(z, sig(z)) : near(z);
+  }
+  // dy/dz, and y
+  __device__ __forceinline__ float slope_near(float y) const {
+    const float w = y * inv;
+    return CAP ? fmaf(-w, w, 1.f) : 1.f;
+  }
+  __device__ __forceinline__ float slope_any(float z, float& y) const {
+    y = near(z);
+    float d = slope_near(y);
+    if (CAP) {
+      const float r = sig(z);
+      if (!(fabsf(z) < half)) {
+        y = far(z, r);
+        d = 4.f * r * (1.f - r);
+      }
+    }
+    return d;
+  }
+  // Whether a vector of logits has one past near's range in any lane here.
+  template <typename V>
+  __device__ __forceinline__ bool some_far(const V& v) const {
+    if (!CAP) return false;
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < V::N; ++j) most = fmaxf(most, fabsf(tof(v.e[j])));
+    return __any(!(most < half));
+  }
 };
-template <int CAP>
-__device__ __forceinline__ float ex(float d) {
-  return __builtin_amdgcn_exp2f(CAP == kCap ? d : d * kLog2eF);
-}
+__device__ __forceinline__ float ex(float d) { return __builtin_amdgcn_exp2f(d * kLog2eF); }
 constexpr float kLowest = -3.402823466e38f;
 
 // The parts of a row: `head` elements before its first 16-byte boundary, then
@@ -95,20 +120,19 @@ struct RowSpan {
 };
 
 // One row's terms from its maximum and sum, in fp64.  Where the token is the maximum, its
-// distance from it is zero: the capped maximum is off by up to cap 2^-23, and a difference from
-// the token's exact value gave log-probabilities above zero (of up to 3e-6 at a cap of 30).
-template <typename E, int CAP>
+// distance from it is zero: the capped maximum is rounded to fp32, and a difference from the
+// token's exact value would give log-probabilities above zero.
+template <typename E, bool CAP>
 __device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, float m, float s, float& lpf, float& coef,
                                           float& logs, double& term) {
-  const double l2 = log2((double)s), top = CAP == kCap ? (double)m * kLn2 : (double)m;
+  const double l2 = log2((double)s);
   const int64_t tok = p.tokens[n];
   double off = (double)NAN;  // the token's logit from the maximum; of a token that is none of the row's
   if (tok >= 0 && tok < p.V) {
     const float z = tof(((const E*)p.z)[n * p.stride + tok]);
     double y = (double)z;
-    if (CAP == kCap) y = (double)p.cap * (1.0 - 2.0 / (1.0 + exp(2.0 * y / (double)p.cap)));
-    if (CAP == kWide) y = (double)p.cap * tanh(y / (double)p.cap);
-    off = CAP && Logit<CAP>(p.cap)(z) >= m ? 0.0 : y - top;
+    if (CAP) y = (double)p.cap * tanh(y / (double)p.cap);
+    off = CAP && Logit<CAP>(p.cap).any(z) >= m ? 0.0 : y - (double)m;
   }
   const double lp = off - l2 * kLn2;
   logs = (float)l2;
@@ -131,7 +155,7 @@ __device__ __forceinline__ void row_terms(const PolicyP& p, int64_t n, float w, 
 constexpr int kScan = 4;  // vectors a thread has on their way at once
 // This thread's share (of LANES) of a row's running maximum and sum: part `part` of
 // `parts` of its vectors, and its ends with the first.
-template <typename E, int CAP, int LANES>
+template <typename E, bool CAP, int LANES>
 __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& f, int li, float& m, float& s,
                                          int part = 0, int parts = 1) {
   constexpr int N = Vec16<E>::N, U = kScan;
@@ -141,7 +165,7 @@ __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& 
   s = 0.f;
   auto one = [&](float x) {
     const float top = fmaxf(m, x);
-    s = fmaf(s, ex<CAP>(m - top), ex<CAP>(x - top));
+    s = fmaf(s, ex(m - top), ex(x - top));
     m = top;
   };
   for (int i = li + part * LANES * U; i < span.vecs; i += parts * LANES * U) {
@@ -153,44 +177,51 @@ __device__ __forceinline__ void row_scan(const E* row, int V, const Logit<CAP>& 
     for (int u = 0; u < U; ++u)
       if (i + u * LANES < span.vecs) {
         float x[N], top = m;
+        if (f.some_far(v[u])) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          x[j] = f(tof(v[u].e[j]));
-          top = fmaxf(top, x[j]);
+          for (int j = 0; j < N; ++j) x[j] = f.any(tof(v[u].e[j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[j] = f.near(tof(v[u].e[j]));
         }
-        s *= ex<CAP>(m - top);
 #pragma unroll
-        for (int j = 0; j < N; ++j) s += ex<CAP>(x[j] - top);
+        for (int j = 0; j < N; ++j) top = fmaxf(top, x[j]);
+        s *= ex(m - top);
+#pragma unroll
+        for (int j = 0; j < N; ++j) s += ex(x[j] - top);
         m = top;
       }
   }
   if (part == 0) {
-    if (li < span.head) one(f(tof(row[li])));
-    for (int i = span.head + span.vecs * N + li; i < V; i += LANES) one(f(tof(row[i])));
+    if (li < span.head) one(f.any(tof(row[li])));
+    for (int i = span.head + span.vecs * N + li; i < V; i += LANES) one(f.any(tof(row[i])));
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(m, m2);
-    s = s * ex<CAP>(m - top) + s2 * ex<CAP>(m2 - top);
+    s = s * ex(m - top) + s2 * ex(m2 - top);
     m = top;
   }
 }
 
 // This thread's share of a row's gradient c dlp/dz: parts of the row's vectors
 // (part of parts), and its ends with the first part.
-template <typename E, int CAP, int LANES>
+template <typename E, bool CAP, int LANES>
 __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read, const Logit<CAP>& f, float c, float top,
                                          float logs, int64_t tok, int li, int part, int parts) {
   constexpr int N = Vec16<E>::N, U = 4;
-  auto grad = [&](float z, int v) {
-    float x = z, slope = 1.f;
-    if (CAP) {
-      const float r = f.sig(z);
-      x = f.of(z, r);
-      slope = 4.f * r * (1.f - r);
-    }
-    const float prob = __builtin_amdgcn_exp2f(CAP == kCap ? (x - top) - logs : fmaf(x - top, kLog2eF, -logs));
+  auto part_of = [&](float x, float slope, int v) {
+    const float prob = __builtin_amdgcn_exp2f(fmaf(x - top, kLog2eF, -logs));
     return c * ((v == tok ? 1.f : 0.f) - prob) * slope;
+  };
+  auto grad = [&](float z, int v) {
+    float x;
+    const float slope = f.slope_any(z, x);
+    return part_of(x, slope, v);
+  };
+  auto grad_near = [&](float z, int v) {
+    const float x = f.near(z);
+    return part_of(x, f.slope_near(x), v);
   };
   // the output's vectors; where the logits' do not start with them, they are read element by element
   const RowSpan<E> span(out, V);
@@ -215,9 +246,13 @@ __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read,
       if (at < span.vecs) {
         Vec16<E> o;
         o.raw = make_uint4(0u, 0u, 0u, 0u);
-        if (read)
+        if (read && f.some_far(v[u])) {
 #pragma unroll
           for (int j = 0; j < N; ++j) o.e[j] = cvt<E>(grad(tof(v[u].e[j]), span.head + at * N + j));
+        } else if (read) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) o.e[j] = cvt<E>(grad_near(tof(v[u].e[j]), span.head + at * N + j));
+        }
         ((Vec16<E>*)(out + span.head))[at].raw = o.raw;
       }
     }
@@ -228,7 +263,7 @@ __device__ __forceinline__ void row_grad(const E* row, E* out, int V, bool read,
 }
 
 // WPR waves a row, R rows one after the other whose terms are formed together.
-template <typename E, int CAP, int WPR, int R>
+template <typename E, bool CAP, int WPR, int R>
 __global__ __launch_bounds__(256) void policy_fwd_kernel(PolicyP p) {
   constexpr int THREADS = 256, GROUPS = THREADS / (64 * WPR), LANES = 64 * WPR;
   __shared__ float sm[WPR == 1 ? 1 : THREADS / 64], ss[WPR == 1 ? 1 : THREADS / 64];
@@ -257,7 +292,7 @@ __global__ __launch_bounds__(256) void policy_fwd_kernel(PolicyP p) {
       for (int w = 0; w < WPR; ++w) m = fmaxf(m, sm[w0 + w]);
       s = 0.f;
 #pragma unroll
-      for (int w = 0; w < WPR; ++w) s = fmaf(ss[w0 + w], ex<CAP>(sm[w0 + w] - m), s);
+      for (int w = 0; w < WPR; ++w) s = fmaf(ss[w0 + w], ex(sm[w0 + w] - m), s);
       __syncthreads();
     }
     if (li == k) {
@@ -292,7 +327,7 @@ __global__ __launch_bounds__(256) void policy_fwd_kernel(PolicyP p) {
 }
 
 // Few long rows: a row's scan in `split` workgroups, each leaving its maximum and sum,
-template <typename E, int CAP>
+template <typename E, bool CAP>
 __global__ __launch_bounds__(256) void policy_scan_kernel(PolicyP p) {
   __shared__ float sm[4], ss[4];
   const int tid = threadIdx.x;
@@ -311,11 +346,11 @@ __global__ __launch_bounds__(256) void policy_scan_kernel(PolicyP p) {
   for (int i = 0; i < 4; ++i) m = fmaxf(m, sm[i]);
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s = fmaf(ss[i], ex<CAP>(sm[i] - m), s);
+  for (int i = 0; i < 4; ++i) s = fmaf(ss[i], ex(sm[i] - m), s);
   p.scans[n * p.split + blockIdx.y] = make_float2(m, s);
 }
 // and the rows' own terms from those, a lane each.
-template <typename E, int CAP>
+template <typename E, bool CAP>
 __global__ __launch_bounds__(64) void policy_join_kernel(PolicyP p) {
   const int64_t n = (int64_t)blockIdx.x * 64 + threadIdx.x;
   double term = 0.0;
@@ -327,7 +362,7 @@ __global__ __launch_bounds__(64) void policy_join_kernel(PolicyP p) {
       for (int i = 0; i < p.split; ++i) m = fmaxf(m, p.scans[n * p.split + i].x);
       for (int i = 0; i < p.split; ++i) {
         const float2 one = p.scans[n * p.split + i];
-        s = fmaf(one.y, ex<CAP>(one.x - m), s);
+        s = fmaf(one.y, ex(one.x - m), s);
       }
       row_terms<E, CAP>(p, n, w, m, s, lpf, coef, logs, term);
     }
@@ -365,7 +400,7 @@ __global__ __launch_bounds__(1024) void policy_sum_kernel(const double* part, in
   if (tid == 0) loss[0] = (float)s[0];
 }
 
-template <typename E, int CAP, int WPR>
+template <typename E, bool CAP, int WPR>
 __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
   constexpr int LANES = 64 * WPR, GROUPS = 256 / LANES;
   const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
@@ -381,7 +416,7 @@ __global__ __launch_bounds__(256) void policy_bwd_kernel(PolicyP p) {
 // Long rows in training: a workgroup scans a row and forms its gradient (for an
 // upstream gradient of one) at once, so that the second reading finds the row in
 // the caches: 8192 rows of 32768 bf16 logits 236 us, against 118 and 169 of the two kernels.
-template <typename E, int CAP>
+template <typename E, bool CAP>
 __global__ __launch_bounds__(256) void policy_fused_kernel(PolicyP p) {
   __shared__ float sm[4], ss[4], sc[3];
   const int tid = threadIdx.x;
@@ -403,7 +438,7 @@ __global__ __launch_bounds__(256) void policy_fused_kernel(PolicyP p) {
     for (int i = 0; i < 4; ++i) m = fmaxf(m, sm[i]);
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s = fmaf(ss[i], ex<CAP>(sm[i] - m), s);
+    for (int i = 0; i < 4; ++i) s = fmaf(ss[i], ex(sm[i] - m), s);
   }
   if (tid == 0) {
     double term = 0.0;
@@ -463,7 +498,7 @@ int64_t forward_blocks(const PolicyP& p) {
   return (p.rows + per - 1) / per;
 }
 
-template <typename E, int CAP>
+template <typename E, bool CAP>
 void forward(const PolicyP& p, hipStream_t stream) {
   const dim3 grid((unsigned)forward_blocks(p));
   if (p.dz)
@@ -479,7 +514,7 @@ void forward(const PolicyP& p, hipStream_t stream) {
   else
     hipLaunchKernelGGL((ts::policy_fwd_kernel<E, CAP, 4, 1>), grid, dim3(256), 0, stream, p);
 }
-template <typename E, int CAP>
+template <typename E, bool CAP>
 void backward(const PolicyP& p, hipStream_t stream) {
   // a long row's vectors over several workgroups where the rows are few (16 rows of 131072:
   // 5.5 us against 37, 128 of 32768: 7.1 and 12.3)
@@ -494,23 +529,13 @@ void backward(const PolicyP& p, hipStream_t stream) {
     hipLaunchKernelGGL((ts::policy_bwd_kernel<E, CAP, 4>), grid, dim3(256), 0, stream, p);
 }
 
-// The form of the cap (without one, up to 64, and above).
-int cap_of(const PolicyP& p) { return p.cap == 0.f ? ts::kPlain : (p.cap <= 64.f ? ts::kCap : ts::kWide); }
 template <typename E>
 void forward(const PolicyP& p, hipStream_t stream) {
-  switch (cap_of(p)) {
-    case ts::kPlain: return forward<E, ts::kPlain>(p, stream);
-    case ts::kCap: return forward<E, ts::kCap>(p, stream);
-    default: return forward<E, ts::kWide>(p, stream);
-  }
+  return p.cap == 0.f ? forward<E, false>(p, stream) : forward<E, true>(p, stream);
 }
 template <typename E>
 void backward(const PolicyP& p, hipStream_t stream) {
-  switch (cap_of(p)) {
-    case ts::kPlain: return backward<E, ts::kPlain>(p, stream);
-    case ts::kCap: return backward<E, ts::kCap>(p, stream);
-    default: return backward<E, ts::kWide>(p, stream);
-  }
+  return p.cap == 0.f ? backward<E, false>(p, stream) : backward<E, true>(p, stream);
 }
 
 int setup(const ts_policy_desc* d, const void* z, const int64_t* tokens, PolicyP* p) {
