@@ -60,8 +60,12 @@ extern "C" {
  *     earlier changed.
  * 20: ts_delta_io has a buffer for the low halves of what a bf16 forward keeps (low,
  *     ts_delta_low_bytes), which ts_delta_bwd reads; ts_policy_loss_scale in place of
- *     ts_policy_scale. */
-#define TS_ABI_VERSION 20
+ *     ts_policy_scale.
+ * 21: ts_window_attention_fwd / ts_window_attention_bwd (with its workspace size),
+ *     ts_window_step (with its workspace size), ts_window_cache_fill, ts_sample_tokens
+ *     and ts_distill_fwd / ts_distill_bwd (with ts_distill_parts); nothing earlier
+ *     changed. */
+#define TS_ABI_VERSION 21
 
 enum ts_status {
   TS_OK = 0,
@@ -1358,6 +1362,114 @@ int ts_capture_id(hipStream_t stream, uint64_t* id);
  * gradient dloss (fp32, on the device). */
 int ts_policy_loss_bwd(const ts_policy_desc* desc, const ts_policy_io* io, const float* dloss, void* dlogits,
                        hipStream_t stream);
+
+/* ------------------------------------------------ windowed attention with sinks */
+
+/* Softmax attention of q [B,H,T,d] against k, v [B,Hkv,T,d] (Hkv divides H: head h reads
+ * head h / (H / Hkv)); query i sees key j where j <= i and (i - j < window or j < sinks):
+ *   out[b,h,i] = sum_j softmax_j(scale q_i . k_j) v_j
+ * bf16 or fp32; d <= 128 in 16-byte vectors; rows 16-byte aligned.  Tokens at or past a
+ * sequence's length are not read and give zeros. */
+typedef struct ts_window_desc {
+  int32_t B, H, Hkv, T, d, dtype;
+  int32_t window, sinks;
+  float scale;
+} ts_window_desc;
+
+typedef struct ts_window_io {
+  ts_strided q, k, v, out;
+  const int64_t* lengths; /* [B] or NULL: T each                                  */
+  float* lse;             /* out [B,H,T] (or NULL): kept for the backward         */
+} ts_window_io;
+
+typedef struct ts_window_grads {
+  ts_strided dout;       /* as out                                               */
+  ts_strided dq, dk, dv; /* out, of the inputs' shapes and dtype                 */
+} ts_window_grads;
+
+int ts_window_attention_fwd(const ts_window_desc* desc, const ts_window_io* io, hipStream_t stream);
+int ts_window_attention_bwd_workspace_bytes(const ts_window_desc* desc, size_t* bytes);
+/* io as the forward had and left it (out and lse are read). */
+int ts_window_attention_bwd(const ts_window_desc* desc, const ts_window_io* io, const ts_window_grads* grads,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* One token of each sequence against its cache [B,Hkv,sinks + window,d]: the token of position
+ * n stands in slot n where n < sinks, else in slot sinks + (n - sinks) % window.  q, out
+ * [B,H,1,d] and k, v [B,Hkv,1,d] are the new token's, positions [B] its position; its key and
+ * value go to their slot, and it sees the sinks and the last `window` positions, its own
+ * among them.  A place of position -1 (or any below zero) is free: its output is zero, its
+ * cache is left as it is.  Slots that hold no token yet are not read.  desc.T is not used. */
+int ts_window_step_workspace_bytes(const ts_window_desc* desc, size_t* bytes);
+int ts_window_step(const ts_window_desc* desc, const ts_window_io* io, ts_strided cache_k, ts_strided cache_v,
+                   const int64_t* positions, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* The cache of a prompt of T keys and values (io.k, io.v; io.lengths or T of them): its sinks and
+ * its last `window` tokens into their slots; other slots are left as they are. */
+int ts_window_cache_fill(const ts_window_desc* desc, const ts_window_io* io, ts_strided cache_k, ts_strided cache_v,
+                         hipStream_t stream);
+
+/* ------------------------------------------------ token sampling */
+
+/* A token of each row of logits (element stride `stride`), y = cap tanh(z / cap) (cap 0: y = z):
+ *   w_i = round(2^44 exp((y_i - max y) / temperature))
+ * Left are the top_k highest logits (ties: the lowest index first); of those, in that order,
+ * while the weight before a token is less than top_p of theirs (the first always); of those,
+ * w_i >= min_p 2^44.  The token is the first, by index, whose running weight is over
+ * floor(u times the weight left).  temperature 0: the highest logit.  A logit of -inf is no token;
+ * a row of none, or with +inf or NaN, has token -1 and log-probability NaN. */
+typedef struct ts_sample_desc {
+  int64_t rows, stride;
+  int32_t V, dtype; /* V < 2^19                                                 */
+  float cap;
+  int32_t reserved;
+  double temperature, top_p, min_p; /* for all rows, where io has none of a row  */
+  int64_t top_k;
+} ts_sample_desc;
+
+typedef struct ts_sample_io {
+  const void* logits;
+  const float* uniforms;                          /* [rows], in [0, 1)           */
+  const float *temperatures, *top_ps, *min_ps;    /* [rows] or NULL              */
+  const int64_t* top_ks;                          /* [rows] or NULL              */
+  int64_t* tokens;                                /* out [rows]                  */
+  float* log_probs; /* out [rows]: of the tokens, log softmax(y) (of all, at temperature one) */
+} ts_sample_io;
+
+int ts_sample_tokens(const ts_sample_desc* desc, const ts_sample_io* io, hipStream_t stream);
+
+/* ------------------------------------------------ distillation from top tokens */
+
+/* Rows of logits z (element stride `stride`), x = cap tanh(z / cap) / temperature (cap 0: z /
+ * temperature), lq = log softmax(x), against K of a teacher's tokens with their log-probabilities:
+ *   tail:  P_k = exp(lp_k), P_r = max(0, 1 - sum P_k), Q_r the student's share of all other tokens
+ *          loss = sum_n w [ sum_k P_k (lp_k - lq_k) + P_r (log P_r - log Q_r) ]
+ *   else:  P = softmax(lp);  loss = sum_n w sum_k P_k (log P_k - lq_k)
+ * An id below zero is no token; one at or past V, or twice in a row, makes its row NaN.  A row of
+ * weight zero is not read. */
+typedef struct ts_distill_desc {
+  int64_t rows, stride;
+  int32_t V, K, dtype, tail; /* V <= 2^20                                        */
+  float cap;
+  int32_t reserved;
+  double temperature;
+} ts_distill_desc;
+
+typedef struct ts_distill_io {
+  const void* logits;
+  const int64_t* ids;     /* [rows, K]                                            */
+  const float* log_probs; /* [rows, K]                                            */
+  const float* weights;   /* [rows] or NULL: 1 / rows each                        */
+  float* each;            /* out [rows]: the rows' losses before their weights    */
+  float* stats;           /* out [4, rows], kept for the backward (or NULL)       */
+  double* parts;          /* scratch, ts_distill_parts of them                    */
+  float* loss;            /* out [1]                                              */
+} ts_distill_io;
+
+int ts_distill_parts(const ts_distill_desc* desc, int64_t* parts);
+int ts_distill_fwd(const ts_distill_desc* desc, const ts_distill_io* io, hipStream_t stream);
+/* dlogits [rows, V] contiguous from the forward's stats and the loss's gradient dloss (fp32, on
+ * the device). */
+int ts_distill_bwd(const ts_distill_desc* desc, const ts_distill_io* io, const float* dloss, void* dlogits,
+                   hipStream_t stream);
 
 #ifdef __cplusplus
 }

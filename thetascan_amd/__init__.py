@@ -5,7 +5,10 @@ from .state import ThetaScanState
 from .decode import DecodeGraph
 from .delta import GatedDelta, GatedDeltaConfig
 from ._core.ops.delta import gated_delta_rule
+from ._core.ops.distill import distill_loss
 from ._core.ops.policy import policy_loss, token_log_probs
+from ._core.ops.sample import sample_tokens
+from ._core.ops.window import fill_window_cache, windowed_attention, windowed_attention_step
 from .config import (
     Backend,
     BankMode,
@@ -40,6 +43,7 @@ __all__ = [
     "DecodeGraph", "KernelBSplineScaleMode", "KernelConfig", "KernelFeatureMap", "KernelReLU2ThresholdMode",
     "KernelReadNormalization", "KernelSharpnessMode", "KernelSparsity", "KernelValueRepresentation",
     "RegularizationConfig", "RoPEConfig", "RoPEMode", "RoPEPlacement", "RuntimeConfig", "TemporalConfig",
-    "TemporalMode", "ThetaScan", "ThetaScanConfig", "ThetaScanState", "gated_delta_rule", "policy_loss",
-    "token_log_probs",
+    "TemporalMode", "ThetaScan", "ThetaScanConfig", "ThetaScanState", "distill_loss", "fill_window_cache",
+    "gated_delta_rule", "policy_loss", "sample_tokens", "token_log_probs", "windowed_attention",
+    "windowed_attention_step",
 ]

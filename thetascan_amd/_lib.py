@@ -571,7 +571,41 @@ class PolicyIO(ctypes.Structure):
                                                "weights", "log_probs", "coef", "lse", "parts", "loss", "dlogits")]
 
 
-ABI_VERSION = 20  # the include/thetascan_hip.h these bindings are written for
+class WindowDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "H", "Hkv", "T", "d", "dtype", "window", "sinks")] + [
+        ("scale", ctypes.c_float)]
+
+
+class WindowIO(ctypes.Structure):
+    _fields_ = [(n, Strided) for n in ("q", "k", "v", "out")] + [(n, ctypes.c_void_p) for n in ("lengths", "lse")]
+
+
+class WindowGrads(ctypes.Structure):
+    _fields_ = [(n, Strided) for n in ("dout", "dq", "dk", "dv")]
+
+
+class SampleDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("stride", ctypes.c_int64), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("cap", ctypes.c_float), ("reserved", ctypes.c_int32), ("temperature", ctypes.c_double),
+                ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", ctypes.c_int64)]
+
+
+class SampleIO(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "uniforms", "temperatures", "top_ps", "min_ps", "top_ks",
+                                               "tokens", "log_probs")]
+
+
+class DistillDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("stride", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("V", "K", "dtype", "tail")] + [
+        ("cap", ctypes.c_float), ("reserved", ctypes.c_int32), ("temperature", ctypes.c_double)]
+
+
+class DistillIO(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "ids", "log_probs", "weights", "each", "stats", "parts", "loss")]
+
+
+ABI_VERSION = 21  # the include/thetascan_hip.h these bindings are written for
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -735,6 +769,18 @@ def load() -> ctypes.CDLL:
         lib.ts_capture_id.argtypes = [ctypes.c_void_p, P(ctypes.c_uint64)]
         lib.ts_policy_loss_fwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p]
         lib.ts_policy_loss_bwd.argtypes = [P(PolicyDesc), P(PolicyIO), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        lib.ts_window_attention_fwd.argtypes = [P(WindowDesc), P(WindowIO), ctypes.c_void_p]
+        lib.ts_window_attention_bwd_workspace_bytes.argtypes = [P(WindowDesc), P(ctypes.c_size_t)]
+        lib.ts_window_attention_bwd.argtypes = [P(WindowDesc), P(WindowIO), P(WindowGrads), ctypes.c_void_p,
+                                                ctypes.c_size_t, ctypes.c_void_p]
+        lib.ts_window_step_workspace_bytes.argtypes = [P(WindowDesc), P(ctypes.c_size_t)]
+        lib.ts_window_step.argtypes = [P(WindowDesc), P(WindowIO), Strided, Strided, ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_size_t, ctypes.c_void_p]
+        lib.ts_window_cache_fill.argtypes = [P(WindowDesc), P(WindowIO), Strided, Strided, ctypes.c_void_p]
+        lib.ts_sample_tokens.argtypes = [P(SampleDesc), P(SampleIO), ctypes.c_void_p]
+        lib.ts_distill_parts.argtypes = [P(DistillDesc), P(ctypes.c_int64)]
+        lib.ts_distill_fwd.argtypes = [P(DistillDesc), P(DistillIO), ctypes.c_void_p]
+        lib.ts_distill_bwd.argtypes = [P(DistillDesc), P(DistillIO), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_scale_add_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 6
         lib.ts_scale_add_norm_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 4 + [ctypes.c_float] + [
             ctypes.c_void_p] * 4
