@@ -63,8 +63,7 @@ extern "C" {
  *     ts_policy_scale.
  * 21: ts_window_attention_fwd / ts_window_attention_bwd (with its workspace size),
  *     ts_window_step (with its workspace size), ts_window_cache_fill, ts_sample_tokens
- *     and ts_distill_fwd / ts_distill_bwd (with ts_distill_parts); nothing earlier
- *     changed. */
+ *     and ts_distill_fwd / ts_distill_bwd / ts_distill_scale; nothing earlier changed. */
 #define TS_ABI_VERSION 21
 
 enum ts_status {
@@ -1449,7 +1448,7 @@ typedef struct ts_distill_desc {
   int64_t rows, stride;
   int32_t V, K, dtype, tail; /* V <= 2^20                                        */
   float cap;
-  int32_t reserved;
+  int32_t aligned; /* every row starts at a multiple of 16 bytes          */
   double temperature;
 } ts_distill_desc;
 
@@ -1460,16 +1459,20 @@ typedef struct ts_distill_io {
   const float* weights;   /* [rows] or NULL: 1 / rows each                        */
   float* each;            /* out [rows]: the rows' losses before their weights    */
   float* stats;           /* out [4, rows], kept for the backward (or NULL)       */
-  double* parts;          /* scratch, ts_distill_parts of them                    */
+  double* parts;          /* scratch [rows]                                       */
   float* loss;            /* out [1]                                              */
+  void* dlogits;          /* out [rows, V] contiguous, 16-byte aligned: the logits' gradient for
+                             a unit gradient of the loss, in the same pass, or NULL */
 } ts_distill_io;
 
-int ts_distill_parts(const ts_distill_desc* desc, int64_t* parts);
 int ts_distill_fwd(const ts_distill_desc* desc, const ts_distill_io* io, hipStream_t stream);
 /* dlogits [rows, V] contiguous from the forward's stats and the loss's gradient dloss (fp32, on
  * the device). */
 int ts_distill_bwd(const ts_distill_desc* desc, const ts_distill_io* io, const float* dloss, void* dlogits,
                    hipStream_t stream);
+/* io.dlogits, as such a forward left it, for the loss's gradient dloss: formed again from the
+ * logits where that is not one.  Once a forward. */
+int ts_distill_scale(const ts_distill_desc* desc, const ts_distill_io* io, const float* dloss, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -93,10 +93,11 @@ def test_the_library_refuses_by_itself():
         assert sample(**bad) == _lib.TS_ERR_VALUE, bad
     assert sample(dict(rows=0)) == _lib.TS_OK
 
-    n = ctypes.c_int64()
+    def call(**kw):
+        return lib.ts_distill_fwd(ctypes.byref(desc(**kw)), ctypes.byref(io()), None)
 
     def desc(**kw):
-        d = dict(rows=3, stride=50, V=50, K=4, dtype=_lib.TS_F32, tail=1, cap=0.0, reserved=0, temperature=1.0)
+        d = dict(rows=3, stride=50, V=50, K=4, dtype=_lib.TS_F32, tail=1, cap=0.0, aligned=0, temperature=1.0)
         d.update(kw)
         return _lib.DistillDesc(*d.values())
 
@@ -104,12 +105,14 @@ def test_the_library_refuses_by_itself():
         return _lib.DistillIO(*(kw.get(n, fake) for n, _ in _lib.DistillIO._fields_))
 
     for bad in (dict(rows=-1), dict(V=0), dict(K=0), dict(cap=-1.0), dict(temperature=0.0), dict(temperature=float("nan"))):
-        assert lib.ts_distill_parts(ctypes.byref(desc(**bad)), ctypes.byref(n)) == _lib.TS_ERR_VALUE, bad
+        assert call(**bad) == _lib.TS_ERR_VALUE, bad
     for bad in (dict(V=(1 << 20) + 1), dict(dtype=7), dict(rows=1 << 24)):
-        assert lib.ts_distill_parts(ctypes.byref(desc(**bad)), ctypes.byref(n)) == _lib.TS_ERR_NOT_IMPLEMENTED, bad
+        assert call(**bad) == _lib.TS_ERR_NOT_IMPLEMENTED, bad
     for bad in (dict(logits=None), dict(logits=fake + 2), dict(ids=None), dict(log_probs=None), dict(each=None),
                 dict(parts=None), dict(loss=None)):
         assert lib.ts_distill_fwd(ctypes.byref(desc()), ctypes.byref(io(**bad)), None) == _lib.TS_ERR_VALUE, bad
+    assert lib.ts_distill_fwd(ctypes.byref(desc(aligned=1)), ctypes.byref(io()), None) == _lib.TS_ERR_VALUE  # 50 apart
+    assert lib.ts_distill_fwd(ctypes.byref(desc()), ctypes.byref(io(dlogits=fake + 4)), None) == _lib.TS_ERR_VALUE
     for bad in (dict(stats=None), dict(logits=None)):
         assert lib.ts_distill_bwd(ctypes.byref(desc()), ctypes.byref(io(**bad)), fake, fake, None) == _lib.TS_ERR_VALUE, bad
     assert lib.ts_distill_bwd(ctypes.byref(desc()), ctypes.byref(io()), None, fake, None) == _lib.TS_ERR_VALUE

@@ -9,73 +9,95 @@ and ``P_k = exp(lp_k)``::
 
 ``P_r = 1 - sum_k P_k`` and ``Q_r`` are the teacher's and the student's share of all other
 tokens; without the tail, P is the softmax of the K log-probabilities and the second term
-is left out.  One pass over the logits a direction (ts_distill_fwd, ts_distill_bwd); no
+is left out.  Where a gradient is recorded, the forward's launch gives it too, for a unit
+upstream gradient (ts_distill_fwd): it is as large as the logits and held to the backward, as
+a saved tensor, which forms it again where the upstream gradient is another (as does a second
+backward of the same loss).  A loss whose value alone is wanted is called without gradients.  No
 probabilities are stored.  A row of weight zero is not read.
 """
 from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 
 import torch
 
 from ... import _lib
 from .delta import _on
-from .dispatch import HipOp, refuse_tangents
-from .policy import _row_values, _rows
+from .dispatch import HipOp, eager_forward, refuse_tangents
+from .policy import _capture, _row_values, _rows
 
 MAX_LOGITS = 1 << 20
 
 
+_GRADIENT = threading.local()  # the gradient that an eager forward leaves for its setup
+
+
 @functools.lru_cache(maxsize=256)
-def _describe(rows, stride, V, K, dtype, tail, cap, temperature) -> tuple[_lib.DistillDesc, int]:
-    """A call's description and the partial sums of its loss."""
-    desc = _lib.DistillDesc(rows, stride if rows > 1 else V, V, K, _lib.dtype_code(dtype), int(tail), cap, 0, temperature)
-    n = ctypes.c_int64()
-    _lib.check(_lib.load().ts_distill_parts(ctypes.byref(desc), ctypes.byref(n)), "ts_distill_parts")
-    return desc, n.value
+def _plan(rows, stride, V, K, dtype, tail, cap, temperature, aligned) -> _lib.DistillDesc:
+    return _lib.DistillDesc(rows, stride if rows > 1 else V, V, K, _lib.dtype_code(dtype), int(tail), cap, int(aligned),
+                            temperature)
+
+
+def _describe(z: torch.Tensor, K: int, tail: bool, cap: float, temperature: float) -> _lib.DistillDesc:
+    rows, V = z.shape
+    stride = z.stride(0)
+    aligned = z.data_ptr() % 16 == 0 and (rows == 1 or stride * z.element_size() % 16 == 0)
+    return _plan(rows, stride, V, K, z.dtype, tail, cap, temperature, aligned)
 
 
 def _forward(z: torch.Tensor, ids: torch.Tensor, lps: torch.Tensor, weights: torch.Tensor | None, cap: float,
              temperature: float, tail: bool) -> list[torch.Tensor]:
     z = _rows(z)
-    rows, V = z.shape
-    desc, parts = _describe(rows, z.stride(0), V, ids.shape[1], z.dtype, tail, cap, temperature)
+    rows = z.shape[0]
+    desc = _describe(z, ids.shape[1], tail, cap, temperature)
     loss = torch.empty((), dtype=torch.float32, device=z.device)
     each = torch.empty(rows, dtype=torch.float32, device=z.device)
-    # the parts of the loss (fp64), then what the backward takes of each row
-    saved = torch.empty(max(2 * parts + 4 * rows, 2), dtype=torch.float32, device=z.device)
+    # parts of the loss (fp64), then what the backward takes of each row
+    saved = torch.empty(6 * rows + 2, dtype=torch.float32, device=z.device)
     at = saved.data_ptr()
-    io = _lib.DistillIO(z.data_ptr(), ids.data_ptr(), lps.data_ptr(), _lib.ptr(weights), each.data_ptr(), at + 8 * parts,
-                        at, loss.data_ptr())
-    with _on(z.device), _lib.timed("ts_distill_fwd", lambda: _lib.nbytes(z, ids, lps, weights, each)):
+    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if rows and eager_forward() else None
+    io = _lib.DistillIO(z.data_ptr(), ids.data_ptr(), lps.data_ptr(), _lib.ptr(weights), each.data_ptr(), at + 8 * rows,
+                        at, loss.data_ptr(), _lib.ptr(dz))
+    with _on(z.device), _lib.timed("ts_distill_fwd", lambda: _lib.nbytes(z, ids, lps, weights, each, dz)):
         status = _lib.load().ts_distill_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(z.device))
+        graph = 0 if dz is None else _capture(z.device)
     _lib.check(status, "ts_distill_fwd")
+    if dz is not None:
+        _GRADIENT.of = (loss, dz, graph)
     return [loss, each, saved]
 
 
 def _forward_fake(z, ids, lps, weights, cap, temperature, tail):
-    # (a traced size becomes a number here: the parts follow no formula of it)
-    parts = _describe(int(z.shape[0]), int(z.shape[1]), int(z.shape[1]), int(ids.shape[1]), z.dtype, tail, cap,
-                      temperature)[1]
     return [z.new_empty((), dtype=torch.float32), z.new_empty(z.shape[0], dtype=torch.float32),
-            z.new_empty(max(2 * parts + 4 * z.shape[0], 2), dtype=torch.float32)]
+            z.new_empty(6 * z.shape[0] + 2, dtype=torch.float32)]
 
 
 def _backward_impl(g: torch.Tensor, z: torch.Tensor, ids: torch.Tensor, lps: torch.Tensor,
                    weights: torch.Tensor | None, saved: torch.Tensor, cap: float, temperature: float,
                    tail: bool) -> torch.Tensor:
+    return _gradient(g, z, ids, lps, weights, saved, cap, temperature, tail, None)
+
+
+def _gradient(g, z, ids, lps, weights, saved, cap, temperature, tail, formed: torch.Tensor | None) -> torch.Tensor:
+    """The logits' gradient; ``formed`` is the forward's, for a unit ``g``, which
+    becomes it."""
     z = _rows(z)
-    rows, V = z.shape
-    desc, _ = _describe(rows, z.stride(0), V, ids.shape[1], z.dtype, tail, cap, temperature)
-    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    rows = z.shape[0]
+    desc = _describe(z, ids.shape[1], tail, cap, temperature)
+    dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if formed is None else formed
     g32 = g if g.dtype == torch.float32 else g.to(torch.float32)
     io = _lib.DistillIO(z.data_ptr(), ids.data_ptr(), lps.data_ptr(), _lib.ptr(weights), None,
-                        saved.data_ptr() + 4 * (saved.numel() - 4 * rows), None, None)
-    with _on(z.device), _lib.timed("ts_distill_bwd", lambda: _lib.nbytes(z, ids, lps, dz)):
-        status = _lib.load().ts_distill_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(),
-                                            _lib.stream_handle(z.device))
-    _lib.check(status, "ts_distill_bwd")
+                        saved.data_ptr() + 8 * rows, None, None, dz.data_ptr())
+    lib, name = _lib.load(), "ts_distill_bwd" if formed is None else "ts_distill_scale"
+    with _on(z.device), _lib.timed(name, lambda: _lib.nbytes(z, ids, lps, dz)):
+        stream = _lib.stream_handle(z.device)
+        if formed is None:
+            status = lib.ts_distill_bwd(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), dz.data_ptr(), stream)
+        else:
+            status = lib.ts_distill_scale(ctypes.byref(desc), ctypes.byref(io), g32.data_ptr(), stream)
+    _lib.check(status, name)
     return dz
 
 
@@ -85,13 +107,24 @@ def _backward_fake(g, z, ids, lps, weights, saved, cap, temperature, tail):
 
 def _setup(ctx, inputs, output):
     z, ids, lps, weights, *ctx.settings = inputs
-    ctx.save_for_backward(z, ids, lps, weights, output[2])
+    left, _GRADIENT.of = getattr(_GRADIENT, "of", None), None
+    dz, ctx.graph = left[1:] if left is not None and left[0] is output[0] else (None, None)
+    ctx.save_for_backward(z, ids, lps, weights, output[2], dz)
 
 
 def _backward(ctx, grads, bwd):
     if grads[0] is None:
         return (None,) * 7
-    z, ids, lps, weights, saved = ctx.saved_tensors
+    z, ids, lps, weights, saved, dz = ctx.saved_tensors
+    graph, ctx.graph = ctx.graph, None
+    if dz is not None and graph is not None:
+        # (a backward in a graph of its own may be replayed more often than the
+        # forward, and would take another gradient's for the unit one's; each is handed out once)
+        with _on(dz.device):
+            same = _capture(dz.device) == graph
+        if same:
+            # (.data: what the caller does with it is no change of the saved tensor)
+            return (_gradient(grads[0], z, ids, lps, weights, saved, *ctx.settings, dz.data), *(None,) * 6)
     return (bwd(grads[0], z, ids, lps, weights, saved, *ctx.settings), *(None,) * 6)
 
 

@@ -598,11 +598,12 @@ class SampleIO(ctypes.Structure):
 class DistillDesc(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("stride", ctypes.c_int64)] + [
         (n, ctypes.c_int32) for n in ("V", "K", "dtype", "tail")] + [
-        ("cap", ctypes.c_float), ("reserved", ctypes.c_int32), ("temperature", ctypes.c_double)]
+        ("cap", ctypes.c_float), ("aligned", ctypes.c_int32), ("temperature", ctypes.c_double)]
 
 
 class DistillIO(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "ids", "log_probs", "weights", "each", "stats", "parts", "loss")]
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "ids", "log_probs", "weights", "each", "stats", "parts", "loss",
+                                               "dlogits")]
 
 
 ABI_VERSION = 21  # the include/thetascan_hip.h these bindings are written for
@@ -778,7 +779,7 @@ def load() -> ctypes.CDLL:
                                        ctypes.c_size_t, ctypes.c_void_p]
         lib.ts_window_cache_fill.argtypes = [P(WindowDesc), P(WindowIO), Strided, Strided, ctypes.c_void_p]
         lib.ts_sample_tokens.argtypes = [P(SampleDesc), P(SampleIO), ctypes.c_void_p]
-        lib.ts_distill_parts.argtypes = [P(DistillDesc), P(ctypes.c_int64)]
+        lib.ts_distill_scale.argtypes = [P(DistillDesc), P(DistillIO), ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_distill_fwd.argtypes = [P(DistillDesc), P(DistillIO), ctypes.c_void_p]
         lib.ts_distill_bwd.argtypes = [P(DistillDesc), P(DistillIO), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.ts_scale_add_fwd.argtypes = [P(RowsDesc)] + [ctypes.c_void_p] * 6

@@ -17,12 +17,13 @@
 #include "ts_tokens.h"
 
 #include <string.h>
+#include <type_traits>
 
 namespace ts {
 
 struct DistillP {
   int64_t rows, stride;
-  int V, K, tail;
+  int V, K, tail, aligned;
   float cap;
   double inv_t;
   const void* z;
@@ -32,12 +33,7 @@ struct DistillP {
   double* part;
   const float* g;
   void* dz;
-};
-
-// What the backward takes of a row: the others' maximum and the factor of their e^{x - maximum}; log of
-// the sum of all e^x; M; the log of the teacher's sum (0 with a tail).
-struct DistillRow {
-  float top, rest, lse, mass;
+  int formed;  // dz holds the gradient for g = 1: nothing is left to do there
 };
 
 // The threads of a row (LANES: a wave, or the workgroup).
@@ -78,133 +74,356 @@ __device__ __forceinline__ double distill_logit(const DistillP& p, float z) {
   return y * p.inv_t;
 }
 
-// One row by LANES threads: its loss, and what the backward takes of it.
-template <typename E, bool CAP, int LANES>
-__device__ __forceinline__ double distill_row(const DistillP& p, int64_t n, const RowTeam<LANES>& team, uint32_t* marks,
-                                              DistillRow& out) {
-  constexpr int N = Vec16<E>::N;
-  const int li = team.li, V = p.V, K = p.K;
-  const E* row = (const E*)p.z + n * p.stride;
-  const int64_t* ids = p.ids + n * K;
-  const float* lps = p.lps + n * K;
-  const Logit<CAP> f(p.cap);
-  const float inv_t = (float)p.inv_t;
-  const int shift = (int)(((uintptr_t)row & 15) / sizeof(E)), vecs = (V + shift + N - 1) / N;
-  // the teacher's tokens, a bit each (from the 16-byte boundary at or before the row's start)
-  team.sync();
-  for (int i = li; i < (vecs * N + 31) / 32; i += LANES) marks[i] = 0;
-  team.sync();
-  bool bad = false;
-  for (int k = li; k < K; k += LANES) {
-    const int64_t id = ids[k];
-    if (id < 0) continue;
-    if (id >= V) {
-      bad = true;
-      continue;
-    }
-    const uint32_t bit = (uint32_t)(id + shift);
-    bad |= atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u;
-  }
-  team.sync();
-  // the others: running maximum and sum
-  const Vec16<E>* vec = (const Vec16<E>*)(row - shift);
-  float m = kLowest, s = 0.f;
-  for (int j = li; j < vecs; j += LANES) {
-    const int i0 = j * N - shift;
-    const uint32_t mark = marks[j * N >> 5] >> (j * N & 31);
-    Vec16<E> v;
-    float x[N], top = m;
-    if (i0 >= 0 && i0 + N <= V) {
-      v.raw = vec[j].raw;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        v.e[e] = (E)0.f;
-        if (i0 + e >= 0 && i0 + e < V) v.e[e] = row[i0 + e];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      x[e] = f.any(tof(v.e[e])) * inv_t;
-      if (mark >> e & 1u || i0 + e < 0 || i0 + e >= V) x[e] = -INFINITY;
-      top = fmaxf(top, x[e]);
-    }
-    s *= ex(m - top);
-#pragma unroll
-    for (int e = 0; e < N; ++e) s += ex(x[e] - top);
-    m = top;
-  }
-  const float mr = team.most(m);
-  const float sr = team.sum(s * ex(m - mr));
-  // the teacher's tokens: the highest of all, the sums, then the terms
-  double hi = sr > 0.f ? (double)mr : -INFINITY, mass = 0.0;
-  for (int k = li; k < K; k += LANES) {
-    const int64_t id = ids[k];
-    if (id < 0 || id >= V) continue;
-    const double x = distill_logit<CAP>(p, tof(row[id]));
-    hi = x > hi ? x : hi;
-    mass += exp((double)lps[k]);
-  }
-  hi = team.most(hi);
-  mass = team.sum(mass);
-  double total = 0.0;
-  for (int k = li; k < K; k += LANES) {
-    const int64_t id = ids[k];
-    if (id >= 0 && id < V) total += exp(distill_logit<CAP>(p, tof(row[id])) - hi);
-  }
-  const bool others = sr != 0.f;  // (or no number)
-  total = team.sum(total) + (others ? (double)sr * exp((double)mr - hi) : 0.0);
-  const double lse = hi + log(total), norm = p.tail ? 0.0 : log(mass);
-  double term = 0.0;
-  for (int k = li; k < K; k += LANES) {
-    const int64_t id = ids[k];
-    if (id < 0 || id >= V) continue;
-    const double lp = (double)lps[k] - norm, P = exp(lp);
-    if (P != 0.0) term += P * (lp - (distill_logit<CAP>(p, tof(row[id])) - lse));
-  }
-  term = team.sum(term);
-  double left = 0.0;
-  if (p.tail) {
-    left = others ? 1.0 - mass : 0.0;
-    left = left < 0.0 ? 0.0 : left;
-    if (left != 0.0) term += left * (log(left) - ((double)mr + log((double)sr) - lse));
-    mass += left;
-  } else {
-    mass = mass > 0.0 ? 1.0 : mass;
-  }
-  if (team.sum(bad ? 1 : 0)) term = (double)NAN;
-  out.top = mr;
-  out.rest = others ? (float)(mass * exp((double)mr - lse) - left / (double)sr) : 0.f;
-  if (term != term) out.rest = NAN;
-  out.lse = (float)lse;
-  out.mass = (float)mass;
-  return term;
+// ------------------------------------------------ rows that fit in registers
+
+// Sums and maxima over a wave: neighbours by data-parallel moves, then halves by row swaps.
+template <typename F>
+__device__ __forceinline__ float wave_fold(float x, F f) {
+  auto mv = [](float v, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  x = f(x, mv(x, std::integral_constant<int, 0xb1>{}));   // lanes 1, 0, 3, 2
+  x = f(x, mv(x, std::integral_constant<int, 0x4e>{}));   // lanes 2, 3, 0, 1
+  x = f(x, mv(x, std::integral_constant<int, 0x141>{}));  // the other half of eight
+  x = f(x, mv(x, std::integral_constant<int, 0x140>{}));  // of sixteen
+  LanePair p = xor16_pair(x);
+  p = xor32_pair(f(p.a, p.b));
+  return f(p.a, p.b);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return wave_fold(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_most(float x) {
+  return wave_fold(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  auto mv = [](double v, auto ctrl) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, decltype(ctrl)::value, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), decltype(ctrl)::value, 0xf, 0xf, false);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+  };
+  x += mv(x, std::integral_constant<int, 0xb1>{});
+  x += mv(x, std::integral_constant<int, 0x4e>{});
+  x += mv(x, std::integral_constant<int, 0x141>{});
+  x += mv(x, std::integral_constant<int, 0x140>{});
+  auto half = [](double v, auto pair) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const LanePair lo = pair(__uint_as_float((uint32_t)b)), hi = pair(__uint_as_float((uint32_t)(b >> 32)));
+    auto both = [](float l, float h) {
+      return __longlong_as_double((long long)((uint64_t)__float_as_uint(h) << 32 | __float_as_uint(l)));
+    };
+    return both(lo.a, hi.a) + both(lo.b, hi.b);
+  };
+  x = half(x, [](float v) { return xor16_pair(v); });
+  return half(x, [](float v) { return xor32_pair(v); });
 }
 
-template <typename E, bool CAP, int LANES>
-__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillP p) {
-  constexpr int GROUPS = 256 / LANES;
-  extern __shared__ uint32_t marks[];
-  __shared__ double sm[4], sums[4];
-  const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
-  const int64_t n = (int64_t)blockIdx.x * GROUPS + gi;
-  RowTeam<LANES> team{sm, li, tid >> 6};
-  double term = 0.0;
-  if (n < p.rows) {  // (uniform over the row's threads)
-    const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
-    DistillRow r{0.f, 0.f, 0.f, 0.f};
-    if (w != 0.f) term = distill_row<E, CAP, LANES>(p, n, team, marks + gi * ((p.V + 15) / 32 + 2), r);
-    if (li == 0) {
-      p.each[n] = (float)term;
-      if (p.stats) {
-        p.stats[n] = r.top;
-        p.stats[p.rows + n] = r.rest;
-        p.stats[2 * p.rows + n] = r.lse;
-        p.stats[3 * p.rows + n] = r.mass;
+// What a row's loss is formed from: log2 of e^x counts from the highest of all, hi.
+struct DistillTerms {
+  double mass, a;   // sum P, sum P (lp - (x - hi))
+  float total;      // sum of all e^{x - hi}
+  float sr, dm;     // the others' sum from their own maximum, and its distance from hi (log2)
+};
+__device__ __forceinline__ double distill_loss_of(const DistillP& p, const DistillTerms& t) {
+  const double lt = log((double)t.total);
+  if (!p.tail) return t.mass > 0.0 ? t.a / t.mass - log(t.mass) + lt : t.a;
+  double loss = t.a + t.mass * lt;
+  const double left = t.sr != 0.f ? 1.0 - t.mass : 0.0;
+  if (left > 0.0) loss += left * (log(left) - (double)t.dm * kLn2 - log((double)t.sr) + lt);
+  return loss + 0.0 * left;  // (a share that is no number)
+}
+
+// What a wave has of a row before it begins: its logits (VPT vectors a lane), which of them are none
+// of its own, and the teacher's tokens with their log-probabilities.
+template <typename E, int VPT, int KS>
+struct DistillIn {
+  static constexpr int N = Vec16<E>::N, LANES = 64;
+  Vec16<E> v[VPT];
+  int shift, vecs;
+  int id[KS];
+  float lp[KS], w;
+  __device__ __forceinline__ void load(const DistillP& p, int64_t n, int li) {
+    w = 0.f;
+    if (n >= p.rows) return;
+    w = p.w ? p.w[n] : 1.f / (float)p.rows;
+    const E* row = (const E*)p.z + n * p.stride;
+    shift = (int)(((uintptr_t)row & 15) / sizeof(E));
+    vecs = (p.V + shift + N - 1) / N;
+    if (w == 0.f) return;  // (uniform over the row's threads)
+#pragma unroll
+    for (int r = 0; r < VPT; ++r) {
+      const int j = li + r * LANES, i0 = j * N - shift;
+      v[r].raw = make_uint4(0u, 0u, 0u, 0u);
+      if (i0 >= 0 && i0 + N <= p.V) {
+        v[r].raw = *(const uint4*)(row + i0);
+      } else if (j < vecs) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i0 + e >= 0 && i0 + e < p.V) v[r].e[e] = row[i0 + e];
       }
     }
-    term = w != 0.f ? term * (double)w : 0.0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int k = li + s * LANES;
+      id[s] = -1;
+      lp[s] = -INFINITY;
+      if (k < p.K) {
+        const int64_t x = p.ids[n * p.K + k];
+        id[s] = x < 0 ? -1 : x < p.V ? (int)x : p.V;
+        lp[s] = p.lps[n * p.K + k];
+      }
+    }
   }
+  // the student's logits of those
+  __device__ __forceinline__ void gather(const DistillP& p, int64_t n, float* zk) const {
+    if (w == 0.f) return;
+    const E* row = (const E*)p.z + n * p.stride;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) zk[s] = id[s] >= 0 && id[s] < p.V ? tof(row[id[s]]) : -INFINITY;
+  }
+  // which elements of vector r are none of the row's
+  __device__ __forceinline__ uint32_t ends(int r, int li, int V) const {
+    const int i0 = (li + r * LANES) * N - shift;
+    const uint32_t before = i0 < 0 ? (1u << min(-i0, N)) - 1u : 0u;
+    const uint32_t behind = i0 + N > V ? ~((1u << max(V - i0, 0)) - 1u) : 0u;
+    return (before | behind) & ((1u << N) - 1u);
+  }
+};
+
+// The factors of a row's gradient: M, the teacher's sum without a tail (one over it), one over all
+// e^{x - hi}, and the others' factor of e^{x - their maximum}; no number where the row's loss is none.
+struct DistillFactors {
+  float mass, norm, inv, rest, total;
+  __device__ __forceinline__ float of_teacher(double P, float q) const {
+    return rest != rest ? rest : fmaf(mass * q, inv, -((float)P * norm));
+  }
+};
+__device__ __forceinline__ DistillFactors distill_factors(const DistillP& p, double mass, double a, float sr, float ek,
+                                                          float dm) {
+  DistillFactors k;
+  const float down = sr != 0.f ? __builtin_amdgcn_exp2f(dm) : 0.f;
+  k.total = fmaf(sr, down, ek);
+  k.inv = rcp(k.total);
+  const double left = p.tail && sr != 0.f ? fmax(1.0 - mass, 0.0) : 0.0;
+  k.mass = p.tail ? (float)(mass + left) : (mass > 0.0 ? 1.f : (float)mass);
+  k.norm = p.tail ? 1.f : rcp((float)mass);
+  k.rest = sr != 0.f ? fmaf(k.mass * down, k.inv, -((float)left * rcp(sr))) : 0.f;
+  if (!(a == a)) k.rest = NAN;
+  return k;
+}
+
+// A wave takes R rows one after the other, each held in registers from its one reading to its
+// gradient; the next row is on its way meanwhile.  The rows' logarithms follow, a lane each.
+template <typename E, bool CAP, int VPT, int KS, int R, bool GRAD>
+__global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
+  constexpr int N = Vec16<E>::N, LANES = 64, GROUPS = 4, WORDS = LANES * VPT * N / 32 + 1;
+  __shared__ uint32_t all_marks[GROUPS][WORDS];
+  __shared__ double sums[GROUPS];
+  const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
+  uint32_t* marks = all_marks[gi];
+  const int V = p.V;
+  const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + gi) * R;
+  const Logit<CAP> f(p.cap);
+  const float inv_t = (float)p.inv_t, c2 = (float)(p.inv_t / kLn2);
+  const Exp64 e64{kPowers64};
+  DistillTerms mine{1.0, 0.0, 1.f, 0.f, 0.f};
+  float mine_w = 0.f, mine_rest = 0.f, mine_hi = 0.f, mine_mr = 0.f, mine_mass = 0.f;
+  DistillIn<E, VPT, KS> in;
+  float zn[KS];
+  in.load(p, row0, li);
+  in.gather(p, row0, zn);
+  for (int rr = 0; rr < R; ++rr) {
+    const int64_t n = row0 + rr;
+    if (n >= p.rows) break;  // (uniform over the row's threads, as all that follows)
+    const float w = in.w;
+    const int shift = in.shift, vecs = in.vecs;
+    E* out = GRAD ? (E*)p.dz + n * (int64_t)V : nullptr;
+    const bool together = GRAD && (((uintptr_t)(out - shift)) & 15) == 0;
+    auto put = [&](int j, const Vec16<E>& x) {
+      const int i0 = j * N - shift;
+      if (together && i0 >= 0 && i0 + N <= V) {
+        *(uint4*)(out + i0) = x.raw;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i0 + e >= 0 && i0 + e < V) out[i0 + e] = x.e[e];
+      }
+    };
+    if (w == 0.f) {
+      if (GRAD) {
+        Vec16<E> zero;
+        zero.raw = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int r = 0; r < VPT; ++r)
+          if (li + r * LANES < vecs) put(li + r * LANES, zero);
+      }
+      if (rr + 1 < R) {
+        in.load(p, n + 1, li);
+        if (n + 1 < p.rows) in.gather(p, n + 1, zn);
+      }
+      continue;
+    }
+    Vec16<E> v[VPT];
+    uint32_t ends[VPT];
+    int id[KS];
+    float lp[KS], zk[KS];
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < VPT; ++r) {
+      v[r].raw = in.v[r].raw;
+      ends[r] = in.ends(r, li, V);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      lp[s] = in.lp[s];
+      zk[s] = zn[s];
+      bad |= in.id[s] >= V;
+      id[s] = in.id[s] < V ? in.id[s] : -1;
+    }
+    if (rr + 1 < R) in.load(p, n + 1, li);
+    for (int i = li; i < WORDS; i += LANES) marks[i] = 0;
+    wave_lds_sync();
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      if (id[s] >= 0) {
+        const uint32_t bit = (uint32_t)(id[s] + shift);
+        bad |= atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u;
+      }
+    wave_lds_sync();
+    // the capped logits and their slopes, the highest, and the sum of all
+    float y[VPT][N], sl[VPT][N], yk[KS], slk[KS], hz = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < VPT; ++r) {
+      if (f.some_far(v[r])) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) sl[r][e] = f.slope_any(tof(v[r].e[e]), y[r][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          y[r][e] = f.near(tof(v[r].e[e]));
+          sl[r][e] = f.slope_near(y[r][e]);
+        }
+      }
+      if (ends[r]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (ends[r] >> e & 1u) y[r][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) hz = fmaxf(hz, y[r][e]);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) slk[s] = f.slope_any(zk[s], yk[s]);
+    const float h2 = wave_most(hz) * c2;
+    double all = 0.0;
+#pragma unroll
+    for (int r = 0; r < VPT; ++r)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(y[r][e], c2, -h2));
+        all += (double)x;
+        sl[r][e] = CAP ? x * sl[r][e] : x;
+      }
+    double mass = 0.0, a = 0.0, ek = 0.0, P[KS];
+    float q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      P[s] = 0.0;
+      q[s] = 0.f;
+      if (id[s] >= 0) {
+        const float off = fmaf(yk[s], c2, -h2);
+        // (in fp64: one less their sum is what the teacher leaves to all others)
+        P[s] = lp[s] > -700.f ? e64((double)lp[s]) : lp[s] == lp[s] ? 0.0 : (double)lp[s];
+        q[s] = __builtin_amdgcn_exp2f(off);
+        ek += (double)q[s];
+        mass += P[s];
+        if (P[s] != 0.0) a += P[s] * ((double)lp[s] - (double)off * kLn2);
+      }
+    }
+    if (bad) a = (double)NAN;
+    all = wave_sum(all - ek);  // the others: the very terms that the sum has of the teacher's tokens leave it
+    ek = wave_sum(ek);
+    mass = wave_sum(mass);
+    a = wave_sum(a);
+    float m2 = h2, sr = (float)all;
+    if (!(all > ek * 0x1p-28)) {
+      // (uniform) next to nothing is left: from the others' own maximum, the teacher's tokens masked
+      float mz = -INFINITY;
+      sr = 0.f;
+#pragma unroll
+      for (int r = 0; r < VPT; ++r) {
+        const int j = li + r * LANES;
+        const uint32_t mask = j < vecs ? marks[j * N >> 5] >> (j * N & 31) : 0u;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (mask >> e & 1u) y[r][e] = -INFINITY;
+          mz = fmaxf(mz, y[r][e]);
+        }
+      }
+      mz = wave_most(mz);
+      // (no other token: any finite stand-in, their sum is zero)
+      m2 = mz == -INFINITY ? 0.f : mz * c2;
+#pragma unroll
+      for (int r = 0; r < VPT; ++r)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(y[r][e], c2, -m2));
+          sr += x;
+          if (CAP && x != 0.f) {
+            float unused;
+            sl[r][e] = x * f.slope_any(tof(v[r].e[e]), unused);
+          } else {
+            sl[r][e] = x;
+          }
+        }
+      sr = wave_sum(sr);
+    }
+    const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, m2 - h2);
+    if (li == rr) {
+      mine = DistillTerms{mass, a, k.total, sr, m2 - h2};
+      mine_w = w;
+      mine_rest = k.rest;
+      mine_mr = m2;
+      mine_hi = h2;
+      mine_mass = k.mass;
+    }
+    if (rr + 1 < R && n + 1 < p.rows) in.gather(p, n + 1, zn);
+    if constexpr (GRAD) {
+      const float c = w * inv_t, cr = c * k.rest;
+#pragma unroll
+      for (int r = 0; r < VPT; ++r) {
+        const int j = li + r * LANES;
+        if (j >= vecs) continue;
+        Vec16<E> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.e[e] = cvt<E>(sl[r][e] * cr);
+        put(j, o);
+      }
+      // the teacher's tokens over those (a wave's stores keep their order)
+      wave_lds_sync();
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        if (id[s] >= 0) out[id[s]] = cvt<E>(c * k.of_teacher(P[s], q[s]) * slk[s]);
+    } else {
+      wave_lds_sync();
+    }
+  }
+  double term = 0.0;
+  const int64_t n = row0 + li;
+  if (li < R && n < p.rows) {
+    const double each = mine_w != 0.f ? distill_loss_of(p, mine) : 0.0;
+    term = mine_w != 0.f ? each * (double)mine_w : 0.0;
+    p.each[n] = (float)each;
+    if (p.stats) {
+      p.stats[n] = mine_mr;
+      p.stats[p.rows + n] = mine_rest;
+      p.stats[2 * p.rows + n] = mine_hi + __log2f(mine.total);
+      p.stats[3 * p.rows + n] = mine_mass;
+    }
+  }
+#pragma unroll
+  for (int o = R / 2; o >= 1; o >>= 1) term += __shfl_xor(term, o, 64);
   if (li == 0) sums[gi] = term;
   __syncthreads();
   if (tid == 0) {
@@ -214,13 +433,242 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillP p) {
   }
 }
 
+// A row's gradient where no token is the teacher's: cr e^{x - maximum} slope, by LANES threads.
+template <typename E, bool CAP, int LANES>
+__device__ __forceinline__ void distill_others(const E* row, E* out, int V, const Logit<CAP>& f, float cr, float c2,
+                                               float m2, int li) {
+  constexpr int N = Vec16<E>::N, U = 4;
+  auto one = [&](float z) {
+    float y;
+    const float slope = f.slope_any(z, y);
+    return __builtin_amdgcn_exp2f(fmaf(y, c2, -m2)) * cr * slope;
+  };
+  // the output's vectors; where the logits' do not start with them, they are read element by element
+  const RowSpan<E> to(out, V);
+  const bool together = (((uintptr_t)(row + to.head)) & 15) == 0;
+  for (int j0 = li; j0 < to.vecs; j0 += U * LANES) {
+    Vec16<E> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * LANES;
+      v[u].raw = make_uint4(0u, 0u, 0u, 0u);
+      if (j >= to.vecs) continue;
+      if (together)
+        v[u].raw = ((const Vec16<E>*)(row + to.head))[j].raw;
+      else
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u].e[e] = row[to.head + j * N + e];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * LANES;
+      if (j >= to.vecs) continue;
+      Vec16<E> o;
+      if (f.some_far(v[u])) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.e[e] = cvt<E>(one(tof(v[u].e[e])));
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float y = f.near(tof(v[u].e[e]));
+          o.e[e] = cvt<E>(__builtin_amdgcn_exp2f(fmaf(y, c2, -m2)) * cr * f.slope_near(y));
+        }
+      }
+      ((Vec16<E>*)(out + to.head))[j].raw = o.raw;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (li < to.head) out[li] = cvt<E>(one(tof(row[li])));
+  for (int i = to.head + to.vecs * N + li; i < V; i += LANES) out[i] = cvt<E>(one(tof(row[i])));
+}
+
+// Longer rows, a workgroup each: a running maximum and sum, then the gradient from a second reading,
+// which finds the row in the caches.
+template <typename E, bool CAP, int THREADS, bool GRAD>
+__global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
+  constexpr int N = Vec16<E>::N, WAVES = THREADS / 64, U = 4;
+  extern __shared__ uint32_t marks[];
+  __shared__ double sm_a[WAVES], sm_mass[WAVES];
+  __shared__ float sm[3][WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = p.V, K = p.K;
+  const int64_t n = blockIdx.x;
+  const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
+  const E* row = (const E*)p.z + n * p.stride;
+  E* out = GRAD ? (E*)p.dz + n * (int64_t)V : nullptr;
+  const RowSpan<E> to(out, V);
+  if (w == 0.f) {  // (uniform)
+    if (GRAD) {
+      Vec16<E> zero;
+      zero.raw = make_uint4(0u, 0u, 0u, 0u);
+      for (int j = tid; j < to.vecs; j += THREADS) ((Vec16<E>*)(out + to.head))[j].raw = zero.raw;
+      if (tid < to.head) out[tid] = (E)0.f;
+      for (int i = to.head + to.vecs * N + tid; i < V; i += THREADS) out[i] = (E)0.f;
+    }
+    if (tid == 0) {
+      p.each[n] = 0.f;
+      p.part[n] = 0.0;
+      if (p.stats)
+        for (int i = 0; i < 4; ++i) p.stats[i * p.rows + n] = 0.f;
+    }
+    return;
+  }
+  const int64_t* ids = p.ids + n * K;
+  const float* lps = p.lps + n * K;
+  const Logit<CAP> f(p.cap);
+  const Exp64 e64{kPowers64};
+  const float inv_t = (float)p.inv_t, c2 = (float)(p.inv_t / kLn2);
+  // the teacher's tokens, a bit each (from the 16-byte boundary at or before the row's start), and
+  // their highest logit
+  const int shift = (int)(((uintptr_t)row & 15) / sizeof(E)), vecs = (V + shift + N - 1) / N;
+  for (int i = tid; i < (vecs * N + 31) / 32; i += THREADS) marks[i] = 0;
+  __syncthreads();
+  bool bad = false;
+  float hz = -INFINITY;
+  for (int k = tid; k < K; k += THREADS) {
+    const int64_t id = ids[k];
+    if (id >= V) bad = true;
+    if (id < 0 || id >= V) continue;
+    const uint32_t bit = (uint32_t)(id + shift);
+    bad |= atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u;
+    hz = fmaxf(hz, tof(row[id]));
+  }
+  __syncthreads();
+  // the others
+  float m2 = kLowest, sr = 0.f;
+  for (int j0 = tid; j0 < vecs; j0 += U * THREADS) {
+    Vec16<E> v[U];
+    uint32_t mask[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * THREADS, i0 = j * N - shift;
+      mask[u] = 0xffu;
+      v[u].raw = make_uint4(0u, 0u, 0u, 0u);
+      if (j >= vecs) continue;
+      mask[u] = marks[j * N >> 5] >> (j * N & 31) & ((1u << N) - 1u);
+      if (i0 >= 0 && i0 + N <= V) {
+        v[u].raw = *(const uint4*)(row + i0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          if (i0 + e >= 0 && i0 + e < V)
+            v[u].e[e] = row[i0 + e];
+          else
+            mask[u] |= 1u << e;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[N], top = m2;
+      if (f.some_far(v[u])) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = f.any(tof(v[u].e[e])) * c2;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = f.near(tof(v[u].e[e])) * c2;
+      }
+      if (mask[u]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = mask[u] >> e & 1u ? -INFINITY : x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) top = fmaxf(top, x[e]);
+      sr *= __builtin_amdgcn_exp2f(m2 - top);
+#pragma unroll
+      for (int e = 0; e < N; ++e) sr += __builtin_amdgcn_exp2f(x[e] - top);
+      m2 = top;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  {
+    const float top = wave_most(m2);
+    sr = wave_sum(sr * __builtin_amdgcn_exp2f(m2 - top));
+    hz = wave_most(hz);
+    if (lane == 0) {
+      sm[0][wave] = top;
+      sm[1][wave] = sr;
+      sm[2][wave] = hz;
+    }
+    __syncthreads();
+    m2 = kLowest;
+#pragma unroll
+    for (int u = 0; u < WAVES; ++u) {
+      m2 = fmaxf(m2, sm[0][u]);
+      hz = fmaxf(hz, sm[2][u]);
+    }
+    sr = 0.f;
+#pragma unroll
+    for (int u = 0; u < WAVES; ++u) sr = fmaf(sm[1][u], __builtin_amdgcn_exp2f(sm[0][u] - m2), sr);
+  }
+  // (no other token: any finite stand-in, their sum is zero)
+  if (sr == 0.f) m2 = 0.f;
+  const float h2 = sr == 0.f ? f.any(hz) * c2 : fmaxf(m2, f.any(hz) * c2);
+  double mass = 0.0, a = 0.0;
+  float ek = 0.f;
+  auto share = [&](float lp) { return lp > -700.f ? e64((double)lp) : lp == lp ? 0.0 : (double)lp; };
+  for (int k = tid; k < K; k += THREADS) {
+    const int64_t id = ids[k];
+    if (id < 0 || id >= V) continue;
+    const float off = fmaf(f.any(tof(row[id])), c2, -h2), lp = lps[k];
+    // (in fp64: one less their sum is what the teacher leaves to all others)
+    const double P = share(lp);
+    ek += __builtin_amdgcn_exp2f(off);
+    mass += P;
+    if (P != 0.0) a += P * ((double)lp - (double)off * kLn2);
+  }
+  if (bad) a = (double)NAN;
+  ek = wave_sum(ek);
+  mass = wave_sum(mass);
+  a = wave_sum(a);
+  __syncthreads();
+  if (lane == 0) {
+    sm[0][wave] = ek;
+    sm_mass[wave] = mass;
+    sm_a[wave] = a;
+  }
+  __syncthreads();
+  ek = 0.f;
+  mass = a = 0.0;
+#pragma unroll
+  for (int u = 0; u < WAVES; ++u) {
+    ek += sm[0][u];
+    mass += sm_mass[u];
+    a += sm_a[u];
+  }
+  const DistillFactors k = distill_factors(p, mass, a, sr, ek, m2 - h2);
+  if (tid == 0) {
+    const double each = distill_loss_of(p, DistillTerms{mass, a, k.total, sr, m2 - h2});
+    p.each[n] = (float)each;
+    p.part[n] = each * (double)w;
+    if (p.stats) {
+      p.stats[n] = m2;
+      p.stats[p.rows + n] = k.rest;
+      p.stats[2 * p.rows + n] = h2 + __log2f(k.total);
+      p.stats[3 * p.rows + n] = k.mass;
+    }
+  }
+  if constexpr (GRAD) {
+    const float c = w * inv_t;
+    distill_others<E, CAP, THREADS>(row, out, V, f, c * k.rest, c2, m2, tid);
+    __threadfence_block();
+    __syncthreads();
+    for (int i = tid; i < K; i += THREADS) {
+      const int64_t id = ids[i];
+      if (id < 0 || id >= V) continue;
+      float y;
+      const float slope = f.slope_any(tof(row[id]), y);
+      out[id] = cvt<E>(c * k.of_teacher(share(lps[i]), __builtin_amdgcn_exp2f(fmaf(y, c2, -h2))) * slope);
+    }
+  }
+}
+
 template <typename E, bool CAP, int LANES>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillP p) {
   constexpr int N = Vec16<E>::N, GROUPS = 256 / LANES;
   __shared__ double sm[4];
   const int tid = threadIdx.x, gi = tid / LANES, li = tid % LANES;
   const int64_t n = (int64_t)blockIdx.x * GROUPS + gi;
-  if (n >= p.rows) return;  // (a whole wave, or none of the workgroup)
+  if (n >= p.rows || (p.formed && p.g[0] == 1.f)) return;  // (a whole wave, or none of the workgroup)
   RowTeam<LANES> team{sm, li, tid >> 6};
   const int V = p.V;
   const E* row = (const E*)p.z + n * p.stride;
@@ -236,27 +684,9 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillP p) {
     return;
   }
   const Logit<CAP> f(p.cap);
-  const float inv_t = (float)p.inv_t, c = w * p.g[0] * inv_t;
+  const float inv_t = (float)p.inv_t, c2 = (float)(p.inv_t / kLn2), c = w * p.g[0] * inv_t;
   const float top = p.stats[n], rest = p.stats[p.rows + n], lse = p.stats[2 * p.rows + n], mass = p.stats[3 * p.rows + n];
-  auto other = [&](float z) {
-    float y;
-    const float slope = f.slope_any(z, y);
-    return c * rest * ex(fmaf(y, inv_t, -top)) * slope;
-  };
-  const bool together = (((uintptr_t)(row + span.head)) & 15) == 0;
-  for (int j = li; j < span.vecs; j += LANES) {
-    Vec16<E> v, o;
-    if (together)
-      v.raw = ((const Vec16<E>*)(row + span.head))[j].raw;
-    else
-#pragma unroll
-      for (int e = 0; e < N; ++e) v.e[e] = row[span.head + j * N + e];
-#pragma unroll
-    for (int e = 0; e < N; ++e) o.e[e] = cvt<E>(other(tof(v.e[e])));
-    ((Vec16<E>*)(out + span.head))[j].raw = o.raw;
-  }
-  if (li < span.head) out[li] = cvt<E>(other(tof(row[li])));
-  for (int i = span.head + span.vecs * N + li; i < V; i += LANES) out[i] = cvt<E>(other(tof(row[i])));
+  distill_others<E, CAP, LANES>(row, out, V, f, c * rest, c2, top, li);
   // the teacher's tokens over those
   double norm = 0.0;
   if (!p.tail) {
@@ -273,7 +703,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillP p) {
     if (id < 0 || id >= V) continue;
     float y;
     const float slope = f.slope_any(tof(row[id]), y);
-    const double q = exp(distill_logit<CAP>(p, tof(row[id])) - (double)lse), P = exp((double)p.lps[n * p.K + k] - norm);
+    const double q = exp(distill_logit<CAP>(p, tof(row[id])) - (double)lse * kLn2), P = exp((double)p.lps[n * p.K + k] - norm);
     const float d = rest != rest ? rest : (float)((double)mass * q - P);
     out[id] = cvt<E>(c * d * slope);
   }
@@ -285,6 +715,8 @@ namespace {
 
 using ts::DistillP;
 using ts::fail;
+
+bool by_wave(int V) { return V <= 2048; }
 
 int setup(const ts_distill_desc* d, const ts_distill_io* io, DistillP* p) {
   if (!d || !io || d->rows < 0 || d->V < 1 || d->K < 1 || d->stride < 0 ||
@@ -298,32 +730,71 @@ int setup(const ts_distill_desc* d, const ts_distill_io* io, DistillP* p) {
     return fail(TS_ERR_VALUE, "distill: missing or misaligned tensors");
   memset(p, 0, sizeof(*p));
   p->rows = d->rows; p->stride = d->stride; p->V = d->V; p->K = d->K; p->tail = d->tail; p->cap = d->cap;
+  p->aligned = d->aligned;
+  if (d->aligned && (((uintptr_t)io->logits & 15u) || (d->rows > 1 && d->stride % (d->dtype == TS_BF16 ? 8 : 4))))
+    return fail(TS_ERR_VALUE, "distill: rows that are not aligned");
   p->inv_t = 1.0 / d->temperature;
   p->z = io->logits; p->ids = io->ids; p->lps = io->log_probs; p->w = io->weights;
   p->each = io->each; p->stats = io->stats; p->part = io->parts;
   return TS_OK;
 }
 
-bool by_wave(int V) { return V <= 2048; }
-int64_t blocks_of(const DistillP& p) { return by_wave(p.V) ? (p.rows + 3) / 4 : p.rows; }
 
-template <typename E, bool CAP>
+// Whether a wave holds a row in its registers, 32 logits a lane (a vector more than the row's bytes has
+// an unaligned one), and 256 of a teacher's tokens.
+constexpr int kPer = 32;
+bool in_registers(const DistillP& p, bool bf) {
+  return p.K <= 256 && p.V + (p.aligned ? 0 : (bf ? 8 : 4) - 1) <= 64 * kPer;
+}
+// Rows of a wave: several, where there are enough to keep every CU busy all the same.
+int rows_of(const DistillP& p) { return p.rows >= 16384 ? 8 : 1; }
+
+int64_t blocks_of(const DistillP& p, bool bf) {
+  if (!in_registers(p, bf)) return p.rows;
+  const int per = 4 * rows_of(p);
+  return (p.rows + per - 1) / per;
+}
+
+template <typename E, bool CAP, bool GRAD>
 int forward(const DistillP& p, hipStream_t stream) {
-  const dim3 grid((unsigned)blocks_of(p));
-  const int lds = ((p.V + 15) / 32 + 2) * 4 * (by_wave(p.V) ? 4 : 1);
-  if (by_wave(p.V)) {
-    hipLaunchKernelGGL((ts::distill_fwd_kernel<E, CAP, 64>), grid, dim3(256), lds, stream, p);
-  } else {
-    const hipError_t e = ts::ensure_lds_limit((const void*)ts::distill_fwd_kernel<E, CAP, 256>, (1 << 17) + 8);
-    if (e != hipSuccess) return fail(TS_ERR_RUNTIME, "distill: %s", hipGetErrorString(e));
-    hipLaunchKernelGGL((ts::distill_fwd_kernel<E, CAP, 256>), grid, dim3(256), lds, stream, p);
+  constexpr bool BF = sizeof(E) == 2;
+  constexpr int VPT = kPer / (BF ? 8 : 4);
+  const dim3 grid((unsigned)blocks_of(p, BF));
+  if (in_registers(p, BF)) {
+#define TS_ROWS(vpt, ks, r) \
+  hipLaunchKernelGGL((ts::distill_rows_kernel<E, CAP, vpt, ks, r, GRAD>), grid, dim3(256), 0, stream, p)
+    if (rows_of(p) == 1)
+      TS_ROWS(VPT, 4, 1);
+    else if (p.K > 64)
+      TS_ROWS(VPT, 4, 8);
+    else if (p.V > 64 * kPer / 2)
+      TS_ROWS(VPT, 1, 8);
+    else
+      TS_ROWS(VPT / 2, 1, 8);
+#undef TS_ROWS
+    return TS_OK;
   }
+  const int lds = ((p.V + 15) / 32 + 2) * 4;
+  const bool few = p.rows < 512;
+  const void* fn = few ? (const void*)ts::distill_long_kernel<E, CAP, 1024, GRAD>
+                       : (const void*)ts::distill_long_kernel<E, CAP, 256, GRAD>;
+  const hipError_t e = ts::ensure_lds_limit(fn, (1 << 17) + 8);
+  if (e != hipSuccess) return fail(TS_ERR_RUNTIME, "distill: %s", hipGetErrorString(e));
+  if (few)
+    hipLaunchKernelGGL((ts::distill_long_kernel<E, CAP, 1024, GRAD>), grid, dim3(1024), lds, stream, p);
+  else
+    hipLaunchKernelGGL((ts::distill_long_kernel<E, CAP, 256, GRAD>), grid, dim3(256), lds, stream, p);
   return TS_OK;
+}
+template <typename E>
+int forward(const DistillP& p, hipStream_t stream) {
+  if (p.cap == 0.f) return p.dz ? forward<E, false, true>(p, stream) : forward<E, false, false>(p, stream);
+  return p.dz ? forward<E, true, true>(p, stream) : forward<E, true, false>(p, stream);
 }
 
 template <typename E, bool CAP>
 int backward(const DistillP& p, hipStream_t stream) {
-  const dim3 grid((unsigned)blocks_of(p));
+  const dim3 grid((unsigned)(by_wave(p.V) ? (p.rows + 3) / 4 : p.rows));
   if (by_wave(p.V))
     hipLaunchKernelGGL((ts::distill_bwd_kernel<E, CAP, 64>), grid, dim3(256), 0, stream, p);
   else
@@ -341,37 +812,25 @@ int finish(const char* what) {
 
 extern "C" {
 
-int ts_distill_parts(const ts_distill_desc* d, int64_t* parts) {
-  ts_distill_io io;
-  memset(&io, 0, sizeof(io));
-  io.logits = io.ids = (const int64_t*)16;
-  io.log_probs = (const float*)16;
-  DistillP p;
-  const int rc = setup(d, &io, &p);
-  if (rc) return rc;
-  if (parts) *parts = blocks_of(p);
-  return TS_OK;
-}
-
 int ts_distill_fwd(const ts_distill_desc* d, const ts_distill_io* io, hipStream_t stream) {
   DistillP p;
   int rc = setup(d, io, &p);
   if (rc) return rc;
   if (!io->loss || (d->rows && (!io->each || !io->parts))) return fail(TS_ERR_VALUE, "distill: missing tensors");
+  p.dz = io->dlogits;
+  const bool bf = d->dtype == TS_BF16;
+  if (p.dz && ((uintptr_t)p.dz & 15u)) return fail(TS_ERR_VALUE, "distill: misaligned gradient");
   if (d->rows) {
-    if (d->dtype == TS_BF16)
-      rc = d->cap == 0.f ? forward<ts::bf16, false>(p, stream) : forward<ts::bf16, true>(p, stream);
-    else
-      rc = d->cap == 0.f ? forward<float, false>(p, stream) : forward<float, true>(p, stream);
+    rc = bf ? forward<ts::bf16>(p, stream) : forward<float>(p, stream);
     if (rc) return rc;
   }
   hipLaunchKernelGGL(ts::rows_sum_kernel, dim3(1), dim3(1024), 0, stream, (const double*)io->parts,
-                     d->rows ? blocks_of(p) : 0, io->loss);
+                     d->rows ? blocks_of(p, bf) : 0, io->loss);
   return finish("distill");
 }
 
-int ts_distill_bwd(const ts_distill_desc* d, const ts_distill_io* io, const float* dloss, void* dlogits,
-                   hipStream_t stream) {
+static int distill_bwd(const ts_distill_desc* d, const ts_distill_io* io, const float* dloss, void* dlogits, bool formed,
+                       hipStream_t stream) {
   DistillP p;
   int rc = setup(d, io, &p);
   if (rc || d->rows == 0) return rc;
@@ -379,11 +838,21 @@ int ts_distill_bwd(const ts_distill_desc* d, const ts_distill_io* io, const floa
     return fail(TS_ERR_VALUE, "distill bwd: missing or misaligned tensors");
   p.g = dloss;
   p.dz = dlogits;
+  p.formed = formed;
   if (d->dtype == TS_BF16)
     rc = d->cap == 0.f ? backward<ts::bf16, false>(p, stream) : backward<ts::bf16, true>(p, stream);
   else
     rc = d->cap == 0.f ? backward<float, false>(p, stream) : backward<float, true>(p, stream);
   return rc ? rc : finish("distill bwd");
+}
+
+int ts_distill_bwd(const ts_distill_desc* d, const ts_distill_io* io, const float* dloss, void* dlogits,
+                   hipStream_t stream) {
+  return distill_bwd(d, io, dloss, dlogits, false, stream);
+}
+
+int ts_distill_scale(const ts_distill_desc* d, const ts_distill_io* io, const float* dloss, hipStream_t stream) {
+  return distill_bwd(d, io, dloss, io ? io->dlogits : nullptr, true, stream);
 }
 
 }  // extern "C"

@@ -42,23 +42,6 @@ constexpr int kBins = 2048;
 constexpr double kUnit = 17592186044416.0;  // 2^44
 constexpr float kSpan = 31.3f;              // e^-kSpan 2^44 < 1 / 2: weights beyond it are zero
 
-// e^t for t in [-745, 0], to some 2^-52 of itself: 2^(n / 64) from a table, the rest by its series.
-struct Exp64 {
-  const double* table;  // 2^(j / 64)
-  __device__ __forceinline__ double operator()(double t) const {
-    const double k = rint(t * (64.0 / kLn2));
-    const int n = (int)k;
-    double r = fma(k, -0x1.62e42fefap-7, t);  // ln 2 / 64 in two parts
-    r = fma(k, -0x1.cf79abc9e3b3ap-46, r);
-    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    return __builtin_ldexp(e * table[n & 63], n >> 6);
-  }
-};
-
 // Keys in the order of their logits (-0 as 0).
 template <typename E> struct KeyOf;
 template <> struct KeyOf<float> {
@@ -111,7 +94,7 @@ struct Sampler {
     vec = (const Vec16<E>*)(row - shift);
     vecs = (V + shift + N - 1) / N;
     e64.table = sh.table;
-    if (tid < 64) sh.table[tid] = exp2((double)tid / 64.0);
+    if (tid < 64) sh.table[tid] = kPowers64[tid];
     cut_key = 0;
     cut_index = 0xffffffffu;
     least = 1;
