@@ -1379,6 +1379,8 @@ typedef struct ts_window_io {
   ts_strided q, k, v, out;
   const int64_t* lengths; /* [B] or NULL: T each                                  */
   float* lse;             /* out [B,H,T] (or NULL): kept for the backward         */
+  ts_strided low;         /* out, as out (or ptr NULL): what rounding leaves of out, kept for the
+                             backward, whose dout . out it gives its digits      */
 } ts_window_io;
 
 typedef struct ts_window_grads {

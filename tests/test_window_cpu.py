@@ -101,16 +101,16 @@ def test_the_library_refuses_by_itself():
     def bytes_of(**kw):
         return lib.ts_window_attention_bwd_workspace_bytes(ctypes.byref(desc(**kw)), ctypes.byref(n))
 
-    row = _lib.Strided(fake, 0, 0, 64)
-    io = _lib.WindowIO(row, row, row, row, None, fake)
+    row, none = _lib.Strided(fake, 0, 0, 64), _lib.Strided(None, 0, 0, 0)
+    io = _lib.WindowIO(row, row, row, row, None, fake, none)
     assert bytes_of() == _lib.TS_OK and n.value >= 4 * 300 * 4
     for bad in (dict(H=3), dict(window=0), dict(sinks=-1), dict(scale=0.0), dict(scale=float("inf")), dict(T=-1), dict(B=0)):
         assert bytes_of(**bad) == _lib.TS_ERR_VALUE, bad
     for bad in (dict(d=136), dict(d=60), dict(dtype=5), dict(T=2 ** 31 - 1), dict(B=2 ** 24)):
         assert bytes_of(**bad) == _lib.TS_ERR_NOT_IMPLEMENTED, bad
-    odd = _lib.WindowIO(row, _lib.Strided(fake + 8, 0, 0, 64), row, row, None, fake)
+    odd = _lib.WindowIO(row, _lib.Strided(fake + 8, 0, 0, 64), row, row, None, fake, none)
     assert lib.ts_window_attention_fwd(ctypes.byref(desc()), ctypes.byref(odd), None) == _lib.TS_ERR_VALUE
-    odd = _lib.WindowIO(row, row, _lib.Strided(fake, 0, 0, 65), row, None, fake)
+    odd = _lib.WindowIO(row, row, _lib.Strided(fake, 0, 0, 65), row, None, fake, none)
     assert lib.ts_window_attention_fwd(ctypes.byref(desc()), ctypes.byref(odd), None) == _lib.TS_ERR_VALUE
     assert lib.ts_window_attention_fwd(ctypes.byref(desc()), None, None) == _lib.TS_ERR_VALUE
     grads = _lib.WindowGrads(row, row, row, row)
@@ -119,7 +119,7 @@ def test_the_library_refuses_by_itself():
     assert call(ctypes.byref(desc()), ctypes.byref(io), ctypes.byref(grads), fake, n.value - 1, None) == _lib.TS_ERR_VALUE
     assert call(ctypes.byref(desc()), ctypes.byref(io), ctypes.byref(grads), fake + 8, n.value, None) == _lib.TS_ERR_VALUE
     assert call(ctypes.byref(desc()), ctypes.byref(io), None, fake, n.value, None) == _lib.TS_ERR_VALUE
-    bare = _lib.WindowIO(row, row, row, row, None, None)
+    bare = _lib.WindowIO(row, row, row, row, None, None, none)
     assert call(ctypes.byref(desc()), ctypes.byref(bare), ctypes.byref(grads), fake, n.value, None) == _lib.TS_ERR_VALUE
     assert lib.ts_window_step_workspace_bytes(ctypes.byref(desc(window=2 ** 31 - 1)), ctypes.byref(n)) == _lib.TS_ERR_NOT_IMPLEMENTED
     assert lib.ts_window_step_workspace_bytes(ctypes.byref(desc()), ctypes.byref(n)) == _lib.TS_OK

@@ -53,21 +53,25 @@ def _forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.T
     (q4, sq), (k4, sk), (v4, sv) = _rows(q, vec), _rows(k, vec), _rows(v, vec)
     out = _rows_like(q, q.dtype, desc.d)
     lse = torch.empty((B, H, T) if keep else 0, dtype=torch.float32, device=q.device)
-    io = _lib.WindowIO(sq, sk, sv, _lib.strided(out), _lib.ptr(lengths), lse.data_ptr() if keep else None)
+    low = _rows_like(q, q.dtype, desc.d) if keep and q.dtype == torch.bfloat16 else None
+    io = _lib.WindowIO(sq, sk, sv, _lib.strided(out), _lib.ptr(lengths), lse.data_ptr() if keep else None,
+                       _lib.strided(low))
     with _on(q.device), _lib.timed("ts_window_attention_fwd", lambda: _lib.nbytes(q4, k4, v4, out)):
         status = lib.ts_window_attention_fwd(ctypes.byref(desc), ctypes.byref(io), _lib.stream_handle(q.device))
     _lib.check(status, "ts_window_attention_fwd")
-    return [out if desc.d == d else out[..., :d], lse]
+    return [out if desc.d == d else out[..., :d], lse, q.new_empty(0) if low is None else low]
 
 
 def _forward_fake(q, k, v, lengths, window, sinks, scale, keep):
     B, H, T, d = q.shape
     out = _rows_like(q, q.dtype, _width(q.dtype, d))[..., :d]
-    return [out, q.new_empty((B, H, T) if keep else (0,), dtype=torch.float32)]
+    kept = keep and q.dtype == torch.bfloat16
+    return [out, q.new_empty((B, H, T) if keep else (0,), dtype=torch.float32),
+            _rows_like(q, q.dtype, _width(q.dtype, d)) if kept else q.new_empty(0)]
 
 
 def _backward_impl(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
-                   lse: torch.Tensor, lengths: torch.Tensor | None, window: int, sinks: int,
+                   lse: torch.Tensor, low: torch.Tensor, lengths: torch.Tensor | None, window: int, sinks: int,
                    scale: float) -> list[torch.Tensor]:
     lib = _lib.load()
     d, vec = q.shape[-1], _vec(q.dtype)
@@ -75,7 +79,7 @@ def _backward_impl(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     (q4, sq), (k4, sk), (v4, sv), (o4, so) = _rows(q, vec), _rows(k, vec), _rows(v, vec), _rows(out, vec)
     do4, sd = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype), vec)
     dq, dk, dv = (_rows_like(x, q.dtype, desc.d) for x in (q, k, v))
-    io = _lib.WindowIO(sq, sk, sv, so, _lib.ptr(lengths), lse.data_ptr())
+    io = _lib.WindowIO(sq, sk, sv, so, _lib.ptr(lengths), lse.data_ptr(), _lib.strided(low if low.numel() else None))
     grads = _lib.WindowGrads(sd, _lib.strided(dq), _lib.strided(dk), _lib.strided(dv))
     work = torch.empty(_backward_bytes(q.shape, k.shape[1], q.dtype, window, sinks, scale), dtype=torch.uint8,
                        device=q.device)
@@ -88,20 +92,20 @@ def _backward_impl(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     return [dq, dk, dv]
 
 
-def _backward_fake(dout, q, k, v, out, lse, lengths, window, sinks, scale):
+def _backward_fake(dout, q, k, v, out, lse, low, lengths, window, sinks, scale):
     return [_rows_like(x, q.dtype, _width(q.dtype, x.shape[-1]))[..., :x.shape[-1]] for x in (q, k, v)]
 
 
 def _setup(ctx, inputs, output):
     q, k, v, lengths, ctx.window, ctx.sinks, ctx.scale, _ = inputs
-    ctx.save_for_backward(q, k, v, output[0], output[1], lengths)
+    ctx.save_for_backward(q, k, v, *output, lengths)
 
 
 def _backward(ctx, grads, bwd):
     if grads[0] is None:
         return (None,) * 8
-    q, k, v, out, lse, lengths = ctx.saved_tensors
-    dq, dk, dv = bwd(grads[0], q, k, v, out, lse, lengths, ctx.window, ctx.sinks, ctx.scale)
+    q, k, v, out, lse, low, lengths = ctx.saved_tensors
+    dq, dk, dv = bwd(grads[0], q, k, v, out, lse, low, lengths, ctx.window, ctx.sinks, ctx.scale)
     return (dq, dk, dv, None, None, None, None, None)
 
 
@@ -265,7 +269,7 @@ def windowed_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, c
     (q4, sq), (k4, sk), (v4, sv) = _rows(q, vec), _rows(k, vec), _rows(v, vec)
     positions = positions.to(torch.int64).contiguous()
     out = _rows_like(q, q.dtype, d)
-    io = _lib.WindowIO(sq, sk, sv, _lib.strided(out), None, None)
+    io = _lib.WindowIO(sq, sk, sv, _lib.strided(out), None, None, _lib.strided(None))
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     with _on(q.device), _lib.timed("ts_window_step", lambda: _lib.nbytes(q4, k4, v4, out, cache_k, cache_v)):
         status = _lib.load().ts_window_step(ctypes.byref(desc), ctypes.byref(io), _lib.strided(cache_k),
@@ -297,7 +301,7 @@ def fill_window_cache(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, c
     (k4, sk), (v4, sv) = _rows(k, vec), _rows(v, vec)
     if lengths is not None:
         lengths = lengths.to(torch.int64).contiguous()
-    io = _lib.WindowIO(sk, sk, sv, sk, _lib.ptr(lengths), None)
+    io = _lib.WindowIO(sk, sk, sv, sk, _lib.ptr(lengths), None, _lib.strided(None))
     with _on(k.device), _lib.timed("ts_window_cache_fill", lambda: 2 * _lib.nbytes(k4[:, :, :window + sinks],
                                                                                    v4[:, :, :window + sinks])):
         status = _lib.load().ts_window_cache_fill(ctypes.byref(desc), ctypes.byref(io), _lib.strided(cache_k),

@@ -577,7 +577,8 @@ class WindowDesc(ctypes.Structure):
 
 
 class WindowIO(ctypes.Structure):
-    _fields_ = [(n, Strided) for n in ("q", "k", "v", "out")] + [(n, ctypes.c_void_p) for n in ("lengths", "lse")]
+    _fields_ = [(n, Strided) for n in ("q", "k", "v", "out")] + [(n, ctypes.c_void_p) for n in ("lengths", "lse")] + [
+        ("low", Strided)]
 
 
 class WindowGrads(ctypes.Structure):

@@ -14,15 +14,17 @@ struct WinP {
   float scale, scale2;  // and scale * log2(e)
   ts_strided q, k, v, out;
   const int64_t* lengths;
-  float* lse;  // [B,H,T]: log2 of the sum of 2^(scale2 q . k), +inf past a sequence's length
+  float* lse;      // [B,H,T]: log2 of the sum of 2^(scale2 q . k), +inf past a sequence's length
+  ts_strided low;  // what rounding leaves of out (bf16), for the backward
   // backward
   ts_strided dout, dq, dk, dv;
   float* delta;  // [B,H,T]: dout . out
-  float* part;   // [B,Hkv][chunks + 1][sinks][2][d]: sums of the sinks' gradients
+  // The keys' gradients in parts: of `owners` heads a batch (the key heads, or where few, the query heads)
+  int owners, reps;
+  float* rows;  // [B,owners][T][2][d], where owners are the query heads
+  float* part;  // [B,owners][chunks + 1][sinks][2][d]: the sinks', near queries', then stretches of the far ones
   int near_tiles, far_tiles, chunks, chunk_tiles;
 };
-
-constexpr int kWinQ = 128;  // queries (or keys, backward) of a workgroup, 32 a wave
 
 // 16 bytes of padding keep a tile's rows 4 banks apart.
 template <typename E, int D>
@@ -51,28 +53,83 @@ __device__ __forceinline__ floatx8 win_row8(const float* row, int col, int d, bo
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// 64 rows of a stream on their way into LDS: 16-byte vectors in registers, zero past
-// the sequence's length and the head's width.
+// 64 rows of a stream on their way into LDS: 16-byte vectors in registers, at fixed offsets from
+// the tile's first row (the host checks that 64 rows lie within 2 GiB).  Rows at or past the
+// sequence's length repeat its last one (what they meet is masked); columns past the head's width
+// are zero.
 template <typename E, int D>
 struct WinTile {
-  static constexpr int VEC = 16 / (int)sizeof(E), PER = D / VEC, N = TT * PER / 256;
+  static constexpr int VEC = 16 / (int)sizeof(E), PER = D / VEC, N = TT * PER / 256, STEP = 256 / PER;
   uint4 r[N];
-  __device__ __forceinline__ void fetch(const E* base, int64_t st, int t0, int len, int d, int tid) {
+  uint32_t col, pitch;  // bytes
+  int row;
+  bool on;
+  __device__ __forceinline__ void init(int64_t st, int d, int tid) {
+    row = tid / PER;
+    col = (uint32_t)(tid % PER * 16);
+    on = tid % PER * VEC < d;
+    pitch = (uint32_t)st * (uint32_t)sizeof(E);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * 256, t = t0 + idx / PER, c = idx % PER * VEC;
-      r[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (t < len && c < d) r[i] = *(const uint4*)(base + (int64_t)t * st + c);
+    for (int i = 0; i < N; ++i) r[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  // the tile from row t0 of a sequence at `base` (both uniform)
+  __device__ __forceinline__ void fetch(const E* base, int64_t st, int t0, int len) {
+    const char* from = (const char*)(base + (int64_t)t0 * st);
+    const int last = len - 1 - t0;
+    if (!on) return;
+    if (last >= TT - 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = *(const uint4*)(from + (size_t)((uint32_t)(row + i * STEP) * pitch + col));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        r[i] = *(const uint4*)(from + (size_t)((uint32_t)min(row + i * STEP, last) * pitch + col));
     }
   }
-  __device__ __forceinline__ void store(E* dst, int tid) const {
+  __device__ __forceinline__ void store(E* dst) const {
+    E* at = dst + row * win_pitch<E, D>() + col / (int)sizeof(E);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * 256;
-      *(uint4*)(dst + idx / PER * win_pitch<E, D>() + idx % PER * VEC) = r[i];
-    }
+    for (int i = 0; i < N; ++i) *(uint4*)(at + i * STEP * win_pitch<E, D>()) = r[i];
   }
 };
+
+// What a tile of 64 keys from k0 is to the queries q0 .. q1: not seen by any, seen whole by all, or
+// cut by their diagonal, by their window's far end (both: that of a short window), or around a sink.
+enum WinCut { kWinNone, kWinWhole, kWinDiagonal, kWinEdge, kWinSome };
+__device__ __forceinline__ int win_cut(int q0, int q1, int k0, int window, int sinks) {
+  const int k1 = k0 + TT - 1;
+  if (k0 > q1 || (q0 - k1 >= window && k0 >= sinks)) return kWinNone;
+  const bool diagonal = k1 > q0, edge = q1 - k0 >= window && k1 >= sinks;
+  if (!diagonal && !edge) return kWinWhole;
+  if (edge && (diagonal || k0 < sinks)) return kWinSome;
+  return edge ? kWinEdge : kWinDiagonal;
+}
+// Puts `what` where query i does not see key k0 + 16 kf + 4 g + e of a cut tile: f(kf, e) is the place.
+template <typename F>
+__device__ __forceinline__ void win_mask(int cut, int i, int k0, int g, int window, int sinks, F f) {
+  const int a = i - k0 - 4 * g;  // the last key that the query sees, counted as 16 kf + e
+  if (cut == kWinDiagonal) {
+#pragma unroll
+    for (int kf = 0; kf < 4; ++kf)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (16 * kf + e > a) f(kf, e);
+  } else if (cut == kWinEdge) {
+    const int b = a - window;  // and the last one before its window
+#pragma unroll
+    for (int kf = 0; kf < 4; ++kf)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (16 * kf + e <= b) f(kf, e);
+  } else if (cut == kWinSome) {
+    const int b = a - window, c = sinks - k0 - 4 * g;
+#pragma unroll
+    for (int kf = 0; kf < 4; ++kf)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (16 * kf + e > a || (16 * kf + e <= b && 16 * kf + e >= c)) f(kf, e);
+  }
+}
 
 // The key tiles (64 keys) that queries q0 .. q1 - 1 see: those of the sinks before the
 // window's, then the window's.
