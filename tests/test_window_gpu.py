@@ -101,6 +101,17 @@ def test_windows_and_sinks(cuda, T, window, sinks, dtype):
         close(name, *x)
 
 
+@pytest.mark.parametrize("B,H,Hk,T,d", [(1, 4, 2, 700, 64), (1, 4, 2, 700, 128), (4, 2, 2, 1200, 64), (4, 2, 2, 1200, 128),
+                                        (1, 1, 1, 1400, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sinks_of_many_queries(cuda, B, H, Hk, T, d, dtype):
+    """Sinks whose queries take several stretches, with the query heads apart and together."""
+    q, k, v, do = inputs(B, H, Hk, T, d, dtype, T)
+    want, bars = reference(q, k, v, do, 20, 70)
+    for name, *x in zip(("out", "dq", "dk", "dv"), run(cuda, q, k, v, do, window=20, sinks=70), want, bars):
+        close(name, *x)
+
+
 @pytest.mark.parametrize("H,Hk,d", [(1, 1, 128), (6, 2, 128), (8, 1, 80), (3, 3, 16), (4, 4, 40), (2, 1, 20), (2, 2, 1),
                                     (4, 2, 96), (5, 5, 65)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -104,30 +104,25 @@ __device__ __forceinline__ int win_cut(int q0, int q1, int k0, int window, int s
   if (edge && (diagonal || k0 < sinks)) return kWinSome;
   return edge ? kWinEdge : kWinDiagonal;
 }
-// Puts `what` where query i does not see key k0 + 16 kf + 4 g + e of a cut tile: f(kf, e) is the place.
+// f(kf, e, hidden) for the keys k0 + 16 kf + 4 g + e of a cut tile (a wave-uniform `cut`): whether
+// query i does not see them.
 template <typename F>
 __device__ __forceinline__ void win_mask(int cut, int i, int k0, int g, int window, int sinks, F f) {
   const int a = i - k0 - 4 * g;  // the last key that the query sees, counted as 16 kf + e
+  const int b = a - window;      // and the last one before its window
   if (cut == kWinDiagonal) {
 #pragma unroll
-    for (int kf = 0; kf < 4; ++kf)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (16 * kf + e > a) f(kf, e);
+    for (int j = 0; j < 16; ++j) f(j >> 2, j & 3, 16 * (j >> 2) + (j & 3) > a);
   } else if (cut == kWinEdge) {
-    const int b = a - window;  // and the last one before its window
 #pragma unroll
-    for (int kf = 0; kf < 4; ++kf)
+    for (int j = 0; j < 16; ++j) f(j >> 2, j & 3, 16 * (j >> 2) + (j & 3) <= b);
+  } else {
+    const int c = min(sinks - k0 - 4 * g, b + 1);  // from here to b: hidden
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (16 * kf + e <= b) f(kf, e);
-  } else if (cut == kWinSome) {
-    const int b = a - window, c = sinks - k0 - 4 * g;
-#pragma unroll
-    for (int kf = 0; kf < 4; ++kf)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (16 * kf + e > a || (16 * kf + e <= b && 16 * kf + e >= c)) f(kf, e);
+    for (int j = 0; j < 16; ++j) {
+      const int x = 16 * (j >> 2) + (j & 3);
+      f(j >> 2, j & 3, (x > a) | ((x <= b) & (x >= c)));
+    }
   }
 }
 

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 128 / D) 
   extern __shared__ __align__(16) unsigned char lds[];
   E* ks = (E*)lds;  // [2][TT * P]
   E* vs = ks + 2 * TT * P;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
   const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
   const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * QT, qw = q0 + w * WQ;
   const int len = win_length(p, b), d = p.d;
@@ -100,7 +100,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 128 / D) 
       if (cut != kWinWhole) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
-          win_mask(cut, qw + 16 * n + l16, k0, g, p.window, p.sinks, [&](int kf, int e) { s[n][kf][e] = -INFINITY; });
+          win_mask(cut, qw + 16 * n + l16, k0, g, p.window, p.sinks, [&](int kf, int e, bool hidden) {
+            s[n][kf][e] = hidden ? -INFINITY : s[n][kf][e];
+          });
       }
       float m[NQ];
       bool higher = false;

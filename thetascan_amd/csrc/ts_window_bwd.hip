@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
   extern __shared__ __align__(16) unsigned char lds[];
   E* kt = (E*)lds;  // [TT * P]
   E* vt = kt + TT * P;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
   const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
   const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * QT, qw = q0 + w * WQ;
   const int len = win_length(p, b), d = p.d;
@@ -114,7 +114,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
       if (cut != kWinWhole) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
-          win_mask(cut, qw + 16 * n + l16, k0, g, p.window, p.sinks, [&](int kf, int e) { s[n][kf][e] = 0.f; });
+          win_mask(cut, qw + 16 * n + l16, k0, g, p.window, p.sinks, [&](int kf, int e, bool hidden) {
+            s[n][kf][e] = hidden ? 0.f : s[n][kf][e];
+          });
       }
 #pragma unroll
       for (int kp = 0; kp < 2; ++kp) {
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? 2 : 1) void window_dkv_kernel
   E* ot = qt + TT * P;
   float* ls = (float*)(ot + TT * P);  // [TT]
   float* dl = ls + TT;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
   const int b = blockIdx.x / p.owners, own = blockIdx.x % p.owners;
   const int h0 = own * p.reps, hk = h0 / p.rep;  // the first query head, and the key head
   const int len = win_length(p, b), d = p.d;
@@ -176,6 +178,8 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? 2 : 1) void window_dkv_kernel
     t1 = min((len + TT - 1) / TT, t0 + p.chunk_tiles);
   }
   const int per_head = k0 < len ? max(0, t1 - t0) : 0, total = per_head * p.reps;
+  // a query is one of this workgroup's where its distance from the key lies in least .. least + span - 1
+  const uint32_t least = far ? (uint32_t)p.window : 0u, span = far ? 0x7fffffffu - (uint32_t)p.window : (uint32_t)p.window;
 
   f8 kf[NK][KB], vf[NK][KB];
   floatx4 dk[NK][DB], dv[NK][DB];
@@ -228,8 +232,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? 2 : 1) void window_dkv_kernel
     // wave-uniform: none of these queries sees a key here, or all of them all
     const int q1 = q0 + TT - 1, k1 = kw + WK - 1;
     if (far ? kw >= p.sinks || q1 - kw < p.window : kw > q1 || q0 - k1 >= p.window) continue;
-    const bool diagonal = !far && k1 > q0;
-    const bool some = far ? k1 >= p.sinks || q0 - k1 < p.window : diagonal || q1 - kw >= p.window;
+    const bool some = far ? k1 >= p.sinks || q0 - k1 < p.window : k1 > q0 || q1 - kw >= p.window;
 #pragma unroll
     for (int qp = 0; qp < 2; ++qp) {
       floatx4 s[NK][2], dp[NK][2];
@@ -252,26 +255,19 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? 2 : 1) void window_dkv_kernel
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][f][i] = __builtin_amdgcn_exp2f(fmaf(s[n][f][i], p.scale2, -l4[i]));
+          for (int i = 0; i < 4; ++i) {
+            s[n][f][i] = __builtin_amdgcn_exp2f(fmaf(s[n][f][i], p.scale2, -l4[i]));
+            dp[n][f][i] -= d4[i];
+          }
           if (some) {
             // the distance of query i from this lane's key is c + i
             const int key = kw + 16 * n + l16, c = q0 + qf * 16 + 4 * g - key;
-            if (far) {
+            const uint32_t from = far && key >= p.sinks ? 0x7fffffffu : least;
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (key >= p.sinks || c + i < p.window) s[n][f][i] = 0.f;
-            } else if (diagonal) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if ((uint32_t)(c + i) >= (uint32_t)p.window) s[n][f][i] = 0.f;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c + i >= p.window) s[n][f][i] = 0.f;
-            }
+            for (int i = 0; i < 4; ++i) s[n][f][i] = (uint32_t)(c + i) - from < span ? s[n][f][i] : 0.f;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dp[n][f][i] = s[n][f][i] * (dp[n][f][i] - d4[i]);
+          for (int i = 0; i < 4; ++i) dp[n][f][i] *= s[n][f][i];
         }
       }
       f8 pf[NK], ef[NK];

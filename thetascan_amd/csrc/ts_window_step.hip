@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(WinStepP p) {
   constexpr int P = win_pitch<E, D>(), DB = D / 16, KB = D / 32, VEC = 16 / (int)sizeof(E), PER = D / VEC;
   constexpr int NV = kStepSlots * PER / 64;
   extern __shared__ __align__(16) unsigned char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, g = lane >> 4;
   E* vt = (E*)lds + w * kStepSlots * P;
   const int b = blockIdx.x / p.Hkv, hk = blockIdx.x % p.Hkv, z = blockIdx.z * 16, d = p.d;
   const int heads = min(16, p.rep - z), h0 = hk * p.rep + z;
