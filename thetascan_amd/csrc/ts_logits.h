@@ -107,6 +107,21 @@ struct Exp64 {
     e = fma(e, r, 1.0);
     return __builtin_ldexp(e * table[n & 63], n >> 6);
   }
+  // round(2^44 e^t) for t in [-32, 0]: the whole parts come from the low bits of sums with 3 2^51 and 2^52, and
+  // the powers of two go into the exponent's bits (conversions and scalings take four times as long).
+  __device__ __forceinline__ unsigned long long whole(double t) const {
+    const double m = fma(t, 64.0 / kLn2, 0x1.8p52), k = m - 0x1.8p52;
+    const int n = (int)(uint32_t)__double_as_longlong(m);
+    double r = fma(k, -0x1.62e42fefap-7, t);
+    r = fma(k, -0x1.cf79abc9e3b3ap-46, r);
+    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    const long long scaled = __double_as_longlong(e * table[n & 63]) + ((long long)((n >> 6) + 44) << 52);
+    return (unsigned long long)(__double_as_longlong(__longlong_as_double(scaled) + 0x1p52) - __double_as_longlong(0x1p52));
+  }
 };
 
 // The parts of a row: `head` elements before its first 16-byte boundary, then

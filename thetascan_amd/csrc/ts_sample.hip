@@ -39,6 +39,7 @@ struct SampleP {
 };
 
 constexpr int kBins = 2048;
+constexpr int kList = 2048;  // tokens that are sorted at once
 constexpr double kUnit = 17592186044416.0;  // 2^44
 constexpr float kSpan = 31.3f;              // e^-kSpan 2^44 < 1 / 2: weights beyond it are zero
 
@@ -65,11 +66,12 @@ struct Sampler {
   static constexpr int N = Vec16<E>::N, WAVES = THREADS / 64;
   struct Shared {
     u64 bins[kBins];
+    u64 list[kList];
     u64 sums[WAVES];
     double table[64];
-    float most[WAVES], total[WAVES];
+    float most[WAVES], total[WAVES], high[WAVES];
     u64 before, inside;
-    int at;
+    int at, count, token;
   };
   Shared& sh;
   const SampleP& p;
@@ -115,14 +117,34 @@ struct Sampler {
     }
     return v;
   }
-  // f(logit, index) of every element (and of -inf past the row's ends)
+  // f(vector's number, its elements) of every vector (what lies past the row's ends stands as -inf), four
+  // on their way at once, one copy of f's code
+  template <typename F>
+  __device__ __forceinline__ void vectors(F f) const {
+#pragma unroll 1
+    for (int j = tid; j < vecs; j += 4 * THREADS) {
+      Vec16<E> a = load(j), b, c, d;
+      if (j + THREADS < vecs) b = load(j + THREADS);
+      if (j + 2 * THREADS < vecs) c = load(j + 2 * THREADS);
+      if (j + 3 * THREADS < vecs) d = load(j + 3 * THREADS);
+#pragma unroll 1
+      for (int i = j; i < min(vecs, j + 4 * THREADS); i += THREADS) {
+        f(i, a);
+        a.raw = b.raw;
+        b.raw = c.raw;
+        c.raw = d.raw;
+      }
+    }
+  }
+  // f(logit, index) of a vector's elements
+  template <typename F>
+  __device__ __forceinline__ void elements(int j, const Vec16<E>& v, F f) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f(tof(v.e[e]), j * N - shift + e);
+  }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (int j = tid; j < vecs; j += THREADS) {
-      const Vec16<E> v = load(j);
-#pragma unroll
-      for (int e = 0; e < N; ++e) f(tof(v.e[e]), j * N - shift + e);
-    }
+    vectors([&](int j, const Vec16<E>& v) { elements(j, v, f); });
   }
 
   // A logit as the softmax takes it, in fp64, less `base`: the cap where the highest logit is near it
@@ -147,7 +169,7 @@ struct Sampler {
     if (CAP ? x == -INFINITY : (x - most) * (float)inv_t < -(kSpan + 1.f)) return 0;
     const double t = (logit(x) - top) * inv_t;
     if (!(t > -(double)kSpan)) return 0;
-    return (u64)(__double_as_longlong(fma(e64(t), kUnit, 0x1p52)) - __double_as_longlong(0x1p52));
+    return e64.whole(t);
   }
   __device__ __forceinline__ bool left(float x, int i) const {
     const uint32_t k = KeyOf<E>::key(x);
@@ -202,7 +224,7 @@ struct Sampler {
 
   // Cuts what is left to the tokens with ok(measure of those before it), in the order of logits.
   template <typename M, typename OK>
-  __device__ void cut(M measure, OK ok) {
+  __device__ __forceinline__ void cut(M measure, OK ok) {
     clear();
     each([&](float x, int i) {
       const u64 w = left(x, i) ? measure(x) : 0;
@@ -280,98 +302,125 @@ struct Sampler {
   __device__ __forceinline__ u64 weights_left() {
     u64 sum = 0;
     each([&](float x, int i) {
-      if (left(x, i)) {
-        const u64 w = weight(x);
-        sum += w >= least ? w : 0;
-      }
+      if (left(x, i)) sum += weight(x);
     });
     return block_sum(sum);
   }
 
-  __device__ void run() {
-    const int64_t n = blockIdx.x;
-    double temperature = p.temperatures ? (double)p.temperatures[n] : p.temperature;
-    const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
-    const double min_p = p.min_ps ? (double)p.min_ps[n] : p.min_p;
-    int64_t top_k = p.top_ks ? p.top_ks[n] : p.top_k;
-    double u = (double)p.u[n];
-    // the highest logit; a row with none, or with one that is no number or +inf, has no token
-    float hi = -INFINITY;
-    bool bad = !(temperature >= 0.0);
-    each([&](float x, int) {
-      hi = fmaxf(hi, x);
-      bad |= !(x < INFINITY);
-    });
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    if (lane == 0) sh.most[wave] = hi;
-    bad = __syncthreads_or(bad);
-    most = -INFINITY;
-    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, sh.most[w]);
-    if (bad || most == -INFINITY) {
-      if (tid == 0) {
-        p.tokens[n] = -1;
-        p.log_probs[n] = NAN;
-      }
-      return;
-    }
-    // log of the sum of e^{y - max}, in fp32
-    const Logit<CAP> f(p.cap);
-    const float ymax = f.any(most);
-    float s = 0.f;
-    each([&](float x, int) { s += CAP && x == -INFINITY ? 0.f : ex(f.any(x) - ymax); });
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (lane == 0) sh.total[wave] = s;
-    __syncthreads();
-    s = 0.f;
-    for (int w = 0; w < WAVES; ++w) s += sh.total[w];
-
-    if (temperature == 0.0) {  // the highest logit
-      temperature = 1.0;
-      top_k = 1;
-    }
-    inv_t = 1.0 / temperature;
-    base = CAP && !(fabsf(most) < 0.25f * p.cap) ? (double)p.cap : 0.0;
-    top = logit(most);
-    scale = (float)fmin((double)kBins / ((double)kSpan * fmin(temperature, 1e30)), 1e30);
-    if (top_k < V) {
-      const u64 k = top_k < 1 ? 1 : (u64)top_k;
-      cut([&](float x) { return (u64)(x > -INFINITY); }, [&](u64 before) { return before < k; });
-    }
-    if (top_p < 1.0) {
-      const double part = top_p * (double)weights_left();
-      cut([&](float x) { return weight(x); }, [&](u64 before) { return before == 0 || (double)before < part; });
-    }
-    if (min_p > 0.0) {
-      const double w = ceil(fmin(min_p, 1.0) * kUnit);
-      least = w > 1.0 ? (u64)w : 1;
-    }
-    // the token: weights over the vectors, then inside the found ones
-    int sv = bits_over((uint32_t)(vecs - 1), 11);
-    clear();
-    u64 sum = 0;
-    for (int j = tid; j < vecs; j += THREADS) {
-      const Vec16<E> v = load(j);
-      u64 ws = 0;
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float x = tof(v.e[e]);
-        if (left(x, j * N - shift + e)) {
-          const u64 w = weight(x);
-          ws += w >= least ? w : 0;
+  // ---- a list of tokens in LDS: key << 32 | ~index sorts them as the logits are ordered (from the top)
+  static __device__ __forceinline__ u64 entry(uint32_t key, int i) { return (u64)key << 32 | (uint32_t)~(uint32_t)i; }
+  static __device__ __forceinline__ uint32_t key_of(u64 x) { return (uint32_t)(x >> 32); }
+  static __device__ __forceinline__ uint32_t index_of(u64 x) { return ~(uint32_t)x; }
+  __device__ __forceinline__ void add_to_list(float x, int i) {
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < kList) sh.list[at] = entry(KeyOf<E>::key(x), i);
+  }
+  // Sorts the list's first n, the highest first; `size`, a power of two from n on, is filled up with zeros.
+  __device__ __forceinline__ void sort_list(int n) {
+    int size = 2;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += THREADS) sh.list[i] = 0;
+    for (int k = 2; k <= size; k *= 2)
+      for (int j = k / 2; j > 0; j /= 2) {
+        __syncthreads();
+        for (int i = tid; i < size / 2; i += THREADS) {
+          const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+          const u64 a = sh.list[lo], b = sh.list[hi];
+          if ((a < b) == ((lo & k) == 0)) {
+            sh.list[lo] = b;
+            sh.list[hi] = a;
+          }
         }
       }
-      if (ws) atomicAdd(&sh.bins[j >> sv], ws);
-      sum += ws;
+    __syncthreads();
+  }
+  // f(i, what comes before i) with the running sum of g(i) over the first n, from `before`; every thread
+  // has a stretch of them.  Gives the whole sum.
+  template <typename G, typename F>
+  __device__ __forceinline__ u64 running(int n, u64 before, G g, F f) {
+    constexpr int PER = kList / THREADS;
+    const int per = (n + THREADS - 1) / THREADS;
+    u64 own[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = tid * per + i;
+      own[i] = i < per && at < n ? g(at) : 0;
+      sum += own[i];
     }
-    const u64 total = block_sum(sum);
-    if (!(u > 0.0)) u = 0.0;
-    const double place = floor(u * (double)total);
-    const u64 want = place >= (double)total ? total - 1 : (u64)place;
+    u64 run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const u64 x = __shfl_up(run, o, 64);
+      if (lane >= o) run += x;
+    }
+    __syncthreads();
+    if (lane == 63) sh.sums[wave] = run;
+    __syncthreads();
+    u64 at = before + run - sum, all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) at += sh.sums[w];
+      all += sh.sums[w];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = tid * per + i;
+      if (i < per && k < n) f(k, at, own[i]);
+      at += own[i];
+    }
+    return all;
+  }
+  __device__ __forceinline__ u64 list_weight(int i) const { return weight(KeyOf<E>::value(key_of(sh.list[i]))); }
+
+  // floor(u total), below the total
+  static __device__ __forceinline__ u64 place_of(double u, u64 total) {
+    const double place = floor((u > 0.0 ? u : 0.0) * (double)total);
+    return place >= (double)total ? total - 1 : (u64)place;
+  }
+
+  // The token where everything that is left stands in the list's first n (sorted): the nucleus among them, the
+  // least share, then the running weights in the order of the indices.
+  __device__ __forceinline__ int pick_of_list(int n, double top_p, double u) {
+    if (top_p < 1.0) {
+      const u64 all = running(n, 0, [&](int i) { return list_weight(i); }, [](int, u64, u64) {});
+      const double part = top_p * (double)all;
+      __syncthreads();
+      if (tid == 0) sh.at = n;
+      __syncthreads();
+      running(n, 0, [&](int i) { return list_weight(i); }, [&](int i, u64 before, u64) {
+        if (before != 0 && !((double)before < part)) atomicMin(&sh.at, i);
+      });
+      __syncthreads();
+      n = sh.at;
+    }
+    // (in the order of their indices: the key goes behind the index)
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS) {
+      const u64 x = sh.list[i];
+      sh.list[i] = (u64)(uint32_t)x << 32 | key_of(x);  // ~index: the lowest index is the highest
+    }
+    __syncthreads();
+    sort_list(n);
+    auto w = [&](int i) {
+      const u64 x = weight(KeyOf<E>::value((uint32_t)sh.list[i]));
+      return x >= least ? x : 0;
+    };
+    const u64 want = place_of(u, running(n, 0, w, [](int, u64, u64) {}));
+    __syncthreads();
+    if (tid == 0) sh.at = 0;
+    __syncthreads();
+    running(n, 0, w, [&](int i, u64 before, u64 own) {
+      if (before <= want && before + own > want) sh.at = i;
+    });
+    __syncthreads();
+    return (int)~(uint32_t)(sh.list[sh.at] >> 32);
+  }
+
+  // The token by the weights over the vectors that stand in the bins (2^sv vectors each), their sum total.
+  __device__ __forceinline__ int pick_of_bins(int sv, u64 total, double u) {
+    const u64 want = place_of(u, total);
     u64 before = 0, inside;
     const int b = find(before, inside, [&](u64 c) { return c <= want; });
-    // (the bin's elements: 2^sv vectors; one wave, each lane the next element in turn)
+    // (the bin's elements; one wave, each lane the next one in turn)
     if (wave == 0) {
       const int i0 = ((b << sv) * N) - shift, i1 = min(V, i0 + (N << sv));
       int found = -1;
@@ -395,14 +444,217 @@ struct Sampler {
         else
           before += __shfl(run, 63, 64);
       }
-      if (lane == 0) {
-        found = max(found, 0);
-        const float x = tof(row[found]);
-        // (as of the fp32 maximum that the sum is taken from)
-        const double off = f.any(x) >= ymax ? 0.0 : logit(x) + base - (double)ymax;
-        p.tokens[n] = found;
-        p.log_probs[n] = (float)(off - log((double)s));
+      if (lane == 0) sh.token = max(found, 0);
+    }
+    __syncthreads();
+    return sh.token;
+  }
+  // Adds the weights of what is left to the bins of their vectors; gives the sum.
+  __device__ __forceinline__ u64 fill_bins(int sv) {
+    clear();
+    u64 sum = 0;
+    vectors([&](int j, const Vec16<E>& v) {
+      u64 ws = 0;
+      elements(j, v, [&](float x, int i) {
+        if (left(x, i)) {
+          const u64 w = weight(x);
+          ws += w >= least ? w : 0;
+        }
+      });
+      if (ws) atomicAdd(&sh.bins[j >> sv], ws);
+      sum += ws;
+    });
+    return block_sum(sum);
+  }
+
+  __device__ __forceinline__ int pick(int64_t top_k, double top_p, double u, float mine) {
+    const int sv = bits_over((uint32_t)(vecs - 1), 11);
+    if (top_k < V && top_k <= kList / 4) {
+      // The k-th highest of the threads' maxima bounds the k-th logit from below: what lies in its bin and
+      // above is little more than k
+      const u64 k = (u64)(top_k < 1 ? 1 : top_k);
+      clear();
+      if (mine > -INFINITY) atomicAdd(&sh.bins[bin_of(mine)], (u64)1);
+      if (tid == 0) sh.count = 0;
+      u64 before = 0, inside;
+      int b = find(before, inside, [&](u64 c) { return c < k; });
+      if (b < 0) b = kBins - 1;
+      each([&](float x, int i) {
+        if (x > -INFINITY && bin_of(x) <= b) add_to_list(x, i);
+      });
+      __syncthreads();
+      const int n = sh.count;
+      if (n <= kList) {
+        __syncthreads();
+        sort_list(n);
+        return pick_of_list(min(n, (int)k), top_p, u);
       }
+    } else if (top_k >= V && top_p < 1.0) {
+      // weights by their distance from the maximum; the bin of the cut is sorted
+      clear();
+      if (tid == 0) sh.count = 0;
+      u64 sum = 0, before = 0, inside;
+      each([&](float x, int) {
+        const u64 w = weight(x);
+        if (w) atomicAdd(&sh.bins[bin_of(x)], w);
+        sum += w;
+      });
+      const double part = top_p * (double)block_sum(sum);
+      auto ok = [&](u64 c) { return c == 0 || (double)c < part; };
+      const int b = find(before, inside, ok);
+      if (b < 0) return pick_of_bins(sv, fill_bins(sv), u);
+      // a small nucleus is sorted whole
+      each([&](float x, int i) {
+        if (bin_of(x) <= b && x > -INFINITY) add_to_list(x, i);
+      });
+      __syncthreads();
+      const int held = sh.count;
+      if (held <= kList) {
+        __syncthreads();
+        sort_list(held);
+        if (tid == 0) sh.at = held;
+        __syncthreads();
+        running(held, 0, [&](int i) { return list_weight(i); }, [&](int i, u64 c, u64) {
+          if (!ok(c)) atomicMin(&sh.at, i);
+        });
+        __syncthreads();
+        return pick_of_list(sh.at, 1.0, u);
+      }
+      clear();
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      sum = 0;
+      vectors([&](int j, const Vec16<E>& v) {
+        u64 ws = 0;
+        elements(j, v, [&](float x, int i) {
+          const int at = bin_of(x);
+          if (at > b || x == -INFINITY) return;
+          if (at == b) {
+            add_to_list(x, i);
+          } else {
+            const u64 w = weight(x);
+            ws += w >= least ? w : 0;
+          }
+        });
+        if (ws) atomicAdd(&sh.bins[j >> sv], ws);
+        sum += ws;
+      });
+      __syncthreads();
+      const int n = sh.count;
+      if (n <= kList) {
+        sum = block_sum(sum);
+        sort_list(n);
+        // the first of the list that is cut, and the weights of those before it
+        __syncthreads();
+        if (tid == 0) sh.at = n;
+        __syncthreads();
+        running(n, before, [&](int i) { return list_weight(i); }, [&](int i, u64 c, u64) {
+          if (!ok(c)) atomicMin(&sh.at, i);
+        });
+        __syncthreads();
+        const int m = sh.at;  // (one at least: ok holds before the bin)
+        u64 more = 0;
+        for (int i = tid; i < m; i += THREADS) {
+          const u64 w = list_weight(i);
+          if (w < least) continue;
+          atomicAdd(&sh.bins[((int)index_of(sh.list[i]) + shift) / N >> sv], w);
+          more += w;
+        }
+        const u64 last = sh.list[m - 1];
+        cut_key = key_of(last);
+        cut_index = index_of(last) + 1;
+        return pick_of_bins(sv, sum + block_sum(more), u);
+      }
+    }
+    // any other: cut after cut
+    if (top_k < V) {
+      const u64 k = top_k < 1 ? 1 : (u64)top_k;
+      cut([&](float x) { return (u64)(x > -INFINITY); }, [&](u64 before) { return before < k; });
+    }
+    if (top_p < 1.0) {
+      const double part = top_p * (double)weights_left();
+      cut([&](float x) { return weight(x); }, [&](u64 before) { return before == 0 || (double)before < part; });
+    }
+    return pick_of_bins(sv, fill_bins(sv), u);
+  }
+
+  __device__ __forceinline__ void run() {
+    const int64_t n = blockIdx.x;
+    double temperature = p.temperatures ? (double)p.temperatures[n] : p.temperature;
+    const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
+    const double min_p = p.min_ps ? (double)p.min_ps[n] : p.min_p;
+    int64_t top_k = p.top_ks ? p.top_ks[n] : p.top_k;
+    const double u = (double)p.u[n];
+    // the highest logit, and the sum of e^{y - max} (fp32); a row with no logit, or with one that is no number or
+    // +inf, has no token
+    const Logit<CAP> f(p.cap);
+    float mine = -INFINITY, ym = kLowest, s = 0.f;
+    bool bad = !(temperature >= 0.0);
+    vectors([&](int, const Vec16<E>& v) {
+      float y[N], top = ym;
+      const bool far = f.some_far(v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float x = tof(v.e[e]);
+        mine = fmaxf(mine, x);
+        bad |= !(x < INFINITY);
+        y[e] = CAP && x == -INFINITY ? -INFINITY : far ? f.any(x) : f.near(x);
+        top = fmaxf(top, y[e]);
+      }
+      s *= ex(ym - top);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s += ex(y[e] - top);
+      ym = top;
+    });
+    float hi = mine;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+      const float y2 = __shfl_xor(ym, o, 64), s2 = __shfl_xor(s, o, 64), top = fmaxf(ym, y2);
+      s = s * ex(ym - top) + s2 * ex(y2 - top);
+      ym = top;
+    }
+    if (lane == 0) {
+      sh.most[wave] = hi;
+      sh.high[wave] = ym;
+      sh.total[wave] = s;
+    }
+    bad = __syncthreads_or(bad);
+    most = -INFINITY;
+    ym = kLowest;
+    for (int w = 0; w < WAVES; ++w) {
+      most = fmaxf(most, sh.most[w]);
+      ym = fmaxf(ym, sh.high[w]);
+    }
+    if (bad || most == -INFINITY) {
+      if (tid == 0) {
+        p.tokens[n] = -1;
+        p.log_probs[n] = NAN;
+      }
+      return;
+    }
+    s = 0.f;
+    for (int w = 0; w < WAVES; ++w) s = fmaf(sh.total[w], ex(sh.high[w] - ym), s);
+
+    if (temperature == 0.0) {  // the highest logit
+      temperature = 1.0;
+      top_k = 1;
+    }
+    inv_t = 1.0 / temperature;
+    base = CAP && !(fabsf(most) < 0.25f * p.cap) ? (double)p.cap : 0.0;
+    top = logit(most);
+    scale = (float)fmin((double)kBins / ((double)kSpan * fmin(temperature, 1e30)), 1e30);
+    if (min_p > 0.0) {
+      const double w = ceil(fmin(min_p, 1.0) * kUnit);
+      least = w > 1.0 ? (u64)w : 1;
+    }
+    const int token = pick(top_k, top_p, u, mine);
+    if (tid == 0) {
+      const float x = tof(row[token]);
+      // (as of the fp32 maximum that the sum is taken from)
+      const double off = f.any(x) >= ym ? 0.0 : logit(x) + base - (double)ym;
+      p.tokens[n] = token;
+      p.log_probs[n] = (float)(off - log((double)s));
     }
   }
 };
