@@ -19,7 +19,10 @@ attention mixer 786,440, FFN hidden 1024).
 
 ``HybridLM(memory="delta")`` has gated delta memories
 (:class:`thetascan_amd.delta.GatedDelta`) in those two layers instead, and
-``policy_loss`` trains either on rollouts.
+``policy_loss`` trains either on rollouts.  ``HybridLM(window=, sinks=)`` gives the
+attention layers a window and sinks (:func:`thetascan_amd.windowed_attention`), so that
+they, as the memories, carry a state of fixed size: ``generate`` draws rollouts from it,
+and ``distill_loss`` learns from a teacher's ``top_log_probs``.
 
 The upstream script is not available, so this model is defined here from
 those facts; its int8 round trip has no reference numbers to match.
@@ -32,7 +35,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._core.ops import attention as hip_attention, policy, rowglue, rownorm
+from ._core.ops import attention as hip_attention, distill, policy, rowglue, rownorm, sample, window as windowed
 from .api import ThetaScan
 from .config import ThetaScanConfig
 from .delta import GatedDelta, GatedDeltaConfig
@@ -96,10 +99,25 @@ def _rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tens
     return torch.cat([x1 * c + x2 * s, x2 * c - x1 * s], -1).to(x.dtype)
 
 
+@dataclasses.dataclass
+class AttentionCache:
+    """What an attention layer carries through a generation: its ring cache, the next
+    tokens' positions, and the rotary phases of all positions to come."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    positions: torch.Tensor
+    cos: torch.Tensor
+    sin: torch.Tensor
+    position: int = 0
+
+
 class CausalSelfAttention(nn.Module):
-    def __init__(self, dim: int = D_MODEL, heads: int = HEADS, kv_heads: int = KV_HEADS, q_gain: float = 1.5):
+    def __init__(self, dim: int = D_MODEL, heads: int = HEADS, kv_heads: int = KV_HEADS, q_gain: float = 1.5,
+                 window: int | None = None, sinks: int = 0):
         super().__init__()
         self.heads, self.kv_heads, self.hd = heads, kv_heads, dim // heads
+        self.window, self.sinks = window, sinks
         self.c_q = nn.Linear(dim, dim, bias=False)
         self.c_k = nn.Linear(dim, kv_heads * self.hd, bias=False)
         self.c_v = nn.Linear(dim, kv_heads * self.hd, bias=False)
@@ -108,12 +126,25 @@ class CausalSelfAttention(nn.Module):
         self.q_gain = nn.Parameter(torch.full((heads,), q_gain))
         self.rotary = Rotary(self.hd)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def initial_cache(self, batch: int, total: int, like: torch.Tensor) -> AttentionCache:
+        """The cache of ``batch`` sequences of up to ``total`` tokens, with none yet."""
+        cos, sin = self.rotary(total, like.device)
+        shape = (batch, self.kv_heads, self.sinks + self.window, self.hd)
+        return AttentionCache(like.new_empty(shape), like.new_empty(shape),
+                              torch.zeros(batch, dtype=torch.int64, device=like.device), cos, sin)
+
+    def forward(self, x: torch.Tensor, cache: AttentionCache | None = None) -> torch.Tensor:
+        """``cache``: continues from it (a prompt where it is new, then single tokens;
+        without gradients) and leaves these tokens in it."""
         B, T, D = x.shape
         q = self.c_q(x).view(B, T, self.heads, self.hd).transpose(1, 2)
         k = self.c_k(x).view(B, T, self.kv_heads, self.hd).transpose(1, 2)
         v = self.c_v(x).view(B, T, self.kv_heads, self.hd).transpose(1, 2)
-        cos, sin = self.rotary(T, x.device)
+        if cache is None:
+            cos, sin = self.rotary(T, x.device)
+        else:
+            at = slice(cache.position, cache.position + T)
+            cos, sin = cache.cos[at], cache.sin[at]
         if rownorm.supported(q, rope=True) and rownorm.supported(k, rope=True):
             # norm, rotary turn and query gain in one launch per stream
             q = rownorm.rms_rows(q, cos, sin, self.q_gain)
@@ -121,7 +152,17 @@ class CausalSelfAttention(nn.Module):
         else:
             q, k = _rotate(_rms(q), cos, sin), _rotate(_rms(k), cos, sin)
             q = q * self.q_gain.to(q.dtype)[None, :, None, None]
-        y = attention(q, k, v)
+        if self.window is None:
+            y = attention(q, k, v)
+        elif cache is not None and cache.position:
+            y = windowed.windowed_attention_step(q, k, v, cache.k, cache.v, cache.positions, sinks=self.sinks)
+        else:
+            y = windowed.windowed_attention(q, k, v, window=self.window, sinks=self.sinks)
+            if cache is not None:
+                windowed.fill_window_cache(k, v, cache.k, cache.v, sinks=self.sinks)
+        if cache is not None:
+            cache.position += T
+            cache.positions += T
         return self.proj(y.transpose(1, 2).reshape(B, T, D))
 
 
@@ -168,14 +209,14 @@ def delta_config() -> GatedDeltaConfig:
 
 
 class Block(nn.Module):
-    def __init__(self, theta: bool, memory: str = "theta"):
+    def __init__(self, theta: bool, memory: str = "theta", window: int | None = None, sinks: int = 0):
         super().__init__()
         self.theta = theta
         if theta and memory == "delta":
             self.attn = GatedDelta(delta_config())
             nn.init.zeros_(self.attn.proj_out.weight)
         else:
-            self.attn = ThetaScan(theta_config()) if theta else CausalSelfAttention()
+            self.attn = ThetaScan(theta_config()) if theta else CausalSelfAttention(window=window, sinks=sinks)
             if theta:
                 # the recipe's memory starts near identity; its projections start
                 # like attention's (the output projection at zero)
@@ -185,11 +226,18 @@ class Block(nn.Module):
         self.mlp_scale = nn.Parameter(torch.ones(D_MODEL))
         self.resid_mix = nn.Parameter(torch.stack((torch.ones(D_MODEL), torch.zeros(D_MODEL))))
 
-    def forward(self, x: torch.Tensor, x0: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, x0: torch.Tensor, states: list | None = None, i: int = 0) -> torch.Tensor:
+        """``states[i]``: the mixer's carried state, replaced by its next one."""
         # mix0 x + mix1 x0, then x + scale * f(x) per sublayer: one row-glue
         # launch each on the GPU, with the norm that the sublayer reads
         x, n = _add_rms(x, x0, self.resid_mix[0], self.resid_mix[1])
-        x, n = _add_rms(x, self.attn(n), None, self.attn_scale)
+        if states is None:
+            y = self.attn(n)
+        elif self.theta:
+            y, states[i] = self.attn(n, states[i])
+        else:
+            y = self.attn(n, states[i])
+        x, n = _add_rms(x, y, None, self.attn_scale)
         return rowglue.scale_add(x, self.mlp(n), None, self.mlp_scale)
 
 
@@ -197,30 +245,37 @@ class HybridLM(nn.Module):
     """Token ids [B,T] -> mean next-token cross-entropy (or logits).
 
     ``memory`` names the mixers of layers 4 and 5: "theta" (ThetaScan-Kernel) or
-    "delta" (gated delta rule)."""
+    "delta" (gated delta rule); ``window`` and ``sinks`` are the attention layers'
+    (None: every earlier token)."""
 
-    def __init__(self, memory: str = "theta"):
+    def __init__(self, memory: str = "theta", window: int | None = None, sinks: int = 0):
         super().__init__()
+        if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
+            raise ValueError(f"window must be a whole number of at least 1 (None: all), got {window!r}")
+        if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+            raise ValueError(f"sinks must be a whole number of at least 0, got {sinks!r}")
+        self.window = window
         if memory not in ("theta", "delta"):
             raise ValueError(f"memory must be 'theta' or 'delta', got {memory!r}")
         self.tok_emb = nn.Embedding(VOCAB, D_MODEL)
         nn.init.normal_(self.tok_emb.weight, std=0.005)
-        self.blocks = nn.ModuleList([Block(i in THETA_LAYERS, memory) for i in range(LAYERS)])
+        self.blocks = nn.ModuleList([Block(i in THETA_LAYERS, memory, window, sinks) for i in range(LAYERS)])
         self.n_enc = LAYERS // 2
         self.skip_weights = nn.Parameter(torch.ones(min(self.n_enc, LAYERS - self.n_enc), D_MODEL))
 
-    def _logits(self, idx: torch.Tensor) -> torch.Tensor:
-        """The logits [B,T,V] before the soft cap, in the weights' dtype."""
+    def _logits(self, idx: torch.Tensor, states: list | None = None) -> torch.Tensor:
+        """The logits [B,T,V] before the soft cap, in the weights' dtype; with the
+        layers' ``states`` continued from them, of the last token alone [B,1,V]."""
         x = _rms(self.tok_emb(idx))
         x0 = x
         skips = []
         for i, block in enumerate(self.blocks):
             if i >= self.n_enc and skips:
                 x = rowglue.scale_add(x, skips.pop(), None, self.skip_weights[i - self.n_enc])
-            x = block(x, x0)
+            x = block(x, x0, states, i)
             if i < self.n_enc:
                 skips.append(x)
-        x = _rms(x)
+        x = _rms(x if states is None else x[:, -1:])
         return F.linear(x, self.tok_emb.weight.to(x.dtype))
 
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None) -> torch.Tensor:
@@ -244,6 +299,45 @@ class HybridLM(nn.Module):
         sampled successors ``tokens`` [B,T] of ``idx`` [B,T] (``options``: its
         keywords but the soft cap)."""
         return policy.policy_loss(self._logits(idx), tokens, old_log_probs, advantages, softcap=LOGIT_SOFTCAP, **options)
+
+
+    def top_log_probs(self, idx: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """``(ids, log_probs)`` [B,T,k] of the most likely successors of ``idx`` [B,T]: what
+        a student's ``distill_loss`` takes of its teacher (without a gradient)."""
+        with torch.no_grad():
+            z = self._logits(idx).float()
+            lp, ids = torch.log_softmax(LOGIT_SOFTCAP * torch.tanh(z / LOGIT_SOFTCAP), -1).topk(k, -1)
+            return ids, lp
+
+    def distill_loss(self, idx: torch.Tensor, ids: torch.Tensor, log_probs: torch.Tensor,
+                     **options) -> tuple[torch.Tensor, torch.Tensor]:
+        """``(loss, each)`` of :func:`thetascan_amd.distill_loss` for a teacher's tokens
+        ``ids`` [B,T,k] as successors of ``idx`` [B,T] (``options``: its keywords but the soft
+        cap)."""
+        return distill.distill_loss(self._logits(idx), ids, log_probs, softcap=LOGIT_SOFTCAP, **options)
+
+    def generate(self, prompts: torch.Tensor, uniforms: torch.Tensor, **options) -> tuple[torch.Tensor, torch.Tensor]:
+        """``(tokens, log_probs)`` [B,n]: each sequence of ``prompts`` [B,T] continued by
+        as many tokens as ``uniforms`` [B,n] has random numbers in [0, 1), and their
+        log-probabilities (``policy_loss``'s ``old_log_probs``).  ``options``: the settings of
+        :func:`thetascan_amd.sample_tokens`.  The layers' states and caches have a fixed
+        size, so the model needs a ``window``."""
+        if self.window is None:
+            raise ValueError("generate needs a model with a window")
+        if prompts.ndim != 2 or uniforms.ndim != 2 or prompts.shape[0] != uniforms.shape[0] or not prompts.shape[1]:
+            raise ValueError(f"prompts [B,T] and uniforms [B,n], got {tuple(prompts.shape)} and {tuple(uniforms.shape)}")
+        B, n = uniforms.shape
+        tokens = torch.empty(B, n, dtype=torch.int64, device=prompts.device)
+        log_probs = torch.empty(B, n, dtype=torch.float32, device=prompts.device)
+        with torch.no_grad():
+            states = [b.attn.initial_state() if b.theta else
+                      b.attn.initial_cache(B, prompts.shape[1] + n, self.tok_emb.weight) for b in self.blocks]
+            idx = prompts
+            for i in range(n):
+                z = self._logits(idx, states)[:, 0]
+                tokens[:, i], log_probs[:, i] = sample.sample_tokens(z, uniforms[:, i], softcap=LOGIT_SOFTCAP, **options)
+                idx = tokens[:, i:i + 1].clamp(min=0)  # (of logits that are no numbers: no token, -1)
+        return tokens, log_probs
 
 
 # ---------------------------------------------------------------- int8 round trip
