@@ -1460,7 +1460,7 @@ typedef struct ts_distill_io {
   const float* log_probs; /* [rows, K]                                            */
   const float* weights;   /* [rows] or NULL: 1 / rows each                        */
   float* each;            /* out [rows]: the rows' losses before their weights    */
-  float* stats;           /* out [4, rows], kept for the backward (or NULL)       */
+  float* stats;           /* out [5, rows], kept for the backward (or NULL)       */
   double* parts;          /* scratch [rows]                                       */
   float* loss;            /* out [1]                                              */
   void* dlogits;          /* out [rows, V] contiguous, 16-byte aligned: the logits' gradient for

@@ -55,7 +55,7 @@ def _forward(z: torch.Tensor, ids: torch.Tensor, lps: torch.Tensor, weights: tor
     loss = torch.empty((), dtype=torch.float32, device=z.device)
     each = torch.empty(rows, dtype=torch.float32, device=z.device)
     # parts of the loss (fp64), then what the backward takes of each row
-    saved = torch.empty(6 * rows + 2, dtype=torch.float32, device=z.device)
+    saved = torch.empty(7 * rows + 2, dtype=torch.float32, device=z.device)
     at = saved.data_ptr()
     dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if rows and eager_forward() else None
     io = _lib.DistillIO(z.data_ptr(), ids.data_ptr(), lps.data_ptr(), _lib.ptr(weights), each.data_ptr(), at + 8 * rows,
@@ -71,7 +71,7 @@ def _forward(z: torch.Tensor, ids: torch.Tensor, lps: torch.Tensor, weights: tor
 
 def _forward_fake(z, ids, lps, weights, cap, temperature, tail):
     return [z.new_empty((), dtype=torch.float32), z.new_empty(z.shape[0], dtype=torch.float32),
-            z.new_empty(6 * z.shape[0] + 2, dtype=torch.float32)]
+            z.new_empty(7 * z.shape[0] + 2, dtype=torch.float32)]
 
 
 def _backward_impl(g: torch.Tensor, z: torch.Tensor, ids: torch.Tensor, lps: torch.Tensor,

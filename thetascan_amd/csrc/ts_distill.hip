@@ -67,6 +67,22 @@ struct RowTeam {
   __device__ __forceinline__ T most(T x) const { return reduce(x, [](T a, T b) { return a > b ? a : b; }); }
 };
 
+// e^{d / temperature} of differences of capped logits, by powers of two: log2(e) / temperature in two parts
+// (a factor that is off by 2^-25 is another temperature: of a teacher and student that all but agree, the
+// loss is small against what that moves their log-probabilities).
+struct TemperedExp {
+  float hi, lo;
+  __device__ __forceinline__ explicit TemperedExp(double inv_t) {
+    const double c = inv_t / kLn2;
+    hi = (float)c;
+    lo = (float)(c - (double)hi);
+  }
+  __device__ __forceinline__ float operator()(float d) const {
+    d = d < kLowest ? kLowest : d;  // (of -inf the parts' products would cancel to no number)
+    return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
+  }
+};
+
 template <bool CAP>
 __device__ __forceinline__ double distill_logit(const DistillP& p, float z) {
   double y = (double)z;
@@ -119,18 +135,19 @@ __device__ __forceinline__ double wave_sum(double x) {
   return half(x, [](float v) { return xor32_pair(v); });
 }
 
-// What a row's loss is formed from: log2 of e^x counts from the highest of all, hi.
+// What a row's loss is formed from: x counts from the highest of all, hi.
 struct DistillTerms {
   double mass, a;   // sum P, sum P (lp - (x - hi))
   float total;      // sum of all e^{x - hi}
-  float sr, dm;     // the others' sum from their own maximum, and its distance from hi (log2)
+  float sr;         // the others' sum from their own maximum,
+  double dm;        // and its distance from hi
 };
 __device__ __forceinline__ double distill_loss_of(const DistillP& p, const DistillTerms& t) {
   const double lt = log((double)t.total);
   if (!p.tail) return t.mass > 0.0 ? t.a / t.mass - log(t.mass) + lt : t.a;
   double loss = t.a + t.mass * lt;
   const double left = t.sr != 0.f ? 1.0 - t.mass : 0.0;
-  if (left > 0.0) loss += left * (log(left) - (double)t.dm * kLn2 - log((double)t.sr) + lt);
+  if (left > 0.0) loss += left * (log(left) - t.dm - log((double)t.sr) + lt);
   return loss + 0.0 * left;  // (a share that is no number)
 }
 
@@ -200,9 +217,9 @@ struct DistillFactors {
   }
 };
 __device__ __forceinline__ DistillFactors distill_factors(const DistillP& p, double mass, double a, float sr, float ek,
-                                                          float dm) {
+                                                          float down) {
   DistillFactors k;
-  const float down = sr != 0.f ? __builtin_amdgcn_exp2f(dm) : 0.f;
+  if (sr == 0.f) down = 0.f;  // of the others' maximum, e^{x - hi}
   k.total = fmaf(sr, down, ek);
   k.inv = rcp(k.total);
   const double left = p.tail && sr != 0.f ? fmax(1.0 - mass, 0.0) : 0.0;
@@ -225,10 +242,11 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
   const int V = p.V;
   const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + gi) * R;
   const Logit<CAP> f(p.cap);
-  const float inv_t = (float)p.inv_t, c2 = (float)(p.inv_t / kLn2);
+  const float inv_t = (float)p.inv_t;
   const Exp64 e64{kPowers64};
-  DistillTerms mine{1.0, 0.0, 1.f, 0.f, 0.f};
-  float mine_w = 0.f, mine_rest = 0.f, mine_hi = 0.f, mine_mr = 0.f, mine_mass = 0.f;
+  const TemperedExp te(p.inv_t);
+  DistillTerms mine{1.0, 0.0, 1.f, 0.f, 0.0};
+  float mine_w = 0.f, mine_rest = 0.f, mine_hi = 0.f, mine_mr = 0.f, mine_inv = 0.f, mine_mass = 0.f;
   DistillIn<E, VPT, KS> in;
   float zn[KS];
   in.load(p, row0, li);
@@ -315,13 +333,13 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) slk[s] = f.slope_any(zk[s], yk[s]);
-    const float h2 = wave_most(hz) * c2;
+    const float high = wave_most(hz);
     double all = 0.0;
 #pragma unroll
     for (int r = 0; r < VPT; ++r)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(y[r][e], c2, -h2));
+        const float x = te(y[r][e] - high);
         all += (double)x;
         sl[r][e] = CAP ? x * sl[r][e] : x;
       }
@@ -332,13 +350,13 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
       P[s] = 0.0;
       q[s] = 0.f;
       if (id[s] >= 0) {
-        const float off = fmaf(yk[s], c2, -h2);
+        const float off = yk[s] - high;
         // (in fp64: one less their sum is what the teacher leaves to all others)
         P[s] = lp[s] > -700.f ? e64((double)lp[s]) : lp[s] == lp[s] ? 0.0 : (double)lp[s];
-        q[s] = __builtin_amdgcn_exp2f(off);
+        q[s] = te(off);
         ek += (double)q[s];
         mass += P[s];
-        if (P[s] != 0.0) a += P[s] * ((double)lp[s] - (double)off * kLn2);
+        if (P[s] != 0.0) a += P[s] * ((double)lp[s] - (double)off * p.inv_t);
       }
     }
     if (bad) a = (double)NAN;
@@ -346,7 +364,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
     ek = wave_sum(ek);
     mass = wave_sum(mass);
     a = wave_sum(a);
-    float m2 = h2, sr = (float)all;
+    float most = high, sr = (float)all;
     if (!(all > ek * 0x1p-28)) {
       // (uniform) next to nothing is left: from the others' own maximum, the teacher's tokens masked
       float mz = -INFINITY;
@@ -363,12 +381,12 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
       }
       mz = wave_most(mz);
       // (no other token: any finite stand-in, their sum is zero)
-      m2 = mz == -INFINITY ? 0.f : mz * c2;
+      most = mz == -INFINITY ? 0.f : mz;
 #pragma unroll
       for (int r = 0; r < VPT; ++r)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(y[r][e], c2, -m2));
+          const float x = te(y[r][e] - most);
           sr += x;
           if (CAP && x != 0.f) {
             float unused;
@@ -379,13 +397,14 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
         }
       sr = wave_sum(sr);
     }
-    const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, m2 - h2);
+    const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, te(most - high));
     if (li == rr) {
-      mine = DistillTerms{mass, a, k.total, sr, m2 - h2};
+      mine = DistillTerms{mass, a, k.total, sr, (double)(most - high) * p.inv_t};
       mine_w = w;
       mine_rest = k.rest;
-      mine_mr = m2;
-      mine_hi = h2;
+      mine_mr = most;
+      mine_hi = high;
+      mine_inv = k.inv;
       mine_mass = k.mass;
     }
     if (rr + 1 < R && n + 1 < p.rows) in.gather(p, n + 1, zn);
@@ -418,8 +437,9 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
     if (p.stats) {
       p.stats[n] = mine_mr;
       p.stats[p.rows + n] = mine_rest;
-      p.stats[2 * p.rows + n] = mine_hi + __log2f(mine.total);
-      p.stats[3 * p.rows + n] = mine_mass;
+      p.stats[2 * p.rows + n] = mine_hi;
+      p.stats[3 * p.rows + n] = mine_inv;
+      p.stats[4 * p.rows + n] = mine_mass;
     }
   }
 #pragma unroll
@@ -435,13 +455,13 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
 
 // A row's gradient where no token is the teacher's: cr e^{x - maximum} slope, by LANES threads.
 template <typename E, bool CAP, int LANES>
-__device__ __forceinline__ void distill_others(const E* row, E* out, int V, const Logit<CAP>& f, float cr, float c2,
-                                               float m2, int li) {
-  constexpr int N = Vec16<E>::N, U = 4;
+__device__ __forceinline__ void distill_others(const E* row, E* out, int V, const Logit<CAP>& f, float cr, const TemperedExp& te,
+                                               float most, int li) {
+  constexpr int N = Vec16<E>::N, U = 2;
   auto one = [&](float z) {
     float y;
     const float slope = f.slope_any(z, y);
-    return __builtin_amdgcn_exp2f(fmaf(y, c2, -m2)) * cr * slope;
+    return te(y - most) * slope * cr;
   };
   // the output's vectors; where the logits' do not start with them, they are read element by element
   const RowSpan<E> to(out, V);
@@ -471,7 +491,7 @@ __device__ __forceinline__ void distill_others(const E* row, E* out, int V, cons
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float y = f.near(tof(v[u].e[e]));
-          o.e[e] = cvt<E>(__builtin_amdgcn_exp2f(fmaf(y, c2, -m2)) * cr * f.slope_near(y));
+          o.e[e] = cvt<E>(te(y - most) * f.slope_near(y) * cr);
         }
       }
       ((Vec16<E>*)(out + to.head))[j].raw = o.raw;
@@ -486,7 +506,7 @@ __device__ __forceinline__ void distill_others(const E* row, E* out, int V, cons
 // which finds the row in the caches.
 template <typename E, bool CAP, int THREADS, bool GRAD>
 __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
-  constexpr int N = Vec16<E>::N, WAVES = THREADS / 64, U = 4;
+  constexpr int N = Vec16<E>::N, WAVES = THREADS / 64, U = 2;
   extern __shared__ uint32_t marks[];
   __shared__ double sm_a[WAVES], sm_mass[WAVES];
   __shared__ float sm[3][WAVES];
@@ -508,7 +528,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
       p.each[n] = 0.f;
       p.part[n] = 0.0;
       if (p.stats)
-        for (int i = 0; i < 4; ++i) p.stats[i * p.rows + n] = 0.f;
+        for (int i = 0; i < 5; ++i) p.stats[i * p.rows + n] = 0.f;
     }
     return;
   }
@@ -516,7 +536,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   const float* lps = p.lps + n * K;
   const Logit<CAP> f(p.cap);
   const Exp64 e64{kPowers64};
-  const float inv_t = (float)p.inv_t, c2 = (float)(p.inv_t / kLn2);
+  const float inv_t = (float)p.inv_t;
   // the teacher's tokens, a bit each (from the 16-byte boundary at or before the row's start), and
   // their highest logit
   const int shift = (int)(((uintptr_t)row & 15) / sizeof(E)), vecs = (V + shift + N - 1) / N;
@@ -534,7 +554,8 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   }
   __syncthreads();
   // the others
-  float m2 = kLowest, sr = 0.f;
+  const TemperedExp te(p.inv_t);
+  float most = kLowest, sr = 0.f;
   for (int j0 = tid; j0 < vecs; j0 += U * THREADS) {
     Vec16<E> v[U];
     uint32_t mask[U];
@@ -559,13 +580,13 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float x[N], top = m2;
+      float x[N], top = most;
       if (f.some_far(v[u])) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = f.any(tof(v[u].e[e])) * c2;
+        for (int e = 0; e < N; ++e) x[e] = f.any(tof(v[u].e[e]));
       } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = f.near(tof(v[u].e[e])) * c2;
+        for (int e = 0; e < N; ++e) x[e] = f.near(tof(v[u].e[e]));
       }
       if (mask[u]) {
 #pragma unroll
@@ -573,16 +594,16 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
       }
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, x[e]);
-      sr *= __builtin_amdgcn_exp2f(m2 - top);
+      sr *= te(most - top);
 #pragma unroll
-      for (int e = 0; e < N; ++e) sr += __builtin_amdgcn_exp2f(x[e] - top);
-      m2 = top;
+      for (int e = 0; e < N; ++e) sr += te(x[e] - top);
+      most = top;
       __builtin_amdgcn_sched_barrier(0);
     }
   }
   {
-    const float top = wave_most(m2);
-    sr = wave_sum(sr * __builtin_amdgcn_exp2f(m2 - top));
+    const float top = wave_most(most);
+    sr = wave_sum(sr * te(most - top));
     hz = wave_most(hz);
     if (lane == 0) {
       sm[0][wave] = top;
@@ -590,31 +611,31 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
       sm[2][wave] = hz;
     }
     __syncthreads();
-    m2 = kLowest;
+    most = kLowest;
 #pragma unroll
     for (int u = 0; u < WAVES; ++u) {
-      m2 = fmaxf(m2, sm[0][u]);
+      most = fmaxf(most, sm[0][u]);
       hz = fmaxf(hz, sm[2][u]);
     }
     sr = 0.f;
 #pragma unroll
-    for (int u = 0; u < WAVES; ++u) sr = fmaf(sm[1][u], __builtin_amdgcn_exp2f(sm[0][u] - m2), sr);
+    for (int u = 0; u < WAVES; ++u) sr = fmaf(sm[1][u], te(sm[0][u] - most), sr);
   }
   // (no other token: any finite stand-in, their sum is zero)
-  if (sr == 0.f) m2 = 0.f;
-  const float h2 = sr == 0.f ? f.any(hz) * c2 : fmaxf(m2, f.any(hz) * c2);
+  if (sr == 0.f) most = 0.f;
+  const float high = sr == 0.f ? f.any(hz) : fmaxf(most, f.any(hz));
   double mass = 0.0, a = 0.0;
   float ek = 0.f;
   auto share = [&](float lp) { return lp > -700.f ? e64((double)lp) : lp == lp ? 0.0 : (double)lp; };
   for (int k = tid; k < K; k += THREADS) {
     const int64_t id = ids[k];
     if (id < 0 || id >= V) continue;
-    const float off = fmaf(f.any(tof(row[id])), c2, -h2), lp = lps[k];
+    const float off = f.any(tof(row[id])) - high, lp = lps[k];
     // (in fp64: one less their sum is what the teacher leaves to all others)
     const double P = share(lp);
-    ek += __builtin_amdgcn_exp2f(off);
+    ek += te(off);
     mass += P;
-    if (P != 0.0) a += P * ((double)lp - (double)off * kLn2);
+    if (P != 0.0) a += P * ((double)lp - (double)off * p.inv_t);
   }
   if (bad) a = (double)NAN;
   ek = wave_sum(ek);
@@ -635,21 +656,22 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
     mass += sm_mass[u];
     a += sm_a[u];
   }
-  const DistillFactors k = distill_factors(p, mass, a, sr, ek, m2 - h2);
+  const DistillFactors k = distill_factors(p, mass, a, sr, ek, te(most - high));
   if (tid == 0) {
-    const double each = distill_loss_of(p, DistillTerms{mass, a, k.total, sr, m2 - h2});
+    const double each = distill_loss_of(p, DistillTerms{mass, a, k.total, sr, (double)(most - high) * p.inv_t});
     p.each[n] = (float)each;
     p.part[n] = each * (double)w;
     if (p.stats) {
-      p.stats[n] = m2;
+      p.stats[n] = most;
       p.stats[p.rows + n] = k.rest;
-      p.stats[2 * p.rows + n] = h2 + __log2f(k.total);
-      p.stats[3 * p.rows + n] = k.mass;
+      p.stats[2 * p.rows + n] = high;
+      p.stats[3 * p.rows + n] = k.inv;
+      p.stats[4 * p.rows + n] = k.mass;
     }
   }
   if constexpr (GRAD) {
     const float c = w * inv_t;
-    distill_others<E, CAP, THREADS>(row, out, V, f, c * k.rest, c2, m2, tid);
+    distill_others<E, CAP, THREADS>(row, out, V, f, c * k.rest, te, most, tid);
     __threadfence_block();
     __syncthreads();
     for (int i = tid; i < K; i += THREADS) {
@@ -657,7 +679,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
       if (id < 0 || id >= V) continue;
       float y;
       const float slope = f.slope_any(tof(row[id]), y);
-      out[id] = cvt<E>(c * k.of_teacher(share(lps[i]), __builtin_amdgcn_exp2f(fmaf(y, c2, -h2))) * slope);
+      out[id] = cvt<E>(c * k.of_teacher(share(lps[i]), te(y - high)) * slope);
     }
   }
 }
@@ -684,28 +706,33 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillP p) {
     return;
   }
   const Logit<CAP> f(p.cap);
-  const float inv_t = (float)p.inv_t, c2 = (float)(p.inv_t / kLn2), c = w * p.g[0] * inv_t;
-  const float top = p.stats[n], rest = p.stats[p.rows + n], lse = p.stats[2 * p.rows + n], mass = p.stats[3 * p.rows + n];
-  distill_others<E, CAP, LANES>(row, out, V, f, c * rest, c2, top, li);
+  const Exp64 e64{kPowers64};
+  const TemperedExp te(p.inv_t);
+  const float c = w * p.g[0] * (float)p.inv_t, most = p.stats[n], high = p.stats[2 * p.rows + n];
+  DistillFactors k;
+  k.rest = p.stats[p.rows + n];
+  k.inv = p.stats[3 * p.rows + n];
+  k.mass = p.stats[4 * p.rows + n];
+  k.norm = 1.f;
+  distill_others<E, CAP, LANES>(row, out, V, f, c * k.rest, te, most, li);
   // the teacher's tokens over those
-  double norm = 0.0;
+  auto share = [&](float lp) { return lp > -700.f ? e64((double)lp) : lp == lp ? 0.0 : (double)lp; };
   if (!p.tail) {
-    for (int k = li; k < p.K; k += LANES) {
-      const int64_t id = p.ids[n * p.K + k];
-      if (id >= 0 && id < V) norm += exp((double)p.lps[n * p.K + k]);
+    double sum = 0.0;
+    for (int i = li; i < p.K; i += LANES) {
+      const int64_t id = p.ids[n * p.K + i];
+      if (id >= 0 && id < V) sum += share(p.lps[n * p.K + i]);
     }
-    norm = log(team.sum(norm));
+    k.norm = rcp((float)team.sum(sum));
   }
   __threadfence_block();
   team.sync();
-  for (int k = li; k < p.K; k += LANES) {
-    const int64_t id = p.ids[n * p.K + k];
+  for (int i = li; i < p.K; i += LANES) {
+    const int64_t id = p.ids[n * p.K + i];
     if (id < 0 || id >= V) continue;
     float y;
     const float slope = f.slope_any(tof(row[id]), y);
-    const double q = exp(distill_logit<CAP>(p, tof(row[id])) - (double)lse * kLn2), P = exp((double)p.lps[n * p.K + k] - norm);
-    const float d = rest != rest ? rest : (float)((double)mass * q - P);
-    out[id] = cvt<E>(c * d * slope);
+    out[id] = cvt<E>(c * k.of_teacher(share(p.lps[n * p.K + i]), te(y - high)) * slope);
   }
 }
 

@@ -7,8 +7,9 @@
 // queries (dq, and D, which the other reads), one owns keys (dk and dv, over the query heads
 // that share them, so that their sums have a fixed order).  Each wave keeps the rows that it
 // owns as MFMA operands and accumulates in fp32; what it walks over is staged in LDS once
-// for both of its uses, by rows and by columns.  In bf16, P and dS enter their products in
-// bf16 (2^-9 of each).
+// for both of its uses, by rows and by columns.  In bf16, P and dS enter the keys' products
+// in bf16 (2^-9 of each, as the gradients' own rounding); the queries' takes dS in two parts: a
+// query's dS add to zero, so that of keys that are alike little is left but what rounding leaves.
 //
 // A sink is seen by every query behind its window: those pairs go to workgroups of their
 // own, a stretch of queries each, which leave sums of the sinks' rows in fp32; where workgroups are
@@ -120,14 +121,23 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
       }
 #pragma unroll
       for (int kp = 0; kp < 2; ++kp) {
-        f8 ds[NQ];
+        f8 ds[NQ], rest[NQ];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) ds[n] = IO::from_acc(s[n][2 * kp], s[n][2 * kp + 1]);
+        for (int n = 0; n < NQ; ++n) {
+          ds[n] = IO::from_acc(s[n][2 * kp], s[n][2 * kp + 1]);
+          if constexpr (sizeof(E) == 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rest[n][e] = (E)(s[n][2 * kp + (e >> 2)][e & 3] - tof(ds[n][e]));
+          }
+        }
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const f8 a = TF::get(kt, P, db * 16, kp, lane);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) acc[n][db] = mma32(a, ds[n], acc[n][db]);
+          for (int n = 0; n < NQ; ++n) {
+            acc[n][db] = mma32(a, ds[n], acc[n][db]);
+            if constexpr (sizeof(E) == 2) acc[n][db] = mma32(a, rest[n], acc[n][db]);
+          }
         }
       }
     }
