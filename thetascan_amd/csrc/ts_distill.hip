@@ -135,15 +135,22 @@ __device__ __forceinline__ double wave_sum(double x) {
   return half(x, [](float v) { return xor32_pair(v); });
 }
 
-// What a row's loss is formed from: x counts from the highest of all, hi.
+// A share, or an exponential of a distance from a maximum; what is no number stays none.
+__device__ __forceinline__ double distill_exp(const Exp64& e64, double t) { return t > -700.0 ? e64(t) : t == t ? 0.0 : t; }
+
+// What a row's loss is formed from: x counts from the highest of all, hi.  Teacher and student that are
+// near leave of these terms some 1e-3 of themselves or less, so they are fp64: the logarithm of the
+// sum is of the very distance dm, and the teacher's tokens' exponentials are of the distances in a.  (With the
+// whole sum in fp32, losses of 1.6e-3 were off by 2.8e-5 of themselves.)  What fp32 rounds in sr moves the
+// loss by Q_r - P_r times that.
 struct DistillTerms {
   double mass, a;   // sum P, sum P (lp - (x - hi))
-  float total;      // sum of all e^{x - hi}
+  double ek;        // sum of the teacher's tokens' e^{x - hi}
   float sr;         // the others' sum from their own maximum,
   double dm;        // and its distance from hi
 };
 __device__ __forceinline__ double distill_loss_of(const DistillP& p, const DistillTerms& t) {
-  const double lt = log((double)t.total);
+  const double lt = log(t.sr != 0.f ? t.ek + (double)t.sr * distill_exp(Exp64{kPowers64}, t.dm) : t.ek);
   if (!p.tail) return t.mass > 0.0 ? t.a / t.mass - log(t.mass) + lt : t.a;
   double loss = t.a + t.mass * lt;
   const double left = t.sr != 0.f ? 1.0 - t.mass : 0.0;
@@ -211,7 +218,7 @@ struct DistillIn {
 // The factors of a row's gradient: M, the teacher's sum without a tail (one over it), one over all
 // e^{x - hi}, and the others' factor of e^{x - their maximum}; no number where the row's loss is none.
 struct DistillFactors {
-  float mass, norm, inv, rest, total;
+  float mass, norm, inv, rest;
   __device__ __forceinline__ float of_teacher(double P, float q) const {
     return rest != rest ? rest : fmaf(mass * q, inv, -((float)P * norm));
   }
@@ -220,8 +227,7 @@ __device__ __forceinline__ DistillFactors distill_factors(const DistillP& p, dou
                                                           float down) {
   DistillFactors k;
   if (sr == 0.f) down = 0.f;  // of the others' maximum, e^{x - hi}
-  k.total = fmaf(sr, down, ek);
-  k.inv = rcp(k.total);
+  k.inv = rcp(fmaf(sr, down, ek));
   const double left = p.tail && sr != 0.f ? fmax(1.0 - mass, 0.0) : 0.0;
   k.mass = p.tail ? (float)(mass + left) : (mass > 0.0 ? 1.f : (float)mass);
   k.norm = p.tail ? 1.f : rcp((float)mass);
@@ -245,7 +251,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
   const float inv_t = (float)p.inv_t;
   const Exp64 e64{kPowers64};
   const TemperedExp te(p.inv_t);
-  DistillTerms mine{1.0, 0.0, 1.f, 0.f, 0.0};
+  DistillTerms mine{1.0, 0.0, 1.0, 0.f, 0.0};
   float mine_w = 0.f, mine_rest = 0.f, mine_hi = 0.f, mine_mr = 0.f, mine_inv = 0.f, mine_mass = 0.f;
   DistillIn<E, VPT, KS> in;
   float zn[KS];
@@ -343,24 +349,25 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
         all += (double)x;
         sl[r][e] = CAP ? x * sl[r][e] : x;
       }
-    double mass = 0.0, a = 0.0, ek = 0.0, P[KS];
+    double mass = 0.0, a = 0.0, ek = 0.0, near = 0.0, P[KS];
     float q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       P[s] = 0.0;
       q[s] = 0.f;
       if (id[s] >= 0) {
-        const float off = yk[s] - high;
+        const double off = ((double)yk[s] - (double)high) * p.inv_t;
         // (in fp64: one less their sum is what the teacher leaves to all others)
-        P[s] = lp[s] > -700.f ? e64((double)lp[s]) : lp[s] == lp[s] ? 0.0 : (double)lp[s];
-        q[s] = te(off);
-        ek += (double)q[s];
+        P[s] = distill_exp(e64, (double)lp[s]);
+        q[s] = te(yk[s] - high);
+        near += (double)q[s];
+        ek += distill_exp(e64, off);
         mass += P[s];
-        if (P[s] != 0.0) a += P[s] * ((double)lp[s] - (double)off * p.inv_t);
+        if (P[s] != 0.0) a += P[s] * ((double)lp[s] - off);
       }
     }
     if (bad) a = (double)NAN;
-    all = wave_sum(all - ek);  // the others: the very terms that the sum has of the teacher's tokens leave it
+    all = wave_sum(all - near);  // the others: the very terms that the sum has of the teacher's tokens leave it
     ek = wave_sum(ek);
     mass = wave_sum(mass);
     a = wave_sum(a);
@@ -399,7 +406,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
     }
     const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, te(most - high));
     if (li == rr) {
-      mine = DistillTerms{mass, a, k.total, sr, (double)(most - high) * p.inv_t};
+      mine = DistillTerms{mass, a, ek, sr, ((double)most - (double)high) * p.inv_t};
       mine_w = w;
       mine_rest = k.rest;
       mine_mr = most;
@@ -508,7 +515,7 @@ template <typename E, bool CAP, int THREADS, bool GRAD>
 __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   constexpr int N = Vec16<E>::N, WAVES = THREADS / 64, U = 2;
   extern __shared__ uint32_t marks[];
-  __shared__ double sm_a[WAVES], sm_mass[WAVES];
+  __shared__ double sm_a[WAVES], sm_mass[WAVES], sm_ek[WAVES];
   __shared__ float sm[3][WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = p.V, K = p.K;
   const int64_t n = blockIdx.x;
@@ -624,18 +631,16 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   // (no other token: any finite stand-in, their sum is zero)
   if (sr == 0.f) most = 0.f;
   const float high = sr == 0.f ? f.any(hz) : fmaxf(most, f.any(hz));
-  double mass = 0.0, a = 0.0;
-  float ek = 0.f;
-  auto share = [&](float lp) { return lp > -700.f ? e64((double)lp) : lp == lp ? 0.0 : (double)lp; };
+  double mass = 0.0, a = 0.0, ek = 0.0;
   for (int k = tid; k < K; k += THREADS) {
     const int64_t id = ids[k];
     if (id < 0 || id >= V) continue;
-    const float off = f.any(tof(row[id])) - high, lp = lps[k];
+    const double off = ((double)f.any(tof(row[id])) - (double)high) * p.inv_t, lp = (double)lps[k];
     // (in fp64: one less their sum is what the teacher leaves to all others)
-    const double P = share(lp);
-    ek += te(off);
+    const double P = distill_exp(e64, lp);
+    ek += distill_exp(e64, off);
     mass += P;
-    if (P != 0.0) a += P * ((double)lp - (double)off * p.inv_t);
+    if (P != 0.0) a += P * (lp - off);
   }
   if (bad) a = (double)NAN;
   ek = wave_sum(ek);
@@ -643,22 +648,21 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   a = wave_sum(a);
   __syncthreads();
   if (lane == 0) {
-    sm[0][wave] = ek;
+    sm_ek[wave] = ek;
     sm_mass[wave] = mass;
     sm_a[wave] = a;
   }
   __syncthreads();
-  ek = 0.f;
-  mass = a = 0.0;
+  mass = a = ek = 0.0;
 #pragma unroll
   for (int u = 0; u < WAVES; ++u) {
-    ek += sm[0][u];
+    ek += sm_ek[u];
     mass += sm_mass[u];
     a += sm_a[u];
   }
-  const DistillFactors k = distill_factors(p, mass, a, sr, ek, te(most - high));
+  const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, te(most - high));
   if (tid == 0) {
-    const double each = distill_loss_of(p, DistillTerms{mass, a, k.total, sr, (double)(most - high) * p.inv_t});
+    const double each = distill_loss_of(p, DistillTerms{mass, a, ek, sr, ((double)most - (double)high) * p.inv_t});
     p.each[n] = (float)each;
     p.part[n] = each * (double)w;
     if (p.stats) {
@@ -679,7 +683,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
       if (id < 0 || id >= V) continue;
       float y;
       const float slope = f.slope_any(tof(row[id]), y);
-      out[id] = cvt<E>(c * k.of_teacher(share(lps[i]), te(y - high)) * slope);
+      out[id] = cvt<E>(c * k.of_teacher(distill_exp(e64, (double)lps[i]), te(y - high)) * slope);
     }
   }
 }
@@ -716,7 +720,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillP p) {
   k.norm = 1.f;
   distill_others<E, CAP, LANES>(row, out, V, f, c * k.rest, te, most, li);
   // the teacher's tokens over those
-  auto share = [&](float lp) { return lp > -700.f ? e64((double)lp) : lp == lp ? 0.0 : (double)lp; };
+  auto share = [&](float lp) { return distill_exp(e64, (double)lp); };
   if (!p.tail) {
     double sum = 0.0;
     for (int i = li; i < p.K; i += LANES) {
