@@ -771,12 +771,11 @@ int setup(const ts_distill_desc* d, const ts_distill_io* io, DistillP* p) {
 }
 
 
-// Whether a wave holds a row in its registers, 32 logits a lane (a vector more than the row's bytes has
-// an unaligned one), and 256 of a teacher's tokens.
+// Whether a wave holds a row in its registers, `per` logits a lane (an unaligned row begins up to a vector
+// less one behind the boundary that they count from), and 256 of a teacher's tokens.
 constexpr int kPer = 32;
-bool in_registers(const DistillP& p, bool bf) {
-  return p.K <= 256 && p.V + (p.aligned ? 0 : (bf ? 8 : 4) - 1) <= 64 * kPer;
-}
+bool fits(const DistillP& p, bool bf, int per) { return p.V + (p.aligned ? 0 : (bf ? 8 : 4) - 1) <= 64 * per; }
+bool in_registers(const DistillP& p, bool bf) { return p.K <= 256 && fits(p, bf, kPer); }
 // Rows of a wave: several, where there are enough to keep every CU busy all the same.
 int rows_of(const DistillP& p) { return p.rows >= 16384 ? 8 : 1; }
 
@@ -798,10 +797,10 @@ int forward(const DistillP& p, hipStream_t stream) {
       TS_ROWS(VPT, 4, 1);
     else if (p.K > 64)
       TS_ROWS(VPT, 4, 8);
-    else if (p.V > 64 * kPer / 2)
-      TS_ROWS(VPT, 1, 8);
-    else
+    else if (fits(p, BF, kPer / 2))
       TS_ROWS(VPT / 2, 1, 8);
+    else
+      TS_ROWS(VPT, 1, 8);
 #undef TS_ROWS
     return TS_OK;
   }
