@@ -8,8 +8,8 @@ and ``P_k = exp(lp_k)``::
     loss = sum_n w_n [ sum_k P_k (lp_k - lq_k) + P_r (log P_r - log Q_r) ]
 
 ``P_r = 1 - sum_k P_k`` and ``Q_r`` are the teacher's and the student's share of all other
-tokens; without the tail, P is the softmax of the K log-probabilities and the second term
-is left out.  Where a gradient is recorded, the forward's launch gives it too, for a unit
+tokens; without the tail, P is the softmax of the K log-probabilities (which may be any scores)
+and the second term is left out.  Where a gradient is recorded, the forward's launch gives it too, for a unit
 upstream gradient (ts_distill_fwd): it is as large as the logits and held to the backward, as
 a saved tensor, which forms it again where the upstream gradient is another (as does a second
 backward of the same loss).  A loss whose value alone is wanted is called without gradients.  No
@@ -143,7 +143,8 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, log_probs: torch.Tenso
     tokens in any order, ``log_probs`` [..., K] their log-probabilities (at the same
     temperature).  An id below zero is no token; one at or past V, or twice in a row, makes
     the row's loss and gradient NaN.  ``tail`` False leaves all other tokens out.
-    ``weights`` [...] multiplies each row's loss (default: the mean over all rows); a row of
+    A log-probability of -inf is a share of zero; without the tail, a row of none but those has no
+    softmax and is NaN.  ``weights`` [...] multiplies each row's loss (default: the mean over all rows); a row of
     weight zero may hold anything in any input, and gives zero and a gradient of zero.
     ``softcap`` caps the logits at ``softcap tanh(z / softcap)``, before the temperature.
     At most 2^24 - 1 rows a call.  Forward-mode and second derivatives are refused.

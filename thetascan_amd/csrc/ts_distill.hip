@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
       }
     wave_lds_sync();
     // the capped logits and their slopes, the highest, and the sum of all
-    float y[VPT][N], sl[VPT][N], yk[KS], slk[KS], hz = -INFINITY;
+    float y[VPT][N], sl[VPT][N], yk[KS], slk[KS], hz = -INFINITY, hl = 0.f;
 #pragma unroll
     for (int r = 0; r < VPT; ++r) {
       if (f.some_far(v[r])) {
@@ -339,6 +339,12 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) slk[s] = f.slope_any(zk[s], yk[s]);
+    if (!p.tail) {  // (uniform) shares of the named tokens alone, from the highest
+      hl = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) hl = id[s] >= 0 ? fmaxf(hl, lp[s]) : hl;
+      hl = wave_most(hl);
+    }
     const float high = wave_most(hz);
     double all = 0.0;
 #pragma unroll
@@ -356,14 +362,14 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
       P[s] = 0.0;
       q[s] = 0.f;
       if (id[s] >= 0) {
-        const double off = ((double)yk[s] - (double)high) * p.inv_t;
+        const double off = ((double)yk[s] - (double)high) * p.inv_t, lps = (double)lp[s] - (double)hl;
         // (in fp64: one less their sum is what the teacher leaves to all others)
-        P[s] = distill_exp(e64, (double)lp[s]);
+        P[s] = distill_exp(e64, lps);
         q[s] = te(yk[s] - high);
         near += (double)q[s];
         ek += distill_exp(e64, off);
         mass += P[s];
-        if (P[s] != 0.0) a += P[s] * ((double)lp[s] - off);
+        if (P[s] != 0.0) a += P[s] * (lps - off);
       }
     }
     if (bad) a = (double)NAN;
@@ -516,7 +522,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   constexpr int N = Vec16<E>::N, WAVES = THREADS / 64, U = 2;
   extern __shared__ uint32_t marks[];
   __shared__ double sm_a[WAVES], sm_mass[WAVES], sm_ek[WAVES];
-  __shared__ float sm[3][WAVES];
+  __shared__ float sm[4][WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = p.V, K = p.K;
   const int64_t n = blockIdx.x;
   const float w = p.w ? p.w[n] : 1.f / (float)p.rows;
@@ -550,7 +556,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   for (int i = tid; i < (vecs * N + 31) / 32; i += THREADS) marks[i] = 0;
   __syncthreads();
   bool bad = false;
-  float hz = -INFINITY;
+  float hz = -INFINITY, hl = -INFINITY;
   for (int k = tid; k < K; k += THREADS) {
     const int64_t id = ids[k];
     if (id >= V) bad = true;
@@ -558,6 +564,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
     const uint32_t bit = (uint32_t)(id + shift);
     bad |= atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u;
     hz = fmaxf(hz, tof(row[id]));
+    hl = fmaxf(hl, lps[k]);
   }
   __syncthreads();
   // the others
@@ -612,10 +619,12 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
     const float top = wave_most(most);
     sr = wave_sum(sr * te(most - top));
     hz = wave_most(hz);
+    hl = wave_most(hl);
     if (lane == 0) {
       sm[0][wave] = top;
       sm[1][wave] = sr;
       sm[2][wave] = hz;
+      sm[3][wave] = hl;
     }
     __syncthreads();
     most = kLowest;
@@ -623,7 +632,9 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
     for (int u = 0; u < WAVES; ++u) {
       most = fmaxf(most, sm[0][u]);
       hz = fmaxf(hz, sm[2][u]);
+      hl = fmaxf(hl, sm[3][u]);
     }
+    if (p.tail) hl = 0.f;
     sr = 0.f;
 #pragma unroll
     for (int u = 0; u < WAVES; ++u) sr = fmaf(sm[1][u], te(sm[0][u] - most), sr);
@@ -635,7 +646,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
   for (int k = tid; k < K; k += THREADS) {
     const int64_t id = ids[k];
     if (id < 0 || id >= V) continue;
-    const double off = ((double)f.any(tof(row[id])) - (double)high) * p.inv_t, lp = (double)lps[k];
+    const double off = ((double)f.any(tof(row[id])) - (double)high) * p.inv_t, lp = (double)lps[k] - (double)hl;
     // (in fp64: one less their sum is what the teacher leaves to all others)
     const double P = distill_exp(e64, lp);
     ek += distill_exp(e64, off);
@@ -683,7 +694,7 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
       if (id < 0 || id >= V) continue;
       float y;
       const float slope = f.slope_any(tof(row[id]), y);
-      out[id] = cvt<E>(c * k.of_teacher(distill_exp(e64, (double)lps[i]), te(y - high)) * slope);
+      out[id] = cvt<E>(c * k.of_teacher(distill_exp(e64, (double)lps[i] - (double)hl), te(y - high)) * slope);
     }
   }
 }
@@ -720,8 +731,15 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillP p) {
   k.norm = 1.f;
   distill_others<E, CAP, LANES>(row, out, V, f, c * k.rest, te, most, li);
   // the teacher's tokens over those
-  auto share = [&](float lp) { return distill_exp(e64, (double)lp); };
+  double top = 0.0;
+  auto share = [&](float lp) { return distill_exp(e64, (double)lp - top); };
   if (!p.tail) {
+    float hl = -INFINITY;
+    for (int i = li; i < p.K; i += LANES) {
+      const int64_t id = p.ids[n * p.K + i];
+      if (id >= 0 && id < V) hl = fmaxf(hl, p.lps[n * p.K + i]);
+    }
+    top = (double)team.most(hl);
     double sum = 0.0;
     for (int i = li; i < p.K; i += LANES) {
       const int64_t id = p.ids[n * p.K + i];
