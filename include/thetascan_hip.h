@@ -1442,7 +1442,8 @@ int ts_sample_tokens(const ts_sample_desc* desc, const ts_sample_io* io, hipStre
 /* Rows of logits z (element stride `stride`), x = cap tanh(z / cap) / temperature (cap 0: z /
  * temperature), lq = log softmax(x), against K of a teacher's tokens with their log-probabilities:
  *   tail:  P_k = exp(lp_k), P_r = max(0, 1 - sum P_k), Q_r the student's share of all other tokens
- *          loss = sum_n w [ sum_k P_k (lp_k - lq_k) + P_r (log P_r - log Q_r) ]
+ *          loss = sum_n w [ sum_k P_k (lp_k - lq_k) + P_r (log P_r - log Q_r) ], without the second term
+ *          where all other tokens' logits are -inf (Q_r = 0)
  *   else:  P = softmax(lp) (any scores);  loss = sum_n w sum_k P_k (log P_k - lq_k)
  * An id below zero is no token; one at or past V, or twice in a row, makes its row NaN.  A row of
  * weight zero is not read. */

@@ -153,6 +153,8 @@ __device__ __forceinline__ double distill_loss_of(const DistillP& p, const Disti
   const double lt = log(t.sr != 0.f ? t.ek + (double)t.sr * distill_exp(Exp64{kPowers64}, t.dm) : t.ek);
   if (!p.tail) return t.mass > 0.0 ? t.a / t.mass - log(t.mass) + lt : t.a;
   double loss = t.a + t.mass * lt;
+  // (the student has no other token, or forbids them all: 1 - mass may be the rounding of what teacher and
+  // student both forbid, so it is no share there)
   const double left = t.sr != 0.f ? 1.0 - t.mass : 0.0;
   if (left > 0.0) loss += left * (log(left) - t.dm - log((double)t.sr) + lt);
   return loss + 0.0 * left;  // (a share that is no number)
