@@ -74,3 +74,33 @@ def test_small_losses_have_their_digits(cuda, N, V, K, temperature, cap, tail, s
     # with the gradient beside it, the same
     leaf = z.requires_grad_()
     assert torch.equal(ts.distill_loss(leaf, ids, lps, temperature=temperature, softcap=cap, tail=tail)[1], each)
+
+
+@pytest.mark.parametrize("N,V,K,temperature", [(600, 1024, 32, 1.0), (600, 2048, 200, 2.0), (20000, 1024, 32, 2.0),
+                                               (20000, 1999, 100, 1.0), (512, 32768, 64, 2.0), (64, 50257, 64, 1.0)])
+@pytest.mark.parametrize("spread", [0.5, 0.02])
+def test_the_others_gradients_have_their_digits(cuda, N, V, K, temperature, spread):
+    """q (1 - P_r / Q_r) of the tokens that are none of the teacher's: an exponential's own error (as above, with
+    eight 2^-24 for the products and the result), and of P_r / Q_r what the others' sum is off by: a sum by 256
+    lanes or more of fp32 terms, whose independent errors average out over the lanes (V / 2^16 of 2^-48), and
+    eight additions of the lanes' sums; rows of up to 2048 are summed in fp64.  Four times that."""
+    import thetascan_amd as ts
+
+    g = torch.Generator(device=cuda).manual_seed(V + K)
+    z = (2.5 * torch.randn(N, V, generator=g, device=cuda)).requires_grad_()
+    y = (z.detach().double() + spread * torch.randn(N, V, generator=g, device=cuda)) / temperature
+    lps, ids = torch.log_softmax(y, -1).topk(K, -1)
+    lps = lps.float()
+    (dz,) = torch.autograd.grad(ts.distill_loss(z, ids, lps, temperature=temperature)[0], z)
+    x = z.detach().double() / temperature
+    q = torch.softmax(x, -1).scatter_(-1, ids, 0.0)
+    Q, left = q.sum(-1, keepdim=True), (1.0 - lps.double().exp().sum(-1, keepdim=True)).clamp(min=0.0)
+    ratio = left / Q
+    own = ((x - x.amax(-1, keepdim=True)).abs() + 8.0).square() * (1.0 - ratio).square()
+    own += ratio.square() * ((V / 65536 + 8) if V > 2048 else 1.0)
+    square = (q * 2.0 ** -24).square() * own
+    err = torch.where(q > 0, N * temperature * dz.double() - q * (1.0 - ratio), 0.0)
+    size = float((q * (1.0 - ratio)).square().sum().sqrt())
+    err, bar = float(err.square().sum().sqrt()), 4.0 * float(square.sum().sqrt())
+    print(f"off by {err / size:.1e} of them; {err / bar:.3f} of the bar", flush=True)
+    assert err <= bar

@@ -225,15 +225,18 @@ struct DistillFactors {
     return rest != rest ? rest : fmaf(mass * q, inv, -((float)P * norm));
   }
 };
-__device__ __forceinline__ DistillFactors distill_factors(const DistillP& p, double mass, double a, float sr, float ek,
-                                                          float down) {
+// (down: of the others' maximum, e^{x - hi}.)  The others' factor M e^{..} / total - P_r / sr is one
+// difference, mass down sr - left ek over total sr: what cancels there, as the student comes near the
+// teacher, is fp64.
+__device__ __forceinline__ DistillFactors distill_factors(const DistillP& p, double mass, double a, double sr, double ek,
+                                                          double down) {
   DistillFactors k;
-  if (sr == 0.f) down = 0.f;  // of the others' maximum, e^{x - hi}
-  k.inv = rcp(fmaf(sr, down, ek));
-  const double left = p.tail && sr != 0.f ? fmax(1.0 - mass, 0.0) : 0.0;
+  if (sr == 0.0) down = 0.0;
+  const double from = down * sr, left = p.tail && sr != 0.0 ? fmax(1.0 - mass, 0.0) : 0.0;
+  k.inv = rcp((float)(from + ek));
   k.mass = p.tail ? (float)(mass + left) : (mass > 0.0 ? 1.f : (float)mass);
   k.norm = p.tail ? 1.f : rcp((float)mass);
-  k.rest = sr != 0.f ? fmaf(k.mass * down, k.inv, -((float)left * rcp(sr))) : 0.f;
+  k.rest = sr != 0.0 ? (float)(p.tail ? mass * from - left * ek : k.mass * from) * k.inv * rcp((float)sr) : 0.f;
   if (!(a == a)) k.rest = NAN;
   return k;
 }
@@ -379,11 +382,12 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
     ek = wave_sum(ek);
     mass = wave_sum(mass);
     a = wave_sum(a);
-    float most = high, sr = (float)all;
+    float most = high;
+    double sr = all, down = 1.0;
     if (!(all > ek * 0x1p-28)) {
       // (uniform) next to nothing is left: from the others' own maximum, the teacher's tokens masked
       float mz = -INFINITY;
-      sr = 0.f;
+      float rest = 0.f;
 #pragma unroll
       for (int r = 0; r < VPT; ++r) {
         const int j = li + r * LANES;
@@ -402,7 +406,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float x = te(y[r][e] - most);
-          sr += x;
+          rest += x;
           if (CAP && x != 0.f) {
             float unused;
             sl[r][e] = x * f.slope_any(tof(v[r].e[e]), unused);
@@ -410,11 +414,12 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
             sl[r][e] = x;
           }
         }
-      sr = wave_sum(sr);
+      sr = (double)wave_sum(rest);
+      down = distill_exp(e64, ((double)most - (double)high) * p.inv_t);
     }
-    const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, te(most - high));
+    const DistillFactors k = distill_factors(p, mass, a, sr, ek, down);
     if (li == rr) {
-      mine = DistillTerms{mass, a, ek, sr, ((double)most - (double)high) * p.inv_t};
+      mine = DistillTerms{mass, a, ek, (float)sr, 0.0};
       mine_w = w;
       mine_rest = k.rest;
       mine_mr = most;
@@ -446,6 +451,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
   double term = 0.0;
   const int64_t n = row0 + li;
   if (li < R && n < p.rows) {
+    mine.dm = ((double)mine_mr - (double)mine_hi) * p.inv_t;
     const double each = mine_w != 0.f ? distill_loss_of(p, mine) : 0.0;
     term = mine_w != 0.f ? each * (double)mine_w : 0.0;
     p.each[n] = (float)each;
@@ -673,9 +679,10 @@ __global__ __launch_bounds__(THREADS) void distill_long_kernel(DistillP p) {
     mass += sm_mass[u];
     a += sm_a[u];
   }
-  const DistillFactors k = distill_factors(p, mass, a, sr, (float)ek, te(most - high));
+  const double dm = ((double)most - (double)high) * p.inv_t;
+  const DistillFactors k = distill_factors(p, mass, a, sr, ek, distill_exp(e64, dm));
   if (tid == 0) {
-    const double each = distill_loss_of(p, DistillTerms{mass, a, ek, sr, ((double)most - (double)high) * p.inv_t});
+    const double each = distill_loss_of(p, DistillTerms{mass, a, ek, sr, dm});
     p.each[n] = (float)each;
     p.part[n] = each * (double)w;
     if (p.stats) {
