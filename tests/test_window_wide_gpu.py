@@ -99,3 +99,14 @@ def test_what_is_not_finite_reaches_who_sees_it_alone(cuda, B, H, Hk, T, d, bad)
                 assert torch.allclose(out[0, h][free], clean[0, h][free], rtol=2 * U[dtype] + 1e-5, atol=2e-2)
                 if name == "v":
                     assert torch.equal(~torch.isfinite(out[0, h, :, 5]), seen[:, at])
+
+
+@pytest.mark.parametrize("B,H,Hk,T,d,sinks", [(16, 8, 8, 1300, 64, 1100), (16, 16, 8, 1300, 16, 700), (4, 8, 8, 1300, 128, 1200),
+                                              (1, 8, 2, 2100, 64, 1500)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_sinks(cuda, B, H, Hk, T, d, sinks, dtype):
+    """So many of them that their queries are not cut into stretches, or into few."""
+    q, k, v, do = inputs(B, H, Hk, T, d, dtype, T + d)
+    want, bars = reference(*(x[-1:] for x in (q, k, v, do)), 20, sinks)
+    for name, x, y, bar in zip(("out", "dq", "dk", "dv"), run(cuda, q, k, v, do, window=20, sinks=sinks), want, bars):
+        close(name, x[-1:], y, bar)

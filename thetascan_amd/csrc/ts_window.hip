@@ -262,6 +262,8 @@ bool window_narrow(const WinP& p, int B, bool bf, int heads) {
   return !bf || (int64_t)B * heads * ((p.T + 127) / 128) < 256;
 }
 
+int window_bwd_takes(const ts_window_desc* d, WinP p);
+
 template <typename E, int D, int NQ>
 static int window_fwd(const WinP& p, int B, hipStream_t stream) {
   const int lds = 4 * TT * win_pitch<E, D>() * (int)sizeof(E);
@@ -286,8 +288,10 @@ extern "C" {
 int ts_window_attention_fwd(const ts_window_desc* d, const ts_window_io* io, hipStream_t stream) {
   ts::WinP p;
   if (!io) return ts::fail(TS_ERR_VALUE, "window attention: missing tensors");
-  const int rc = ts::window_setup(d, io, &p);
+  int rc = ts::window_setup(d, io, &p);
   if (rc || d->T == 0) return rc;
+  // (kept for a backward: what that refuses is refused here)
+  if (io->lse && (rc = ts::window_bwd_takes(d, p))) return rc;
   const bool bf = d->dtype == TS_BF16;
   return d->d <= 64 ? ts::window_fwd<64>(p, d->B, bf, stream) : ts::window_fwd<128>(p, d->B, bf, stream);
 }

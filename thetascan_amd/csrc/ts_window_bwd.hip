@@ -381,7 +381,10 @@ static WinSplit window_split(const ts_window_desc* d, WinP* p) {
   if (p->sinks > 0 && behind > 0) {
     const int tiles = (behind + TT - 1) / TT + 1;
     p->far_tiles = (p->sinks + keys - 1) / keys;
-    p->chunk_tiles = max(apart ? 4 : 16, (tiles + 63) / 64);
+    // Stretches only until every CU has several workgroups: each leaves sums of all the sinks' rows (8192
+    // sinks of 32 heads of 64 in 31 stretches of 32768 queries were 4.4 GB, in one they are 0.3)
+    const int64_t groups = (int64_t)d->B * p->owners * p->far_tiles, most = groups < 2048 ? 2048 / groups : 1;
+    p->chunk_tiles = max(max(apart ? 4 : 16, (tiles + 63) / 64), (int)((tiles + most - 1) / most));
     p->chunks = (tiles + p->chunk_tiles - 1) / p->chunk_tiles;
   }
   WinSplit s;
@@ -389,6 +392,18 @@ static WinSplit window_split(const ts_window_desc* d, WinP* p) {
   s.rows = apart ? (size_t)d->B * d->H * d->T * 2 * d->d * 4 : 0;
   s.part = p->chunks ? (size_t)d->B * p->owners * (p->chunks + 1) * p->sinks * 2 * d->d * 4 : 0;
   return s;
+}
+
+// Whether the backward takes a call: the forward that keeps what it needs asks too.
+static int window_bwd_fits(const WinP& p) {
+  // (a launch counts its rows of workgroups in 16 bits)
+  if ((int64_t)p.near_tiles + (int64_t)p.far_tiles * p.chunks > 65535 || (int64_t)p.sinks * p.d / 2 > 65535 * 256)
+    return fail(TS_ERR_NOT_IMPLEMENTED, "window attention bwd: too many tokens or sinks");
+  return TS_OK;
+}
+int window_bwd_takes(const ts_window_desc* d, WinP p) {
+  window_split(d, &p);
+  return window_bwd_fits(p);
 }
 
 template <typename E, int D, int NQ, int NK>
@@ -426,9 +441,10 @@ extern "C" {
 
 int ts_window_attention_bwd_workspace_bytes(const ts_window_desc* d, size_t* bytes) {
   ts::WinP p;
-  const int rc = ts::window_setup(d, nullptr, &p);
+  int rc = ts::window_setup(d, nullptr, &p);
   if (rc) return rc;
   const size_t n = ts::window_split(d, &p).all();
+  if ((rc = ts::window_bwd_fits(p))) return rc;
   if (bytes) *bytes = n;
   return TS_OK;
 }
@@ -446,8 +462,7 @@ int ts_window_attention_bwd(const ts_window_desc* d, const ts_window_io* io, con
   const ts::WinSplit need = ts::window_split(d, &p);
   if (!workspace || ((uintptr_t)workspace & 15u) || workspace_bytes < need.all())
     return ts::fail(TS_ERR_VALUE, "window attention bwd: workspace of %zu bytes, 16-byte aligned", need.all());
-  if ((int64_t)p.near_tiles + (int64_t)p.far_tiles * p.chunks > 65535 || (int64_t)p.sinks * d->d / 2 > 65535 * 256)
-    return ts::fail(TS_ERR_NOT_IMPLEMENTED, "window attention bwd: too many sinks");
+  if ((rc = ts::window_bwd_fits(p))) return rc;
   p.dout = grads->dout; p.dq = grads->dq; p.dk = grads->dk; p.dv = grads->dv;
   char* work = (char*)workspace;
   p.delta = (float*)work;
