@@ -8,9 +8,8 @@ ts_window_attention_bwd), and single tokens against a cache of fixed size
 (ts_window_step), a ring of ``window`` slots behind those of the sinks.
 
 bf16 inputs: products take bf16 operands (the probabilities and their gradients rounded
-once) and fp32 sums; fp32 inputs compute in fp32.  A key or value that is not finite
-reaches no output that does not see it; gradients have it in every key and query within 64
-tokens of those that do.
+once) and fp32 sums; fp32 inputs compute in fp32.  A value that is not finite reaches the
+outputs and gradients alone that its formula has it in.
 """
 from __future__ import annotations
 

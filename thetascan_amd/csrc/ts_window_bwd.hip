@@ -15,16 +15,37 @@
 // own, a stretch of queries each, which leave sums of the sinks' rows in fp32; where workgroups are
 // few, the query heads that share a key head have workgroups (and sums) of their own.  A third
 // kernel adds the sums in order.  In bf16, D takes out with what its rounding left of it.
+//
+// A hidden pair's zero times a key or a query that is not finite would be no number: where a workgroup's
+// sums are not finite, it goes over its tiles again and adds only the pairs that there are, as the forward.
 
 #include "ts_window.h"
 
 #include <string.h>
+#include <type_traits>
 
 namespace ts {
 
 int window_setup(const ts_window_desc* d, const ts_window_io* io, WinP* p);
 int window_rows(const ts_strided& s, int vec);
 bool window_narrow(const WinP& p, int B, bool bf, int heads);
+
+// Whether a lane's sums are not all finite (a sum of magnitudes is where all are, or where none is near
+// the border of its type).
+template <int N, int DB>
+__device__ __forceinline__ bool win_odd(const floatx4 (&acc)[N][DB]) {
+  bool odd = false;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float all = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all += fabsf(acc[n][db][i]);
+    odd |= !(all < INFINITY);
+  }
+  return odd;
+}
 
 // A wave owns 16 NQ queries.
 template <typename E, int D, int NQ>
@@ -67,11 +88,15 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
     del[n] = sum_g(s);
     lse[n] = on ? p.lse[row0 + t] : INFINITY;
     if (g == 0 && t < p.T) p.delta[row0 + t] = del[n];
-#pragma unroll
-    for (int db = 0; db < DB; ++db) acc[n][db] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  if (q0 < len) {
+  auto pass = [&](auto careful) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[n][db] = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (q0 >= len) return;
     const WinTiles tiles(q0, min(q0 + QT, len), p.window, p.sinks);
     WinTile<E, D> kr, vr;
     kr.init(p.k.st, d, tid);
@@ -119,6 +144,25 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
             s[n][kf][e] = hidden ? 0.f : s[n][kf][e];
           });
       }
+      if constexpr (CAREFUL) {
+        for (int gg = 0; gg < 4; ++gg)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int kf = 0; kf < 4; ++kf)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float x = __shfl(s[n][kf][i], gg * 16 + l16, 64);
+                const int key = kf * 16 + 4 * gg + i;
+                if (!win_hidden(qw + 16 * n + l16, k0 + key, p.window, p.sinks))
+#pragma unroll
+                  for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      acc[n][db][e] = fmaf(x, tof(kt[key * P + db * 16 + 4 * g + e]), acc[n][db][e]);
+              }
+        continue;
+      }
 #pragma unroll
       for (int kp = 0; kp < 2; ++kp) {
         f8 ds[NQ], rest[NQ];
@@ -141,7 +185,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
         }
       }
     }
-  }
+  };
+  pass(std::false_type{});
+  if (__syncthreads_or(win_odd<NQ, DB>(acc))) pass(std::true_type{});
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int t = qw + 16 * n + l16;
@@ -163,7 +209,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 1) void w
 // them, or query heads); blockIdx.y: the key tiles over the queries of their window, then the sinks'
 // tiles over the queries behind it, a stretch of chunk_tiles query tiles each.
 template <typename E, int D, int NK>
-__global__ __launch_bounds__(256, sizeof(E) == 2 ? 2 : 1) void window_dkv_kernel(WinP p) {
+__global__ __launch_bounds__(256, sizeof(E) == 2 ? (D * NK == 64 ? 4 : 2) : 1) void window_dkv_kernel(WinP p) {
   typedef LdsIO<E> IO;
   typedef TokFrag<E> TF;
   typedef typename Frag<E>::f8 f8;
@@ -203,100 +249,131 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? 2 : 1) void window_dkv_kernel
       kf[n][kk] = win_row8(k, 32 * kk + 8 * g, d, t < len);
       vf[n][kk] = win_row8(v, 32 * kk + 8 * g, d, t < len);
     }
-#pragma unroll
-    for (int db = 0; db < DB; ++db) dk[n][db] = dv[n][db] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  WinTile<E, D> qr, dr;
-  qr.init(p.q.st, d, tid);
-  dr.init(p.dout.st, d, tid);
-  float lr = INFINITY, er = 0.f;
-  int at_h = h0, at_t = t0;  // of the tile on its way
-  auto fetch = [&]() {
-    const int q0 = at_t * TT;
-    qr.fetch((const E*)p.q.ptr + b * p.q.sb + at_h * p.q.sh, p.q.st, q0, len);
-    dr.fetch((const E*)p.dout.ptr + b * p.dout.sb + at_h * p.dout.sh, p.dout.st, q0, len);
-    if (tid < TT) {
-      const bool on = q0 + tid < len;
-      const int64_t at = ((int64_t)b * p.H + at_h) * p.T + q0 + tid;
-      lr = on ? p.lse[at] : INFINITY;  // (no query: its probabilities are zero)
-      er = on ? p.delta[at] : 0.f;
-    }
-  };
-  if (total) fetch();
-  for (int it = 0; it < total; ++it) {
-    const int q0 = at_t * TT;
-    if (it) __syncthreads();  // the last tile is read
-    qr.store(qt);
-    dr.store(ot);
-    if (tid < TT) {
-      ls[tid] = lr;
-      dl[tid] = er;
-    }
-    if (++at_t == t0 + per_head) {
-      at_t = t0;
-      ++at_h;
-    }
-    if (it + 1 < total) fetch();
-    __syncthreads();
-    // wave-uniform: none of these queries sees a key here, or all of them all
-    const int q1 = q0 + TT - 1, k1 = kw + WK - 1;
-    if (far ? kw >= p.sinks || q1 - kw < p.window : kw > q1 || q0 - k1 >= p.window) continue;
-    const bool some = far ? k1 >= p.sinks || q0 - k1 < p.window : k1 > q0 || q1 - kw >= p.window;
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
-    for (int qp = 0; qp < 2; ++qp) {
-      floatx4 s[NK][2], dp[NK][2];
+    for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const int qf = 2 * qp + f;
+      for (int db = 0; db < DB; ++db) dk[n][db] = dv[n][db] = floatx4{0.f, 0.f, 0.f, 0.f};
+    WinTile<E, D> qr, dr;
+    qr.init(p.q.st, d, tid);
+    dr.init(p.dout.st, d, tid);
+    float lr = INFINITY, er = 0.f;
+    int at_h = h0, at_t = t0;  // of the tile on its way
+    auto fetch = [&]() {
+      const int q0 = at_t * TT;
+      qr.fetch((const E*)p.q.ptr + b * p.q.sb + at_h * p.q.sh, p.q.st, q0, len);
+      dr.fetch((const E*)p.dout.ptr + b * p.dout.sb + at_h * p.dout.sh, p.dout.st, q0, len);
+      if (tid < TT) {
+        const bool on = q0 + tid < len;
+        const int64_t at = ((int64_t)b * p.H + at_h) * p.T + q0 + tid;
+        lr = on ? p.lse[at] : INFINITY;  // (no query: its probabilities are zero)
+        er = on ? p.delta[at] : 0.f;
+      }
+    };
+    if (total) fetch();
+    for (int it = 0; it < total; ++it) {
+      const int q0 = at_t * TT;
+      if (it) __syncthreads();  // the last tile is read
+      qr.store(qt);
+      dr.store(ot);
+      if (tid < TT) {
+        ls[tid] = lr;
+        dl[tid] = er;
+      }
+      if (++at_t == t0 + per_head) {
+        at_t = t0;
+        ++at_h;
+      }
+      if (it + 1 < total) fetch();
+      __syncthreads();
+      // wave-uniform: none of these queries sees a key here, or all of them all
+      const int q1 = q0 + TT - 1, k1 = kw + WK - 1;
+      if (far ? kw >= p.sinks || q1 - kw < p.window : kw > q1 || q0 - k1 >= p.window) continue;
+      const bool some = far ? k1 >= p.sinks || q0 - k1 < p.window : k1 > q0 || q1 - kw >= p.window;
 #pragma unroll
-        for (int n = 0; n < NK; ++n) s[n][f] = dp[n][f] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int qp = 0; qp < 2; ++qp) {
+        floatx4 s[NK][2], dp[NK][2];
 #pragma unroll
-        for (int kk = 0; kk < KB; ++kk) {
-          const f8 a = IO::ld8(qt + (qf * 16 + l16) * P + 32 * kk + 8 * g);
-          const f8 c = IO::ld8(ot + (qf * 16 + l16) * P + 32 * kk + 8 * g);
+        for (int f = 0; f < 2; ++f) {
+          const int qf = 2 * qp + f;
+#pragma unroll
+          for (int n = 0; n < NK; ++n) s[n][f] = dp[n][f] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < KB; ++kk) {
+            const f8 a = IO::ld8(qt + (qf * 16 + l16) * P + 32 * kk + 8 * g);
+            const f8 c = IO::ld8(ot + (qf * 16 + l16) * P + 32 * kk + 8 * g);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+              s[n][f] = mma32(a, kf[n][kk], s[n][f]);
+              dp[n][f] = mma32(c, vf[n][kk], dp[n][f]);
+            }
+          }
+          const floatx4 l4 = *(const floatx4*)(ls + qf * 16 + 4 * g), d4 = *(const floatx4*)(dl + qf * 16 + 4 * g);
 #pragma unroll
           for (int n = 0; n < NK; ++n) {
-            s[n][f] = mma32(a, kf[n][kk], s[n][f]);
-            dp[n][f] = mma32(c, vf[n][kk], dp[n][f]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[n][f][i] = __builtin_amdgcn_exp2f(fmaf(s[n][f][i], p.scale2, -l4[i]));
+              dp[n][f][i] -= d4[i];
+            }
+            if (some) {
+              // the distance of query i from this lane's key is c + i
+              const int key = kw + 16 * n + l16, c = q0 + qf * 16 + 4 * g - key;
+              const uint32_t from = far && key >= p.sinks ? 0x7fffffffu : least;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[n][f][i] = (uint32_t)(c + i) - from < span ? s[n][f][i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[n][f][i] *= s[n][f][i];
           }
         }
-        const floatx4 l4 = *(const floatx4*)(ls + qf * 16 + 4 * g), d4 = *(const floatx4*)(dl + qf * 16 + 4 * g);
+        if constexpr (CAREFUL) {
+#pragma unroll 1
+          for (int gg = 0; gg < 4; ++gg)
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
+            for (int n = 0; n < NK; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[n][f][i] = __builtin_amdgcn_exp2f(fmaf(s[n][f][i], p.scale2, -l4[i]));
-            dp[n][f][i] -= d4[i];
-          }
-          if (some) {
-            // the distance of query i from this lane's key is c + i
-            const int key = kw + 16 * n + l16, c = q0 + qf * 16 + 4 * g - key;
-            const uint32_t from = far && key >= p.sinks ? 0x7fffffffu : least;
+              for (int f = 0; f < 2; ++f)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][f][i] = (uint32_t)(c + i) - from < span ? s[n][f][i] : 0.f;
-          }
+                for (int i = 0; i < 4; ++i) {
+                  const float x = __shfl(s[n][f][i], gg * 16 + l16, 64), y = __shfl(dp[n][f][i], gg * 16 + l16, 64);
+                  const int row = (2 * qp + f) * 16 + 4 * gg + i, key = kw + 16 * n + l16;
+                  const uint32_t from = far && key >= p.sinks ? 0x7fffffffu : least;
+                  if (q0 + row < len && (uint32_t)(q0 + row - key) - from < span)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dp[n][f][i] *= s[n][f][i];
+                    for (int db = 0; db < DB; ++db)
+#pragma unroll
+                      for (int e = 0; e < 4; ++e) {
+                        dv[n][db][e] = fmaf(x, tof(ot[row * P + db * 16 + 4 * g + e]), dv[n][db][e]);
+                        dk[n][db][e] = fmaf(y, tof(qt[row * P + db * 16 + 4 * g + e]), dk[n][db][e]);
+                      }
+                }
+          continue;
         }
-      }
-      f8 pf[NK], ef[NK];
-#pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        pf[n] = IO::from_acc(s[n][0], s[n][1]);
-        ef[n] = IO::from_acc(dp[n][0], dp[n][1]);
-      }
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const f8 a = TF::get(ot, P, db * 16, qp, lane), c = TF::get(qt, P, db * 16, qp, lane);
+        f8 pf[NK], ef[NK];
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
-          dv[n][db] = mma32(a, pf[n], dv[n][db]);
-          dk[n][db] = mma32(c, ef[n], dk[n][db]);
+          pf[n] = IO::from_acc(s[n][0], s[n][1]);
+          ef[n] = IO::from_acc(dp[n][0], dp[n][1]);
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const f8 a = TF::get(ot, P, db * 16, qp, lane), c = TF::get(qt, P, db * 16, qp, lane);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            dv[n][db] = mma32(a, pf[n], dv[n][db]);
+            dk[n][db] = mma32(c, ef[n], dk[n][db]);
+          }
         }
       }
     }
-  }
+  };
+  pass(std::false_type{});
+  const bool odd = win_odd<NK, DB>(dk) | win_odd<NK, DB>(dv);
+  if (__builtin_expect(__syncthreads_or(odd), 0)) pass(std::true_type{});
   const int64_t bo = (int64_t)b * p.owners + own;
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
