@@ -1,0 +1,110 @@
+"""Windowed attention, distillation and generation in the uses that their documents allow: saved tensors
+offloaded or formed again, a backward captured without its forward, autocast."""
+from __future__ import annotations
+
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from tests.test_distill_gpu import teacher
+from tests.test_generation_gpu import _model
+from tests.test_window_gpu import inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d", [64, 20])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_offloaded_and_checkpointed(cuda, d, dtype):
+    import thetascan_amd as ts
+
+    q, k, v, do = (x.to(cuda) for x in inputs(2, 4, 2, 150, d, dtype))
+    lengths = torch.tensor([150, 77], device=cuda)
+
+    def f(q, k, v):
+        return ts.windowed_attention(q, k, v, window=40, sinks=2, lengths=lengths)
+
+    def grads(g, **kw):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        out = g(*leaves, **kw)
+        return [out, *torch.autograd.grad(out, leaves, do)]
+
+    base = grads(f)
+    again = grads(lambda *x: checkpoint(f, *x, use_reentrant=False))
+    with torch.autograd.graph.save_on_cpu():
+        offloaded = grads(f)
+    for got in (again, offloaded):
+        assert all(torch.equal(a, b) for a, b in zip(base, got))
+
+
+@pytest.mark.parametrize("V", [1000, 5001])
+def test_distillation_offloaded_and_checkpointed(cuda, V):
+    import thetascan_amd as ts
+
+    g = torch.Generator().manual_seed(V)
+    z = (2.0 * torch.randn(33, V, generator=g)).bfloat16()
+    ids, lps = (x.to(cuda) for x in teacher(z, 12, g))
+    z = z.to(cuda)
+
+    def f(z):
+        return ts.distill_loss(z, ids, lps, temperature=1.3, softcap=30.0)[0]
+
+    def grads(h, scale):
+        leaf = z.detach().requires_grad_(True)
+        loss = h(leaf) * scale
+        return [loss, *torch.autograd.grad(loss, [leaf])]
+
+    for scale in (1.0, 3.0):
+        base = grads(f, scale)
+        again = grads(lambda z: checkpoint(f, z, use_reentrant=False), scale)
+        with torch.autograd.graph.save_on_cpu():
+            offloaded = grads(f, scale)
+        for got in (again, offloaded):
+            assert all(torch.equal(a, b) for a, b in zip(base, got))
+
+
+@pytest.mark.parametrize("V", [1000, 5001])
+def test_a_distillation_backward_captured_alone(cuda, V):
+    """The forward runs before the capture; every replay takes the upstream gradient of its time."""
+    import thetascan_amd as ts
+
+    g = torch.Generator().manual_seed(V)
+    z = (2.0 * torch.randn(33, V, generator=g)).bfloat16()
+    ids, lps = (x.to(cuda) for x in teacher(z, 12, g))
+    up = torch.ones((), device=cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = z.to(cuda).requires_grad_(True)
+        torch.autograd.grad(ts.distill_loss(warm, ids, lps)[0], warm, up)
+        leaf = z.to(cuda).requires_grad_(True)
+        loss = ts.distill_loss(leaf, ids, lps)[0]
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            (held,) = torch.autograd.grad(loss, leaf, up)
+    torch.cuda.current_stream().wait_stream(side)
+    for x in (2.0, 1.0, -0.5, 1.0):
+        up.fill_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        other = z.to(cuda).requires_grad_(True)
+        (want,) = torch.autograd.grad(ts.distill_loss(other, ids, lps)[0], other, torch.tensor(x, device=cuda))
+        # (a unit gradient stands from the forward, another is formed by the backward: one rounding apart)
+        assert torch.allclose(held.float(), want.float(), rtol=2.0 ** -7, atol=1e-30)
+
+
+@pytest.mark.parametrize("memory", ["theta", "delta"])
+def test_generation_under_autocast(cuda, memory):
+    """An fp32 model under autocast to bf16 generates as it trains: its products in bf16."""
+    model = _model(memory, torch.float32, cuda, window=16, sinks=2)
+    g = torch.Generator().manual_seed(1)
+    idx = torch.randint(0, 1024, (3, 21), generator=g).to(cuda)
+    u = torch.rand(3, 25, generator=g).to(cuda)
+    with torch.autocast("cuda", torch.bfloat16):
+        tokens, lps = model.generate(idx, u, top_k=50)
+        whole = torch.cat([idx, tokens], 1)
+        want = model.log_probs(whole[:, :-1], whole[:, 1:])[:, 20:]
+    # (bf16 logits of some ones: a rounding or two of 2^-8 at each of nine layers' ends)
+    assert torch.isfinite(lps).all() and (lps - want).abs().max() < 0.15

@@ -101,15 +101,16 @@ def _rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tens
 
 @dataclasses.dataclass
 class AttentionCache:
-    """What an attention layer carries through a generation: its ring cache, the next
-    tokens' positions, and the rotary phases of all positions to come."""
+    """What an attention layer carries through a generation: the next tokens' positions, the
+    rotary phases of all positions to come, and its ring cache, made with the prompt (an
+    autocast chooses its dtype)."""
 
-    k: torch.Tensor
-    v: torch.Tensor
     positions: torch.Tensor
     cos: torch.Tensor
     sin: torch.Tensor
     position: int = 0
+    k: torch.Tensor | None = None
+    v: torch.Tensor | None = None
 
 
 class CausalSelfAttention(nn.Module):
@@ -129,9 +130,7 @@ class CausalSelfAttention(nn.Module):
     def initial_cache(self, batch: int, total: int, like: torch.Tensor) -> AttentionCache:
         """The cache of ``batch`` sequences of up to ``total`` tokens, with none yet."""
         cos, sin = self.rotary(total, like.device)
-        shape = (batch, self.kv_heads, self.sinks + self.window, self.hd)
-        return AttentionCache(like.new_empty(shape), like.new_empty(shape),
-                              torch.zeros(batch, dtype=torch.int64, device=like.device), cos, sin)
+        return AttentionCache(torch.zeros(batch, dtype=torch.int64, device=like.device), cos, sin)
 
     def forward(self, x: torch.Tensor, cache: AttentionCache | None = None) -> torch.Tensor:
         """``cache``: continues from it (a prompt where it is new, then single tokens;
@@ -159,6 +158,7 @@ class CausalSelfAttention(nn.Module):
         else:
             y = windowed.windowed_attention(q, k, v, window=self.window, sinks=self.sinks)
             if cache is not None:
+                cache.k, cache.v = (x.new_empty(B, self.kv_heads, self.sinks + self.window, self.hd) for x in (k, v))
                 windowed.fill_window_cache(k, v, cache.k, cache.v, sinks=self.sinks)
         if cache is not None:
             cache.position += T
