@@ -1,7 +1,8 @@
 """Windowed attention, distillation and generation in the uses that their documents allow: saved tensors
-offloaded or formed again, a backward captured without its forward, autocast."""
+offloaded or formed again, a backward captured without its forward, autocast, scales at the ends of fp32."""
 from __future__ import annotations
 
+import math
 
 import pytest
 import torch
@@ -9,7 +10,7 @@ from torch.utils.checkpoint import checkpoint
 
 from tests.test_distill_gpu import teacher
 from tests.test_generation_gpu import _model
-from tests.test_window_gpu import inputs
+from tests.test_window_gpu import inputs, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +109,33 @@ def test_generation_under_autocast(cuda, memory):
         want = model.log_probs(whole[:, :-1], whole[:, 1:])[:, 20:]
     # (bf16 logits of some ones: a rounding or two of 2^-8 at each of nine layers' ends)
     assert torch.isfinite(lps).all() and (lps - want).abs().max() < 0.15
+
+
+@pytest.mark.parametrize("scale", [1.2e-38, 1e-30, 2e38])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scales_at_the_ends_of_fp32(cuda, scale, dtype):
+    """Scores of next to zero: every query's mean of the values that it sees; the largest scale that is
+    taken: of scores far apart, the highest alone."""
+    import thetascan_amd as ts
+
+    T = 100
+    q, k, v, do = (x.to(cuda) for x in inputs(1, 2, 2, T, 64, dtype))
+    seen = visible(T, 30, 2)
+    if scale > 1.0:
+        q, k = (torch.zeros_like(x) for x in (q, k))
+        k[..., 0] = torch.arange(T, device=cuda).remainder(30).to(dtype)  # (within a window, the highest is one token)
+        q[..., 0] = 1e-36
+        seen = visible(T, 30, 0)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    sinks = 2 if scale < 1.0 else 0
+    out = ts.windowed_attention(*leaves, window=30, sinks=sinks, scale=scale)
+    grads = torch.autograd.grad(out, leaves, do)
+    if scale < 1.0:
+        P = seen.double() / seen.double().sum(-1, keepdim=True)
+    else:
+        s = torch.where(seen, k[0, 0, :, 0].double().cpu(), -math.inf)
+        P = torch.nn.functional.one_hot(s.argmax(-1), T).double()
+    want = (P @ v.double().cpu(), P.T @ do.double().cpu())
+    for x, y in zip((out, grads[2]), want):
+        assert torch.allclose(x.detach().double().cpu(), y, rtol=2.0 ** -7, atol=2.0 ** -7 if dtype == torch.bfloat16 else 1e-5)
+    assert all(torch.isfinite(x).all() for x in grads)

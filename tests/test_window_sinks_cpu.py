@@ -42,3 +42,18 @@ def test_what_the_backward_refuses_the_forward_refuses():
         assert lib.ts_window_attention_fwd(ctypes.byref(one), ctypes.byref(io), None) == _lib.TS_ERR_NOT_IMPLEMENTED
         assert lib.ts_window_attention_bwd(ctypes.byref(one), ctypes.byref(io), ctypes.byref(grads), FAKE, 1 << 62,
                                            None) == _lib.TS_ERR_NOT_IMPLEMENTED
+
+
+def test_scales_that_fp32_does_not_hold():
+    import pytest
+    import torch
+
+    import thetascan_amd as ts
+
+    n = ctypes.c_size_t()
+    for scale in (1e-39, 2.4e38, 3e38, float("inf"), float("nan")):
+        one = desc(scale=scale)
+        assert _lib.load().ts_window_attention_bwd_workspace_bytes(ctypes.byref(one), ctypes.byref(n)) == _lib.TS_ERR_VALUE
+        x = torch.zeros(1, 1, 2, 16)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            ts.windowed_attention(x, x, x, scale=scale)

@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 
@@ -25,6 +24,7 @@ from .dispatch import HipOp, refuse_tangents
 from .scan_hip import _vec
 
 MAX_HEAD = 128
+LEAST_SCALE, MOST_SCALE = 1.2e-38, 2.3e38  # (fp32 holds them, and the latter times log2(e))
 _MOST = 2 ** 31 - 1
 
 
@@ -121,8 +121,8 @@ def _count(what: str, name: str, x, least: int) -> int:
 def _scale(what: str, scale: float | None, d: int) -> float:
     if scale is None:
         return d ** -0.5
-    if not (0.0 < float(scale) < math.inf):
-        raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
+    if not LEAST_SCALE <= float(scale) <= MOST_SCALE:
+        raise ValueError(f"{what}: scale must be positive, in [{LEAST_SCALE}, {MOST_SCALE}], got {scale}")
     return float(scale)
 
 
@@ -167,7 +167,8 @@ def windowed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, win
     ``q`` [B,H,T,d], ``k`` and ``v`` [B,Hk,T,d] (bf16 or fp32, any strides, d at most
     128; H a multiple of Hk: query head h reads key head h // (H / Hk)).  ``window``: tokens
     that a query sees back to, its own among them (None: all); ``sinks``: first tokens
-    that stay visible.  ``scale`` multiplies the scores (None: d ** -0.5).  ``lengths`` [B]
+    that stay visible.  ``scale`` multiplies the scores (None: d ** -0.5; scores past 2^30 in
+    size are not held, and may give NaN).  ``lengths`` [B]
     (integers, on the GPU, clamped to [0, T]) makes a padded batch: tokens at or past a
     sequence's length are not read, give zeros and gradients of zero.
 

@@ -53,7 +53,8 @@ __global__ __launch_bounds__(256, sizeof(E) == 2 ? (D == 64 ? 3 : 2) : 128 / D) 
   }
   // The reference is the highest score so far or up to 2^8 below it: terms to 2^8 lose nothing, and the
   // sums are seldom scaled.
-  const float slack = 8.f / p.scale2;
+  // (the least scales have no such slack in fp32: 1e38 of their scores is less than 2^8)
+  const float slack = fminf(8.f / p.scale2, 1e38f);
 
   auto pass = [&](auto careful) {
     constexpr bool CAREFUL = decltype(careful)::value;
@@ -230,7 +231,7 @@ int window_rows(const ts_strided& s, int vec) {
 // The kernels' parameters of a call; without io, of its sizes.
 int window_setup(const ts_window_desc* d, const ts_window_io* io, WinP* p) {
   if (!d || d->B < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv || d->T < 0 || d->d < 1 || d->window < 1 ||
-      d->sinks < 0 || !(d->scale > 0.f && d->scale < INFINITY))
+      d->sinks < 0 || !(d->scale >= 1.17549435e-38f && d->scale * 1.44269504088896340736f < INFINITY))
     return fail(TS_ERR_VALUE, "window attention: bad shape, window, sinks or scale");
   if (d->dtype != TS_BF16 && d->dtype != TS_F32)
     return fail(TS_ERR_NOT_IMPLEMENTED, "window attention: bf16 or fp32 only");
