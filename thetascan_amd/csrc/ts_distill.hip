@@ -83,13 +83,6 @@ struct TemperedExp {
   }
 };
 
-template <bool CAP>
-__device__ __forceinline__ double distill_logit(const DistillP& p, float z) {
-  double y = (double)z;
-  if (CAP) y = (double)p.cap * tanh(y / (double)p.cap);
-  return y * p.inv_t;
-}
-
 // ------------------------------------------------ rows that fit in registers
 
 // Sums and maxima over a wave: neighbours by data-parallel moves, then halves by row swaps.
