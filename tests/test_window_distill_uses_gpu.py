@@ -139,3 +139,19 @@ def test_scales_at_the_ends_of_fp32(cuda, scale, dtype):
     for x, y in zip((out, grads[2]), want):
         assert torch.allclose(x.detach().double().cpu(), y, rtol=2.0 ** -7, atol=2.0 ** -7 if dtype == torch.bfloat16 else 1e-5)
     assert all(torch.isfinite(x).all() for x in grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_cache_filled_from_itself(cuda, dtype):
+    """Tokens dropped from the front: the slots' rows move within the cache, each read before it is written."""
+    import thetascan_amd as ts
+
+    g = torch.Generator().manual_seed(3)
+    for drop, sinks in ((1, 0), (3, 2), (500, 16)):
+        caches = [torch.randn(3, 4, 2000, 64, generator=g).to(dtype).to(cuda) for _ in range(2)]
+        want = [x.clone() for x in caches]
+        rows = [x[:, :, drop:] for x in caches]
+        for x in want:
+            x[:, :, :2000 - drop] = x[:, :, drop:].clone()
+        ts.fill_window_cache(*rows, *caches, sinks=sinks)
+        assert all(torch.equal(x, y) for x, y in zip(caches, want))

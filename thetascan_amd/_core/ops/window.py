@@ -217,6 +217,13 @@ def _cache(what: str, k: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Ten
     return min(cache_k.shape[2] - sinks, _MOST)
 
 
+def _meets(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether the stretches of memory that hold two tensors overlap."""
+    (a, b), (c, d) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+                      for t in (x, y))
+    return a < d and c < b
+
+
 def _changed(*caches: torch.Tensor) -> None:
     for x in caches:
         if not x.is_inference():
@@ -296,6 +303,8 @@ def fill_window_cache(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, c
     _same_place(what, k, (v, cache_k, cache_v, lengths))
     if T == 0:
         return
+    # (what stands in a cache itself is read from a copy: slots are written while others are read)
+    k, v = (x.clone() if _meets(x, cache_k) or _meets(x, cache_v) else x for x in (k, v))
     vec = _vec(k.dtype)
     desc = _describe(k.shape, Hk, k.dtype, window, sinks, 1.0)
     (k4, sk), (v4, sv) = _rows(k, vec), _rows(v, vec)
