@@ -1416,7 +1416,8 @@ int ts_window_cache_fill(const ts_window_desc* desc, const ts_window_io* io, ts_
  * while the weight before a token is less than top_p of theirs (the first always); of those,
  * w_i >= min_p 2^44.  The token is the first, by index, whose running weight is over
  * floor(u times the weight left).  temperature 0: the highest logit.  A logit of -inf is no token;
- * a row of none, or with +inf or NaN, has token -1 and log-probability NaN. */
+ * a row of none, or with +inf or NaN, or of a setting that is NaN, has token -1 and log-probability
+ * NaN.  Fewer than 2^22 rows a call. */
 typedef struct ts_sample_desc {
   int64_t rows, stride;
   int32_t V, dtype; /* V < 2^19                                                 */

@@ -1,5 +1,6 @@
 """Windowed attention, distillation and generation in the uses that their documents allow: saved tensors
-offloaded or formed again, a backward captured without its forward, autocast, scales at the ends of fp32."""
+offloaded or formed again, a backward captured without its forward, autocast, scales at the ends of fp32, settings that are
+no numbers."""
 from __future__ import annotations
 
 import math
@@ -155,3 +156,22 @@ def test_a_cache_filled_from_itself(cuda, dtype):
             x[:, :, :2000 - drop] = x[:, :, drop:].clone()
         ts.fill_window_cache(*rows, *caches, sinks=sinks)
         assert all(torch.equal(x, y) for x, y in zip(caches, want))
+
+
+@pytest.mark.parametrize("V", [100, 9000])
+def test_a_row_of_a_setting_that_is_no_number_draws_nothing(cuda, V):
+    import thetascan_amd as ts
+
+    g = torch.Generator().manual_seed(4)
+    z, u = torch.randn(4, V, generator=g).to(cuda), torch.rand(4, generator=g).to(cuda)
+    usual = dict(temperature=torch.full((4,), 0.8), top_p=torch.full((4,), 0.9), min_p=torch.full((4,), 0.01))
+    want = ts.sample_tokens(z, u, **{n: x.to(cuda) for n, x in usual.items()})
+    for row, name in enumerate(usual):
+        one = {n: x.clone() for n, x in usual.items()}
+        one[name][row] = math.nan
+        for more in (dict(), dict(top_k=7)):
+            tokens, lps = ts.sample_tokens(z, u, **{n: x.to(cuda) for n, x in one.items()}, **more)
+            assert int(tokens[row]) == -1 and math.isnan(float(lps[row]))
+            if not more:
+                others = torch.arange(4, device=cuda) != row
+                assert torch.equal(tokens[others], want[0][others]) and torch.equal(lps[others], want[1][others])

@@ -58,7 +58,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     tensors, a ``top_k`` below one counts as one, a ``top_p`` at or below zero leaves the
     first token, a ``min_p`` over one counts as one.  ``softcap`` caps the logits at
     ``softcap tanh(z / softcap)``.  A logit of -inf is no token, whatever the cap; a row that has no
-    token, or +inf or NaN in it, or a temperature below zero or NaN, gives token -1 and NaN.
+    token, or +inf or NaN in it, or a temperature below zero, or a setting that is NaN, gives
+    token -1 and NaN.  Fewer than 2^22 rows a call.
     """
     what = "sample_tokens"
     if logits.ndim < 1 or logits.shape[-1] < 1:

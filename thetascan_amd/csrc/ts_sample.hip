@@ -589,7 +589,7 @@ struct Sampler {
     // +inf, has no token
     const Logit<CAP> f(p.cap);
     float mine = -INFINITY, ym = kLowest, s = 0.f;
-    bool bad = !(temperature >= 0.0);
+    bool bad = !(temperature >= 0.0) || top_p != top_p || min_p != min_p;
     vectors([&](int, const Vec16<E>& v) {
       float y[N], top = ym;
       const bool far = f.some_far(v);
