@@ -10,11 +10,12 @@ and ``P_k = exp(lp_k)``::
 ``P_r = 1 - sum_k P_k`` and ``Q_r`` are the teacher's and the student's share of all other
 tokens; without the tail, P is the softmax of the K log-probabilities (which may be any scores)
 and the second term is left out; so it is where the student forbids all other tokens (logits of
--inf: what the teacher's log-probabilities leave there may be their rounding alone).  Where a gradient is recorded, the forward's launch gives it too, for a unit
-upstream gradient (ts_distill_fwd): it is as large as the logits and held to the backward, as
-a saved tensor, which forms it again where the upstream gradient is another (as does a second
-backward of the same loss).  A loss whose value alone is wanted is called without gradients.  No
-probabilities are stored.  A row of weight zero is not read.
+-inf: what the teacher's log-probabilities leave there may be their rounding alone).  Where a
+gradient is recorded, the forward's launch gives it too, for a unit upstream gradient
+(ts_distill_fwd): it is as large as the logits and held to the backward, as a saved tensor, which
+forms it again where the upstream gradient is another (as does a second backward of the same
+loss).  A loss whose value alone is wanted is called without gradients.  No probabilities are
+stored.  A row of weight zero is not read.
 """
 from __future__ import annotations
 

@@ -9,7 +9,9 @@ ts_window_attention_bwd), and single tokens against a cache of fixed size
 
 bf16 inputs: products take bf16 operands (the probabilities and their gradients rounded
 once) and fp32 sums; fp32 inputs compute in fp32.  A value that is not finite reaches the
-outputs and gradients alone that its formula has it in.
+outputs and gradients alone that its formula has it in.  Where a gradient is recorded, a
+call keeps its inputs, its output, a log-sum a query (fp32) and, in bf16, what the output's
+rounding left (as large as the output), which the gradients' digits need.
 """
 from __future__ import annotations
 

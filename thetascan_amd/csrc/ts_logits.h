@@ -91,8 +91,9 @@ static __device__ const double kPowers64[64] = {
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
-// e^t for t in [-745, 0], to some 2^-52 of itself: 2^(n / 64) from the table above (or a copy in
-// LDS), the rest by its series.
+// e^t for t in [-745, 0], to some 2^-52 of itself, by a table and a short polynomial (the table-driven
+// method of P. T. P. Tang, 1989): t = n ln 2 / 64 + r, 2^(n / 64) from the table above (or a copy in
+// LDS), e^r by its series.
 struct Exp64 {
   const double* table;
   __device__ __forceinline__ double operator()(double t) const {

@@ -12,7 +12,9 @@
 // A workgroup takes a row.  A cut (of top-k by counts, of top-p by weights) is found without
 // sorting: a histogram over the distance from the maximum, in LDS by integer atomics, then
 // histograms of the keys inside the bin that the cut falls into, down to one key, then of
-// the indices of its ties.  The token is found the same way, by weights over the indices.
+// the indices of its ties.  The token is found the same way, by weights over the indices.  Few tokens
+// or a small nucleus are sorted in LDS instead.  256 rows of 131072 logits, settings a row: 160 us, bound by
+// the passes over a row that one CU makes, two of them with fp64 exponentials.
 
 #include "ts_common.h"
 #include "ts_logits.h"
@@ -469,6 +471,9 @@ struct Sampler {
 
   __device__ __forceinline__ int pick(int64_t top_k, double top_p, double u, float mine) {
     const int sv = bits_over((uint32_t)(vecs - 1), 11);
+    // (a list of them or cut after cut, 64 rows in us: 131072 logits, top_k 20 44 either way, 100 48 and 96, 500 64
+    // and 103, past kList / 4 900 132 and 108; 32768, 500 43 and 44, 900 54 and 46; short rows' lists overflow
+    // from 100 on: 8192, 250 56 and 30; 1024, 250 33 and 16)
     if (top_k < V && top_k <= kList / 4) {
       // The k-th highest of the threads' maxima bounds the k-th logit from below: what lies in its bin and
       // above is little more than k
@@ -678,6 +683,8 @@ using ts::SampleP;
 template <typename E, bool CAP>
 void launch(const SampleP& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.rows);
+  // (256 and 1024 threads a row, a nucleus in us: 1024 logits, 16 rows 22 and 27, 1024 rows 28 and 100; 8192, 40 and
+  // 37, 71 and 146; 16384, 70 and 49, 100 and 195; 32768, 133 and 71, 188 and 280)
   if (p.V <= 8192)
     hipLaunchKernelGGL((ts::sample_kernel<E, CAP, 256>), grid, dim3(256), 0, stream, p);
   else

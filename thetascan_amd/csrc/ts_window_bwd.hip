@@ -10,6 +10,10 @@
 // for both of its uses, by rows and by columns.  In bf16, P and dS enter the keys' products
 // in bf16 (2^-9 of each, as the gradients' own rounding); the queries' takes dS in two parts: a
 // query's dS add to zero, so that of keys that are alike little is left but what rounding leaves.
+// At B8 H8 T4096 (64-wide on 4 key heads, window 1024) the keys' kernel takes 219 us and the queries' 170, the
+// matrix cores busy in 24 and 31 % of them, other vector instructions in 20 and 40; at 16384 tokens of 8
+// 128-wide heads 439 and 302 us, busy in 25 and 36 %: one tile in LDS with two barriers, not either unit, bounds
+// the keys'.
 //
 // A sink is seen by every query behind its window: those pairs go to workgroups of their
 // own, a stretch of queries each, which leave sums of the sinks' rows in fp32; where workgroups are
@@ -437,7 +441,9 @@ __global__ __launch_bounds__(256) void window_parts_kernel(WinP p) {
   st4f<E>((E*)to.ptr + b * to.sb + hk * to.sh + (int64_t)t * to.st + c % p.d, r);
 }
 
-// Keys of a workgroup of the second kernel: 128 where their sums fit twice in a SIMD's registers.
+// Keys of a workgroup of the second kernel: 128 where their sums fit twice in a SIMD's registers and workgroups
+// are many (with gradients in us, 128 and 64 keys, 64-wide heads, at 128, 256, 512 and 1024 of the former: 2048
+// tokens of 8 key heads 89 74, 109 105, 137 134, 221 222; 4096 of 4 131 124, 175 165, 260 258, 438 453).
 static int window_keys(const WinP& p, int B, bool bf) { return bf && p.d <= 64 && !window_narrow(p, B, bf, p.Hkv) ? 128 : 64; }
 
 struct WinSplit {
@@ -449,7 +455,9 @@ static WinSplit window_split(const ts_window_desc* d, WinP* p) {
   const bool bf = d->dtype == TS_BF16;
   const int keys = window_keys(*p, d->B, bf);
   p->near_tiles = (p->T + keys - 1) / keys;
-  // query heads apart, where the key heads' workgroups would leave half of the CUs idle
+  // query heads apart, where the key heads' workgroups would leave half of the CUs idle (8 on 2 heads, with
+  // gradients in us, apart and together, at 32, 64, 128 and 256 of those: 64-wide 48 79, 54 114, 78 132, 108
+  // 162; 128-wide 69 112, 77 154, 116 179, 175 234: the border could lie higher)
   const bool apart = p->rep > 1 && (int64_t)d->B * d->Hkv * p->near_tiles < 128;
   p->owners = apart ? d->H : d->Hkv;
   p->reps = apart ? 1 : p->rep;
@@ -458,7 +466,9 @@ static WinSplit window_split(const ts_window_desc* d, WinP* p) {
   if (p->sinks > 0 && behind > 0) {
     const int tiles = (behind + TT - 1) / TT + 1;
     p->far_tiles = (p->sinks + keys - 1) / keys;
-    // Stretches only until every CU has several workgroups: each leaves sums of all the sinks' rows (8192
+    // Stretches of 16 tiles, of 4 where few workgroups are (us with gradients: one sequence of 16384 tokens of 8
+    // heads on 2 in stretches of 4, 8, 16 and 32 tiles 291, 286, 308, 411; of 3000 in 1, 2, 4, 8 and 16 65, 59, 54, 58,
+    // 64).  Only until every CU has several workgroups: each leaves sums of all the sinks' rows (8192
     // sinks of 32 heads of 64 in 31 stretches of 32768 queries were 4.4 GB, in one they are 0.3)
     const int64_t groups = (int64_t)d->B * p->owners * p->far_tiles, most = groups < 2048 ? 2048 / groups : 1;
     p->chunk_tiles = max(max(apart ? 4 : 16, (tiles + 63) / 64), (int)((tiles + most - 1) / most));

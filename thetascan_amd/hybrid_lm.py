@@ -246,7 +246,7 @@ class HybridLM(nn.Module):
 
     ``memory`` names the mixers of layers 4 and 5: "theta" (ThetaScan-Kernel) or
     "delta" (gated delta rule); ``window`` and ``sinks`` are the attention layers'
-    (None: every earlier token)."""
+    (None: every earlier token, the first ones among them whatever ``sinks`` is)."""
 
     def __init__(self, memory: str = "theta", window: int | None = None, sinks: int = 0):
         super().__init__()
