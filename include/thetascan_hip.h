@@ -1367,8 +1367,9 @@ int ts_policy_loss_bwd(const ts_policy_desc* desc, const ts_policy_io* io, const
 /* Softmax attention of q [B,H,T,d] against k, v [B,Hkv,T,d] (Hkv divides H: head h reads
  * head h / (H / Hkv)); query i sees key j where j <= i and (i - j < window or j < sinks):
  *   out[b,h,i] = sum_j softmax_j(scale q_i . k_j) v_j
- * bf16 or fp32; d <= 128 in 16-byte vectors; rows 16-byte aligned.  Tokens at or past a
- * sequence's length are not read and give zeros. */
+ * bf16 or fp32; d <= 128 in 16-byte vectors; rows 16-byte aligned; a scale that fp32 holds as a normal
+ * number, as it does scale log2(e).  Tokens at or past a sequence's length are not read and give
+ * zeros.  A forward with lse refuses what its backward would. */
 typedef struct ts_window_desc {
   int32_t B, H, Hkv, T, d, dtype;
   int32_t window, sinks;
