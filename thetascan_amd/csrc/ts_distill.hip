@@ -11,7 +11,7 @@
 // those tokens alone (the teacher's are marked in LDS, a bit each), from a maximum of their own, not
 // taken from one.  Exponentials are fp32; the K tokens' terms are formed and added in fp64 (they all
 // but cancel), as are a row's last sums, the rows in fp64 in a fixed order.  65536 rows of 1024
-// (capped, K 32, with gradient): 141 us, of which vector instructions issue in 62 %; 8192 of
+// (capped, K 32, with gradient): 136 us, of which vector instructions issue in 62 %; 8192 of
 // 32768: 272 us, 3.9 TB/s of what has to move.
 
 #include "ts_common.h"
@@ -238,8 +238,10 @@ __device__ __forceinline__ DistillFactors distill_factors(const DistillP& p, dou
 
 // A wave takes R rows one after the other, each held in registers from its one reading to its
 // gradient; the next row is on its way meanwhile.  The rows' logarithms follow, a lane each.
+// (Three waves a SIMD where 16 logits a lane and a token leave the registers for it: with 172 of them, two,
+// 65536 rows of 1024 took 169 us instead of 136.)
 template <typename E, bool CAP, int VPT, int KS, int R, bool GRAD>
-__global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
+__global__ __launch_bounds__(256, VPT * Vec16<E>::N <= 16 && KS == 1 ? 3 : 1) void distill_rows_kernel(DistillP p) {
   constexpr int N = Vec16<E>::N, LANES = 64, GROUPS = 4, WORDS = LANES * VPT * N / 32 + 1;
   __shared__ uint32_t all_marks[GROUPS][WORDS];
   __shared__ double sums[GROUPS];
@@ -357,19 +359,36 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillP p) {
       }
     double mass = 0.0, a = 0.0, ek = 0.0, near = 0.0, P[KS];
     float q[KS];
+    if (KS == 1 && p.K <= 32) {
+      // (uniform) the upper lanes have no token: they form the lower ones' e^off while those form P
+      const bool on = id[0] >= 0;
+      const double off = on ? ((double)yk[0] - (double)high) * p.inv_t : -INFINITY;
+      const double lps = on ? (double)lp[0] - (double)hl : -INFINITY;
+      const uint64_t bits = (uint64_t)__double_as_longlong(off);
+      const LanePair lo = xor32_pair(__uint_as_float((uint32_t)bits)), hi = xor32_pair(__uint_as_float((uint32_t)(bits >> 32)));
+      const double up = __longlong_as_double((long long)((uint64_t)__float_as_uint(hi.a) << 32 | __float_as_uint(lo.a)));
+      const double x = distill_exp(e64, li < 32 ? lps : up);
+      P[0] = li < 32 ? x : 0.0;
+      ek = li < 32 ? 0.0 : x;
+      q[0] = on ? te(yk[0] - high) : 0.f;
+      near = (double)q[0];
+      mass = P[0];
+      if (P[0] != 0.0) a = P[0] * (lps - off);
+    } else {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      P[s] = 0.0;
-      q[s] = 0.f;
-      if (id[s] >= 0) {
-        const double off = ((double)yk[s] - (double)high) * p.inv_t, lps = (double)lp[s] - (double)hl;
-        // (in fp64: one less their sum is what the teacher leaves to all others)
-        P[s] = distill_exp(e64, lps);
-        q[s] = te(yk[s] - high);
-        near += (double)q[s];
-        ek += distill_exp(e64, off);
-        mass += P[s];
-        if (P[s] != 0.0) a += P[s] * (lps - off);
+      for (int s = 0; s < KS; ++s) {
+        P[s] = 0.0;
+        q[s] = 0.f;
+        if (id[s] >= 0) {
+          const double off = ((double)yk[s] - (double)high) * p.inv_t, lps = (double)lp[s] - (double)hl;
+          // (in fp64: one less their sum is what the teacher leaves to all others)
+          P[s] = distill_exp(e64, lps);
+          q[s] = te(yk[s] - high);
+          near += (double)q[s];
+          ek += distill_exp(e64, off);
+          mass += P[s];
+          if (P[s] != 0.0) a += P[s] * (lps - off);
+        }
       }
     }
     if (bad) a = (double)NAN;
