@@ -11,7 +11,7 @@
 // those tokens alone (the teacher's are marked in LDS, a bit each), from a maximum of their own, not
 // taken from one.  Exponentials are fp32; the K tokens' terms are formed and added in fp64 (they all
 // but cancel), as are a row's last sums, the rows in fp64 in a fixed order.  65536 rows of 1024
-// (capped, K 32, with gradient): 136 us, of which vector instructions issue in 62 %; 8192 of
+// (capped, K 32, with gradient): 136 us, of which vector instructions issue in 63 %; 8192 of
 // 32768: 272 us, 3.9 TB/s of what has to move.
 
 #include "ts_common.h"
@@ -819,7 +819,7 @@ bool fits(const DistillP& p, bool bf, int per) { return p.V + (p.aligned ? 0 : (
 bool in_registers(const DistillP& p, bool bf) { return p.K <= 256 && fits(p, bf, kPer); }
 // Rows of a wave: several (the next row's loads then hide behind a row's arithmetic), where there are enough to
 // keep every CU busy all the same.  Loss and gradient in us, eight and one: 2048 rows of 1024 (K 32, capped)
-// 36 and 18, 8192 41 and 44, 16384 51 and 76, 32768 81 and 137; of 2048 (K 64) 16384 59 and 54, 32768 129 and 111.
+// 35 and 18, 8192 41 and 44, 16384 50 and 76, 32768 80 and 136; of 2048 (K 64) 16384 59 and 55, 32768 128 and 112.
 int rows_of(const DistillP& p) { return p.rows >= 16384 ? 8 : 1; }
 
 int64_t blocks_of(const DistillP& p, bool bf) {
